@@ -526,6 +526,104 @@ int32_t tk_quant_fp8_rows(const void* x, int32_t dtype, int64_t M, int64_t K, in
                           int64_t stride_qm, float* scales, tk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Row operators around the experts
+ * ---------------------------------------------------------------------------------------------- */
+
+/*
+ * Layer norm of the rows of x [n_rows, n_cols] (unit stride along the columns, rows at any element stride and address):
+ *   y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps),   var = mean((x - mean)^2)
+ * x and y share `dtype` (fp32 / bf16 / fp16); weight and bias [n_cols] are optional (NULL) and have a type of their own;
+ * mean and rstd [n_rows] fp32 are optional outputs, which the backward pass reads.  Statistics and arithmetic in fp32, one
+ * rounding to `dtype`.  No counterpart in the reference's operator library.
+ */
+int32_t tk_layer_norm(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols, int64_t stride_xm, const void* weight,
+                      int32_t weight_dtype, const void* bias, int32_t bias_dtype, float eps, void* y, int64_t stride_ym,
+                      float* mean, float* rstd, tk_stream_t stream);
+
+/*
+ * Gradients of tk_layer_norm for dy (x's type):  with h = (x - mean) * rstd and g = dy * weight,
+ *   dx = (g - mean(g) - h * mean(g * h)) * rstd,   dweight = sum over rows of dy * h,   dbias = sum over rows of dy.
+ * Each of dx, dweight, dbias may be NULL (not wanted).  The sums over rows are taken in fp32 in an order that depends on the sizes
+ * alone, through `workspace` of tk_layer_norm_backward_workspace_bytes(...) bytes (needed with dweight or dbias; 16-byte aligned,
+ * not cleared).
+ */
+int64_t tk_layer_norm_backward_workspace_bytes(int64_t n_rows, int64_t n_cols);
+int32_t tk_layer_norm_backward(const void* dy, int64_t stride_dym, const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,
+                               int64_t stride_xm, const void* weight, int32_t weight_dtype, const float* mean, const float* rstd,
+                               void* dx, int64_t stride_dxm, void* dweight, void* dbias, int32_t bias_dtype, void* workspace,
+                               tk_stream_t stream);
+
+/*
+ * Rows of logits over a whole vocabulary, logits [n_rows, vocab] with unit stride along the vocabulary, rows at any element
+ * stride and address.  With z = logits / temperature, m = max z, s = sum exp(z - m), p = exp(z - m) / s:
+ *
+ *   tk_token_logprobs            logprobs[t] = z[tokens[t]] - m - ln s;  entropy[t] = -sum p ln p;  the k largest logits, larger
+ *                                first, equal ones by index, as top_indx and top_logprobs = z - m - ln s
+ *   tk_token_logprobs_backward   d_logits = (d_logprobs (1[v = token] - p) - d_entropy p (ln p + entropy)) / temperature
+ *   tk_distill_topk              a = softmax(teacher_logits / temperature) over the entries of a row;
+ *                                loss[t] = sum_j a_j (ln a_j - (z[teacher_indx[t, j]] - m - ln s))
+ *   tk_distill_topk_backward     d_logits = d_loss (p - sum of a_j over the entries j that name v) / temperature
+ *
+ * Outputs and their gradients are fp32.  `stats` [2, n_rows] fp32 (m as a logit, not divided by the temperature; ln s) and
+ * `teacher_stats` [2, n_rows] (the same of a row's teacher entries) are written by the forward calls where given (optional there)
+ * and read by the backward calls.  Rows that are no distribution:
+ *   - a logit of -inf has probability zero.  A row of nothing else: logprobs -inf, entropy 0, loss +inf, gradient 0;
+ *   - a row with a NaN or +inf: logprobs, entropy, top_logprobs, loss and gradient are NaN, top_indx is -1;
+ *   - a token outside [0, vocab): logprobs 0, and no gradient through it;
+ *   - a teacher entry whose index is outside [0, vocab), or whose logit is -inf, carries no weight; a row without any other has loss 0
+ *     and gradient 0.  An index that occurs twice counts twice.
+ * A row whose given gradients are all zero has the gradient zero.
+ * No counterpart in the reference's operator library; tk/topk.py:25-141 is the router's selection.
+ */
+#define TK_VOCAB_MAX_TOP 128            /* k of tk_token_logprobs */
+#define TK_VOCAB_MAX_TOP_COLUMNS 524288 /* vocab, where k > 0 */
+#define TK_VOCAB_MAX_TEACHER 1024       /* teacher entries a row */
+typedef struct tk_vocab_desc {
+  const void* logits;
+  int32_t logits_dtype; /* TK_F32, TK_BF16, TK_F16; also d_logits' */
+  int64_t logits_stride_m;
+  int32_t n_rows;
+  int32_t vocab;
+  float temperature; /* > 0, finite */
+  float* stats;
+  /* token_logprobs */
+  const void* tokens; /* [n_rows] */
+  int32_t tokens_i64; /* int64 instead of int32 */
+  float* logprobs;
+  float* entropy; /* read by the backward call */
+  int32_t k;      /* <= TK_VOCAB_MAX_TOP and vocab; 0 = no alternatives */
+  float* top_logprobs;
+  int32_t* top_indx; /* [n_rows, k] contiguous */
+  /* distill_topk */
+  const void* teacher_logits; /* [n_rows, n_teacher], unit stride along the entries */
+  int32_t teacher_dtype;      /* TK_F32, TK_BF16, TK_F16 */
+  int64_t teacher_stride_m;
+  const void* teacher_indx;
+  int32_t teacher_indx_i64;
+  int64_t teacher_indx_stride_m;
+  int32_t n_teacher; /* <= TK_VOCAB_MAX_TEACHER */
+  float* teacher_stats;
+  float* loss;
+  /* backward: gradients of the outputs, element stride 0 = one value for all rows; NULL = zero */
+  const float* d_logprobs;
+  int64_t d_logprobs_stride;
+  const float* d_entropy;
+  int64_t d_entropy_stride;
+  const float* d_loss;
+  int64_t d_loss_stride;
+  void* d_logits;
+  int64_t d_logits_stride_m;
+  /* tk_vocab_workspace_bytes(n_rows, vocab, k) bytes, 16-byte aligned, not cleared; the forward calls use it (k = 0 for distill_topk) */
+  void* workspace;
+} tk_vocab_desc;
+
+int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k);
+int32_t tk_token_logprobs(const tk_vocab_desc* desc, tk_stream_t stream);
+int32_t tk_token_logprobs_backward(const tk_vocab_desc* desc, tk_stream_t stream);
+int32_t tk_distill_topk(const tk_vocab_desc* desc, tk_stream_t stream);
+int32_t tk_distill_topk_backward(const tk_vocab_desc* desc, tk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Host check hooks (no device work, no GPU needed)
  * ---------------------------------------------------------------------------------------------- */
 

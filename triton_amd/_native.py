@@ -96,6 +96,18 @@ class DecodeLayerDesc(_c.Structure):
     ]
 
 
+class VocabDesc(_c.Structure):
+    """struct tk_vocab_desc (field order and types follow include/triton_amd.h)."""
+    _fields_ = [
+        ("logits", _ptr), ("logits_dtype", _i32), ("logits_stride_m", _i64), ("n_rows", _i32), ("vocab", _i32), ("temperature", _f32),
+        ("stats", _ptr), ("tokens", _ptr), ("tokens_i64", _i32), ("logprobs", _ptr), ("entropy", _ptr), ("k", _i32), ("top_logprobs", _ptr),
+        ("top_indx", _ptr), ("teacher_logits", _ptr), ("teacher_dtype", _i32), ("teacher_stride_m", _i64), ("teacher_indx", _ptr),
+        ("teacher_indx_i64", _i32), ("teacher_indx_stride_m", _i64), ("n_teacher", _i32), ("teacher_stats", _ptr), ("loss", _ptr),
+        ("d_logprobs", _ptr), ("d_logprobs_stride", _i64), ("d_entropy", _ptr), ("d_entropy_stride", _i64), ("d_loss", _ptr),
+        ("d_loss_stride", _i64), ("d_logits", _ptr), ("d_logits_stride_m", _i64), ("workspace", _ptr),
+    ]
+
+
 # name -> (restype, argtypes); must list every symbol include/triton_amd.h declares.
 SIGNATURES = {
     "tk_version": (_i32, []),
@@ -119,6 +131,14 @@ SIGNATURES = {
     "tk_reduce_mid_backward": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr]),
     "tk_quant_fp8_rows": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr]),
     "tk_mx_upcast": (_i32, [_ptr, _ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _i64, _ptr]),
+    "tk_layer_norm": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _i32, _f32, _ptr, _i64, _ptr, _ptr, _ptr]),
+    "tk_layer_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "tk_layer_norm_backward": (_i32, [_ptr, _i64, _ptr, _i32, _i64, _i64, _i64, _ptr, _i32, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i32, _ptr, _ptr]),
+    "tk_vocab_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "tk_token_logprobs": (_i32, [_c.POINTER(VocabDesc), _ptr]),
+    "tk_token_logprobs_backward": (_i32, [_c.POINTER(VocabDesc), _ptr]),
+    "tk_distill_topk": (_i32, [_c.POINTER(VocabDesc), _ptr]),
+    "tk_distill_topk_backward": (_i32, [_c.POINTER(VocabDesc), _ptr]),
     # host check hooks (no device work)
     "tk_host_mx_convert": (_i32, [_ptr, _i64, _i32, _ptr]),
     "tk_host_mx_scale": (_i32, [_ptr, _i64, _i32, _i32, _ptr]),

@@ -334,3 +334,50 @@ def matmul_ogs_torch(x, w, bias, routing_data=None, gather_indx=None, scatter_in
     if scatter_indx is None:
         return y
     return reduce_torch(y.view(y.shape[0] // k, k, -1), dim=1)[0]
+
+
+# ---- rows around the experts ------------------------------------------------------------------------------
+
+def layer_norm_torch(x, weight=None, bias=None, eps: float = 1e-5):
+    """Layer norm over the last dimension with its arithmetic in fp32."""
+    xf = x.to(torch.float32)
+    centred = xf - xf.mean(-1, keepdim=True)
+    y = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
+    y = y if weight is None else y * weight.to(torch.float32)
+    return (y if bias is None else y + bias.to(torch.float32)).to(x.dtype)
+
+
+def _log_softmax_rows(logits, temperature):
+    """fp32 log probabilities; rows of -inf alone stay -inf."""
+    x = logits.to(torch.float32)
+    m = x.amax(1, keepdim=True)
+    z = (x - torch.where(m == float("-inf"), torch.zeros_like(m), m)) / temperature
+    s = z.exp().sum(1, keepdim=True)
+    return z - torch.where(s == 0, torch.zeros_like(s), s.log())
+
+
+def token_logprobs_torch(logits, tokens, k: int = 0, temperature: float = 1.0):
+    """Log probabilities of the given tokens, entropies, and the k largest entries of each row (ties to the lower index)."""
+    from .logprobs import TokenLogprobs
+    V = logits.shape[1]
+    lp = _log_softmax_rows(logits, temperature)
+    live = (tokens >= 0) & (tokens < V)
+    at = torch.where(live, tokens, torch.zeros_like(tokens)).to(torch.int64)
+    logprobs = torch.where(live, lp.gather(1, at[:, None]).squeeze(1), lp.new_zeros(()))
+    p = lp.exp()
+    entropy = -torch.where(p > 0, p * lp, p).sum(1)
+    top = torch.sort(logits.to(torch.float32), dim=1, descending=True, stable=True).indices[:, :k]
+    bad = entropy.isnan()[:, None]
+    return TokenLogprobs(logprobs, entropy, torch.where(bad, lp.new_full((), float("nan")), lp.gather(1, top)) if k else None,
+                         torch.where(bad, top.new_full((), -1), top).to(torch.int32) if k else None)
+
+
+def distill_topk_torch(logits, teacher_logits, teacher_indx, temperature: float = 1.0):
+    """Kullback-Leibler divergence of each row from the teacher that its entries describe."""
+    lp = _log_softmax_rows(logits, temperature)
+    live = (teacher_indx >= 0) & (teacher_indx < logits.shape[1]) & (teacher_logits != float("-inf"))
+    q = torch.where(live, teacher_logits.to(torch.float32), lp.new_full((), float("-inf")))
+    la = _log_softmax_rows(q, temperature)
+    a = torch.where(live, la.exp(), lp.new_zeros(()))
+    at = torch.where(live, teacher_indx, torch.zeros_like(teacher_indx)).to(torch.int64)
+    return torch.where(a != 0, a * (la - lp.gather(1, at)), a).sum(1)
