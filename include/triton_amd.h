@@ -583,7 +583,7 @@ typedef struct tk_vocab_desc {
   int32_t logits_dtype; /* TK_F32, TK_BF16, TK_F16; also d_logits' */
   int64_t logits_stride_m;
   int32_t n_rows;
-  int32_t vocab;
+  int32_t vocab;     /* <= 2^30 */
   float temperature; /* > 0, finite */
   float* stats;
   /* token_logprobs */

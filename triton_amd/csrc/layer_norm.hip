@@ -7,17 +7,17 @@ namespace {
 template <int DT>
 __global__ __launch_bounds__(256) void layer_norm_kernel(const void* x, int64_t M, int64_t C, int64_t sx, const void* w, int wt, const void* b, int bt,
                                                          float eps, void* y, int64_t sy, float* mean, float* rstd) {
-  __shared__ float buf[256];
+  __shared__ float buf[3][4];
   for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
     float s = 0.f;
     for (int64_t c = threadIdx.x; c < C; c += 256) s += RowType<DT>::load(x, m * sx + c);
-    const float mu = block_sum<256>(s, buf) / (float)C;
+    const float mu = block_sum<256>(s, buf[0]) / (float)C;
     s = 0.f;
     for (int64_t c = threadIdx.x; c < C; c += 256) {
       const float d = RowType<DT>::load(x, m * sx + c) - mu;
       s = fmaf(d, d, s);
     }
-    const float r = 1.0f / sqrtf(block_sum<256>(s, buf) / (float)C + eps);
+    const float r = 1.0f / sqrtf(block_sum<256>(s, buf[1]) / (float)C + eps);
     for (int64_t c = threadIdx.x; c < C; c += 256) {
       const float h = (RowType<DT>::load(x, m * sx + c) - mu) * r;
       RowType<DT>::store(y, m * sy + c, fmaf(h, w ? load_any(w, wt, c) : 1.0f, b ? load_any(b, bt, c) : 0.0f));
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const void* x, int64_t 
 template <int DT>
 __global__ __launch_bounds__(256) void layer_norm_dx_kernel(const void* dy, int64_t sdy, const void* x, int64_t M, int64_t C, int64_t sx, const void* w, int wt,
                                                             const float* mean, const float* rstd, void* dx, int64_t sdx) {
-  __shared__ float buf[256];
+  __shared__ float buf[3][4];
   for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
     const float mu = mean[m], r = rstd[m];
     float sg = 0.f, sgh = 0.f;
@@ -41,8 +41,8 @@ __global__ __launch_bounds__(256) void layer_norm_dx_kernel(const void* dy, int6
       sg += g;
       sgh = fmaf(g, (RowType<DT>::load(x, m * sx + c) - mu) * r, sgh);
     }
-    sg = block_sum<256>(sg, buf) / (float)C;
-    sgh = block_sum<256>(sgh, buf) / (float)C;
+    sg = block_sum<256>(sg, buf[0]) / (float)C;
+    sgh = block_sum<256>(sgh, buf[1]) / (float)C;
     for (int64_t c = threadIdx.x; c < C; c += 256) {
       const float g = RowType<DT>::load(dy, m * sdy + c) * (w ? load_any(w, wt, c) : 1.0f), h = (RowType<DT>::load(x, m * sx + c) - mu) * r;
       RowType<DT>::store(dx, m * sdx + c, (g - sg - h * sgh) * r);

@@ -1,8 +1,12 @@
 // Pieces that the row operators share (layer norm, operators over a vocabulary): typed element access and sums over a workgroup.
 #pragma once
 #include "common.h"
+#include "route_common.h"
 
 namespace tk {
+
+typedef uint32_t row_u32x4 __attribute__((ext_vector_type(4)));
+typedef row_u32x4 row_u32x4_at2 __attribute__((aligned(2)));  // sixteen bytes at the address of any element
 
 template <int DT>
 struct RowType {
@@ -19,6 +23,34 @@ struct RowType {
       static_cast<uint16_t*>(p)[i] = f32_to_bf16_bits(v);
     else
       static_cast<uint16_t*>(p)[i] = f32_to_f16_bits(v);
+  }
+
+  // Sixteen bytes of a row: VE elements.  Rows of an odd number of 16-bit elements begin at any even address; the memory pipe takes such
+  // addresses in one instruction.
+  static constexpr int VE = 16 / BYTES;
+  static constexpr uint32_t NEG_INF_BITS = DT == TK_F32 ? 0xFF800000u : DT == TK_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // a dword of -inf
+  static __device__ __forceinline__ row_u32x4 load_vec(const void* p, int64_t i) {
+    return *reinterpret_cast<const row_u32x4_at2*>(static_cast<const char*>(p) + i * BYTES);
+  }
+  // The same where the elements from `end` on are not there: they read as `fill` (a dword of it), and nothing behind `end` is touched.
+  static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int64_t i, int64_t end, uint32_t fill) {
+    if (i + VE <= end) return load_vec(p, i);
+    row_u32x4 v = {fill, fill, fill, fill};
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (i + e < end) {
+        if constexpr (DT == TK_F32)
+          v[e] = static_cast<const uint32_t*>(p)[i + e];
+        else
+          v[e >> 1] = e & 1 ? (v[e >> 1] & 0xFFFFu) | (uint32_t) static_cast<const uint16_t*>(p)[i + e] << 16
+                            : (v[e >> 1] & 0xFFFF0000u) | static_cast<const uint16_t*>(p)[i + e];
+      }
+    return v;
+  }
+  static __device__ __forceinline__ float element(row_u32x4 v, int e) {
+    if constexpr (DT == TK_F32) return bits_f32(v[e]);
+    if constexpr (DT == TK_BF16) return bits_f32(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
+    return f16_bits_to_f32((uint16_t)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1]));
   }
 };
 
@@ -38,19 +70,38 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
 
 inline bool is_row_dtype(int32_t t) { return t == TK_F32 || t == TK_BF16 || t == TK_F16; }
 
-// The sum over a workgroup of THREADS, in every lane; `buf`: THREADS floats of LDS.  Begins and ends with a barrier.
+__device__ __forceinline__ float wave_max_f32(float v) {
+  int x = __builtin_bit_cast(int, v);
+#define TK_STEP(ctrl) x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
+  TK_ROW16(TK_STEP)
+#undef TK_STEP
+  const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 0)), b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 16));
+  const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 32)), d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 48));
+  return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
+
+// Over a workgroup of THREADS, in every lane: the waves' results by lane exchanges, then through `buf` (THREADS / 64 floats of LDS, not in
+// use by anything in front of the call).  One barrier; the caller puts another one in front of the next use of `buf`.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* buf) {
+  v = wave_sum_f32(v);
+  if constexpr (THREADS == 64) return v;
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
-  buf[threadIdx.x] = v;
-  __syncthreads();
+  float s = buf[0];
 #pragma unroll
-  for (int d = THREADS / 2; d; d >>= 1) {
-    if ((int)threadIdx.x < d) buf[threadIdx.x] += buf[threadIdx.x + d];
-    __syncthreads();
-  }
-  const float s = buf[0];
+  for (int w = 1; w < THREADS / 64; ++w) s += buf[w];
+  return s;
+}
+template <int THREADS>
+__device__ __forceinline__ float block_max(float v, float* buf) {
+  v = wave_max_f32(v);
+  if constexpr (THREADS == 64) return v;
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
+  float s = buf[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) s = fmaxf(s, buf[w]);
   return s;
 }
 

@@ -7,96 +7,416 @@ namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
 
-__device__ __forceinline__ float block_max(float v, float* buf) {
-  __syncthreads();
-  buf[threadIdx.x] = v;
-  __syncthreads();
-  for (int d = 128; d; d >>= 1) {
-    if ((int)threadIdx.x < d) buf[threadIdx.x] = fmaxf(buf[threadIdx.x], buf[threadIdx.x + d]);
-    __syncthreads();
-  }
-  return buf[0];
-}
-
-// Order of a logit as an unsigned number; the two zeros are one value.
-__device__ __forceinline__ uint32_t order_of(float f) {
-  const uint32_t u = f32_bits(f + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int THREADS = 256, WAVES = 4;
+constexpr int MAX_GRID = 1 << 23;  // workgroups of a launch (2^32 threads are its limit)
+constexpr int GROUP = 64;      // consecutive columns whose largest logit is kept while a row streams by
+constexpr int MAX_CHUNKS = 256;  // pieces that a row is split into where there are few rows
 
 __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
 }
 
-// m = the largest logit, ln s = ln sum exp((x - m) / t), and the entropy of a row.
-struct RowSums {
-  float m, log_s, entropy;
-  bool bad, empty;
+// What a call needs of the temperature: exponentials are taken to the base two, exp((x - m) / t) = 2^((x - m) c2).
+struct Scales {
+  float inv_t, c2;
 };
-template <int DT>
-__device__ RowSums row_sums(const void* row, int V, float inv_t, float* buf) {
-  float m = NEG_INF;
-  for (int v = threadIdx.x; v < V; v += 256) m = fmaxf(m, RowType<DT>::load(row, v));
-  m = block_max(m, buf);
-  const float ref = m == NEG_INF ? 0.f : m;
-  float s = 0.f, e = 0.f;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float d = (RowType<DT>::load(row, v) - ref) * inv_t, p = expf(d);
-    s += p;
-    e = fmaf(p, fmaxf(d, -200.f), e);
+
+// ---- the pass over the logits -------------------------------------------------------------------------------
+// Softmax statistics of the logits seen so far, as one pass takes them: m the largest, s = sum 2^d and e = sum 2^d d with
+// d = (x - m) c2.  A larger m rescales both: with f = 2^((m - m') c2), s' = f s and e' = f (e + s (m - m') c2).
+// (x - m) is taken before the scaling: the product x c2 of a mask of the type's lowest value would overflow.  d is bounded by
+// D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero in 32 bits.
+constexpr float D_MIN = -300.f;
+struct Softmax {
+  float m, s, e;
+  __device__ __forceinline__ float reference() const { return m == NEG_INF ? 0.f : m; }
+  __device__ __forceinline__ void raise(float to, float c2) {
+    const float d = m == NEG_INF ? 0.f : (m - to) * c2, f = __builtin_amdgcn_exp2f(d);  // (nothing seen yet: both sums are zero)
+    e = f * fmaf(s, fmaxf(d, D_MIN), e);
+    s *= f;
+    m = to;
   }
-  s = block_sum<256>(s, buf);
-  e = block_sum<256>(e, buf);
-  RowSums r;
-  r.m = m;
-  r.log_s = logf(s);
-  r.bad = !(s >= 0.f) || m == __builtin_inff();
-  r.empty = !r.bad && s == 0.f;
-  r.entropy = r.bad ? __builtin_nanf("") : r.empty ? 0.f : r.log_s - e / s;
+};
+
+// A row's statistics in every lane, from those of the lanes; `buf`: 3 * WAVES floats of LDS.
+__device__ __forceinline__ Softmax block_softmax(Softmax r, float c2, float* buf) {
+  r.raise(block_max<THREADS>(r.m, buf), c2);
+  r.s = wave_sum_f32(r.s);
+  r.e = wave_sum_f32(r.e);
+  if ((threadIdx.x & 63) == 0) {
+    buf[WAVES + (threadIdx.x >> 6)] = r.s;
+    buf[2 * WAVES + (threadIdx.x >> 6)] = r.e;
+  }
+  __syncthreads();
+  r.s = (buf[WAVES] + buf[WAVES + 1]) + (buf[WAVES + 2] + buf[WAVES + 3]);
+  r.e = (buf[2 * WAVES] + buf[2 * WAVES + 1]) + (buf[2 * WAVES + 2] + buf[2 * WAVES + 3]);
   return r;
 }
 
+// Order of a logit as an unsigned number of KEY_BITS; the two zeros are one value, and no logit's number is zero.
 template <int DT>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(tk_vocab_desc d, float inv_t) {
-  __shared__ float buf[256];
-  __shared__ unsigned long long best;
-  for (int t = blockIdx.x; t < d.n_rows; t += gridDim.x) {
-    const void* row = static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
-    const RowSums r = row_sums<DT>(row, d.vocab, inv_t, buf);
-    if (threadIdx.x == 0) {
-      const int64_t at = index_at(d.tokens, d.tokens_i64, t);
-      float lp = 0.f;
-      if (at >= 0 && at < d.vocab) lp = r.bad ? __builtin_nanf("") : r.empty ? NEG_INF : (RowType<DT>::load(row, at) - r.m) * inv_t - r.log_s;
-      d.logprobs[t] = lp;
-      d.entropy[t] = r.entropy;
-      if (d.stats) {
-        d.stats[t] = r.m;
-        d.stats[d.n_rows + t] = r.bad ? __builtin_nanf("") : r.log_s;
-      }
-    }
-    // the next one in the order (larger logit, then lower index), one after the other
-    unsigned long long last = ~0ull;
-    for (int j = 0; j < d.k; ++j) {
-      __syncthreads();
-      if (threadIdx.x == 0) best = 0;
-      __syncthreads();
-      unsigned long long mine = 0;
-      for (int v = threadIdx.x; v < d.vocab; v += 256) {
-        const unsigned long long key = (unsigned long long)order_of(RowType<DT>::load(row, v)) << 32 | (uint32_t)~v;
-        if (key < last && key > mine) mine = key;
-      }
-      atomicMax(&best, mine);
-      __syncthreads();
-      last = best;
-      const int at = (int)~(uint32_t)last;
-      if (threadIdx.x == 0) {
-        const int64_t o = (int64_t)t * d.k + j;
-        d.top_indx[o] = r.bad ? -1 : at;
-        d.top_logprobs[o] = r.bad ? __builtin_nanf("") : r.empty ? NEG_INF : (RowType<DT>::load(row, at) - r.m) * inv_t - r.log_s;
-      }
-    }
-    __syncthreads();
+struct Key {
+  static constexpr int SHIFT = DT == TK_F32 ? 0 : DT == TK_BF16 ? 16 : 13, BITS = 32 - SHIFT;
+  static __device__ __forceinline__ uint32_t of(float f) { return ordered_key(f + 0.0f) >> SHIFT; }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    const uint32_t low = (1u << SHIFT) - 1u;
+    return key_to_float(k << SHIFT | (k >> (BITS - 1) ? 0u : low));
   }
+};
+
+// Columns [c0, c1) of a row; `keys` takes the order numbers of the groups' largest logits (group = column / GROUP; c0 is a multiple
+// of GROUP).
+template <int DT, bool ENTROPY, bool TOP>
+__device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float c2, uint32_t* keys) {
+  typedef RowType<DT> R;
+  constexpr int VE = R::VE, U = 4, STEP = THREADS * VE * U;
+  Softmax r = {NEG_INF, 0.f, 0.f};
+  for (int base = c0; base < c1; base += STEP) {
+    const int at = base + (int)threadIdx.x * VE;
+    row_u32x4 raw[U];
+    if (base + STEP <= c1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = R::load_vec(row, at + u * THREADS * VE);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
+    }
+    float mx[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mx[u] = R::element(raw[u], 0);
+#pragma unroll
+      for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
+    }
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    if (top > r.m) r.raise(top, c2);
+    const float ref = r.reference();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float s = 0.f, en = 0.f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float d = (R::element(raw[u], e) - ref) * c2, p = __builtin_amdgcn_exp2f(d);
+        s += p;
+        if (ENTROPY) en = fmaf(p, fmaxf(d, D_MIN), en);
+      }
+      r.s += s;
+      r.e += en;
+    }
+    if (TOP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        int x = __builtin_bit_cast(int, mx[u]);
+#define TK_STEP(ctrl) \
+  x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
+        TK_STEP(TK_DPP_QUAD_XOR1)
+        TK_STEP(TK_DPP_QUAD_XOR2)
+        TK_STEP(TK_DPP_ROW_HALF_MIRROR)
+        if (VE == 4) TK_STEP(TK_DPP_ROW_MIRROR)
+#undef TK_STEP
+        const int c = at + u * THREADS * VE;
+        if ((threadIdx.x & (GROUP / VE - 1)) == 0 && c < c1) keys[c / GROUP] = Key<DT>::of(__builtin_bit_cast(float, x));
+      }
+    }
+  }
+  return r;
+}
+
+// ---- the k largest ------------------------------------------------------------------------------------------
+// A row's k largest logits lie in the k groups whose largest logits are the largest (equal ones: the lower groups): were one of them in
+// another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per
+// group, and then at the k groups' elements again: the rest of the row is read once, whatever stands in it.
+// Each of the two selections finds the k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum
+// in the order of the columns.
+struct SelectLds {
+  int count[2][WAVES];
+  int scan[WAVES];
+  int group[TK_VOCAB_MAX_TOP];
+  uint32_t key[TK_VOCAB_MAX_TOP];
+  int indx[TK_VOCAB_MAX_TOP];
+};
+
+// The workgroup's count of keys >= `at` (threads own their keys in order; `turn` alternates between calls).
+template <int N>
+__device__ __forceinline__ int count_from(const uint32_t (&key)[N], uint32_t at, int turn, SelectLds& lds) {
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) c += __builtin_popcountll(__ballot(key[i] >= at));
+  if ((threadIdx.x & 63) == 0) lds.count[turn][threadIdx.x >> 6] = c;
+  __syncthreads();
+  return (lds.count[turn][0] + lds.count[turn][1]) + (lds.count[turn][2] + lds.count[turn][3]);
+}
+
+// Calls take(slot, i) for the k first keys in the order (larger key, then lower position), slots counted by position; at least k keys are not 0.
+template <int N, int BITS, class F>
+__device__ __forceinline__ void select(const uint32_t (&key)[N], int k, SelectLds& lds, F&& take) {
+  uint32_t from = 0;
+  int n = -1;  // keys >= from, once known
+  for (int b = BITS - 1; b >= 0; --b) {
+    const int c = count_from<N>(key, from | 1u << b, b & 1, lds);
+    if (c >= k) {
+      from |= 1u << b;
+      n = c;
+      if (c == k) break;
+    }
+  }
+  // more than k from there on: all larger ones, and the first of the equal ones
+  int larger = 0, equal = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    larger += key[i] > from;
+    equal += key[i] == from;
+  }
+  if (n == k) {
+    larger += equal;
+    equal = 0;
+  }
+  const int mine = larger | equal << 16, upto = wave_scan_i32(mine);
+  if ((threadIdx.x & 63) == 63) lds.scan[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  int before = upto - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) before += lds.scan[w];
+    all += lds.scan[w];
+  }
+  const int need = k - (all & 0xFFFF);  // equal ones that are taken
+  int l = before & 0xFFFF, q = before >> 16;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool eq = key[i] == from, in = key[i] > from || (eq && (n == k || q < need));
+    if (in) take(l + (q < need ? q : need), i);
+    l += key[i] > from || (eq && n == k);
+    q += eq && n != k;
+  }
+}
+
+// N / 4 = the most alternatives that this instance takes.
+template <int DT, int N>
+__device__ __forceinline__ void top_of_groups(const void* row, int V, int k, int n_groups, SelectLds& lds) {
+  typedef RowType<DT> R;
+  constexpr int VE = R::VE;
+  uint32_t key[N];
+  const int first = (int)threadIdx.x * N;
+#pragma unroll
+  for (int v = 0; v < N / VE; ++v) {
+    const int c = first + v * VE;
+    const int at = c < n_groups * GROUP ? lds.group[c / GROUP] * GROUP + c % GROUP : V;
+    const row_u32x4 raw = R::load_vec_to(row, at, V, 0u);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) key[v * VE + e] = at + e < V ? Key<DT>::of(R::element(raw, e)) : 0u;
+  }
+  select<N, Key<DT>::BITS>(key, k, lds, [&](int slot, int i) {
+    const int c = first + i;
+    lds.key[slot] = key[i];
+    lds.indx[slot] = lds.group[c / GROUP] * GROUP + c % GROUP;
+  });
+  __syncthreads();
+}
+
+// The k largest of a row from its groups' numbers; leaves them in lds.key / lds.indx by column.  NG = groups a thread.
+template <int DT, int NG>
+__device__ __forceinline__ void top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
+  const int groups = (V + GROUP - 1) / GROUP, n = k < groups ? k : groups;
+  uint32_t key[NG];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const int g = (int)threadIdx.x * NG + i;
+    key[i] = g < groups ? group_keys[g] : 0u;
+  }
+  select<NG, Key<DT>::BITS>(key, n, lds, [&](int slot, int i) { lds.group[slot] = (int)threadIdx.x * NG + i; });
+  __syncthreads();
+  if (k <= 32)
+    top_of_groups<DT, 8>(row, V, k, n, lds);
+  else if (k <= 64)
+    top_of_groups<DT, 16>(row, V, k, n, lds);
+  else
+    top_of_groups<DT, 32>(row, V, k, n, lds);
+}
+
+// ---- what comes out of a row's statistics ---------------------------------------------------------------------
+struct RowResult {
+  float m, log_s;
+  bool bad, empty;
+  __device__ __forceinline__ RowResult(const Softmax& r) : m(r.m) {
+    bad = !(r.s >= 0.f) || r.m == __builtin_inff();
+    empty = !bad && r.s == 0.f;
+    log_s = bad ? __builtin_nanf("") : logf(r.s);
+  }
+  __device__ __forceinline__ float logprob(float x, float inv_t) const { return bad ? __builtin_nanf("") : empty ? NEG_INF : (x - m) * inv_t - log_s; }
+};
+
+template <int DT, bool TOP>
+__device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, const uint32_t* group_keys,
+                                                SelectLds* lds) {
+  const RowResult o(r);
+  if (threadIdx.x == 0) {
+    const int64_t at = index_at(d.tokens, d.tokens_i64, t);
+    d.logprobs[t] = at >= 0 && at < d.vocab ? o.logprob(RowType<DT>::load(row, at), sc.inv_t) : 0.f;
+    d.entropy[t] = o.bad ? __builtin_nanf("") : o.empty ? 0.f : o.log_s - LN2 * (r.e / r.s);
+    if (d.stats) {
+      d.stats[t] = o.m;
+      d.stats[(int64_t)d.n_rows + t] = o.log_s;
+    }
+  }
+  if constexpr (TOP) {
+    const int64_t out = (int64_t)t * d.k;
+    if (o.bad) {
+      if ((int)threadIdx.x < d.k) {
+        d.top_indx[out + threadIdx.x] = -1;
+        d.top_logprobs[out + threadIdx.x] = __builtin_nanf("");
+      }
+      return;
+    }
+    if (d.vocab <= 8 * THREADS * GROUP)
+      top_of_row<DT, 8>(row, d.vocab, d.k, group_keys, *lds);
+    else
+      top_of_row<DT, 32>(row, d.vocab, d.k, group_keys, *lds);
+    if ((int)threadIdx.x < d.k) {
+      const uint32_t key = lds->key[threadIdx.x];
+      int rank = 0;
+      for (int j = 0; j < d.k; ++j) rank += lds->key[j] > key || (lds->key[j] == key && j < (int)threadIdx.x);
+      d.top_indx[out + rank] = lds->indx[threadIdx.x];
+      d.top_logprobs[out + rank] = o.logprob(Key<DT>::value(key), sc.inv_t);
+    }
+  }
+}
+
+// The teacher's entry j of row t: its index, or -1 where it carries no weight, and its logit.
+__device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int j, float* q) {
+  *q = load_any(d.teacher_logits, d.teacher_dtype, (int64_t)t * d.teacher_stride_m + j);
+  const int64_t i = index_at(d.teacher_indx, d.teacher_indx_i64, (int64_t)t * d.teacher_indx_stride_m + j);
+  return i < 0 || i >= d.vocab || *q == NEG_INF ? -1 : (int)i;
+}
+
+template <int DT>
+__device__ __forceinline__ void finish_distill(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, float (*buf)[WAVES]) {
+  const RowResult o(r);
+  float qm = NEG_INF, q, qs = 0.f, loss = 0.f;
+  int bad = 0;
+  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS)
+    if (teacher_entry(d, t, j, &q) >= 0) {
+      qm = fmaxf(qm, q);
+      bad |= q != q;
+    }
+  qm = block_max<THREADS>(qm, buf[0]);
+  bad = __syncthreads_or(bad) || qm == __builtin_inff();
+  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS)
+    if (teacher_entry(d, t, j, &q) >= 0) qs += expf((q - qm) * sc.inv_t);
+  qs = block_sum<THREADS>(qs, buf[1]);
+  const float log_qs = bad ? __builtin_nanf("") : logf(qs);
+  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS) {
+    const int at = teacher_entry(d, t, j, &q);
+    if (at < 0) continue;
+    const float la = (q - qm) * sc.inv_t - log_qs, a = expf(la);
+    if (a != 0.f) loss = fmaf(a, la - o.logprob(RowType<DT>::load(row, at), sc.inv_t), loss);
+  }
+  loss = block_sum<THREADS>(loss, buf[2]);
+  if (threadIdx.x == 0) {
+    d.loss[t] = loss;
+    if (d.stats) {
+      d.stats[t] = o.m;
+      d.stats[(int64_t)d.n_rows + t] = o.log_s;
+    }
+    if (d.teacher_stats) {
+      d.teacher_stats[t] = bad ? __builtin_nanf("") : qm;
+      d.teacher_stats[(int64_t)d.n_rows + t] = log_qs;
+    }
+  }
+}
+
+enum { LOGPROBS = 0, LOGPROBS_TOP = 1, DISTILL = 2 };
+
+struct RowLds {
+  float softmax[3 * WAVES];
+  float teacher[3][WAVES];
+  SelectLds select;
+};
+
+template <int DT, int OP>
+__device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, const uint32_t* keys, RowLds& lds) {
+  if constexpr (OP == DISTILL)
+    finish_distill<DT>(d, sc, t, row, r, lds.teacher);
+  else
+    finish_logprobs<DT, OP == LOGPROBS_TOP>(d, sc, t, row, r, keys, &lds.select);
+}
+
+template <int DT>
+__device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t) {
+  return static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
+}
+
+// A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
+template <int DT, int OP>
+__global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0) {
+  extern __shared__ uint32_t keys[];
+  __shared__ RowLds lds;
+  const int t = t0 + (int)blockIdx.x;
+  const void* row = logits_row<DT>(d, t);
+  const Softmax r = block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
+  finish<DT, OP>(d, sc, t, row, r, keys, lds);
+}
+
+// Few rows: pieces of a row, whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
+template <int DT, int OP>
+__global__ __launch_bounds__(THREADS) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
+  __shared__ float buf[3 * WAVES];
+  const int t = blockIdx.x / n_chunks, c = blockIdx.x % n_chunks, c0 = c * chunk;
+  const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
+  const Softmax r =
+      block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
+  if (threadIdx.x < 3) parts[((int64_t)t * n_chunks + c) * 3 + threadIdx.x] = threadIdx.x == 0 ? r.m : threadIdx.x == 1 ? r.s : r.e;
+}
+
+template <int DT, int OP>
+__global__ __launch_bounds__(THREADS) void vocab_join_kernel(tk_vocab_desc d, Scales sc, int n_chunks, const float* parts, const uint32_t* keys, int groups) {
+  __shared__ RowLds lds;
+  const int t = blockIdx.x;
+  Softmax r = {NEG_INF, 0.f, 0.f};
+  if ((int)threadIdx.x < n_chunks) {
+    const float* p = parts + ((int64_t)t * n_chunks + threadIdx.x) * 3;
+    r = {p[0], p[1], p[2]};
+  }
+  r = block_softmax(r, sc.c2, lds.softmax);
+  finish<DT, OP>(d, sc, t, logits_row<DT>(d, t), r, keys + (int64_t)t * groups, lds);
+}
+
+// Pieces that the rows of a call are split into: enough for eight workgroups a CU, of at least a load a thread.
+struct Split {
+  int n, chunk, groups;
+  int64_t parts_bytes, bytes;
+};
+Split split_of(int32_t n_rows, int32_t vocab, int32_t k) {
+  Split s;
+  const int64_t want = cdiv(2048, n_rows > 0 ? n_rows : 1), most = cdiv(vocab, 2048);
+  int64_t n = want < most ? want : most;
+  n = n < MAX_CHUNKS ? n : MAX_CHUNKS;
+  s.chunk = (int)(cdiv(cdiv(vocab, n), 2048) * 2048 < vocab ? cdiv(cdiv(vocab, n), 2048) * 2048 : vocab);
+  s.n = (int)cdiv(vocab, s.chunk);
+  s.groups = k ? (int)cdiv(vocab, GROUP) : 0;
+  s.parts_bytes = cdiv((int64_t)n_rows * s.n * 12, 16) * 16;
+  s.bytes = s.n > 1 ? s.parts_bytes + (int64_t)n_rows * s.groups * 4 : 0;
+  return s;
+}
+
+template <int DT, int OP>
+int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
+  const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0);
+  const Scales sc = {(float)(1.0 / d->temperature), (float)(1.4426950408889634 / d->temperature)};
+  if (s.n == 1) {
+    for (int64_t t = 0; t < d->n_rows; t += MAX_GRID) {
+      const int rows = (int)(d->n_rows - t < MAX_GRID ? d->n_rows - t : MAX_GRID);
+      hipLaunchKernelGGL((vocab_rows_kernel<DT, OP>), dim3(rows), dim3(THREADS), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
+    }
+    return check_launch(who);
+  }
+  if (!d->workspace) return fail(TK_ERR_INVALID, "%s: null workspace", who);
+  float* parts = static_cast<float*>(d->workspace);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(static_cast<char*>(d->workspace) + s.parts_bytes);
+  hipLaunchKernelGGL((vocab_chunk_kernel<DT, OP>), dim3((unsigned)(d->n_rows * s.n)), dim3(THREADS), 0, stream, *d, sc, s.chunk, s.n, parts, keys, s.groups);
+  hipLaunchKernelGGL((vocab_join_kernel<DT, OP>), dim3(d->n_rows), dim3(THREADS), 0, stream, *d, sc, s.n, parts, keys, s.groups);
+  return check_launch(who);
 }
 
 template <int DT>
@@ -119,56 +439,6 @@ __global__ __launch_bounds__(256) void token_logprobs_backward_kernel(tk_vocab_d
   }
 }
 
-// The teacher's entry j of row t: its index, or -1 where it carries no weight, and its logit.
-template <int DT>
-__device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int j, float* q) {
-  *q = load_any(d.teacher_logits, d.teacher_dtype, (int64_t)t * d.teacher_stride_m + j);
-  const int64_t i = index_at(d.teacher_indx, d.teacher_indx_i64, (int64_t)t * d.teacher_indx_stride_m + j);
-  return i < 0 || i >= d.vocab || *q == NEG_INF ? -1 : (int)i;
-}
-
-template <int DT>
-__global__ __launch_bounds__(256) void distill_kernel(tk_vocab_desc d, float inv_t) {
-  __shared__ float buf[256];
-  for (int t = blockIdx.x; t < d.n_rows; t += gridDim.x) {
-    const void* row = static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
-    const RowSums r = row_sums<DT>(row, d.vocab, inv_t, buf);
-    float qm = NEG_INF, q, qs = 0.f, loss = 0.f;
-    int bad = 0;
-    for (int j = threadIdx.x; j < d.n_teacher; j += 256)
-      if (teacher_entry<DT>(d, t, j, &q) >= 0) {
-        qm = fmaxf(qm, q);
-        bad |= q != q;
-      }
-    qm = block_max(qm, buf);
-    bad = __syncthreads_or(bad) || qm == __builtin_inff();
-    for (int j = threadIdx.x; j < d.n_teacher; j += 256)
-      if (teacher_entry<DT>(d, t, j, &q) >= 0) qs += expf((q - qm) * inv_t);
-    qs = block_sum<256>(qs, buf);
-    const float log_qs = bad ? __builtin_nanf("") : logf(qs);
-    for (int j = threadIdx.x; j < d.n_teacher; j += 256) {
-      const int at = teacher_entry<DT>(d, t, j, &q);
-      if (at < 0) continue;
-      const float la = (q - qm) * inv_t - log_qs, a = expf(la);
-      const float lp = r.bad ? __builtin_nanf("") : r.empty ? NEG_INF : (RowType<DT>::load(row, at) - r.m) * inv_t - r.log_s;
-      if (a != 0.f) loss = fmaf(a, la - lp, loss);
-    }
-    loss = block_sum<256>(loss, buf);
-    if (threadIdx.x == 0) {
-      d.loss[t] = loss;
-      if (d.stats) {
-        d.stats[t] = r.m;
-        d.stats[d.n_rows + t] = r.bad ? __builtin_nanf("") : r.log_s;
-      }
-      if (d.teacher_stats) {
-        d.teacher_stats[t] = bad ? __builtin_nanf("") : qm;
-        d.teacher_stats[d.n_rows + t] = log_qs;
-      }
-    }
-    __syncthreads();
-  }
-}
-
 template <int DT>
 __global__ __launch_bounds__(256) void distill_backward_kernel(tk_vocab_desc d, float inv_t) {
   __shared__ float a[TK_VOCAB_MAX_TEACHER];
@@ -182,7 +452,7 @@ __global__ __launch_bounds__(256) void distill_backward_kernel(tk_vocab_desc d, 
     __syncthreads();
     for (int j = threadIdx.x; j < d.n_teacher; j += 256) {
       float q;
-      at[j] = teacher_entry<DT>(d, t, j, &q);
+      at[j] = teacher_entry(d, t, j, &q);
       a[j] = expf((q - qm) * inv_t - log_qs);
     }
     __syncthreads();
@@ -198,6 +468,7 @@ __global__ __launch_bounds__(256) void distill_backward_kernel(tk_vocab_desc d, 
 int32_t check(const tk_vocab_desc* d, const char* who) {
   if (!d) return fail(TK_ERR_INVALID, "%s: null descriptor", who);
   if (d->n_rows < 0 || d->vocab <= 0) return fail(TK_ERR_INVALID, "%s: bad sizes %d x %d", who, d->n_rows, d->vocab);
+  if (d->vocab > 1 << 30) return fail(TK_ERR_UNSUPPORTED, "%s: %d columns, at most 2^30", who, d->vocab);
   if (!(d->temperature > 0.f) || d->temperature == __builtin_inff()) return fail(TK_ERR_INVALID, "%s: the temperature must be positive and finite", who);
   if (!is_row_dtype(d->logits_dtype)) return fail(TK_ERR_UNSUPPORTED, "%s: logits are fp32, bf16 or fp16", who);
   if (d->n_rows && !d->logits) return fail(TK_ERR_INVALID, "%s: null logits", who);
@@ -225,7 +496,7 @@ using namespace tk;
     hipLaunchKernelGGL(f, dim3(rows_grid(d->n_rows)), dim3(256), 0, static_cast<hipStream_t>(stream), *d, 1.0f / d->temperature);             \
   } while (0)
 
-extern "C" int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k) { return 0; }
+extern "C" int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k) { return n_rows > 0 && vocab > 0 ? split_of(n_rows, vocab, k).bytes : 0; }
 
 extern "C" int32_t tk_token_logprobs(const tk_vocab_desc* d, tk_stream_t stream) {
   if (int32_t e = check(d, "tk_token_logprobs")) return e;
@@ -234,8 +505,11 @@ extern "C" int32_t tk_token_logprobs(const tk_vocab_desc* d, tk_stream_t stream)
     return fail(TK_ERR_UNSUPPORTED, "tk_token_logprobs: at most %d alternatives, of at most %d columns", TK_VOCAB_MAX_TOP, TK_VOCAB_MAX_TOP_COLUMNS);
   if (d->n_rows == 0) return TK_OK;
   if (!d->tokens || !d->logprobs || !d->entropy || (d->k && (!d->top_logprobs || !d->top_indx))) return fail(TK_ERR_INVALID, "tk_token_logprobs: null pointer");
-  TK_VOCAB_LAUNCH(token_logprobs_kernel);
-  return check_launch("token_logprobs_kernel");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto f = d->logits_dtype == TK_F32 ? (d->k ? forward<TK_F32, LOGPROBS_TOP> : forward<TK_F32, LOGPROBS>)
+           : d->logits_dtype == TK_BF16 ? (d->k ? forward<TK_BF16, LOGPROBS_TOP> : forward<TK_BF16, LOGPROBS>)
+                                        : (d->k ? forward<TK_F16, LOGPROBS_TOP> : forward<TK_F16, LOGPROBS>);
+  return f(d, st, "tk_token_logprobs");
 }
 
 extern "C" int32_t tk_token_logprobs_backward(const tk_vocab_desc* d, tk_stream_t stream) {
@@ -251,8 +525,8 @@ extern "C" int32_t tk_distill_topk(const tk_vocab_desc* d, tk_stream_t stream) {
   if (int32_t e = check_teacher(d, "tk_distill_topk")) return e;
   if (d->n_rows == 0) return TK_OK;
   if (!d->loss) return fail(TK_ERR_INVALID, "tk_distill_topk: null pointer");
-  TK_VOCAB_LAUNCH(distill_kernel);
-  return check_launch("distill_kernel");
+  auto f = d->logits_dtype == TK_F32 ? forward<TK_F32, DISTILL> : d->logits_dtype == TK_BF16 ? forward<TK_BF16, DISTILL> : forward<TK_F16, DISTILL>;
+  return f(d, static_cast<hipStream_t>(stream), "tk_distill_topk");
 }
 
 extern "C" int32_t tk_distill_topk_backward(const tk_vocab_desc* d, tk_stream_t stream) {
