@@ -133,7 +133,7 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
         return d
 
     entries = {e: getattr(lib, e) for e in ("tk_token_logprobs", "tk_token_logprobs_backward", "tk_distill_topk", "tk_distill_topk_backward")}
-    shared = [dict(n_rows=-1), dict(vocab=0), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=INF), dict(temperature=float("nan")), dict(logits=None)]
+    shared = [dict(n_rows=-1), dict(vocab=0), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=1e-39), dict(temperature=INF), dict(temperature=float("nan")), dict(logits=None)]
     own = {"tk_token_logprobs": [dict(k=-1), dict(k=101), dict(tokens=None), dict(logprobs=None), dict(entropy=None), dict(top_indx=None), dict(top_logprobs=None)],
            "tk_token_logprobs_backward": [dict(tokens=None), dict(entropy=None), dict(stats=None), dict(d_logits=None)],
            "tk_distill_topk": [dict(n_teacher=-1), dict(teacher_logits=None), dict(teacher_indx=None), dict(loss=None)],

@@ -52,6 +52,34 @@ struct RowType {
     if constexpr (DT == TK_BF16) return bits_f32(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
     return f16_bits_to_f32((uint16_t)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1]));
   }
+  // Results rounded to nearest even.
+  static __device__ __forceinline__ row_u32x4 pack(const float (&x)[VE]) {
+    row_u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == TK_F32)
+        v[i] = f32_bits(x[i]);
+      else if constexpr (DT == TK_BF16)
+        v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x[2 * i], x[2 * i + 1]}), bf16x2_t));
+      else
+        v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x[2 * i], x[2 * i + 1]}), f16x2_t));
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void store_vec(void* p, int64_t i, row_u32x4 v) {
+    *reinterpret_cast<row_u32x4_at2*>(static_cast<char*>(p) + i * BYTES) = v;
+  }
+  static __device__ __forceinline__ void store_vec_to(void* p, int64_t i, int64_t end, row_u32x4 v) {
+    if (i + VE <= end) return store_vec(p, i, v);
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (i + e < end) {
+        if constexpr (DT == TK_F32)
+          static_cast<uint32_t*>(p)[i + e] = v[e];
+        else
+          static_cast<uint16_t*>(p)[i + e] = (uint16_t)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1]);
+      }
+  }
 };
 
 // An element of a type that is only known at run time (weights, of which there are few).

@@ -7,7 +7,7 @@ namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
 
-constexpr float LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int THREADS = 256, WAVES = 4;
 constexpr int MAX_GRID = 1 << 23;  // workgroups of a launch (2^32 threads are its limit)
 constexpr int GROUP = 64;      // consecutive columns whose largest logit is kept while a row streams by
@@ -400,10 +400,12 @@ Split split_of(int32_t n_rows, int32_t vocab, int32_t k) {
   return s;
 }
 
+Scales scales_of(const tk_vocab_desc* d) { return {(float)(1.0 / d->temperature), (float)(1.4426950408889634 / d->temperature)}; }
+
 template <int DT, int OP>
 int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0);
-  const Scales sc = {(float)(1.0 / d->temperature), (float)(1.4426950408889634 / d->temperature)};
+  const Scales sc = scales_of(d);
   if (s.n == 1) {
     for (int64_t t = 0; t < d->n_rows; t += MAX_GRID) {
       const int rows = (int)(d->n_rows - t < MAX_GRID ? d->n_rows - t : MAX_GRID);
@@ -419,57 +421,118 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   return check_launch(who);
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void token_logprobs_backward_kernel(tk_vocab_desc d, float inv_t) {
-  for (int t = blockIdx.x; t < d.n_rows; t += gridDim.x) {
-    const void* row = static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
-    void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * RowType<DT>::BYTES;
+// ---- gradients ----------------------------------------------------------------------------------------------
+// A piece of a row a workgroup: one read and one write of the row's size.  With p = 2^d2, d2 = (x - m) c2 - log2 s:
+//   log probabilities   g = p (A + B d2) everywhere, A = -(d_lp + d_h H) / t, B = -d_h ln 2 / t, and d_lp / t more at the token
+//   distillation        g = p G, G = d_loss / t, and a_j G less at the teacher's entry j
+// The few columns that get more are found by a bit a column in LDS (the teacher's), so that each element is written once.
+constexpr int GRAD_CHUNK = 16384;
+
+template <int DT, int OP>
+__global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d, Scales sc, int t0, int n_chunks, int chunk) {
+  typedef RowType<DT> R;
+  constexpr int VE = R::VE, U = 2, STEP = THREADS * VE * U;
+  extern __shared__ uint32_t teacher[];  // [n_teacher] columns, [n_teacher] a_j (OP == DISTILL)
+  __shared__ uint32_t named[OP == DISTILL ? GRAD_CHUNK / 32 : 1];
+  const int t = t0 + (int)(blockIdx.x / (unsigned)n_chunks), c0 = (int)(blockIdx.x % (unsigned)n_chunks) * chunk;
+  const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
+  const void* row = logits_row<DT>(d, t);
+  void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * R::BYTES;
+  const float m = d.stats[t], log_s = d.stats[(int64_t)d.n_rows + t], log2_s = log_s * LOG2E;
+  float A, B = 0.f, more = 0.f;
+  int token = -1;
+  bool zero;
+  if constexpr (OP == DISTILL) {
+    const float qm = d.teacher_stats[t], log_qs = d.teacher_stats[(int64_t)d.n_rows + t], g = d.d_loss ? d.d_loss[t * d.d_loss_stride] : 0.f;
+    zero = g == 0.f || log_s == NEG_INF || qm == NEG_INF;  // (sums of nothing)
+    A = qm == qm ? g * sc.inv_t : qm;
+    if (!zero) {
+      for (int i = threadIdx.x; i < GRAD_CHUNK / 32; i += THREADS) named[i] = 0;
+      __syncthreads();
+      for (int j = threadIdx.x; j < d.n_teacher; j += THREADS) {
+        float q;
+        const int at = teacher_entry(d, t, j, &q);
+        teacher[j] = (uint32_t)at;
+        teacher[d.n_teacher + j] = f32_bits(expf((q - qm) * sc.inv_t - log_qs));
+        if (at >= c0 && at < c1) atomicOr(&named[(at - c0) >> 5], 1u << ((at - c0) & 31));
+      }
+      __syncthreads();
+    }
+  } else {
     const int64_t at = index_at(d.tokens, d.tokens_i64, t);
-    const float g_lp = d.d_logprobs && at >= 0 && at < d.vocab ? d.d_logprobs[t * d.d_logprobs_stride] : 0.f;
-    const float g_h = d.d_entropy ? d.d_entropy[t * d.d_entropy_stride] : 0.f;
-    const float m = d.stats[t], log_s = d.stats[d.n_rows + t], h = d.entropy[t];
-    const bool zero = (g_lp == 0.f && g_h == 0.f) || log_s == NEG_INF;  // (a sum of nothing)
-    for (int v = threadIdx.x; v < d.vocab; v += 256) {
-      const float lp = (RowType<DT>::load(row, v) - m) * inv_t - log_s, p = expf(lp);
-      float g = -p * (g_lp + g_h * (fmaxf(lp, -200.f) + h));
-      if (v == at) g += g_lp;
-      if (lp != lp) g = lp;
-      RowType<DT>::store(out, v, zero ? 0.f : g * inv_t);
+    const bool live = at >= 0 && at < d.vocab;
+    const float g_lp = live && d.d_logprobs ? d.d_logprobs[t * d.d_logprobs_stride] : 0.f, g_h = d.d_entropy ? d.d_entropy[t * d.d_entropy_stride] : 0.f;
+    zero = (g_lp == 0.f && g_h == 0.f) || log_s == NEG_INF;  // (a sum of nothing)
+    token = live ? (int)at : -1;
+    A = -(g_lp + g_h * d.entropy[t]) * sc.inv_t;
+    B = -g_h * LN2 * sc.inv_t;
+    more = g_lp * sc.inv_t;
+  }
+  for (int base = c0; base < c1; base += STEP) {
+    const int at = base + (int)threadIdx.x * VE;
+    if (zero) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) R::store_vec_to(out, at + u * THREADS * VE, c1, row_u32x4{0, 0, 0, 0});
+      continue;
+    }
+    const bool full = base + STEP <= c1;
+    row_u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = full ? R::load_vec(row, at + u * THREADS * VE) : R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = at + u * THREADS * VE;
+      float g[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float d2 = fmaf(R::element(raw[u], e) - m, sc.c2, -log2_s), p = __builtin_amdgcn_exp2f(d2);
+        g[e] = OP == DISTILL ? p * A : p * fmaf(fmaxf(d2, D_MIN), B, A);
+      }
+      if constexpr (OP == DISTILL) {
+        const uint32_t bits = v < c1 ? named[(v - c0) >> 5] >> ((v - c0) & 31) & ((1u << VE) - 1u) : 0u;
+        if (bits)
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if (bits >> e & 1) {
+              float a = 0.f;
+              for (int j = 0; j < d.n_teacher; ++j)
+                if ((int)teacher[j] == v + e) a += bits_f32(teacher[d.n_teacher + j]);
+              g[e] = fmaf(-a, A, g[e]);
+            }
+      } else if ((unsigned)(token - v) < (unsigned)VE) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (v + e == token) g[e] += more;
+      }
+      if (full)
+        R::store_vec(out, v, R::pack(g));
+      else
+        R::store_vec_to(out, v, c1, R::pack(g));
     }
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void distill_backward_kernel(tk_vocab_desc d, float inv_t) {
-  __shared__ float a[TK_VOCAB_MAX_TEACHER];
-  __shared__ int at[TK_VOCAB_MAX_TEACHER];
-  for (int t = blockIdx.x; t < d.n_rows; t += gridDim.x) {
-    const void* row = static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
-    void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * RowType<DT>::BYTES;
-    const float m = d.stats[t], log_s = d.stats[d.n_rows + t], qm = d.teacher_stats[t], log_qs = d.teacher_stats[d.n_rows + t];
-    const float g = d.d_loss ? d.d_loss[t * d.d_loss_stride] : 0.f;
-    const bool zero = g == 0.f || log_s == NEG_INF || qm == NEG_INF;  // (sums of nothing)
-    __syncthreads();
-    for (int j = threadIdx.x; j < d.n_teacher; j += 256) {
-      float q;
-      at[j] = teacher_entry(d, t, j, &q);
-      a[j] = expf((q - qm) * inv_t - log_qs);
-    }
-    __syncthreads();
-    for (int v = threadIdx.x; v < d.vocab; v += 256) {
-      float p = expf((RowType<DT>::load(row, v) - m) * inv_t - log_s);
-      for (int j = 0; j < d.n_teacher; ++j)
-        if (at[j] == v) p -= a[j];
-      RowType<DT>::store(out, v, zero ? 0.f : qm != qm ? qm : p * g * inv_t);
-    }
+template <int DT, int OP>
+int32_t backward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
+  // pieces of up to GRAD_CHUNK columns; fewer where that leaves less than sixteen workgroups a CU
+  const int64_t want = cdiv(4096, d->n_rows), most = cdiv(d->vocab, 2048), least = cdiv(d->vocab, GRAD_CHUNK);
+  const int64_t n = want > most ? most : want < least ? least : want;
+  const int64_t chunk = cdiv(cdiv(d->vocab, n), 2048) * 2048;
+  const int n_chunks = (int)cdiv(d->vocab, chunk), rows = MAX_GRID / n_chunks;
+  for (int64_t t = 0; t < d->n_rows; t += rows) {
+    const int now = (int)(d->n_rows - t < rows ? d->n_rows - t : rows);
+    hipLaunchKernelGGL((vocab_backward_kernel<DT, OP>), dim3((unsigned)(now * n_chunks)), dim3(THREADS), OP == DISTILL ? d->n_teacher * 8 : 0, stream, *d,
+                       scales_of(d), (int)t, n_chunks, (int)chunk);
   }
+  return check_launch(who);
 }
 
 int32_t check(const tk_vocab_desc* d, const char* who) {
   if (!d) return fail(TK_ERR_INVALID, "%s: null descriptor", who);
   if (d->n_rows < 0 || d->vocab <= 0) return fail(TK_ERR_INVALID, "%s: bad sizes %d x %d", who, d->n_rows, d->vocab);
   if (d->vocab > 1 << 30) return fail(TK_ERR_UNSUPPORTED, "%s: %d columns, at most 2^30", who, d->vocab);
-  if (!(d->temperature > 0.f) || d->temperature == __builtin_inff()) return fail(TK_ERR_INVALID, "%s: the temperature must be positive and finite", who);
+  if (!(d->temperature >= 1.17549435e-38f) || d->temperature == __builtin_inff())  // (a smaller one has no reciprocal)
+    return fail(TK_ERR_INVALID, "%s: the temperature must be a positive, finite normal number", who);
   if (!is_row_dtype(d->logits_dtype)) return fail(TK_ERR_UNSUPPORTED, "%s: logits are fp32, bf16 or fp16", who);
   if (d->n_rows && !d->logits) return fail(TK_ERR_INVALID, "%s: null logits", who);
   return TK_OK;
@@ -483,18 +546,14 @@ int32_t check_teacher(const tk_vocab_desc* d, const char* who) {
   return TK_OK;
 }
 
-unsigned rows_grid(int n) { return n < 65536 ? n : 65536; }
-
 }  // namespace
 }  // namespace tk
 
 using namespace tk;
 
-#define TK_VOCAB_LAUNCH(kernel)                                                                                                              \
-  do {                                                                                                                                       \
-    auto f = d->logits_dtype == TK_F32 ? kernel<TK_F32> : d->logits_dtype == TK_BF16 ? kernel<TK_BF16> : kernel<TK_F16>;                        \
-    hipLaunchKernelGGL(f, dim3(rows_grid(d->n_rows)), dim3(256), 0, static_cast<hipStream_t>(stream), *d, 1.0f / d->temperature);             \
-  } while (0)
+// f<type of the logits, op>(descriptor, stream, name)
+#define TK_VOCAB_CALL(f, op, who)                                                                                                            \
+  (d->logits_dtype == TK_F32 ? f<TK_F32, op> : d->logits_dtype == TK_BF16 ? f<TK_BF16, op> : f<TK_F16, op>)(d, static_cast<hipStream_t>(stream), who)
 
 extern "C" int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k) { return n_rows > 0 && vocab > 0 ? split_of(n_rows, vocab, k).bytes : 0; }
 
@@ -505,19 +564,14 @@ extern "C" int32_t tk_token_logprobs(const tk_vocab_desc* d, tk_stream_t stream)
     return fail(TK_ERR_UNSUPPORTED, "tk_token_logprobs: at most %d alternatives, of at most %d columns", TK_VOCAB_MAX_TOP, TK_VOCAB_MAX_TOP_COLUMNS);
   if (d->n_rows == 0) return TK_OK;
   if (!d->tokens || !d->logprobs || !d->entropy || (d->k && (!d->top_logprobs || !d->top_indx))) return fail(TK_ERR_INVALID, "tk_token_logprobs: null pointer");
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  auto f = d->logits_dtype == TK_F32 ? (d->k ? forward<TK_F32, LOGPROBS_TOP> : forward<TK_F32, LOGPROBS>)
-           : d->logits_dtype == TK_BF16 ? (d->k ? forward<TK_BF16, LOGPROBS_TOP> : forward<TK_BF16, LOGPROBS>)
-                                        : (d->k ? forward<TK_F16, LOGPROBS_TOP> : forward<TK_F16, LOGPROBS>);
-  return f(d, st, "tk_token_logprobs");
+  return d->k ? TK_VOCAB_CALL(forward, LOGPROBS_TOP, "tk_token_logprobs") : TK_VOCAB_CALL(forward, LOGPROBS, "tk_token_logprobs");
 }
 
 extern "C" int32_t tk_token_logprobs_backward(const tk_vocab_desc* d, tk_stream_t stream) {
   if (int32_t e = check(d, "tk_token_logprobs_backward")) return e;
   if (d->n_rows == 0) return TK_OK;
   if (!d->tokens || !d->entropy || !d->stats || !d->d_logits) return fail(TK_ERR_INVALID, "tk_token_logprobs_backward: null pointer");
-  TK_VOCAB_LAUNCH(token_logprobs_backward_kernel);
-  return check_launch("token_logprobs_backward_kernel");
+  return TK_VOCAB_CALL(backward, LOGPROBS, "tk_token_logprobs_backward");
 }
 
 extern "C" int32_t tk_distill_topk(const tk_vocab_desc* d, tk_stream_t stream) {
@@ -525,8 +579,7 @@ extern "C" int32_t tk_distill_topk(const tk_vocab_desc* d, tk_stream_t stream) {
   if (int32_t e = check_teacher(d, "tk_distill_topk")) return e;
   if (d->n_rows == 0) return TK_OK;
   if (!d->loss) return fail(TK_ERR_INVALID, "tk_distill_topk: null pointer");
-  auto f = d->logits_dtype == TK_F32 ? forward<TK_F32, DISTILL> : d->logits_dtype == TK_BF16 ? forward<TK_BF16, DISTILL> : forward<TK_F16, DISTILL>;
-  return f(d, static_cast<hipStream_t>(stream), "tk_distill_topk");
+  return TK_VOCAB_CALL(forward, DISTILL, "tk_distill_topk");
 }
 
 extern "C" int32_t tk_distill_topk_backward(const tk_vocab_desc* d, tk_stream_t stream) {
@@ -534,6 +587,5 @@ extern "C" int32_t tk_distill_topk_backward(const tk_vocab_desc* d, tk_stream_t 
   if (int32_t e = check_teacher(d, "tk_distill_topk_backward")) return e;
   if (d->n_rows == 0) return TK_OK;
   if (!d->stats || !d->teacher_stats || !d->d_logits) return fail(TK_ERR_INVALID, "tk_distill_topk_backward: null pointer");
-  TK_VOCAB_LAUNCH(distill_backward_kernel);
-  return check_launch("distill_backward_kernel");
+  return TK_VOCAB_CALL(backward, DISTILL, "tk_distill_topk_backward");
 }
