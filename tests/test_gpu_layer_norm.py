@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 SIZES = [(1, 1), (1, 7), (3, 8), (5, 63), (2, 64), (17, 100), (4, 128), (33, 257), (9, 512), (70, 520), (5, 1023), (3, 2049), (16, 2880), (2, 4096), (3, 8191),
-         (1, 16384), (2, 33001), (300, 72), (1000, 130)]
+         (1, 16384), (3, 10000), (2, 16385), (2, 33001), (300, 72), (1000, 130)]
 
 
 def _make(M, C, dtype, weights, seed=0, shift=0.0):

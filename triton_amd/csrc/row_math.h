@@ -32,13 +32,21 @@ struct RowType {
   static __device__ __forceinline__ row_u32x4 load_vec(const void* p, int64_t i) {
     return *reinterpret_cast<const row_u32x4_at2*>(static_cast<const char*>(p) + i * BYTES);
   }
+  // What is left of a row from element i on; opaque, since the compiler would keep a mask for each element of each vector over a loop
+  // over rows, at a hundred registers.
+  static __device__ __forceinline__ int left(int i, int end) {
+    int n = end - i;
+    asm volatile("" : "+v"(n));
+    return n;
+  }
   // The same where the elements from `end` on are not there: they read as `fill` (a dword of it), and nothing behind `end` is touched.
-  static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int64_t i, int64_t end, uint32_t fill) {
-    if (i + VE <= end) return load_vec(p, i);
+  static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int i, int end, uint32_t fill) {
+    const int n = left(i, end);
+    if (n >= VE) return load_vec(p, i);
     row_u32x4 v = {fill, fill, fill, fill};
 #pragma unroll
     for (int e = 0; e < VE; ++e)
-      if (i + e < end) {
+      if (e < n) {
         if constexpr (DT == TK_F32)
           v[e] = static_cast<const uint32_t*>(p)[i + e];
         else
@@ -69,11 +77,12 @@ struct RowType {
   static __device__ __forceinline__ void store_vec(void* p, int64_t i, row_u32x4 v) {
     *reinterpret_cast<row_u32x4_at2*>(static_cast<char*>(p) + i * BYTES) = v;
   }
-  static __device__ __forceinline__ void store_vec_to(void* p, int64_t i, int64_t end, row_u32x4 v) {
-    if (i + VE <= end) return store_vec(p, i, v);
+  static __device__ __forceinline__ void store_vec_to(void* p, int i, int end, row_u32x4 v) {
+    const int n = left(i, end);
+    if (n >= VE) return store_vec(p, i, v);
 #pragma unroll
     for (int e = 0; e < VE; ++e)
-      if (i + e < end) {
+      if (e < n) {
         if constexpr (DT == TK_F32)
           static_cast<uint32_t*>(p)[i + e] = v[e];
         else
