@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from oracle import rows as orc
+from triton_amd import _native as nt
 from triton_kernels.layer_norm import layer_norm, layer_norm_backward, layer_norm_forward
 
 pytestmark = pytest.mark.gpu
@@ -127,7 +128,11 @@ def test_no_rows():
     assert layer_norm(x.view(3, 0, 64), w, b).shape == (3, 0, 64)
 
 
-def test_autograd_gives_the_same_and_only_what_is_asked():
+@pytest.mark.parametrize("native", [True, False])
+def test_autograd_gives_the_same_and_only_what_is_asked(native, monkeypatch):
+    """Through the native host path and through the general one."""
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
     x, w, b, dy = _make(50, 300, BF16, F32)
     y0, mean, rstd = layer_norm_forward(x, w, b)
     want = layer_norm_backward(dy, x, mean, rstd, w, b)
@@ -145,8 +150,18 @@ def test_autograd_gives_the_same_and_only_what_is_asked():
     g, = torch.autograd.grad(layer_norm(leaf, w, b).sum(), leaf)
     assert torch.equal(g, layer_norm_backward(torch.ones_like(x), x, mean, rstd, w, b)[0])
     g, = torch.autograd.grad(layer_norm(leaf, w, b), leaf, dy, create_graph=True)
-    with pytest.raises(RuntimeError):
+    assert torch.equal(g, want[0])
+    with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()
+    leaf = x.clone().requires_grad_()
+    y = layer_norm(leaf, w, b)
+    with torch.no_grad():
+        leaf.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    turned = x.t().contiguous().t().requires_grad_()  # (goes the general way)
+    layer_norm(turned, w, b).backward(dy.t().contiguous().t())
+    assert torch.equal(turned.grad, want[0])
 
 
 def test_equal_calls_give_equal_bits():

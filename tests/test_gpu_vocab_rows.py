@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oracle import rows as orc
+from triton_amd import _native as nt
 from triton_kernels.distill import _forward as distill_forward
 from triton_kernels.distill import distill_topk, distill_topk_backward
 from triton_kernels.layer_norm import layer_norm
@@ -246,7 +247,11 @@ def test_no_rows():
     assert torch.autograd.grad(distill_topk(leaf, q[:0], at[:0]).sum(), leaf)[0].shape == (0, 100)
 
 
-def test_autograd():
+@pytest.mark.parametrize("native", [True, False])
+def test_autograd(native, monkeypatch):
+    """Through the native host path and through the general one."""
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
     z, tokens, a, b = _logits(40, 3001, F32)
     lp, h, _, _, stats = logprobs_forward(z, tokens, 6, 0.7, True)
     for ga, gb in ((a, b), (a, None), (None, b)):
@@ -265,9 +270,13 @@ def test_autograd():
     distill_topk(leaf, q, at, temperature=2.0).mean().backward()
     orc.check(leaf.grad, *orc.distill_topk_backward(z, q, at, torch.full((1, ), 1 / 40), 2.0), "dlogits")
     leaf = z.clone().requires_grad_()
-    g, = torch.autograd.grad(distill_topk(leaf, q, at).sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    for f in (lambda t: distill_topk(t, q, at), lambda t: token_logprobs(t, tokens, 3).entropy):
+        g, = torch.autograd.grad(f(leaf).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
+    turned = z.t().contiguous().t().requires_grad_()  # (goes the general way)
+    token_logprobs(turned, tokens, temperature=0.7).logprobs.backward(a)
+    assert torch.equal(turned.grad, token_logprobs_backward(z, tokens, h, stats, a, None, 0.7))
     with torch.no_grad():
         assert not token_logprobs(leaf, tokens).logprobs.requires_grad
     with pytest.raises(NotImplementedError, match="teacher"):

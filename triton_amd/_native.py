@@ -173,7 +173,9 @@ def lib():
 
 _host = None
 _HOST_ENTRIES = ("tk_moe_gemm", "tk_route", "tk_route_workspace_bytes", "tk_reduce_mid", "tk_quant_fp8_rows", "tk_mx_downcast",
-                 "tk_mx_upcast", "tk_ragged_k_gemm", "tk_moe_decode_layer", "tk_moe_decode_layer_workspace_bytes")
+                 "tk_mx_upcast", "tk_ragged_k_gemm", "tk_moe_decode_layer", "tk_moe_decode_layer_workspace_bytes", "tk_layer_norm",
+                 "tk_layer_norm_backward", "tk_layer_norm_backward_workspace_bytes", "tk_vocab_workspace_bytes", "tk_token_logprobs",
+                 "tk_token_logprobs_backward", "tk_distill_topk", "tk_distill_topk_backward", "tk_last_error")
 
 
 def _load_host():

@@ -1,6 +1,6 @@
 // The host side of the common calls: a CPython extension module (`triton_amd._host`) that checks the operands, allocates the
 // results, fills the descriptor of the C ABI and launches, for the calls a layer is made of (routing, the expert GEMM, the top-k
-// combine, the quantisers, the ragged-K GEMM, the one-launch decode layer).
+// combine, the quantisers, the ragged-K GEMM, the one-launch decode layer, and the row operators around them in host_rows.h).
 //
 // What bounds it: these calls come one after another from Python, and at small sizes the GPU waits for them.  The same steps
 // written in Python cost 15 us for a GEMM, 20 us for the router and 11 us for the combine, most of it attribute and tensor
@@ -47,6 +47,15 @@ struct Bound {
   decltype(&tk_ragged_k_gemm) ragged_k_gemm = nullptr;
   decltype(&tk_moe_decode_layer) decode_layer = nullptr;
   decltype(&tk_moe_decode_layer_workspace_bytes) decode_workspace_bytes = nullptr;
+  decltype(&tk_layer_norm) layer_norm = nullptr;
+  decltype(&tk_layer_norm_backward) layer_norm_backward = nullptr;
+  decltype(&tk_layer_norm_backward_workspace_bytes) layer_norm_workspace = nullptr;
+  decltype(&tk_vocab_workspace_bytes) vocab_workspace = nullptr;
+  decltype(&tk_token_logprobs) token_logprobs = nullptr;
+  decltype(&tk_token_logprobs_backward) token_logprobs_backward = nullptr;
+  decltype(&tk_distill_topk) distill_topk = nullptr;
+  decltype(&tk_distill_topk_backward) distill_topk_backward = nullptr;
+  decltype(&tk_last_error) last_error = nullptr;
   PyObject *check, *raw_stream, *current_device;              // _native.check, torch's raw stream and device getters
   PyObject *tile_counters, *combine_counters, *decode_workspace;  // per device and stream
   PyObject *tensor_type, *mx_value, *mx_scale, *fp8_value, *fp4;  // Tensor, its layouts, the FP4 data type
@@ -799,6 +808,12 @@ PyObject* run_decode_layer(PyObject* const* v) {
   return THPVariable_Wrap(std::move(out));
 }
 
+}  // namespace
+
+#include "host_rows.h"
+
+namespace {
+
 // ---- module -----------------------------------------------------------------------------------------------------------------
 
 // f(args) with the number of arguments checked and C++ exceptions turned into Python's
@@ -912,6 +927,15 @@ PyObject* bind(PyObject*, PyObject* dict) {
   ENTRY(ragged_k_gemm, tk_ragged_k_gemm)
   ENTRY(decode_layer, tk_moe_decode_layer)
   ENTRY(decode_workspace_bytes, tk_moe_decode_layer_workspace_bytes)
+  ENTRY(layer_norm, tk_layer_norm)
+  ENTRY(layer_norm_backward, tk_layer_norm_backward)
+  ENTRY(layer_norm_workspace, tk_layer_norm_backward_workspace_bytes)
+  ENTRY(vocab_workspace, tk_vocab_workspace_bytes)
+  ENTRY(token_logprobs, tk_token_logprobs)
+  ENTRY(token_logprobs_backward, tk_token_logprobs_backward)
+  ENTRY(distill_topk, tk_distill_topk)
+  ENTRY(distill_topk_backward, tk_distill_topk_backward)
+  ENTRY(last_error, tk_last_error)
 #undef ENTRY
 #define OBJECT(name)                            \
   if (!(B.name = get(#name))) return nullptr;   \
@@ -935,6 +959,9 @@ PyMethodDef methods[] = {
     METHOD("mx_upcast", run_mx_upcast, 4),
     METHOD("ragged_k", run_ragged_k, 4),
     METHOD("decode_layer", run_decode_layer, 13),
+    METHOD("layer_norm", run_layer_norm, 4),
+    METHOD("token_logprobs", run_token_logprobs, 4),
+    METHOD("distill_topk", run_distill_topk, 4),
     METHOD("x_extent", rule_x_extent, 4),
     METHOD("dma_runs_16bit", rule_dma_16bit, 5),
     METHOD("dma_block_m", rule_dma, 4),

@@ -7,9 +7,9 @@ once more.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nt
+from ._autograd import once
 from .logprobs import DTYPES, check_index, check_logits, logits_desc, row_gradient, workspace
 
 MAX_TEACHER = 1024
@@ -72,7 +72,7 @@ class _DistillTopK(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, d_loss):
         return distill_topk_backward(*ctx.saved_tensors, d_loss, ctx.temperature), None, None, None
 
@@ -87,6 +87,10 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     int64; K up to 1024).  An entry whose index lies outside `[0, V)` or whose logit is -inf carries no weight; a row without any
     other has the loss 0 and no gradient (padding, fewer alternatives than K).  A student that gives one of the others no
     probability has the loss +inf; one with a NaN or +inf, or a teacher with one, NaN.  Differentiable once in `logits`."""
+    host = nt.host()
+    loss = host.distill_topk(logits, teacher_logits, teacher_indx, temperature) if host is not None else None
+    if loss is not None:
+        return loss
     logits = check_logits(logits, temperature)
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distill_topk has no gradient for the teacher: pass its logits detached")

@@ -9,9 +9,9 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nt
+from ._autograd import once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -96,7 +96,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -109,6 +109,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x, weight and bias are fp32, bf16 or fp16, each its own; weight and bias are `[C]` and optional.  Rows may have any stride.
     Differentiable once in all three."""
+    host = nt.host()
+    y = host.layer_norm(x, weight, bias, eps) if host is not None else None
+    if y is not None:
+        return y
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, with_stats=False)[0]

@@ -11,9 +11,9 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nt
+from ._autograd import once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_TOP = 128
@@ -123,7 +123,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprobs, entropy, top_logprobs, top_indx
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, d_logprobs, d_entropy, *_unused):
         logits, tokens, entropy, stats = ctx.saved_tensors
         if d_logprobs is None and d_entropy is None:
@@ -139,6 +139,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0, tempe
     has log probabilities of -inf, entropy 0 and no gradient.  A row with a NaN or +inf gives NaN, and -1 as its alternatives.  A token
     outside `[0, V)` (padding) has the log probability 0 and no gradient through it.  The log probabilities and the entropies are
     differentiable once in the logits, the alternatives are not."""
+    host = nt.host()
+    r = host.token_logprobs(logits, tokens, k, temperature) if host is not None else None
+    if r is not None:
+        return TokenLogprobs(*r)
     logits = check_logits(logits, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, k, temperature))
