@@ -1,5 +1,7 @@
 // Operators over rows of logits of a whole vocabulary: log probabilities of given tokens with entropy and top alternatives, the
 // distillation loss against a teacher's top logits, and the gradients of both.
+#include <type_traits>
+
 #include "row_math.h"
 
 namespace tk {
@@ -12,6 +14,7 @@ constexpr int THREADS = 256, WAVES = 4;
 constexpr int MAX_GRID = 1 << 23;  // workgroups of a launch (2^32 threads are its limit)
 constexpr int GROUP = 64;      // consecutive columns whose largest logit is kept while a row streams by
 constexpr int MAX_CHUNKS = 256;  // pieces that a row is split into where there are few rows
+constexpr int LEAST_CHUNK = 4096;
 
 __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
   return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
@@ -66,15 +69,15 @@ struct Key {
 };
 
 // Columns [c0, c1) of a row; `keys` takes the order numbers of the groups' largest logits (group = column / GROUP; c0 is a multiple
-// of GROUP).
-template <int DT, bool ENTROPY, bool TOP>
+// of GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
+template <int DT, bool ENTROPY, bool TOP, int U>
 __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float c2, uint32_t* keys) {
   typedef RowType<DT> R;
-  constexpr int VE = R::VE, U = 4, STEP = THREADS * VE * U;
+  constexpr int VE = R::VE, STEP = THREADS * VE * U;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 64 * VE;
   Softmax r = {NEG_INF, 0.f, 0.f};
-  for (int base = c0; base < c1; base += STEP) {
+  const auto fetch = [&](row_u32x4 (&raw)[U], int base) {
     const int at = base + (int)threadIdx.x * VE;
-    row_u32x4 raw[U];
     if (base + STEP <= c1) {
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = R::load_vec(row, at + u * THREADS * VE);
@@ -82,18 +85,31 @@ __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
     }
-    float mx[U];
+  };
+  row_u32x4 next[U];
+  fetch(next, c0);
+  for (int base = c0; base < c1; base += STEP) {
+    const int at = base + (int)threadIdx.x * VE;
+    row_u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
+    if (base + STEP < c1) fetch(next, base + STEP);
+    __builtin_amdgcn_sched_barrier(0);  // (the requests first)
+    float mx[U], top = NEG_INF;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      mx[u] = NEG_INF;
+      if (base + u * THREADS * VE + wave >= c1) continue;  // (of a row's last step only; the wave as a whole)
       mx[u] = R::element(raw[u], 0);
 #pragma unroll
       for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
+      top = fmaxf(top, mx[u]);
     }
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
     if (top > r.m) r.raise(top, c2);
     const float ref = r.reference();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (base + u * THREADS * VE + wave >= c1) continue;
       float s = 0.f, en = 0.f;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
@@ -103,10 +119,7 @@ __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float
       }
       r.s += s;
       r.e += en;
-    }
-    if (TOP) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
+      if (TOP) {
         int x = __builtin_bit_cast(int, mx[u]);
 #define TK_STEP(ctrl) \
   x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
@@ -127,52 +140,48 @@ __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float
 // A row's k largest logits lie in the k groups whose largest logits are the largest (equal ones: the lower groups): were one of them in
 // another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per
 // group, and then at the k groups' elements again: the rest of the row is read once, whatever stands in it.
-// Each of the two selections finds the k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum
-// in the order of the columns.
+// A bound from below narrows both: k threads' largest group numbers are at least the k-th largest of the threads' largest ones, so that
+// only groups, and then only elements, from there on can be among the k; as a rule they are few more than k, which are ranked by
+// counting.  Where they are many (equal logits, logits masked to one value, neighbours sorted together), each of the two selections finds the
+// k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum in the order of the columns.
+constexpr int MANY = 512;
 struct SelectLds {
   int count[2][WAVES];
   int scan[WAVES];
-  int group[TK_VOCAB_MAX_TOP];
-  uint32_t key[TK_VOCAB_MAX_TOP];
-  int indx[TK_VOCAB_MAX_TOP];
+  int n_groups, n_found;
+  row_u32x4 most[THREADS / 4];
+  int group[MANY];
+  uint64_t found[MANY];  // key << 32 | ~column: a larger one comes first
 };
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, int column) { return (uint64_t)key << 32 | (uint32_t)~column; }
 
-// The workgroup's count of keys >= `at` (threads own their keys in order; `turn` alternates between calls).
-template <int N>
-__device__ __forceinline__ int count_from(const uint32_t (&key)[N], uint32_t at, int turn, SelectLds& lds) {
-  int c = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) c += __builtin_popcountll(__ballot(key[i] >= at));
-  if ((threadIdx.x & 63) == 0) lds.count[turn][threadIdx.x >> 6] = c;
-  __syncthreads();
-  return (lds.count[turn][0] + lds.count[turn][1]) + (lds.count[turn][2] + lds.count[turn][3]);
-}
-
-// Calls take(slot, i) for the k first keys in the order (larger key, then lower position), slots counted by position; at least k keys are not 0.
-template <int N, int BITS, class F>
-__device__ __forceinline__ void select(const uint32_t (&key)[N], int k, SelectLds& lds, F&& take) {
+// Calls take(slot, i) for the k first of n items in the order (larger key, then lower i), slots by i; at least k keys are not 0.  A thread looks
+// at consecutive items.  This is the way for the rows that the ranking does not serve: it reads the keys again for each bit.
+template <int BITS, class KeyOf, class F>
+__device__ __forceinline__ void select(int n, int k, SelectLds& lds, KeyOf&& key_of, F&& take) {
+  const int per = (n + THREADS - 1) / THREADS, i0 = (int)threadIdx.x * per, i1 = i0 + per < n ? i0 + per : n;
   uint32_t from = 0;
-  int n = -1;  // keys >= from, once known
-  for (int b = BITS - 1; b >= 0; --b) {
-    const int c = count_from<N>(key, from | 1u << b, b & 1, lds);
-    if (c >= k) {
-      from |= 1u << b;
-      n = c;
-      if (c == k) break;
-    }
+  bool exact = false;  // k keys are >= from
+  for (int b = BITS - 1; b >= 0 && !exact; --b) {
+    const uint32_t at = from | 1u << b;
+    int mine = 0;
+    for (int i = i0; i < i1; ++i) mine += key_of(i) >= at;
+    mine = wave_scan_i32(mine);
+    if ((threadIdx.x & 63) == 63) lds.count[b & 1][threadIdx.x >> 6] = mine;
+    __syncthreads();
+    const int c = (lds.count[b & 1][0] + lds.count[b & 1][1]) + (lds.count[b & 1][2] + lds.count[b & 1][3]);
+    if (c >= k) from = at;
+    exact = c == k;
   }
-  // more than k from there on: all larger ones, and the first of the equal ones
+  // all larger ones, and the first of the equal ones
   int larger = 0, equal = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    larger += key[i] > from;
-    equal += key[i] == from;
-  }
-  if (n == k) {
-    larger += equal;
-    equal = 0;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t key = key_of(i);
+    larger += key > from;
+    equal += key == from;
   }
   const int mine = larger | equal << 16, upto = wave_scan_i32(mine);
+  __syncthreads();
   if ((threadIdx.x & 63) == 63) lds.scan[threadIdx.x >> 6] = upto;
   __syncthreads();
   int before = upto - mine, all = 0;
@@ -183,56 +192,96 @@ __device__ __forceinline__ void select(const uint32_t (&key)[N], int k, SelectLd
   }
   const int need = k - (all & 0xFFFF);  // equal ones that are taken
   int l = before & 0xFFFF, q = before >> 16;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const bool eq = key[i] == from, in = key[i] > from || (eq && (n == k || q < need));
-    if (in) take(l + (q < need ? q : need), i);
-    l += key[i] > from || (eq && n == k);
-    q += eq && n != k;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t key = key_of(i);
+    if (key > from || (key == from && q < need)) take(l + (q < need ? q : need), i);
+    l += key > from;
+    q += key == from;
   }
 }
 
-// N / 4 = the most alternatives that this instance takes.
-template <int DT, int N>
-__device__ __forceinline__ void top_of_groups(const void* row, int V, int k, int n_groups, SelectLds& lds) {
+// The k-th largest of the threads' numbers, each wave by itself; 1 (less than any logit's) where fewer than k threads have one.
+template <int BITS>
+__device__ __forceinline__ uint32_t kth_of_threads(uint32_t mine, int k, SelectLds& lds) {
+  reinterpret_cast<uint32_t*>(lds.most)[threadIdx.x] = mine;
+  __syncthreads();
+  const row_u32x4 four = lds.most[threadIdx.x & 63];
+  uint32_t from = 0;
+  for (int b = BITS - 1; b >= 0; --b) {
+    const uint32_t at = from | 1u << b;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c += __builtin_popcountll(__ballot(four[i] >= at));
+    if (c < k) continue;
+    from = at;
+    if (c == k) break;
+  }
+  return from ? from : 1u;
+}
+
+// Leaves at least the k largest of a row in lds.found, in any order, and returns how many; from the groups' numbers.
+template <int DT>
+__device__ __forceinline__ int top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
   typedef RowType<DT> R;
-  constexpr int VE = R::VE;
-  uint32_t key[N];
-  const int first = (int)threadIdx.x * N;
+  constexpr int VE = R::VE, BITS = Key<DT>::BITS, OWN = 8;
+  const int groups = (V + GROUP - 1) / GROUP;
+  if (threadIdx.x == 0) lds.n_groups = lds.n_found = 0;
+  uint32_t most = 0, own[OWN];  // (the first OWN of a thread's stay in registers)
 #pragma unroll
-  for (int v = 0; v < N / VE; ++v) {
-    const int c = first + v * VE;
-    const int at = c < n_groups * GROUP ? lds.group[c / GROUP] * GROUP + c % GROUP : V;
-    const row_u32x4 raw = R::load_vec_to(row, at, V, 0u);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) key[v * VE + e] = at + e < V ? Key<DT>::of(R::element(raw, e)) : 0u;
+  for (int i = 0; i < OWN; ++i) {
+    const int g = i * THREADS + (int)threadIdx.x;
+    own[i] = g < groups ? group_keys[g] : 0u;
+    most = own[i] > most ? own[i] : most;
   }
-  select<N, Key<DT>::BITS>(key, k, lds, [&](int slot, int i) {
-    const int c = first + i;
-    lds.key[slot] = key[i];
-    lds.indx[slot] = lds.group[c / GROUP] * GROUP + c % GROUP;
-  });
-  __syncthreads();
-}
-
-// The k largest of a row from its groups' numbers; leaves them in lds.key / lds.indx by column.  NG = groups a thread.
-template <int DT, int NG>
-__device__ __forceinline__ void top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
-  const int groups = (V + GROUP - 1) / GROUP, n = k < groups ? k : groups;
-  uint32_t key[NG];
+  for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) most = group_keys[g] > most ? group_keys[g] : most;
+  if (groups < k)  // a row so short that the threads' elements tell more
+    for (int v = threadIdx.x * VE; v < V; v += THREADS * VE) {
+      const row_u32x4 raw = R::load_vec_to(row, v, V, R::NEG_INF_BITS);
+      uint32_t mx = 0;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    const int g = (int)threadIdx.x * NG + i;
-    key[i] = g < groups ? group_keys[g] : 0u;
-  }
-  select<NG, Key<DT>::BITS>(key, n, lds, [&](int slot, int i) { lds.group[slot] = (int)threadIdx.x * NG + i; });
+      for (int e = 0; e < VE; ++e) {
+        const uint32_t one = Key<DT>::of(R::element(raw, e));
+        mx = one > mx ? one : mx;
+      }
+      most = v == (int)threadIdx.x * VE || mx > most ? mx : most;
+    }
+  const uint32_t from = kth_of_threads<BITS>(most, k, lds);
+  const auto add_group = [&](uint32_t key, int g) {
+    if (key < from) return;
+    const int slot = atomicAdd(&lds.n_groups, 1);
+    if (slot < MANY) lds.group[slot] = g;
+  };
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) add_group(own[i], i * THREADS + (int)threadIdx.x);
+  for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) add_group(group_keys[g], g);
   __syncthreads();
-  if (k <= 32)
-    top_of_groups<DT, 8>(row, V, k, n, lds);
-  else if (k <= 64)
-    top_of_groups<DT, 16>(row, V, k, n, lds);
-  else
-    top_of_groups<DT, 32>(row, V, k, n, lds);
+  const int n_groups = lds.n_groups;
+  if (n_groups <= MANY) {
+    constexpr int PER = GROUP / VE;
+    for (int v = threadIdx.x; v < n_groups * PER; v += THREADS) {
+      const int at = lds.group[v / PER] * GROUP + v % PER * VE;
+      const row_u32x4 raw = R::load_vec_to(row, at, V, R::NEG_INF_BITS);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const uint32_t one = Key<DT>::of(R::element(raw, e));
+        if (one >= from && at + e < V) {
+          const int i = atomicAdd(&lds.n_found, 1);
+          if (i < MANY) lds.found[i] = entry_of(one, at + e);
+        }
+      }
+    }
+    __syncthreads();
+    const int n = lds.n_found;
+    if (n <= MANY) return n;
+  }
+  const int n = k < groups ? k : groups;
+  select<BITS>(groups, n, lds, [&](int i) { return group_keys[i]; }, [&](int to, int i) { lds.group[to] = i; });
+  __syncthreads();
+  const auto column = [&](int i) { return lds.group[i / GROUP] * GROUP + i % GROUP; };
+  const auto element = [&](int i) { return column(i) < V ? Key<DT>::of(R::load(row, column(i))) : 0u; };
+  select<BITS>(n * GROUP, k, lds, element, [&](int to, int i) { lds.found[to] = entry_of(element(i), column(i)); });
+  __syncthreads();
+  return k;
 }
 
 // ---- what comes out of a row's statistics ---------------------------------------------------------------------
@@ -247,13 +296,24 @@ struct RowResult {
   __device__ __forceinline__ float logprob(float x, float inv_t) const { return bad ? __builtin_nanf("") : empty ? NEG_INF : (x - m) * inv_t - log_s; }
 };
 
+// What a row's results take from single elements, requested before the row streams by.
+template <int DT>
+struct Token {
+  float x = 0.f;
+  bool live;
+  __device__ __forceinline__ Token(const tk_vocab_desc& d, int t, const void* row) {
+    const int64_t at = index_at(d.tokens, d.tokens_i64, t);
+    live = at >= 0 && at < d.vocab;
+    if (live) x = RowType<DT>::load(row, at);
+  }
+};
+
 template <int DT, bool TOP>
-__device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, const uint32_t* group_keys,
-                                                SelectLds* lds) {
+__device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Token<DT>& token, const Softmax& r,
+                                                const uint32_t* group_keys, SelectLds* lds) {
   const RowResult o(r);
   if (threadIdx.x == 0) {
-    const int64_t at = index_at(d.tokens, d.tokens_i64, t);
-    d.logprobs[t] = at >= 0 && at < d.vocab ? o.logprob(RowType<DT>::load(row, at), sc.inv_t) : 0.f;
+    d.logprobs[t] = token.live ? o.logprob(token.x, sc.inv_t) : 0.f;
     d.entropy[t] = o.bad ? __builtin_nanf("") : o.empty ? 0.f : o.log_s - LN2 * (r.e / r.s);
     if (d.stats) {
       d.stats[t] = o.m;
@@ -269,16 +329,15 @@ __device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales s
       }
       return;
     }
-    if (d.vocab <= 8 * THREADS * GROUP)
-      top_of_row<DT, 8>(row, d.vocab, d.k, group_keys, *lds);
-    else
-      top_of_row<DT, 32>(row, d.vocab, d.k, group_keys, *lds);
-    if ((int)threadIdx.x < d.k) {
-      const uint32_t key = lds->key[threadIdx.x];
+    const int n = top_of_row<DT>(row, d.vocab, d.k, group_keys, *lds);
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const uint64_t mine = lds->found[i];
       int rank = 0;
-      for (int j = 0; j < d.k; ++j) rank += lds->key[j] > key || (lds->key[j] == key && j < (int)threadIdx.x);
-      d.top_indx[out + rank] = lds->indx[threadIdx.x];
-      d.top_logprobs[out + rank] = o.logprob(Key<DT>::value(key), sc.inv_t);
+      for (int j = 0; j < n; ++j) rank += lds->found[j] > mine;
+      if (rank < d.k) {
+        d.top_indx[out + rank] = (int)~(uint32_t)mine;
+        d.top_logprobs[out + rank] = o.logprob(Key<DT>::value((uint32_t)(mine >> 32)), sc.inv_t);
+      }
     }
   }
 }
@@ -290,28 +349,51 @@ __device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int 
   return i < 0 || i >= d.vocab || *q == NEG_INF ? -1 : (int)i;
 }
 
+// The teacher's entries of a thread: their logits, -inf where they carry no weight, and the student's at their indices.
+constexpr int ENTRIES = TK_VOCAB_MAX_TEACHER / THREADS;
 template <int DT>
-__device__ __forceinline__ void finish_distill(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, float (*buf)[WAVES]) {
-  const RowResult o(r);
-  float qm = NEG_INF, q, qs = 0.f, loss = 0.f;
-  int bad = 0;
-  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS)
-    if (teacher_entry(d, t, j, &q) >= 0) {
-      qm = fmaxf(qm, q);
-      bad |= q != q;
+struct Teacher {
+  float q[ENTRIES], x[ENTRIES];
+  __device__ __forceinline__ Teacher(const tk_vocab_desc& d, int t, const void* row) {
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      const int j = i * THREADS + (int)threadIdx.x;
+      q[i] = NEG_INF;
+      x[i] = 0.f;
+      if (j < d.n_teacher) {
+        const int at = teacher_entry(d, t, j, &q[i]);
+        if (at >= 0)
+          x[i] = RowType<DT>::load(row, at);
+        else
+          q[i] = NEG_INF;
+      }
     }
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void finish_distill(const tk_vocab_desc& d, Scales sc, int t, const Teacher<DT>& teacher, const Softmax& r, float (*buf)[WAVES]) {
+  const RowResult o(r);
+  float qm = NEG_INF, qs = 0.f, loss = 0.f;
+  int bad = 0;
+#pragma unroll
+  for (int i = 0; i < ENTRIES; ++i) {
+    qm = fmaxf(qm, teacher.q[i]);
+    bad |= teacher.q[i] != teacher.q[i];
+  }
   qm = block_max<THREADS>(qm, buf[0]);
   bad = __syncthreads_or(bad) || qm == __builtin_inff();
-  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS)
-    if (teacher_entry(d, t, j, &q) >= 0) qs += expf((q - qm) * sc.inv_t);
+#pragma unroll
+  for (int i = 0; i < ENTRIES; ++i)
+    if (teacher.q[i] != NEG_INF) qs += expf((teacher.q[i] - qm) * sc.inv_t);
   qs = block_sum<THREADS>(qs, buf[1]);
   const float log_qs = bad ? __builtin_nanf("") : logf(qs);
-  for (int j = threadIdx.x; j < d.n_teacher; j += THREADS) {
-    const int at = teacher_entry(d, t, j, &q);
-    if (at < 0) continue;
-    const float la = (q - qm) * sc.inv_t - log_qs, a = expf(la);
-    if (a != 0.f) loss = fmaf(a, la - o.logprob(RowType<DT>::load(row, at), sc.inv_t), loss);
-  }
+#pragma unroll
+  for (int i = 0; i < ENTRIES; ++i)
+    if (teacher.q[i] != NEG_INF) {
+      const float la = (teacher.q[i] - qm) * sc.inv_t - log_qs, a = expf(la);
+      if (a != 0.f) loss = fmaf(a, la - o.logprob(teacher.x[i], sc.inv_t), loss);
+    }
   loss = block_sum<THREADS>(loss, buf[2]);
   if (threadIdx.x == 0) {
     d.loss[t] = loss;
@@ -335,11 +417,14 @@ struct RowLds {
 };
 
 template <int DT, int OP>
-__device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Softmax& r, const uint32_t* keys, RowLds& lds) {
+using Single = std::conditional_t<OP == DISTILL, Teacher<DT>, Token<DT>>;
+template <int DT, int OP>
+__device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Single<DT, OP>& single, const Softmax& r,
+                                       const uint32_t* keys, RowLds& lds) {
   if constexpr (OP == DISTILL)
-    finish_distill<DT>(d, sc, t, row, r, lds.teacher);
+    finish_distill<DT>(d, sc, t, single, r, lds.teacher);
   else
-    finish_logprobs<DT, OP == LOGPROBS_TOP>(d, sc, t, row, r, keys, &lds.select);
+    finish_logprobs<DT, OP == LOGPROBS_TOP>(d, sc, t, row, single, r, keys, &lds.select);
 }
 
 template <int DT>
@@ -348,14 +433,15 @@ __device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t)
 }
 
 // A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
-template <int DT, int OP>
+template <int DT, int OP, int U>
 __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0) {
   extern __shared__ uint32_t keys[];
   __shared__ RowLds lds;
   const int t = t0 + (int)blockIdx.x;
   const void* row = logits_row<DT>(d, t);
-  const Softmax r = block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
-  finish<DT, OP>(d, sc, t, row, r, keys, lds);
+  const Single<DT, OP> single(d, t, row);
+  const Softmax r = block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
+  finish<DT, OP>(d, sc, t, row, single, r, keys, lds);
 }
 
 // Few rows: pieces of a row, whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
@@ -365,7 +451,7 @@ __global__ __launch_bounds__(THREADS) void vocab_chunk_kernel(tk_vocab_desc d, S
   const int t = blockIdx.x / n_chunks, c = blockIdx.x % n_chunks, c0 = c * chunk;
   const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
   const Softmax r =
-      block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
+      block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, 2>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
   if (threadIdx.x < 3) parts[((int64_t)t * n_chunks + c) * 3 + threadIdx.x] = threadIdx.x == 0 ? r.m : threadIdx.x == 1 ? r.s : r.e;
 }
 
@@ -373,26 +459,31 @@ template <int DT, int OP>
 __global__ __launch_bounds__(THREADS) void vocab_join_kernel(tk_vocab_desc d, Scales sc, int n_chunks, const float* parts, const uint32_t* keys, int groups) {
   __shared__ RowLds lds;
   const int t = blockIdx.x;
+  const void* row = logits_row<DT>(d, t);
+  const Single<DT, OP> single(d, t, row);
   Softmax r = {NEG_INF, 0.f, 0.f};
   if ((int)threadIdx.x < n_chunks) {
     const float* p = parts + ((int64_t)t * n_chunks + threadIdx.x) * 3;
     r = {p[0], p[1], p[2]};
   }
   r = block_softmax(r, sc.c2, lds.softmax);
-  finish<DT, OP>(d, sc, t, logits_row<DT>(d, t), r, keys + (int64_t)t * groups, lds);
+  finish<DT, OP>(d, sc, t, row, single, r, keys + (int64_t)t * groups, lds);
 }
 
-// Pieces that the rows of a call are split into: enough for eight workgroups a CU, of at least a load a thread.
+// Pieces that the rows of a call are split into: about four workgroups a CU; no more, since a second launch joins them (us, pieces for 500, 1000
+// and 2048 workgroups: 1000 x 131072 bf16 with 20 alternatives 61, 61, 76; 300 x 131072 22.9, 22.5, 23.4; 100 x 131072 13.4, 12.6, 11.8; 61 x 50001
+// fp16 with 8 13.1, 14.4, 16.3).
 struct Split {
   int n, chunk, groups;
   int64_t parts_bytes, bytes;
 };
 Split split_of(int32_t n_rows, int32_t vocab, int32_t k) {
   Split s;
-  const int64_t want = cdiv(2048, n_rows > 0 ? n_rows : 1), most = cdiv(vocab, 2048);
+  const int64_t want = cdiv(1000, n_rows > 0 ? n_rows : 1), most = cdiv(vocab, LEAST_CHUNK);
   int64_t n = want < most ? want : most;
   n = n < MAX_CHUNKS ? n : MAX_CHUNKS;
-  s.chunk = (int)(cdiv(cdiv(vocab, n), 2048) * 2048 < vocab ? cdiv(cdiv(vocab, n), 2048) * 2048 : vocab);
+  const int64_t chunk = cdiv(cdiv(vocab, n), LEAST_CHUNK) * LEAST_CHUNK;
+  s.chunk = (int)(chunk < vocab ? chunk : vocab);
   s.n = (int)cdiv(vocab, s.chunk);
   s.groups = k ? (int)cdiv(vocab, GROUP) : 0;
   s.parts_bytes = cdiv((int64_t)n_rows * s.n * 12, 16) * 16;
@@ -407,9 +498,14 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0);
   const Scales sc = scales_of(d);
   if (s.n == 1) {
+    // Four vectors a lane under way, or two: two waste less of a row's last step and start sooner, four carry long rows when the chip is full of them.
+    // us with two, four (softmax statistics alone; * with 64 alternatives): 4096 x 131072 bf16 196, 188 (* 208, 204); 2048 x 32000 fp32 50.2, 47.6;
+    // 1000 x 50001 fp16 25.4, 27.5, fp32 38.4, 39.8; 16000 x 4000 bf16 with 20 alternatives 74, 90.
+    constexpr int STEP = 4 * THREADS * RowType<DT>::VE;
+    auto f = d->n_rows >= 2048 && d->vocab >= 6 * STEP ? vocab_rows_kernel<DT, OP, 4> : vocab_rows_kernel<DT, OP, 2>;
     for (int64_t t = 0; t < d->n_rows; t += MAX_GRID) {
       const int rows = (int)(d->n_rows - t < MAX_GRID ? d->n_rows - t : MAX_GRID);
-      hipLaunchKernelGGL((vocab_rows_kernel<DT, OP>), dim3(rows), dim3(THREADS), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
+      hipLaunchKernelGGL(f, dim3(rows), dim3(THREADS), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
     }
     return check_launch(who);
   }
