@@ -32,6 +32,13 @@ struct RowType {
   static __device__ __forceinline__ row_u32x4 load_vec(const void* p, int64_t i) {
     return *reinterpret_cast<const row_u32x4_at2*>(static_cast<const char*>(p) + i * BYTES);
   }
+  // The same with the hint that the elements are not looked at again.
+  static __device__ __forceinline__ row_u32x4 load_vec_once(const void* p, int64_t i) {
+    return __builtin_nontemporal_load(reinterpret_cast<const row_u32x4_at2*>(static_cast<const char*>(p) + i * BYTES));
+  }
+  static __device__ __forceinline__ void store_vec_once(void* p, int64_t i, row_u32x4 v) {
+    __builtin_nontemporal_store(v, reinterpret_cast<row_u32x4_at2*>(static_cast<char*>(p) + i * BYTES));
+  }
   // What is left of a row from element i on; opaque, since the compiler would keep a mask for each element of each vector over a loop
   // over rows, at a hundred registers.
   static __device__ __forceinline__ int left(int i, int end) {

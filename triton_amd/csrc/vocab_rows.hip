@@ -10,7 +10,6 @@ namespace {
 constexpr float NEG_INF = -__builtin_inff();
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int THREADS = 256, WAVES = 4;
 constexpr int MAX_GRID = 1 << 23;  // workgroups of a launch (2^32 threads are its limit)
 constexpr int GROUP = 64;      // consecutive columns whose largest logit is kept while a row streams by
 constexpr int MAX_CHUNKS = 256;  // pieces that a row is split into where there are few rows
@@ -42,22 +41,7 @@ struct Softmax {
   }
 };
 
-// A row's statistics in every lane, from those of the lanes; `buf`: 3 * WAVES floats of LDS.
-__device__ __forceinline__ Softmax block_softmax(Softmax r, float c2, float* buf) {
-  r.raise(block_max<THREADS>(r.m, buf), c2);
-  r.s = wave_sum_f32(r.s);
-  r.e = wave_sum_f32(r.e);
-  if ((threadIdx.x & 63) == 0) {
-    buf[WAVES + (threadIdx.x >> 6)] = r.s;
-    buf[2 * WAVES + (threadIdx.x >> 6)] = r.e;
-  }
-  __syncthreads();
-  r.s = (buf[WAVES] + buf[WAVES + 1]) + (buf[WAVES + 2] + buf[WAVES + 3]);
-  r.e = (buf[2 * WAVES] + buf[2 * WAVES + 1]) + (buf[2 * WAVES + 2] + buf[2 * WAVES + 3]);
-  return r;
-}
-
-// Order of a logit as an unsigned number of KEY_BITS; the two zeros are one value, and no logit's number is zero.
+// Order of a logit as an unsigned number of BITS; the two zeros are one value, and no logit's number is zero.
 template <int DT>
 struct Key {
   static constexpr int SHIFT = DT == TK_F32 ? 0 : DT == TK_BF16 ? 16 : 13, BITS = 32 - SHIFT;
@@ -68,223 +52,8 @@ struct Key {
   }
 };
 
-// Columns [c0, c1) of a row; `keys` takes the order numbers of the groups' largest logits (group = column / GROUP; c0 is a multiple
-// of GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
-template <int DT, bool ENTROPY, bool TOP, int U>
-__device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float c2, uint32_t* keys) {
-  typedef RowType<DT> R;
-  constexpr int VE = R::VE, STEP = THREADS * VE * U;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 64 * VE;
-  Softmax r = {NEG_INF, 0.f, 0.f};
-  const auto fetch = [&](row_u32x4 (&raw)[U], int base) {
-    const int at = base + (int)threadIdx.x * VE;
-    if (base + STEP <= c1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = R::load_vec(row, at + u * THREADS * VE);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
-    }
-  };
-  row_u32x4 next[U];
-  fetch(next, c0);
-  for (int base = c0; base < c1; base += STEP) {
-    const int at = base + (int)threadIdx.x * VE;
-    row_u32x4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = next[u];
-    if (base + STEP < c1) fetch(next, base + STEP);
-    __builtin_amdgcn_sched_barrier(0);  // (the requests first)
-    float mx[U], top = NEG_INF;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      mx[u] = NEG_INF;
-      if (base + u * THREADS * VE + wave >= c1) continue;  // (of a row's last step only; the wave as a whole)
-      mx[u] = R::element(raw[u], 0);
-#pragma unroll
-      for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
-      top = fmaxf(top, mx[u]);
-    }
-    if (top > r.m) r.raise(top, c2);
-    const float ref = r.reference();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (base + u * THREADS * VE + wave >= c1) continue;
-      float s = 0.f, en = 0.f;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float d = (R::element(raw[u], e) - ref) * c2, p = __builtin_amdgcn_exp2f(d);
-        s += p;
-        if (ENTROPY) en = fmaf(p, fmaxf(d, D_MIN), en);
-      }
-      r.s += s;
-      r.e += en;
-      if (TOP) {
-        int x = __builtin_bit_cast(int, mx[u]);
-#define TK_STEP(ctrl) \
-  x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
-        TK_STEP(TK_DPP_QUAD_XOR1)
-        TK_STEP(TK_DPP_QUAD_XOR2)
-        TK_STEP(TK_DPP_ROW_HALF_MIRROR)
-        if (VE == 4) TK_STEP(TK_DPP_ROW_MIRROR)
-#undef TK_STEP
-        const int c = at + u * THREADS * VE;
-        if ((threadIdx.x & (GROUP / VE - 1)) == 0 && c < c1) keys[c / GROUP] = Key<DT>::of(__builtin_bit_cast(float, x));
-      }
-    }
-  }
-  return r;
-}
-
-// ---- the k largest ------------------------------------------------------------------------------------------
-// A row's k largest logits lie in the k groups whose largest logits are the largest (equal ones: the lower groups): were one of them in
-// another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per
-// group, and then at the k groups' elements again: the rest of the row is read once, whatever stands in it.
-// A bound from below narrows both: k threads' largest group numbers are at least the k-th largest of the threads' largest ones, so that
-// only groups, and then only elements, from there on can be among the k; as a rule they are few more than k, which are ranked by
-// counting.  Where they are many (equal logits, logits masked to one value, neighbours sorted together), each of the two selections finds the
-// k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum in the order of the columns.
-constexpr int MANY = 512;
-struct SelectLds {
-  int count[2][WAVES];
-  int scan[WAVES];
-  int n_groups, n_found;
-  row_u32x4 most[THREADS / 4];
-  int group[MANY];
-  uint64_t found[MANY];  // key << 32 | ~column: a larger one comes first
-};
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int column) { return (uint64_t)key << 32 | (uint32_t)~column; }
 
-// Calls take(slot, i) for the k first of n items in the order (larger key, then lower i), slots by i; at least k keys are not 0.  A thread looks
-// at consecutive items.  This is the way for the rows that the ranking does not serve: it reads the keys again for each bit.
-template <int BITS, class KeyOf, class F>
-__device__ __forceinline__ void select(int n, int k, SelectLds& lds, KeyOf&& key_of, F&& take) {
-  const int per = (n + THREADS - 1) / THREADS, i0 = (int)threadIdx.x * per, i1 = i0 + per < n ? i0 + per : n;
-  uint32_t from = 0;
-  bool exact = false;  // k keys are >= from
-  for (int b = BITS - 1; b >= 0 && !exact; --b) {
-    const uint32_t at = from | 1u << b;
-    int mine = 0;
-    for (int i = i0; i < i1; ++i) mine += key_of(i) >= at;
-    mine = wave_scan_i32(mine);
-    if ((threadIdx.x & 63) == 63) lds.count[b & 1][threadIdx.x >> 6] = mine;
-    __syncthreads();
-    const int c = (lds.count[b & 1][0] + lds.count[b & 1][1]) + (lds.count[b & 1][2] + lds.count[b & 1][3]);
-    if (c >= k) from = at;
-    exact = c == k;
-  }
-  // all larger ones, and the first of the equal ones
-  int larger = 0, equal = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t key = key_of(i);
-    larger += key > from;
-    equal += key == from;
-  }
-  const int mine = larger | equal << 16, upto = wave_scan_i32(mine);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) lds.scan[threadIdx.x >> 6] = upto;
-  __syncthreads();
-  int before = upto - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) before += lds.scan[w];
-    all += lds.scan[w];
-  }
-  const int need = k - (all & 0xFFFF);  // equal ones that are taken
-  int l = before & 0xFFFF, q = before >> 16;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t key = key_of(i);
-    if (key > from || (key == from && q < need)) take(l + (q < need ? q : need), i);
-    l += key > from;
-    q += key == from;
-  }
-}
-
-// The k-th largest of the threads' numbers, each wave by itself; 1 (less than any logit's) where fewer than k threads have one.
-template <int BITS>
-__device__ __forceinline__ uint32_t kth_of_threads(uint32_t mine, int k, SelectLds& lds) {
-  reinterpret_cast<uint32_t*>(lds.most)[threadIdx.x] = mine;
-  __syncthreads();
-  const row_u32x4 four = lds.most[threadIdx.x & 63];
-  uint32_t from = 0;
-  for (int b = BITS - 1; b >= 0; --b) {
-    const uint32_t at = from | 1u << b;
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c += __builtin_popcountll(__ballot(four[i] >= at));
-    if (c < k) continue;
-    from = at;
-    if (c == k) break;
-  }
-  return from ? from : 1u;
-}
-
-// Leaves at least the k largest of a row in lds.found, in any order, and returns how many; from the groups' numbers.
-template <int DT>
-__device__ __forceinline__ int top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
-  typedef RowType<DT> R;
-  constexpr int VE = R::VE, BITS = Key<DT>::BITS, OWN = 8;
-  const int groups = (V + GROUP - 1) / GROUP;
-  if (threadIdx.x == 0) lds.n_groups = lds.n_found = 0;
-  uint32_t most = 0, own[OWN];  // (the first OWN of a thread's stay in registers)
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    const int g = i * THREADS + (int)threadIdx.x;
-    own[i] = g < groups ? group_keys[g] : 0u;
-    most = own[i] > most ? own[i] : most;
-  }
-  for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) most = group_keys[g] > most ? group_keys[g] : most;
-  if (groups < k)  // a row so short that the threads' elements tell more
-    for (int v = threadIdx.x * VE; v < V; v += THREADS * VE) {
-      const row_u32x4 raw = R::load_vec_to(row, v, V, R::NEG_INF_BITS);
-      uint32_t mx = 0;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const uint32_t one = Key<DT>::of(R::element(raw, e));
-        mx = one > mx ? one : mx;
-      }
-      most = v == (int)threadIdx.x * VE || mx > most ? mx : most;
-    }
-  const uint32_t from = kth_of_threads<BITS>(most, k, lds);
-  const auto add_group = [&](uint32_t key, int g) {
-    if (key < from) return;
-    const int slot = atomicAdd(&lds.n_groups, 1);
-    if (slot < MANY) lds.group[slot] = g;
-  };
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) add_group(own[i], i * THREADS + (int)threadIdx.x);
-  for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) add_group(group_keys[g], g);
-  __syncthreads();
-  const int n_groups = lds.n_groups;
-  if (n_groups <= MANY) {
-    constexpr int PER = GROUP / VE;
-    for (int v = threadIdx.x; v < n_groups * PER; v += THREADS) {
-      const int at = lds.group[v / PER] * GROUP + v % PER * VE;
-      const row_u32x4 raw = R::load_vec_to(row, at, V, R::NEG_INF_BITS);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const uint32_t one = Key<DT>::of(R::element(raw, e));
-        if (one >= from && at + e < V) {
-          const int i = atomicAdd(&lds.n_found, 1);
-          if (i < MANY) lds.found[i] = entry_of(one, at + e);
-        }
-      }
-    }
-    __syncthreads();
-    const int n = lds.n_found;
-    if (n <= MANY) return n;
-  }
-  const int n = k < groups ? k : groups;
-  select<BITS>(groups, n, lds, [&](int i) { return group_keys[i]; }, [&](int to, int i) { lds.group[to] = i; });
-  __syncthreads();
-  const auto column = [&](int i) { return lds.group[i / GROUP] * GROUP + i % GROUP; };
-  const auto element = [&](int i) { return column(i) < V ? Key<DT>::of(R::load(row, column(i))) : 0u; };
-  select<BITS>(n * GROUP, k, lds, element, [&](int to, int i) { lds.found[to] = entry_of(element(i), column(i)); });
-  __syncthreads();
-  return k;
-}
-
-// ---- what comes out of a row's statistics ---------------------------------------------------------------------
 struct RowResult {
   float m, log_s;
   bool bad, empty;
@@ -308,40 +77,6 @@ struct Token {
   }
 };
 
-template <int DT, bool TOP>
-__device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Token<DT>& token, const Softmax& r,
-                                                const uint32_t* group_keys, SelectLds* lds) {
-  const RowResult o(r);
-  if (threadIdx.x == 0) {
-    d.logprobs[t] = token.live ? o.logprob(token.x, sc.inv_t) : 0.f;
-    d.entropy[t] = o.bad ? __builtin_nanf("") : o.empty ? 0.f : o.log_s - LN2 * (r.e / r.s);
-    if (d.stats) {
-      d.stats[t] = o.m;
-      d.stats[(int64_t)d.n_rows + t] = o.log_s;
-    }
-  }
-  if constexpr (TOP) {
-    const int64_t out = (int64_t)t * d.k;
-    if (o.bad) {
-      if ((int)threadIdx.x < d.k) {
-        d.top_indx[out + threadIdx.x] = -1;
-        d.top_logprobs[out + threadIdx.x] = __builtin_nanf("");
-      }
-      return;
-    }
-    const int n = top_of_row<DT>(row, d.vocab, d.k, group_keys, *lds);
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const uint64_t mine = lds->found[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += lds->found[j] > mine;
-      if (rank < d.k) {
-        d.top_indx[out + rank] = (int)~(uint32_t)mine;
-        d.top_logprobs[out + rank] = o.logprob(Key<DT>::value((uint32_t)(mine >> 32)), sc.inv_t);
-      }
-    }
-  }
-}
-
 // The teacher's entry j of row t: its index, or -1 where it carries no weight, and its logit.
 __device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int j, float* q) {
   *q = load_any(d.teacher_logits, d.teacher_dtype, (int64_t)t * d.teacher_stride_m + j);
@@ -349,83 +84,366 @@ __device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int 
   return i < 0 || i >= d.vocab || *q == NEG_INF ? -1 : (int)i;
 }
 
-// The teacher's entries of a thread: their logits, -inf where they carry no weight, and the student's at their indices.
-constexpr int ENTRIES = TK_VOCAB_MAX_TEACHER / THREADS;
-template <int DT>
-struct Teacher {
-  float q[ENTRIES], x[ENTRIES];
-  __device__ __forceinline__ Teacher(const tk_vocab_desc& d, int t, const void* row) {
+enum { LOGPROBS = 0, LOGPROBS_TOP = 1, DISTILL = 2 };
+
+// ---- a row by a workgroup of THREADS lanes: four waves, or one for short rows, of which the chip then holds four times as many ----------
+template <int THREADS>
+struct Workgroup {
+  static constexpr int WAVES = THREADS / 64;
+  static constexpr int MANY = THREADS == 64 ? 256 : 512;  // candidates that are ranked by counting
+  static constexpr int ENTRIES = TK_VOCAB_MAX_TEACHER / 256;  // teacher entries a lane
+
+  // A row's statistics in every lane, from those of the lanes; `buf`: 3 * WAVES floats of LDS.
+  static __device__ __forceinline__ Softmax block_softmax(Softmax r, float c2, float* buf) {
+    r.raise(block_max<THREADS>(r.m, buf), c2);
+    r.s = wave_sum_f32(r.s);
+    r.e = wave_sum_f32(r.e);
+    if constexpr (WAVES == 1) return r;
+    if ((threadIdx.x & 63) == 0) {
+      buf[WAVES + (threadIdx.x >> 6)] = r.s;
+      buf[2 * WAVES + (threadIdx.x >> 6)] = r.e;
+    }
+    __syncthreads();
+    r.s = buf[WAVES];
+    r.e = buf[2 * WAVES];
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
-      const int j = i * THREADS + (int)threadIdx.x;
-      q[i] = NEG_INF;
-      x[i] = 0.f;
-      if (j < d.n_teacher) {
-        const int at = teacher_entry(d, t, j, &q[i]);
-        if (at >= 0)
-          x[i] = RowType<DT>::load(row, at);
-        else
-          q[i] = NEG_INF;
+    for (int w = 1; w < WAVES; ++w) {
+      r.s += buf[WAVES + w];
+      r.e += buf[2 * WAVES + w];
+    }
+    return r;
+  }
+
+  // Columns [c0, c1) of a row; `keys` takes the order numbers of the groups' largest logits (group = column / GROUP; c0 is a multiple
+  // of GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
+  template <int DT, bool ENTROPY, bool TOP, int U>
+  static __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float c2, uint32_t* keys) {
+    typedef RowType<DT> R;
+    constexpr int VE = R::VE, STEP = THREADS * VE * U;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 64 * VE;
+    Softmax r = {NEG_INF, 0.f, 0.f};
+    const auto fetch = [&](row_u32x4 (&raw)[U], int base) {
+      const int at = base + (int)threadIdx.x * VE;
+      if (base + STEP <= c1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = R::load_vec(row, at + u * THREADS * VE);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
+      }
+    };
+    row_u32x4 next[U];
+    fetch(next, c0);
+    for (int base = c0; base < c1; base += STEP) {
+      const int at = base + (int)threadIdx.x * VE;
+      row_u32x4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      if (base + STEP < c1) fetch(next, base + STEP);
+      __builtin_amdgcn_sched_barrier(0);  // (the requests first)
+      float mx[U], top = NEG_INF;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        mx[u] = NEG_INF;
+        if (base + u * THREADS * VE + wave >= c1) continue;  // (of a row's last step only; the wave as a whole)
+        mx[u] = R::element(raw[u], 0);
+#pragma unroll
+        for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
+        top = fmaxf(top, mx[u]);
+      }
+      if (top > r.m) r.raise(top, c2);
+      const float ref = r.reference();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (base + u * THREADS * VE + wave >= c1) continue;
+        float s = 0.f, en = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float d = (R::element(raw[u], e) - ref) * c2, p = __builtin_amdgcn_exp2f(d);
+          s += p;
+          if (ENTROPY) en = fmaf(p, fmaxf(d, D_MIN), en);
+        }
+        r.s += s;
+        r.e += en;
+        if (TOP) {
+          int x = __builtin_bit_cast(int, mx[u]);
+#define TK_STEP(ctrl) \
+    x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
+          TK_STEP(TK_DPP_QUAD_XOR1)
+          TK_STEP(TK_DPP_QUAD_XOR2)
+          TK_STEP(TK_DPP_ROW_HALF_MIRROR)
+          if (VE == 4) TK_STEP(TK_DPP_ROW_MIRROR)
+#undef TK_STEP
+          const int c = at + u * THREADS * VE;
+          if ((threadIdx.x & (GROUP / VE - 1)) == 0 && c < c1) keys[c / GROUP] = Key<DT>::of(__builtin_bit_cast(float, x));
+        }
+      }
+    }
+    return r;
+  }
+
+  // ---- the k largest ------------------------------------------------------------------------------------------
+  // A row's k largest logits lie in the k groups whose largest logits are the largest (equal ones: the lower groups): were one of them in
+  // another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per
+  // group, and then at the k groups' elements again: the rest of the row is read once, whatever stands in it.
+  // A bound from below narrows both: k threads' largest group numbers are at least the k-th largest of the threads' largest ones, so that
+  // only groups, and then only elements, from there on can be among the k; as a rule they are few more than k, which are ranked by
+  // counting.  Where they are many (equal logits, logits masked to one value, neighbours sorted together), each of the two selections finds the
+  // k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum in the order of the columns.
+  struct SelectLds {
+    int count[2][WAVES];
+    int scan[WAVES];
+    int n_groups, n_found;
+    alignas(16) uint32_t most[THREADS];
+    int group[MANY];
+    uint64_t found[MANY];  // key << 32 | ~column: a larger one comes first
+  };
+  // Calls take(slot, i) for the k first of n items in the order (larger key, then lower i), slots by i; at least k keys are not 0.  A thread looks
+  // at consecutive items.  This is the way for the rows that the ranking does not serve: it reads the keys again for each bit.
+  template <int BITS, class KeyOf, class F>
+  static __device__ __forceinline__ void select(int n, int k, SelectLds& lds, KeyOf&& key_of, F&& take) {
+    const int per = (n + THREADS - 1) / THREADS, i0 = (int)threadIdx.x * per, i1 = i0 + per < n ? i0 + per : n;
+    uint32_t from = 0;
+    bool exact = false;  // k keys are >= from
+    for (int b = BITS - 1; b >= 0 && !exact; --b) {
+      const uint32_t at = from | 1u << b;
+      int mine = 0;
+      for (int i = i0; i < i1; ++i) mine += key_of(i) >= at;
+      mine = wave_scan_i32(mine);
+      if ((threadIdx.x & 63) == 63) lds.count[b & 1][threadIdx.x >> 6] = mine;
+      __syncthreads();
+      int c = lds.count[b & 1][0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) c += lds.count[b & 1][w];
+      if (c >= k) from = at;
+      exact = c == k;
+    }
+    // all larger ones, and the first of the equal ones
+    int larger = 0, equal = 0;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t key = key_of(i);
+      larger += key > from;
+      equal += key == from;
+    }
+    const int mine = larger | equal << 16, upto = wave_scan_i32(mine);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) lds.scan[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    int before = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) before += lds.scan[w];
+      all += lds.scan[w];
+    }
+    const int need = k - (all & 0xFFFF);  // equal ones that are taken
+    int l = before & 0xFFFF, q = before >> 16;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t key = key_of(i);
+      if (key > from || (key == from && q < need)) take(l + (q < need ? q : need), i);
+      l += key > from;
+      q += key == from;
+    }
+  }
+
+  // The k-th largest of the threads' numbers, each wave by itself; 1 (less than any logit's) where fewer than k threads have one.
+  template <int BITS>
+  static __device__ __forceinline__ uint32_t kth_of_threads(uint32_t mine, int k, SelectLds& lds) {
+    lds.most[threadIdx.x] = mine;
+    __syncthreads();
+    typedef uint32_t own __attribute__((ext_vector_type(WAVES == 1 ? 2 : WAVES)));  // (a lane's share of them; a wave alone has one)
+    own share;
+    if constexpr (WAVES == 1)
+      share = own{mine, 0u};
+    else
+      share = reinterpret_cast<const own*>(lds.most)[threadIdx.x & 63];
+    uint32_t from = 0;
+    for (int b = BITS - 1; b >= 0; --b) {
+      const uint32_t at = from | 1u << b;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) c += __builtin_popcountll(__ballot(share[i] >= at));
+      if (c < k) continue;
+      from = at;
+      if (c == k) break;
+    }
+    return from ? from : 1u;
+  }
+
+  // Leaves at least the k largest of a row in lds.found, in any order, and returns how many; from the groups' numbers.
+  template <int DT>
+  static __device__ __forceinline__ int top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
+    typedef RowType<DT> R;
+    constexpr int VE = R::VE, BITS = Key<DT>::BITS, OWN = 8;
+    const int groups = (V + GROUP - 1) / GROUP;
+    if (threadIdx.x == 0) lds.n_groups = lds.n_found = 0;
+    uint32_t most = 0, own[OWN];  // (the first OWN of a thread's stay in registers)
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int g = i * THREADS + (int)threadIdx.x;
+      own[i] = g < groups ? group_keys[g] : 0u;
+      most = own[i] > most ? own[i] : most;
+    }
+    for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) most = group_keys[g] > most ? group_keys[g] : most;
+    if (groups < k)  // a row so short that the threads' elements tell more
+      for (int v = threadIdx.x * VE; v < V; v += THREADS * VE) {
+        const row_u32x4 raw = R::load_vec_to(row, v, V, R::NEG_INF_BITS);
+        uint32_t mx = 0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const uint32_t one = Key<DT>::of(R::element(raw, e));
+          mx = one > mx ? one : mx;
+        }
+        most = v == (int)threadIdx.x * VE || mx > most ? mx : most;
+      }
+    const uint32_t from = kth_of_threads<BITS>(most, k, lds);
+    const auto add_group = [&](uint32_t key, int g) {
+      if (key < from) return;
+      const int slot = atomicAdd(&lds.n_groups, 1);
+      if (slot < MANY) lds.group[slot] = g;
+    };
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) add_group(own[i], i * THREADS + (int)threadIdx.x);
+    for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) add_group(group_keys[g], g);
+    __syncthreads();
+    const int n_groups = lds.n_groups;
+    if (n_groups <= MANY) {
+      constexpr int PER = GROUP / VE;
+      for (int v = threadIdx.x; v < n_groups * PER; v += THREADS) {
+        const int at = lds.group[v / PER] * GROUP + v % PER * VE;
+        const row_u32x4 raw = R::load_vec_to(row, at, V, R::NEG_INF_BITS);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const uint32_t one = Key<DT>::of(R::element(raw, e));
+          if (one >= from && at + e < V) {
+            const int i = atomicAdd(&lds.n_found, 1);
+            if (i < MANY) lds.found[i] = entry_of(one, at + e);
+          }
+        }
+      }
+      __syncthreads();
+      const int n = lds.n_found;
+      if (n <= MANY) return n;
+    }
+    const int n = k < groups ? k : groups;
+    select<BITS>(groups, n, lds, [&](int i) { return group_keys[i]; }, [&](int to, int i) { lds.group[to] = i; });
+    __syncthreads();
+    const auto column = [&](int i) { return lds.group[i / GROUP] * GROUP + i % GROUP; };
+    const auto element = [&](int i) { return column(i) < V ? Key<DT>::of(R::load(row, column(i))) : 0u; };
+    select<BITS>(n * GROUP, k, lds, element, [&](int to, int i) { lds.found[to] = entry_of(element(i), column(i)); });
+    __syncthreads();
+    return k;
+  }
+
+  // ---- what comes out of a row's statistics ---------------------------------------------------------------------
+  template <int DT, bool TOP>
+  static __device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Token<DT>& token, const Softmax& r,
+                                                  const uint32_t* group_keys, SelectLds* lds) {
+    const RowResult o(r);
+    if (threadIdx.x == 0) {
+      d.logprobs[t] = token.live ? o.logprob(token.x, sc.inv_t) : 0.f;
+      d.entropy[t] = o.bad ? __builtin_nanf("") : o.empty ? 0.f : o.log_s - LN2 * (r.e / r.s);
+      if (d.stats) {
+        d.stats[t] = o.m;
+        d.stats[(int64_t)d.n_rows + t] = o.log_s;
+      }
+    }
+    if constexpr (TOP) {
+      const int64_t out = (int64_t)t * d.k;
+      if (o.bad) {
+        if ((int)threadIdx.x < d.k) {
+          d.top_indx[out + threadIdx.x] = -1;
+          d.top_logprobs[out + threadIdx.x] = __builtin_nanf("");
+        }
+        return;
+      }
+      const int n = top_of_row<DT>(row, d.vocab, d.k, group_keys, *lds);
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        const uint64_t mine = lds->found[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += lds->found[j] > mine;
+        if (rank < d.k) {
+          d.top_indx[out + rank] = (int)~(uint32_t)mine;
+          d.top_logprobs[out + rank] = o.logprob(Key<DT>::value((uint32_t)(mine >> 32)), sc.inv_t);
+        }
       }
     }
   }
-};
 
-template <int DT>
-__device__ __forceinline__ void finish_distill(const tk_vocab_desc& d, Scales sc, int t, const Teacher<DT>& teacher, const Softmax& r, float (*buf)[WAVES]) {
-  const RowResult o(r);
-  float qm = NEG_INF, qs = 0.f, loss = 0.f;
-  int bad = 0;
+  // The teacher's entries of a thread: their logits, -inf where they carry no weight, and the student's at their indices.
+  template <int DT>
+  struct Teacher {
+    float q[ENTRIES], x[ENTRIES];
+    __device__ __forceinline__ Teacher(const tk_vocab_desc& d, int t, const void* row) {
 #pragma unroll
-  for (int i = 0; i < ENTRIES; ++i) {
-    qm = fmaxf(qm, teacher.q[i]);
-    bad |= teacher.q[i] != teacher.q[i];
+      for (int i = 0; i < ENTRIES; ++i) {
+        const int j = i * THREADS + (int)threadIdx.x;
+        q[i] = NEG_INF;
+        x[i] = 0.f;
+        if (j < d.n_teacher) {
+          const int at = teacher_entry(d, t, j, &q[i]);
+          if (at >= 0)
+            x[i] = RowType<DT>::load(row, at);
+          else
+            q[i] = NEG_INF;
+        }
+      }
+    }
+  };
+
+  template <int DT>
+  static __device__ __forceinline__ void finish_distill(const tk_vocab_desc& d, Scales sc, int t, const Teacher<DT>& teacher, const Softmax& r, float (*buf)[WAVES]) {
+    const RowResult o(r);
+    float qm = NEG_INF, qs = 0.f, loss = 0.f;
+    int bad = 0;
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      qm = fmaxf(qm, teacher.q[i]);
+      bad |= teacher.q[i] != teacher.q[i];
+    }
+    qm = block_max<THREADS>(qm, buf[0]);
+    bad = __syncthreads_or(bad) || qm == __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i)
+      if (teacher.q[i] != NEG_INF) qs += expf((teacher.q[i] - qm) * sc.inv_t);
+    qs = block_sum<THREADS>(qs, buf[1]);
+    const float log_qs = bad ? __builtin_nanf("") : logf(qs);
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i)
+      if (teacher.q[i] != NEG_INF) {
+        const float la = (teacher.q[i] - qm) * sc.inv_t - log_qs, a = expf(la);
+        if (a != 0.f) loss = fmaf(a, la - o.logprob(teacher.x[i], sc.inv_t), loss);
+      }
+    loss = block_sum<THREADS>(loss, buf[2]);
+    if (threadIdx.x == 0) {
+      d.loss[t] = loss;
+      if (d.stats) {
+        d.stats[t] = o.m;
+        d.stats[(int64_t)d.n_rows + t] = o.log_s;
+      }
+      if (d.teacher_stats) {
+        d.teacher_stats[t] = bad ? __builtin_nanf("") : qm;
+        d.teacher_stats[(int64_t)d.n_rows + t] = log_qs;
+      }
+    }
   }
-  qm = block_max<THREADS>(qm, buf[0]);
-  bad = __syncthreads_or(bad) || qm == __builtin_inff();
-#pragma unroll
-  for (int i = 0; i < ENTRIES; ++i)
-    if (teacher.q[i] != NEG_INF) qs += expf((teacher.q[i] - qm) * sc.inv_t);
-  qs = block_sum<THREADS>(qs, buf[1]);
-  const float log_qs = bad ? __builtin_nanf("") : logf(qs);
-#pragma unroll
-  for (int i = 0; i < ENTRIES; ++i)
-    if (teacher.q[i] != NEG_INF) {
-      const float la = (teacher.q[i] - qm) * sc.inv_t - log_qs, a = expf(la);
-      if (a != 0.f) loss = fmaf(a, la - o.logprob(teacher.x[i], sc.inv_t), loss);
-    }
-  loss = block_sum<THREADS>(loss, buf[2]);
-  if (threadIdx.x == 0) {
-    d.loss[t] = loss;
-    if (d.stats) {
-      d.stats[t] = o.m;
-      d.stats[(int64_t)d.n_rows + t] = o.log_s;
-    }
-    if (d.teacher_stats) {
-      d.teacher_stats[t] = bad ? __builtin_nanf("") : qm;
-      d.teacher_stats[(int64_t)d.n_rows + t] = log_qs;
-    }
+
+  struct RowLds {
+    float softmax[3 * WAVES];
+    float teacher[3][WAVES];
+    SelectLds select;
+  };
+
+  template <int DT, int OP>
+  using Single = std::conditional_t<OP == DISTILL, Teacher<DT>, Token<DT>>;
+  template <int DT, int OP>
+  static __device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Single<DT, OP>& single, const Softmax& r,
+                                         const uint32_t* keys, RowLds& lds) {
+    if constexpr (OP == DISTILL)
+      finish_distill<DT>(d, sc, t, single, r, lds.teacher);
+    else
+      finish_logprobs<DT, OP == LOGPROBS_TOP>(d, sc, t, row, single, r, keys, &lds.select);
   }
-}
-
-enum { LOGPROBS = 0, LOGPROBS_TOP = 1, DISTILL = 2 };
-
-struct RowLds {
-  float softmax[3 * WAVES];
-  float teacher[3][WAVES];
-  SelectLds select;
 };
-
-template <int DT, int OP>
-using Single = std::conditional_t<OP == DISTILL, Teacher<DT>, Token<DT>>;
-template <int DT, int OP>
-__device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Single<DT, OP>& single, const Softmax& r,
-                                       const uint32_t* keys, RowLds& lds) {
-  if constexpr (OP == DISTILL)
-    finish_distill<DT>(d, sc, t, single, r, lds.teacher);
-  else
-    finish_logprobs<DT, OP == LOGPROBS_TOP>(d, sc, t, row, single, r, keys, &lds.select);
-}
 
 template <int DT>
 __device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t) {
@@ -433,41 +451,43 @@ __device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t)
 }
 
 // A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
-template <int DT, int OP, int U>
+template <int DT, int OP, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0) {
+  typedef Workgroup<THREADS> W;
   extern __shared__ uint32_t keys[];
-  __shared__ RowLds lds;
+  __shared__ typename W::RowLds lds;
   const int t = t0 + (int)blockIdx.x;
   const void* row = logits_row<DT>(d, t);
-  const Single<DT, OP> single(d, t, row);
-  const Softmax r = block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
-  finish<DT, OP>(d, sc, t, row, single, r, keys, lds);
+  const typename W::template Single<DT, OP> single(d, t, row);
+  const Softmax r = W::block_softmax(W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
+  W::template finish<DT, OP>(d, sc, t, row, single, r, keys, lds);
 }
 
 // Few rows: pieces of a row, whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
+typedef Workgroup<256> Wide;
 template <int DT, int OP>
-__global__ __launch_bounds__(THREADS) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
-  __shared__ float buf[3 * WAVES];
+__global__ __launch_bounds__(256) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
+  __shared__ float buf[3 * Wide::WAVES];
   const int t = blockIdx.x / n_chunks, c = blockIdx.x % n_chunks, c0 = c * chunk;
   const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
-  const Softmax r =
-      block_softmax(stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, 2>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
+  const Softmax r = Wide::block_softmax(
+      Wide::stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, 2>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
   if (threadIdx.x < 3) parts[((int64_t)t * n_chunks + c) * 3 + threadIdx.x] = threadIdx.x == 0 ? r.m : threadIdx.x == 1 ? r.s : r.e;
 }
 
 template <int DT, int OP>
-__global__ __launch_bounds__(THREADS) void vocab_join_kernel(tk_vocab_desc d, Scales sc, int n_chunks, const float* parts, const uint32_t* keys, int groups) {
-  __shared__ RowLds lds;
+__global__ __launch_bounds__(256) void vocab_join_kernel(tk_vocab_desc d, Scales sc, int n_chunks, const float* parts, const uint32_t* keys, int groups) {
+  __shared__ Wide::RowLds lds;
   const int t = blockIdx.x;
   const void* row = logits_row<DT>(d, t);
-  const Single<DT, OP> single(d, t, row);
+  const Wide::Single<DT, OP> single(d, t, row);
   Softmax r = {NEG_INF, 0.f, 0.f};
   if ((int)threadIdx.x < n_chunks) {
     const float* p = parts + ((int64_t)t * n_chunks + threadIdx.x) * 3;
     r = {p[0], p[1], p[2]};
   }
-  r = block_softmax(r, sc.c2, lds.softmax);
-  finish<DT, OP>(d, sc, t, row, single, r, keys + (int64_t)t * groups, lds);
+  r = Wide::block_softmax(r, sc.c2, lds.softmax);
+  Wide::finish<DT, OP>(d, sc, t, row, single, r, keys + (int64_t)t * groups, lds);
 }
 
 // Pieces that the rows of a call are split into: about four workgroups a CU; no more, since a second launch joins them (us, pieces for 500, 1000
@@ -493,6 +513,12 @@ Split split_of(int32_t n_rows, int32_t vocab, int32_t k) {
 
 Scales scales_of(const tk_vocab_desc* d) { return {(float)(1.0 / d->temperature), (float)(1.4426950408889634 / d->temperature)}; }
 
+// Rows of up to SHORT_ROW columns have a wave each, where there are enough of them (us, a workgroup and a wave: 16000 x 1000 bf16 22.9, 12.1, its gradient
+// 35, 19; x 4000 23.5, 28, its gradient 52, 56), longer ones with alternatives up to SHORT_TOP, whose ranking is the same work for four waves and one
+// (with 20: 16000 x 2000 71, 34; x 4000 74, 44; x 8000 84, 67; x 16000 121, 118).  No more of those than half a wave ranks, nor more teacher
+// entries than four a lane.
+constexpr int SHORT_ROW = 2048, SHORT_TOP = 8192;
+
 template <int DT, int OP>
 int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0);
@@ -501,19 +527,21 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
     // Four vectors a lane under way, or two: two waste less of a row's last step and start sooner, four carry long rows when the chip is full of them.
     // us with two, four (softmax statistics alone; * with 64 alternatives): 4096 x 131072 bf16 196, 188 (* 208, 204); 2048 x 32000 fp32 50.2, 47.6;
     // 1000 x 50001 fp16 25.4, 27.5, fp32 38.4, 39.8; 16000 x 4000 bf16 with 20 alternatives 74, 90.
-    constexpr int STEP = 4 * THREADS * RowType<DT>::VE;
-    auto f = d->n_rows >= 2048 && d->vocab >= 6 * STEP ? vocab_rows_kernel<DT, OP, 4> : vocab_rows_kernel<DT, OP, 2>;
+    constexpr int STEP = 4 * 256 * RowType<DT>::VE;
+    const bool wave = d->n_rows >= 1000 && (OP == LOGPROBS_TOP ? d->k <= 32 && d->vocab <= SHORT_TOP : d->vocab <= SHORT_ROW)
+                      && (OP != DISTILL || d->n_teacher <= 64 * Workgroup<64>::ENTRIES);
+    auto f = wave ? vocab_rows_kernel<DT, OP, 64, 2> : d->n_rows >= 2048 && d->vocab >= 6 * STEP ? vocab_rows_kernel<DT, OP, 256, 4> : vocab_rows_kernel<DT, OP, 256, 2>;
     for (int64_t t = 0; t < d->n_rows; t += MAX_GRID) {
       const int rows = (int)(d->n_rows - t < MAX_GRID ? d->n_rows - t : MAX_GRID);
-      hipLaunchKernelGGL(f, dim3(rows), dim3(THREADS), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
+      hipLaunchKernelGGL(f, dim3(rows), dim3(wave ? 64 : 256), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
     }
     return check_launch(who);
   }
   if (!d->workspace) return fail(TK_ERR_INVALID, "%s: null workspace", who);
   float* parts = static_cast<float*>(d->workspace);
   uint32_t* keys = reinterpret_cast<uint32_t*>(static_cast<char*>(d->workspace) + s.parts_bytes);
-  hipLaunchKernelGGL((vocab_chunk_kernel<DT, OP>), dim3((unsigned)(d->n_rows * s.n)), dim3(THREADS), 0, stream, *d, sc, s.chunk, s.n, parts, keys, s.groups);
-  hipLaunchKernelGGL((vocab_join_kernel<DT, OP>), dim3(d->n_rows), dim3(THREADS), 0, stream, *d, sc, s.n, parts, keys, s.groups);
+  hipLaunchKernelGGL((vocab_chunk_kernel<DT, OP>), dim3((unsigned)(d->n_rows * s.n)), dim3(256), 0, stream, *d, sc, s.chunk, s.n, parts, keys, s.groups);
+  hipLaunchKernelGGL((vocab_join_kernel<DT, OP>), dim3(d->n_rows), dim3(256), 0, stream, *d, sc, s.n, parts, keys, s.groups);
   return check_launch(who);
 }
 
@@ -521,39 +549,34 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
 // A piece of a row a workgroup: one read and one write of the row's size.  With p = 2^d2, d2 = (x - m) c2 - log2 s:
 //   log probabilities   g = p (A + B d2) everywhere, A = -(d_lp + d_h H) / t, B = -d_h ln 2 / t, and d_lp / t more at the token
 //   distillation        g = p G, G = d_loss / t, and a_j G less at the teacher's entry j
-// The few columns that get more are found by a bit a column in LDS (the teacher's), so that each element is written once.
+// The teacher's few columns are written once more at the end, by the piece that they lie in: looking each column up while the row streams by
+// cost as much as the row where a wave's columns hold some of them (2000 x 1500 fp16 with 50 entries 31 us).
 constexpr int GRAD_CHUNK = 16384;
+// Gradients from this size on are read and written with the read-once hint: they would only push the logits, which come from the last-level cache in part, out
+// of it (forward and backward, us without and with: 2048 x 32000 fp32, 262 MB, 159, 129; 4096 x 131072 bf16, 1074 MB, 604, 590; 1000 x 50001 fp16,
+// 100 MB, 79, 74.5; 200 x 32000 bf16, 13 MB, 18, 18, where whoever reads the gradient next may find it cached).
+constexpr int64_t ONCE_BYTES = 64 << 20;
 
-template <int DT, int OP>
+template <int DT, int OP, int THREADS, bool ONCE>
 __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d, Scales sc, int t0, int n_chunks, int chunk) {
   typedef RowType<DT> R;
   constexpr int VE = R::VE, U = 2, STEP = THREADS * VE * U;
-  extern __shared__ uint32_t teacher[];  // [n_teacher] columns, [n_teacher] a_j (OP == DISTILL)
-  __shared__ uint32_t named[OP == DISTILL ? GRAD_CHUNK / 32 : 1];
-  const int t = t0 + (int)(blockIdx.x / (unsigned)n_chunks), c0 = (int)(blockIdx.x % (unsigned)n_chunks) * chunk;
+  // (from the last row back: its logits were read last and may still be in the last-level cache)
+  const unsigned place = gridDim.x - 1 - blockIdx.x;
+  const int t = t0 + (int)(place / (unsigned)n_chunks), c0 = (int)(place % (unsigned)n_chunks) * chunk;
   const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
   const void* row = logits_row<DT>(d, t);
   void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * R::BYTES;
   const float m = d.stats[t], log_s = d.stats[(int64_t)d.n_rows + t], log2_s = log_s * LOG2E;
-  float A, B = 0.f, more = 0.f;
+  float A, B = 0.f, more = 0.f, qm = 0.f, log_qs = 0.f;
   int token = -1;
   bool zero;
   if constexpr (OP == DISTILL) {
-    const float qm = d.teacher_stats[t], log_qs = d.teacher_stats[(int64_t)d.n_rows + t], g = d.d_loss ? d.d_loss[t * d.d_loss_stride] : 0.f;
+    qm = d.teacher_stats[t];
+    log_qs = d.teacher_stats[(int64_t)d.n_rows + t];
+    const float g = d.d_loss ? d.d_loss[t * d.d_loss_stride] : 0.f;
     zero = g == 0.f || log_s == NEG_INF || qm == NEG_INF;  // (sums of nothing)
     A = qm == qm ? g * sc.inv_t : qm;
-    if (!zero) {
-      for (int i = threadIdx.x; i < GRAD_CHUNK / 32; i += THREADS) named[i] = 0;
-      __syncthreads();
-      for (int j = threadIdx.x; j < d.n_teacher; j += THREADS) {
-        float q;
-        const int at = teacher_entry(d, t, j, &q);
-        teacher[j] = (uint32_t)at;
-        teacher[d.n_teacher + j] = f32_bits(expf((q - qm) * sc.inv_t - log_qs));
-        if (at >= c0 && at < c1) atomicOr(&named[(at - c0) >> 5], 1u << ((at - c0) & 31));
-      }
-      __syncthreads();
-    }
   } else {
     const int64_t at = index_at(d.tokens, d.tokens_i64, t);
     const bool live = at >= 0 && at < d.vocab;
@@ -564,6 +587,10 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
     B = -g_h * LN2 * sc.inv_t;
     more = g_lp * sc.inv_t;
   }
+  const auto gradient = [&](float x) {
+    const float d2 = fmaf(x - m, sc.c2, -log2_s), p = __builtin_amdgcn_exp2f(d2);
+    return OP == DISTILL ? p * A : p * fmaf(fmaxf(d2, D_MIN), B, A);
+  };
   for (int base = c0; base < c1; base += STEP) {
     const int at = base + (int)threadIdx.x * VE;
     if (zero) {
@@ -574,36 +601,56 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
     const bool full = base + STEP <= c1;
     row_u32x4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = full ? R::load_vec(row, at + u * THREADS * VE) : R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
+    for (int u = 0; u < U; ++u) {
+      const int v = at + u * THREADS * VE;
+      raw[u] = !full ? R::load_vec_to(row, v, c1, R::NEG_INF_BITS) : ONCE ? R::load_vec_once(row, v) : R::load_vec(row, v);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = at + u * THREADS * VE;
       float g[VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float d2 = fmaf(R::element(raw[u], e) - m, sc.c2, -log2_s), p = __builtin_amdgcn_exp2f(d2);
-        g[e] = OP == DISTILL ? p * A : p * fmaf(fmaxf(d2, D_MIN), B, A);
-      }
-      if constexpr (OP == DISTILL) {
-        const uint32_t bits = v < c1 ? named[(v - c0) >> 5] >> ((v - c0) & 31) & ((1u << VE) - 1u) : 0u;
-        if (bits)
-#pragma unroll
-          for (int e = 0; e < VE; ++e)
-            if (bits >> e & 1) {
-              float a = 0.f;
-              for (int j = 0; j < d.n_teacher; ++j)
-                if ((int)teacher[j] == v + e) a += bits_f32(teacher[d.n_teacher + j]);
-              g[e] = fmaf(-a, A, g[e]);
-            }
-      } else if ((unsigned)(token - v) < (unsigned)VE) {
+      for (int e = 0; e < VE; ++e) g[e] = gradient(R::element(raw[u], e));
+      if (OP != DISTILL && (unsigned)(token - v) < (unsigned)VE)
 #pragma unroll
         for (int e = 0; e < VE; ++e)
           if (v + e == token) g[e] += more;
-      }
-      if (full)
-        R::store_vec(out, v, R::pack(g));
-      else
+      if (!full)
         R::store_vec_to(out, v, c1, R::pack(g));
+      else if (ONCE)
+        R::store_vec_once(out, v, R::pack(g));
+      else
+        R::store_vec(out, v, R::pack(g));
+    }
+  }
+  if constexpr (OP == DISTILL) {
+    if (zero) return;
+    extern __shared__ uint32_t lds[];  // [n_teacher] columns, [n_teacher] logits, [chunk / 32] a bit a column that an entry names, whether two name one
+    const int n = d.n_teacher;
+    uint32_t *column = lds, *logit = lds + n, *named = lds + 2 * n, *twice = named + chunk / 32;
+    for (int i = threadIdx.x; i <= chunk / 32; i += THREADS) named[i] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += THREADS) {
+      float q;
+      const int v = teacher_entry(d, t, j, &q);
+      column[j] = (uint32_t)v;
+      logit[j] = f32_bits(q);
+      const uint32_t bit = 1u << ((v - c0) & 31);
+      if (v >= c0 && v < c1 && (atomicOr(&named[(v - c0) >> 5], bit) & bit)) *twice = 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's part of the row has arrived where the second writing of a column finds it)
+    __syncthreads();
+    const auto weight = [&](int j) { return expf((bits_f32(logit[j]) - qm) * sc.inv_t - log_qs); };
+    for (int j = threadIdx.x; j < n; j += THREADS) {
+      const int v = (int)column[j];
+      if (v < c0 || v >= c1) continue;
+      float a = 0.f;
+      if (!*twice)
+        a = weight(j);
+      else  // (all entries that name a column write the same)
+        for (int i = 0; i < n; ++i)
+          if ((int)column[i] == v) a += weight(i);
+      R::store(out, v, fmaf(-a, A, gradient(R::load(row, v))));
     }
   }
 }
@@ -615,10 +662,12 @@ int32_t backward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   const int64_t n = want > most ? most : want < least ? least : want;
   const int64_t chunk = cdiv(cdiv(d->vocab, n), 2048) * 2048;
   const int n_chunks = (int)cdiv(d->vocab, chunk), rows = MAX_GRID / n_chunks;
+  const bool wave = d->n_rows >= 1000 && d->vocab <= SHORT_ROW, once = (int64_t)d->n_rows * d->vocab * RowType<DT>::BYTES >= ONCE_BYTES;
+  auto f = wave ? vocab_backward_kernel<DT, OP, 64, false> : once ? vocab_backward_kernel<DT, OP, 256, true> : vocab_backward_kernel<DT, OP, 256, false>;
   for (int64_t t = 0; t < d->n_rows; t += rows) {
     const int now = (int)(d->n_rows - t < rows ? d->n_rows - t : rows);
-    hipLaunchKernelGGL((vocab_backward_kernel<DT, OP>), dim3((unsigned)(now * n_chunks)), dim3(THREADS), OP == DISTILL ? d->n_teacher * 8 : 0, stream, *d,
-                       scales_of(d), (int)t, n_chunks, (int)chunk);
+    hipLaunchKernelGGL(f, dim3((unsigned)(now * n_chunks)), dim3(wave ? 64 : 256), OP == DISTILL ? d->n_teacher * 8 + chunk / 8 + 4 : 0, stream, *d, scales_of(d),
+                       (int)t, n_chunks, (int)chunk);
   }
   return check_launch(who);
 }
