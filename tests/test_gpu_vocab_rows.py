@@ -205,6 +205,26 @@ def test_teacher_entries_that_do_not_count(dtype):
     _check_distill(z, q[:, :0], at[:, :0], 1.0, a)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("first", [1, 3, 5, 7])
+def test_padding_beside_rows_that_begin_between_boundaries(first, dtype):
+    """Entries and tokens of -1 where a row's loads begin in front of its first column: nothing in front of it is read or written."""
+    for T, V in ((7, 501), (5, 20003), (1200, 301)):
+        wide, tokens, a, b = _logits(T, V + 8, dtype)
+        z = wide[:, first:first + V]
+        tokens = tokens % V
+        tokens[::2] = -1
+        q, at = _teacher(z, 9)
+        at[:, ::2] = -1
+        at[1::3, 1] = 0
+        at[2::3, 3] = V - 1
+        _check_distill(z, q, at, 1.0, a)
+        wide[:, :first] = float("nan")
+        wide[:, first + V:] = INF
+        _check_logprobs(z, tokens, 5, 1.0, (a, b))
+        _check_distill(z, q, at, 1.0, a)
+
+
 def test_the_largest_number_of_teacher_entries():
     z, _, a, _ = _logits(3, 5003, BF16)
     _check_distill(z, *_teacher(z, 1024, dtype=F32), 1.0, a)

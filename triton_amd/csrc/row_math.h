@@ -46,22 +46,29 @@ struct RowType {
     asm volatile("" : "+v"(n));
     return n;
   }
-  // The same where the elements from `end` on are not there: they read as `fill` (a dword of it), and nothing behind `end` is touched.
-  static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int i, int end, uint32_t fill) {
-    const int n = left(i, end);
-    if (n >= VE) return load_vec(p, i);
+  // The same where the elements in front of `begin` and from `end` on are not there: they read as `fill` (a dword of it), and nothing there is
+  // touched.  Pairs of 16-bit elements are requested together, from the nearest element that there is, and chosen afterwards: one by one under their
+  // conditions, each waits for the one that it shares a register with, up to seven memory latencies in a row at the end of each row.
+  static __device__ __forceinline__ row_u32x4 load_vec_in(const void* p, int i, int begin, int end, uint32_t fill) {
+    const int n = left(i, end), skip = begin - i;
+    if (skip <= 0 && n >= VE) return load_vec(p, i);
     row_u32x4 v = {fill, fill, fill, fill};
+    if constexpr (DT == TK_F32) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      if (e < n) {
-        if constexpr (DT == TK_F32)
-          v[e] = static_cast<const uint32_t*>(p)[i + e];
-        else
-          v[e >> 1] = e & 1 ? (v[e >> 1] & 0xFFFFu) | (uint32_t) static_cast<const uint16_t*>(p)[i + e] << 16
-                            : (v[e >> 1] & 0xFFFF0000u) | static_cast<const uint16_t*>(p)[i + e];
-      }
+      for (int e = 0; e < VE; ++e)
+        if (e >= skip && e < n) v[e] = static_cast<const uint32_t*>(p)[i + e];
+    } else if (n > 0 && skip < VE) {
+      uint32_t x[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = static_cast<const uint16_t*>(p)[i + (e < skip ? skip : e < n ? e : n - 1)];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = e >= skip && e < n ? x[e] : fill & 0xFFFFu;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = x[2 * e] | x[2 * e + 1] << 16;
+    }
     return v;
   }
+  static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int i, int end, uint32_t fill) { return load_vec_in(p, i, i, end, fill); }
   static __device__ __forceinline__ float element(row_u32x4 v, int e) {
     if constexpr (DT == TK_F32) return bits_f32(v[e]);
     if constexpr (DT == TK_BF16) return bits_f32(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);

@@ -86,6 +86,23 @@ __device__ __forceinline__ int teacher_entry(const tk_vocab_desc& d, int t, int 
 
 enum { LOGPROBS = 0, LOGPROBS_TOP = 1, DISTILL = 2 };
 
+template <int DT>
+__device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t) {
+  return static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
+}
+
+// A row from the sixteen-byte boundary at or in front of it: place `begin` is its column 0, what lies in front is not touched.  Loads that do not begin at such
+// boundaries take a quarter longer (4096 x 130001 bf16 222 us, x 130000 180).
+struct Placed {
+  const void* base;
+  int begin;
+};
+template <int DT>
+__device__ __forceinline__ Placed placed(const void* row) {
+  const int begin = (int)(reinterpret_cast<uintptr_t>(row) & 15) / RowType<DT>::BYTES;
+  return {static_cast<const char*>(row) - begin * RowType<DT>::BYTES, begin};
+}
+
 // ---- a row by a workgroup of THREADS lanes: four waves, or one for short rows, of which the chip then holds four times as many ----------
 template <int THREADS>
 struct Workgroup {
@@ -114,22 +131,22 @@ struct Workgroup {
     return r;
   }
 
-  // Columns [c0, c1) of a row; `keys` takes the order numbers of the groups' largest logits (group = column / GROUP; c0 is a multiple
-  // of GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
-  template <int DT, bool ENTROPY, bool TOP, int U>
-  static __device__ __forceinline__ Softmax stream(const void* row, int c0, int c1, float c2, uint32_t* keys) {
+  // Places [c0, c1) of a row from `begin` on; `keys` takes the order numbers of the groups' largest logits (group = place / GROUP; c0 is a multiple of
+  // GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
+  template <int DT, bool ENTROPY, bool TOP, int U, bool ONCE>
+  static __device__ __forceinline__ Softmax stream(const void* row, int begin, int c0, int c1, float c2, uint32_t* keys) {
     typedef RowType<DT> R;
     constexpr int VE = R::VE, STEP = THREADS * VE * U;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 64 * VE;
     Softmax r = {NEG_INF, 0.f, 0.f};
     const auto fetch = [&](row_u32x4 (&raw)[U], int base) {
       const int at = base + (int)threadIdx.x * VE;
-      if (base + STEP <= c1) {
+      if (base >= begin && base + STEP <= c1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = R::load_vec(row, at + u * THREADS * VE);
+        for (int u = 0; u < U; ++u) raw[u] = ONCE ? R::load_vec_once(row, at + u * THREADS * VE) : R::load_vec(row, at + u * THREADS * VE);
       } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = R::load_vec_to(row, at + u * THREADS * VE, c1, R::NEG_INF_BITS);
+        for (int u = 0; u < U; ++u) raw[u] = R::load_vec_in(row, at + u * THREADS * VE, begin, c1, R::NEG_INF_BITS);
       }
     };
     row_u32x4 next[U];
@@ -269,12 +286,12 @@ struct Workgroup {
     return from ? from : 1u;
   }
 
-  // Leaves at least the k largest of a row in lds.found, in any order, and returns how many; from the groups' numbers.
+  // Leaves at least the k largest of places [begin, end) of a row in lds.found, in any order, and returns how many; from the groups' numbers.
   template <int DT>
-  static __device__ __forceinline__ int top_of_row(const void* row, int V, int k, const uint32_t* group_keys, SelectLds& lds) {
+  static __device__ __forceinline__ int top_of_row(const void* row, int begin, int end, int k, const uint32_t* group_keys, SelectLds& lds) {
     typedef RowType<DT> R;
     constexpr int VE = R::VE, BITS = Key<DT>::BITS, OWN = 8;
-    const int groups = (V + GROUP - 1) / GROUP;
+    const int groups = (end + GROUP - 1) / GROUP;
     if (threadIdx.x == 0) lds.n_groups = lds.n_found = 0;
     uint32_t most = 0, own[OWN];  // (the first OWN of a thread's stay in registers)
 #pragma unroll
@@ -285,8 +302,8 @@ struct Workgroup {
     }
     for (int g = OWN * THREADS + (int)threadIdx.x; g < groups; g += THREADS) most = group_keys[g] > most ? group_keys[g] : most;
     if (groups < k)  // a row so short that the threads' elements tell more
-      for (int v = threadIdx.x * VE; v < V; v += THREADS * VE) {
-        const row_u32x4 raw = R::load_vec_to(row, v, V, R::NEG_INF_BITS);
+      for (int v = (int)threadIdx.x * VE; v < end; v += THREADS * VE) {
+        const row_u32x4 raw = R::load_vec_in(row, v, begin, end, R::NEG_INF_BITS);
         uint32_t mx = 0;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -310,13 +327,13 @@ struct Workgroup {
       constexpr int PER = GROUP / VE;
       for (int v = threadIdx.x; v < n_groups * PER; v += THREADS) {
         const int at = lds.group[v / PER] * GROUP + v % PER * VE;
-        const row_u32x4 raw = R::load_vec_to(row, at, V, R::NEG_INF_BITS);
+        const row_u32x4 raw = R::load_vec_in(row, at, begin, end, R::NEG_INF_BITS);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const uint32_t one = Key<DT>::of(R::element(raw, e));
-          if (one >= from && at + e < V) {
+          if (one >= from && at + e >= begin && at + e < end) {
             const int i = atomicAdd(&lds.n_found, 1);
-            if (i < MANY) lds.found[i] = entry_of(one, at + e);
+            if (i < MANY) lds.found[i] = entry_of(one, at + e - begin);
           }
         }
       }
@@ -327,16 +344,16 @@ struct Workgroup {
     const int n = k < groups ? k : groups;
     select<BITS>(groups, n, lds, [&](int i) { return group_keys[i]; }, [&](int to, int i) { lds.group[to] = i; });
     __syncthreads();
-    const auto column = [&](int i) { return lds.group[i / GROUP] * GROUP + i % GROUP; };
-    const auto element = [&](int i) { return column(i) < V ? Key<DT>::of(R::load(row, column(i))) : 0u; };
-    select<BITS>(n * GROUP, k, lds, element, [&](int to, int i) { lds.found[to] = entry_of(element(i), column(i)); });
+    const auto place = [&](int i) { return lds.group[i / GROUP] * GROUP + i % GROUP; };
+    const auto element = [&](int i) { return place(i) >= begin && place(i) < end ? Key<DT>::of(R::load(row, place(i))) : 0u; };
+    select<BITS>(n * GROUP, k, lds, element, [&](int to, int i) { lds.found[to] = entry_of(element(i), place(i) - begin); });
     __syncthreads();
     return k;
   }
 
   // ---- what comes out of a row's statistics ---------------------------------------------------------------------
   template <int DT, bool TOP>
-  static __device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Token<DT>& token, const Softmax& r,
+  static __device__ __forceinline__ void finish_logprobs(const tk_vocab_desc& d, Scales sc, int t, Placed row, const Token<DT>& token, const Softmax& r,
                                                   const uint32_t* group_keys, SelectLds* lds) {
     const RowResult o(r);
     if (threadIdx.x == 0) {
@@ -356,7 +373,7 @@ struct Workgroup {
         }
         return;
       }
-      const int n = top_of_row<DT>(row, d.vocab, d.k, group_keys, *lds);
+      const int n = top_of_row<DT>(row.base, row.begin, row.begin + d.vocab, d.k, group_keys, *lds);
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint64_t mine = lds->found[i];
         int rank = 0;
@@ -436,7 +453,7 @@ struct Workgroup {
   template <int DT, int OP>
   using Single = std::conditional_t<OP == DISTILL, Teacher<DT>, Token<DT>>;
   template <int DT, int OP>
-  static __device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, const void* row, const Single<DT, OP>& single, const Softmax& r,
+  static __device__ __forceinline__ void finish(const tk_vocab_desc& d, Scales sc, int t, Placed row, const Single<DT, OP>& single, const Softmax& r,
                                          const uint32_t* keys, RowLds& lds) {
     if constexpr (OP == DISTILL)
       finish_distill<DT>(d, sc, t, single, r, lds.teacher);
@@ -445,22 +462,21 @@ struct Workgroup {
   }
 };
 
-template <int DT>
-__device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t) {
-  return static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
-}
-
 // A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
 template <int DT, int OP, int THREADS, int U>
-__global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0) {
+__global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0, int keep_from) {
   typedef Workgroup<THREADS> W;
   extern __shared__ uint32_t keys[];
   __shared__ typename W::RowLds lds;
   const int t = t0 + (int)blockIdx.x;
   const void* row = logits_row<DT>(d, t);
   const typename W::template Single<DT, OP> single(d, t, row);
-  const Softmax r = W::block_softmax(W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U>(row, 0, d.vocab, sc.c2, keys), sc.c2, lds.softmax);
-  W::template finish<DT, OP>(d, sc, t, row, single, r, keys, lds);
+  const Placed p = THREADS == 64 ? Placed{row, 0} : placed<DT>(row);  // (a short row is over before it pays)
+  const int end = p.begin + d.vocab;
+  const Softmax mine = THREADS == 64 || t >= keep_from ? W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U, false>(p.base, p.begin, 0, end, sc.c2, keys)
+                                                       : W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U, THREADS != 64>(p.base, p.begin, 0, end, sc.c2, keys);
+  const Softmax r = W::block_softmax(mine, sc.c2, lds.softmax);
+  W::template finish<DT, OP>(d, sc, t, p, single, r, keys, lds);
 }
 
 // Few rows: pieces of a row, whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
@@ -469,9 +485,10 @@ template <int DT, int OP>
 __global__ __launch_bounds__(256) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
   __shared__ float buf[3 * Wide::WAVES];
   const int t = blockIdx.x / n_chunks, c = blockIdx.x % n_chunks, c0 = c * chunk;
-  const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
-  const Softmax r = Wide::block_softmax(
-      Wide::stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, 2>(logits_row<DT>(d, t), c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
+  const Placed p = placed<DT>(logits_row<DT>(d, t));
+  const int end = p.begin + d.vocab, c1 = end - c0 < chunk ? end : c0 + chunk;
+  const Softmax r =
+      Wide::block_softmax(Wide::stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, 2, false>(p.base, p.begin, c0, c1, sc.c2, keys + (int64_t)t * groups), sc.c2, buf);
   if (threadIdx.x < 3) parts[((int64_t)t * n_chunks + c) * 3 + threadIdx.x] = threadIdx.x == 0 ? r.m : threadIdx.x == 1 ? r.s : r.e;
 }
 
@@ -487,8 +504,17 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(tk_vocab_desc d, Scales
     r = {p[0], p[1], p[2]};
   }
   r = Wide::block_softmax(r, sc.c2, lds.softmax);
-  Wide::finish<DT, OP>(d, sc, t, row, single, r, keys + (int64_t)t * groups, lds);
+  Wide::finish<DT, OP>(d, sc, t, placed<DT>(row), single, r, keys + (int64_t)t * groups, lds);
 }
+
+// Gradients from this size on are read and written with the read-once hint: they would only push the logits, which come from the last-level cache in part, out
+// of it (forward and backward, us without and with: 2048 x 32000 fp32, 262 MB, 159, 129; 4096 x 131072 bf16, 1074 MB, 604, 590; 1000 x 50001 fp16,
+// 100 MB, 79, 74.5; 200 x 32000 bf16, 13 MB, 18, 18, where whoever reads the gradient next may find it cached).
+constexpr int64_t ONCE_BYTES = 64 << 20;
+// The forward pass reads its logits with the hint, too (nothing follows it: 4096 x 131072 bf16 189, 165, 2048 x 32000 fp32 48.6, 42.6), but where a backward pass is to follow,
+// the last rows without: that many bytes are still cached when it begins with them (forward and backward, all rows hinted, none, the last 192 MB not:
+// 2048 x 32000 fp32 143, 129, 127; 2048 x 64000 281, 270, 263; 4096 x 96000 bf16 422, 416, 400; 4096 x 131072 542, 586, 548; 8192 x 100000 978, 924, 960).
+constexpr int64_t KEPT_BYTES = 192 << 20;
 
 // Pieces that the rows of a call are split into: about four workgroups a CU; no more, since a second launch joins them (us, pieces for 500, 1000
 // and 2048 workgroups: 1000 x 131072 bf16 with 20 alternatives 61, 61, 76; 300 x 131072 22.9, 22.5, 23.4; 100 x 131072 13.4, 12.6, 11.8; 61 x 50001
@@ -497,8 +523,10 @@ struct Split {
   int n, chunk, groups;
   int64_t parts_bytes, bytes;
 };
-Split split_of(int32_t n_rows, int32_t vocab, int32_t k) {
+// `shift`: columns that the rows' addresses may add in front.
+Split split_of(int32_t n_rows, int64_t vocab, int32_t k, int shift) {
   Split s;
+  vocab += shift;
   const int64_t want = cdiv(1000, n_rows > 0 ? n_rows : 1), most = cdiv(vocab, LEAST_CHUNK);
   int64_t n = want < most ? want : most;
   n = n < MAX_CHUNKS ? n : MAX_CHUNKS;
@@ -521,7 +549,8 @@ constexpr int SHORT_ROW = 2048, SHORT_TOP = 8192;
 
 template <int DT, int OP>
 int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
-  const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0);
+  const bool aligned = ((reinterpret_cast<uintptr_t>(d->logits) | (uintptr_t)(d->logits_stride_m * RowType<DT>::BYTES)) & 15) == 0;
+  const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0, aligned ? 0 : RowType<DT>::VE - 1);
   const Scales sc = scales_of(d);
   if (s.n == 1) {
     // Four vectors a lane under way, or two: two waste less of a row's last step and start sooner, four carry long rows when the chip is full of them.
@@ -531,9 +560,11 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
     const bool wave = d->n_rows >= 1000 && (OP == LOGPROBS_TOP ? d->k <= 32 && d->vocab <= SHORT_TOP : d->vocab <= SHORT_ROW)
                       && (OP != DISTILL || d->n_teacher <= 64 * Workgroup<64>::ENTRIES);
     auto f = wave ? vocab_rows_kernel<DT, OP, 64, 2> : d->n_rows >= 2048 && d->vocab >= 6 * STEP ? vocab_rows_kernel<DT, OP, 256, 4> : vocab_rows_kernel<DT, OP, 256, 2>;
+    const int64_t row_bytes = (int64_t)d->vocab * RowType<DT>::BYTES, kept = d->stats ? KEPT_BYTES / row_bytes : 0;
+    const int keep_from = d->n_rows * row_bytes < ONCE_BYTES ? 0 : (int)(d->n_rows > kept ? d->n_rows - kept : 0);
     for (int64_t t = 0; t < d->n_rows; t += MAX_GRID) {
       const int rows = (int)(d->n_rows - t < MAX_GRID ? d->n_rows - t : MAX_GRID);
-      hipLaunchKernelGGL(f, dim3(rows), dim3(wave ? 64 : 256), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t);
+      hipLaunchKernelGGL(f, dim3(rows), dim3(wave ? 64 : 256), OP == LOGPROBS_TOP ? s.groups * 4 : 0, stream, *d, sc, (int)t, keep_from);
     }
     return check_launch(who);
   }
@@ -552,10 +583,6 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
 // The teacher's few columns are written once more at the end, by the piece that they lie in: looking each column up while the row streams by
 // cost as much as the row where a wave's columns hold some of them (2000 x 1500 fp16 with 50 entries 31 us).
 constexpr int GRAD_CHUNK = 16384;
-// Gradients from this size on are read and written with the read-once hint: they would only push the logits, which come from the last-level cache in part, out
-// of it (forward and backward, us without and with: 2048 x 32000 fp32, 262 MB, 159, 129; 4096 x 131072 bf16, 1074 MB, 604, 590; 1000 x 50001 fp16,
-// 100 MB, 79, 74.5; 200 x 32000 bf16, 13 MB, 18, 18, where whoever reads the gradient next may find it cached).
-constexpr int64_t ONCE_BYTES = 64 << 20;
 
 template <int DT, int OP, int THREADS, bool ONCE>
 __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d, Scales sc, int t0, int n_chunks, int chunk) {
@@ -563,9 +590,10 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
   constexpr int VE = R::VE, U = 2, STEP = THREADS * VE * U;
   // (from the last row back: its logits were read last and may still be in the last-level cache)
   const unsigned place = gridDim.x - 1 - blockIdx.x;
-  const int t = t0 + (int)(place / (unsigned)n_chunks), c0 = (int)(place % (unsigned)n_chunks) * chunk;
-  const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
+  const int t = t0 + (int)(place / (unsigned)n_chunks);
   const void* row = logits_row<DT>(d, t);
+  const int c0 = (int)(place % (unsigned)n_chunks) * chunk;
+  const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
   void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * R::BYTES;
   const float m = d.stats[t], log_s = d.stats[(int64_t)d.n_rows + t], log2_s = log_s * LOG2E;
   float A, B = 0.f, more = 0.f, qm = 0.f, log_qs = 0.f;
@@ -700,7 +728,15 @@ using namespace tk;
 #define TK_VOCAB_CALL(f, op, who)                                                                                                            \
   (d->logits_dtype == TK_F32 ? f<TK_F32, op> : d->logits_dtype == TK_BF16 ? f<TK_BF16, op> : f<TK_F16, op>)(d, static_cast<hipStream_t>(stream), who)
 
-extern "C" int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k) { return n_rows > 0 && vocab > 0 ? split_of(n_rows, vocab, k).bytes : 0; }
+extern "C" int64_t tk_vocab_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t k) {
+  if (n_rows <= 0 || vocab <= 0) return 0;
+  int64_t most = 0;  // (of what the logits' type and addresses may call for)
+  for (int shift : {0, 3, 7}) {
+    const int64_t n = split_of(n_rows, vocab, k, shift).bytes;
+    most = n > most ? n : most;
+  }
+  return most;
+}
 
 extern "C" int32_t tk_token_logprobs(const tk_vocab_desc* d, tk_stream_t stream) {
   if (int32_t e = check(d, "tk_token_logprobs")) return e;
