@@ -58,22 +58,13 @@ __device__ __forceinline__ void once_more(row_u32x4 (&v)[N]) {
 
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
-// TPR lanes a row, NV vectors of 16 bytes a lane, FULL of which lie within any row that comes here: the row is read once, into registers; mean, then the sum of squares around it.
+// One row's mean and reciprocal deviation from its registers (TPR lanes a row, NV vectors of 16 bytes a lane, the first FULL of them within any
+// row that comes here): the mean first, then the sum of squares around it.  `buf`: 2 x 16 floats of LDS from 256 lanes a row on.
 template <int DT, int TPR, int NV, int FULL>
-__global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x, int64_t M, int C, int64_t sx, const void* w, int wt, const void* b, int bt,
-                                                                   float eps, void* y, int64_t sy, float* mean, float* rstd, int64_t m0) {
+__device__ __forceinline__ void row_statistics(row_u32x4 (&raw)[NV], int lane, int C, float inv_c, float eps, float (*buf)[16], float* mean, float* rstd) {
   typedef RowType<DT> R;
-  constexpr int VE = R::VE, ROWS = block_of(TPR) / TPR;
-  __shared__ float buf[2][16];
-  const int lane = (int)threadIdx.x % TPR;
-  const float inv_c = 1.0f / (float)C;
-  const int64_t m = m0 + (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  if (m >= M) return;  // (lanes that share a row leave together)
-  const char* row = static_cast<const char*>(x) + m * sx * R::BYTES;
-  row_u32x4 raw[NV];
+  constexpr int VE = R::VE;
   float s = 0.f;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) raw[v] = v < FULL ? R::load_vec(row, (v * TPR + lane) * VE) : R::load_vec_to(row, (v * TPR + lane) * VE, C, 0u);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -82,29 +73,70 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x
   once_more(raw);
   s = 0.f;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const bool full = v < FULL;
+  for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const float d = R::element(raw[v], e) - mu;
-      s = fmaf(d, full || (v * TPR + lane) * VE + e < C ? d : 0.f, s);
+      s = fmaf(d, v < FULL || (v * TPR + lane) * VE + e < C ? d : 0.f, s);
     }
-  }
-  const float r = 1.0f / sqrtf(row_sum<TPR>(s, buf[1]) * inv_c + eps);
+  *mean = mu;
+  *rstd = 1.0f / sqrtf(row_sum<TPR>(s, buf[1]) * inv_c + eps);
   once_more(raw);
+}
+
+// A row's vectors, and what is to be done with them before they are used: elements behind the row's end are zero then.  (Rows shorter than a vector come element by element.)
+template <int DT, int TPR, int NV, int FULL>
+__device__ __forceinline__ void load_row(const void* x, int64_t at, int lane, int C, row_u32x4 (&raw)[NV]) {
+  typedef RowType<DT> R;
+  const void* row = static_cast<const char*>(x) + at * R::BYTES;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i = (v * TPR + lane) * R::VE;
+    raw[v] = v < FULL ? R::load_vec(row, i) : TPR == 8 && C < R::VE ? R::load_vec_to(row, i, C, 0u) : R::load_last(row, i, C);
+  }
+}
+template <int DT, int TPR, int NV, int FULL>
+__device__ __forceinline__ void place_row(int lane, int C, row_u32x4 (&raw)[NV]) {
+  typedef RowType<DT> R;
+#pragma unroll
+  for (int v = FULL; v < NV; ++v)
+    if (!(TPR == 8 && C < R::VE)) raw[v] = R::last(raw[v], (v * TPR + lane) * R::VE, C);
+}
+
+// A row a group of TPR lanes.  The weights are requested with the row, so that its latency covers theirs.
+template <int DT, int TPR, int NV, int FULL>
+__global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x, int64_t M, int C, int64_t sx, const void* w, int wt, const void* b, int bt,
+                                                                   float eps, void* y, int64_t sy, float* mean, float* rstd, int64_t m0) {
+  typedef RowType<DT> R;
+  constexpr int VE = R::VE, ROWS = block_of(TPR) / TPR;
+  __shared__ float buf[2][16];
+  const int lane = (int)threadIdx.x % TPR;
+  const int64_t m = m0 + (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (m >= M) return;  // (lanes that share a row leave together)
+  row_u32x4 raw[NV];
+  load_row<DT, TPR, NV, FULL>(x, m * sx, lane, C, raw);
+  float wv[NV][VE], bv[NV][VE], mu, r;
+  const auto weights = [&](int v) {
+    load_weights<VE>(w, wt, (v * TPR + lane) * VE, C, 1.f, wv[v]);
+    load_weights<VE>(b, bt, (v * TPR + lane) * VE, C, 0.f, bv[v]);
+  };
+  constexpr bool EARLY = NV * VE <= 16;  // (beyond that their registers cost more rows at a time than their latency: 8192 x 8192 bf16 65 us, 56)
+  if (EARLY)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) weights(v);
+  place_row<DT, TPR, NV, FULL>(lane, C, raw);
+  row_statistics<DT, TPR, NV, FULL>(raw, lane, C, 1.0f / (float)C, eps, buf, &mu, &r);
   void* out = static_cast<char*>(y) + m * sy * R::BYTES;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * TPR + lane) * VE;
-    float wv[VE], bv[VE], o[VE];
-    load_weights<VE>(w, wt, c, C, 1.f, wv);
-    load_weights<VE>(b, bt, c, C, 0.f, bv);
+    float o[VE];
+    if (!EARLY) weights(v);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) o[e] = fmaf((R::element(raw[v], e) - mu) * r, wv[e], bv[e]);
+    for (int e = 0; e < VE; ++e) o[e] = fmaf((R::element(raw[v], e) - mu) * r, wv[v][e], bv[v][e]);
     if (v < FULL)
-      R::store_vec(out, c, R::pack(o));
+      R::store_vec(out, (v * TPR + lane) * VE, R::pack(o));
     else
-      R::store_vec_to(out, c, C, R::pack(o));
+      R::store_vec_to(out, (v * TPR + lane) * VE, C, R::pack(o));
   }
   if (lane == 0 && mean) {
     mean[m] = mu;
@@ -112,18 +144,94 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x
   }
 }
 
+// Many rows: workgroups of four waves that stay, the weights read once each, into registers (up to 16 elements a lane) or LDS; a group's next
+// rows are requested before the present ones are summed.  AT rows a group at a time, so that short rows keep as many bytes under way as long ones.
+template <int DT, int TPR, int NV, int FULL>
+__global__ __launch_bounds__(256) void layer_norm_many_kernel(const void* x, int64_t M, int C, int64_t sx, const void* w, int wt, const void* b, int bt,
+                                                              float eps, void* y, int64_t sy, float* mean, float* rstd) {
+  typedef RowType<DT> R;
+  constexpr int VE = R::VE, GROUPS = 256 / TPR, AT = NV == 1 ? 2 : 1;
+  constexpr bool IN_LDS = NV * VE > 16;
+  __shared__ row_u32x4 wl[IN_LDS ? 2 : 1][IN_LDS ? NV : 1][VE / 4][IN_LDS ? TPR : 1];
+  const int lane = (int)threadIdx.x % TPR;
+  const float inv_c = 1.0f / (float)C;
+  float wv[IN_LDS ? 1 : NV][VE], bv[IN_LDS ? 1 : NV][VE];
+  if constexpr (IN_LDS) {
+    for (int i = threadIdx.x; i < 2 * NV * TPR; i += 256) {
+      const int which = i / (NV * TPR), j = i % (NV * TPR);
+      float o[VE];
+      load_weights<VE>(which ? b : w, which ? bt : wt, j * VE, C, which ? 0.f : 1.f, o);
+#pragma unroll
+      for (int q = 0; q < VE / 4; ++q)
+        wl[which][j / TPR][q][j % TPR] = row_u32x4{f32_bits(o[4 * q]), f32_bits(o[4 * q + 1]), f32_bits(o[4 * q + 2]), f32_bits(o[4 * q + 3])};
+    }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      load_weights<VE>(w, wt, (v * TPR + lane) * VE, C, 1.f, wv[v]);
+      load_weights<VE>(b, bt, (v * TPR + lane) * VE, C, 0.f, bv[v]);
+    }
+  }
+  const int64_t step = (int64_t)gridDim.x * GROUPS * AT;
+  int64_t m = ((int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR) * AT;
+  if (m >= M) return;  // (lanes that share a row leave together)
+  row_u32x4 next[AT][NV];
+#pragma unroll
+  for (int i = 0; i < AT; ++i) load_row<DT, TPR, NV, FULL>(x, (m + i < M ? m + i : M - 1) * sx, lane, C, next[i]);
+  for (; m < M; m += step) {
+    row_u32x4 raw[AT][NV];
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) raw[i][v] = next[i][v];
+      if (m + step < M) load_row<DT, TPR, NV, FULL>(x, (m + step + i < M ? m + step + i : M - 1) * sx, lane, C, next[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (the requests first)
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      float mu, r;
+      place_row<DT, TPR, NV, FULL>(lane, C, raw[i]);
+      row_statistics<DT, TPR, NV, FULL>(raw[i], lane, C, inv_c, eps, nullptr, &mu, &r);
+      if (m + i >= M) break;
+      void* out = static_cast<char*>(y) + (m + i) * sy * R::BYTES;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float o[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float we = IN_LDS ? bits_f32(wl[0][IN_LDS ? v : 0][e / 4][IN_LDS ? lane : 0][e % 4]) : wv[IN_LDS ? 0 : v][e];
+          const float be = IN_LDS ? bits_f32(wl[IN_LDS ? 1 : 0][IN_LDS ? v : 0][e / 4][IN_LDS ? lane : 0][e % 4]) : bv[IN_LDS ? 0 : v][e];
+          o[e] = fmaf((R::element(raw[i][v], e) - mu) * r, we, be);
+        }
+        if (v < FULL)
+          R::store_vec(out, (v * TPR + lane) * VE, R::pack(o));
+        else
+          R::store_vec_to(out, (v * TPR + lane) * VE, C, R::pack(o));
+        if (IN_LDS) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (lane == 0 && mean) {
+        mean[m + i] = mu;
+        rstd[m + i] = r;
+      }
+    }
+  }
+}
+
 // The gradients.  Workgroups stay for many rows: a lane's columns are the same in each of them, so that their sums over rows stay in
 // registers (`SUMS`), are joined over the workgroup's rows in LDS, and leave as one row of partial sums a workgroup (parts [2][gridDim.x][C]),
 // which layer_norm_sums_kernel adds in their order.  The weight lies in LDS in 32 bits, in the order in which lanes take it.
-template <int DT, int TPR, int NV, int FULL, bool SUMS>
-__global__ __launch_bounds__(block_of(TPR)) void layer_norm_backward_kernel(const void* dy, int64_t sdy, const void* x, int64_t M, int C, int64_t sx,
-                                                                            const void* w, int wt, const float* mean, const float* rstd, void* dx,
-                                                                            int64_t sdx, float* parts) {
+template <int DT, int TPR, int NV, int FULL, int BLOCK, bool SUMS>
+__global__ __launch_bounds__(BLOCK) void layer_norm_backward_kernel(const void* dy, int64_t sdy, const void* x, int64_t M, int C, int64_t sx, const void* w,
+                                                                    int wt, const float* mean, const float* rstd, void* dx, int64_t sdx, float* parts) {
   typedef RowType<DT> R;
-  constexpr int VE = R::VE, BLOCK = block_of(TPR), ROWS = BLOCK / TPR, WIDTH = NV * TPR * VE;
+  constexpr int VE = R::VE, ROWS = BLOCK / TPR, WIDTH = NV * TPR * VE, WPR = TPR / 64;
+  // The next row is requested before the present one is summed, where there are registers for both (us without and with: 16384 x 2880 bf16 76.8, 65.6,
+  // x 4096 98.7, 92.4, 135168 x 128 31.7, 29.8).
+  constexpr bool AHEAD = NV * VE <= 32;
   __shared__ float buf[2][2][16];
   __shared__ row_u32x4 wl[NV][VE / 4][TPR];
-  const int lane = (int)threadIdx.x % TPR;
+  const int lane = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
   const float inv_c = 1.0f / (float)C;
   for (int i = threadIdx.x; i < NV * TPR; i += BLOCK) {
     float o[VE];
@@ -138,18 +246,42 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_backward_kernel(cons
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int e = 0; e < VE; ++e) dw[v][e] = db[v][e] = 0.f;
+  row_u32x4 xn[AHEAD ? NV : 1], gn[AHEAD ? NV : 1];
+  float mu_n = 0.f, r_n = 0.f;
+  // (groups of a workgroup go through the loop together: those without a row take the last one and count it as nothing)
+  const auto fetch = [&](int64_t m, row_u32x4* xv, row_u32x4* gv, float* mu, float* r) {
+    const int64_t at = m < M ? m : M - 1;
+    row_u32x4(&xa)[NV] = *reinterpret_cast<row_u32x4(*)[NV]>(xv);
+    row_u32x4(&ga)[NV] = *reinterpret_cast<row_u32x4(*)[NV]>(gv);
+    load_row<DT, TPR, NV, FULL>(x, at * sx, lane, C, xa);
+    load_row<DT, TPR, NV, FULL>(dy, at * sdy, lane, C, ga);
+    *mu = mean[at];
+    *r = rstd[at];
+  };
+  const int64_t first = (int64_t)blockIdx.x * ROWS + group, step = (int64_t)gridDim.x * ROWS;
+  if constexpr (AHEAD) fetch(first, xn, gn, &mu_n, &r_n);
   int turn = 0;
-  for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; m < M; m += (int64_t)gridDim.x * ROWS, turn ^= 1) {
-    const char *xr = static_cast<const char*>(x) + m * sx * R::BYTES, *gr = static_cast<const char*>(dy) + m * sdy * R::BYTES;
+  for (int64_t m = first; m - group < M; m += step, turn ^= 1) {
     row_u32x4 xv[NV], gv[NV];
+    float mu, r;
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * TPR + lane) * VE;
-      const bool full = v < FULL;
-      xv[v] = full ? R::load_vec(xr, c) : R::load_vec_to(xr, c, C, 0u);
-      gv[v] = full ? R::load_vec(gr, c) : R::load_vec_to(gr, c, C, 0u);
+      for (int v = 0; v < NV; ++v) {
+        xv[v] = xn[v];
+        gv[v] = gn[v];
+      }
+      mu = mu_n;
+      r = r_n;
+      if (m - group + step < M) fetch(m + step, xn, gn, &mu_n, &r_n);
+      __builtin_amdgcn_sched_barrier(0);  // (the requests first)
+    } else {
+      fetch(m, xv, gv, &mu, &r);
     }
-    const float mu = mean[m], r = rstd[m];
+    place_row<DT, TPR, NV, FULL>(lane, C, xv);
+    place_row<DT, TPR, NV, FULL>(lane, C, gv);
+    if (m >= M)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) gv[v] = row_u32x4{0, 0, 0, 0};
     float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -167,7 +299,7 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_backward_kernel(cons
       }
       __builtin_amdgcn_sched_barrier(0);  // (a vector after the other: all of them at once would not fit the registers)
     }
-    if constexpr (TPR >= 256) {
+    if constexpr (TPR > 64) {
       sg = wave_sum_f32(sg);
       sgh = wave_sum_f32(sgh);
       if ((threadIdx.x & 63) == 0) {
@@ -177,15 +309,15 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_backward_kernel(cons
       __syncthreads();
       sg = sgh = 0.f;
 #pragma unroll
-      for (int i = 0; i < TPR / 64; ++i) {
-        sg += buf[turn][0][i];
-        sgh += buf[turn][1][i];
+      for (int i = 0; i < WPR; ++i) {
+        sg += buf[turn][0][group * WPR + i];
+        sgh += buf[turn][1][group * WPR + i];
       }
     } else {
       sg = row_sum<TPR>(sg, nullptr);
       sgh = row_sum<TPR>(sgh, nullptr);
     }
-    if (!dx) continue;
+    if (!dx || m >= M) continue;
     once_more(xv);
     once_more(gv);
     asm volatile("" ::: "memory");  // (the weight comes from LDS once more, too)
@@ -244,28 +376,34 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_backward_kernel(cons
   }
 }
 
-// The partial sums' sums: 32 columns a workgroup, eight lanes a row of 128 bytes, 32 rows at a time; then the rows' sums in their order.
+// The partial sums' sums: 16 columns a workgroup, four lanes a row of 64 bytes, 64 rows at a time and eight such requested together; then over the lanes and
+// waves that hold the same columns.
 __global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts, int n, int C, void* dw, int wt, void* db, int bt) {
-  __shared__ float acc[32][33];
-  const int c = (int)blockIdx.x * 32 + (int)(threadIdx.x & 7) * 4;
+  __shared__ float acc[4][16];
+  const int c = (int)blockIdx.x * 16 + (int)(threadIdx.x & 3) * 4;
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   const float* p = parts + (int64_t)blockIdx.y * n * C;
-  for (int i = threadIdx.x >> 3; i < n; i += 32) {
-    const row_u32x4 v = RowType<TK_F32>::load_vec_to(p + (int64_t)i * C, c, C, 0u);
+  for (int i0 = threadIdx.x >> 2; i0 < n; i0 += 512) {
+    row_u32x4 v[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += bits_f32(v[e]);
+    for (int u = 0; u < 8; ++u) v[u] = i0 + u * 64 < n ? RowType<TK_F32>::load_vec_to(p + (int64_t)(i0 + u * 64) * C, c, C, 0u) : row_u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += bits_f32(v[u][e]);
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[threadIdx.x >> 3][(threadIdx.x & 7) * 4 + e] = s[e];
+  for (int d = 4; d < 64; d *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], d);
+  if ((threadIdx.x & 63) < 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[threadIdx.x >> 6][(threadIdx.x & 3) * 4 + e] = s[e];
   __syncthreads();
-  if (threadIdx.x < 32 && (int)blockIdx.x * 32 + (int)threadIdx.x < C) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t += acc[i][threadIdx.x];
-    store_any(out, blockIdx.y ? bt : wt, (int)blockIdx.x * 32 + threadIdx.x, t);
-  }
+  if (threadIdx.x < 16 && (int)blockIdx.x * 16 + (int)threadIdx.x < C)
+    store_any(out, blockIdx.y ? bt : wt, (int)blockIdx.x * 16 + threadIdx.x, (acc[0][threadIdx.x] + acc[1][threadIdx.x]) + (acc[2][threadIdx.x] + acc[3][threadIdx.x]));
 }
 
 // ---- rows of any length: read once for each step ----------------------------------------------------------------
@@ -333,7 +471,14 @@ __global__ __launch_bounds__(256) void layer_norm_parts_long_kernel(const void* 
 }
 
 constexpr int64_t MAX_COLS = 1 << 30;
-constexpr int MAX_PARTS = 512;  // rows of partial sums: two workgroups a CU
+// Lanes a workgroup of the backward pass, and the most workgroups, each of which leaves a row of partial sums: eight waves a CU carry long rows, short ones want more
+// (us at 256, 512, 768, 1024 workgroups: 65000 x 500 bf16 86, 59, 49, 50; 135168 x 128 43, 32, 29, 30; 32768 x 1024 64, 48, 49, 50; rows shared by two waves,
+// workgroups of eight: 16384 x 4096 85, 94, 104, 113).
+constexpr int backward_block(int tpr) { return tpr == 128 ? 512 : block_of(tpr); }
+constexpr int backward_parts(int tpr, int nv) { return nv == 1 ? 768 : tpr == 128 ? 256 : 512; }
+// Rows from this many on go through workgroups that stay; fewer have a workgroup each (16 x 2880 bf16 4.0 us, by waves 6.4; 1024 x 2880 6.7, 9.4; 4096 x 2880 14.4, by workgroups 17.9).
+constexpr int64_t MANY_ROWS = 2048;
+constexpr int64_t STAYING = 2048;  // such workgroups, at most (16384 x 4096 bf16 with 1024, 2048, 4096: 53.6, 54.5, 51.2 us; 65000 x 500 fp16 42.0, 35.5, 36.0)
 unsigned rows_grid(int64_t rows) { return (unsigned)(rows < 1 << 20 ? rows : 1 << 20); }
 
 struct Forward {
@@ -350,10 +495,20 @@ struct Forward {
   hipStream_t s;
   template <int DT, int TPR, int NV, int FULL>
   void run() const {
-    constexpr int64_t rows = block_of(TPR) / TPR, most = 1 << 21;  // (workgroups of a launch: 2^32 threads are its limit)
-    for (int64_t m0 = 0; m0 < M; m0 += most * rows)
-      hipLaunchKernelGGL((layer_norm_kernel<DT, TPR, NV, FULL>), dim3((unsigned)(cdiv(M - m0, rows) < most ? cdiv(M - m0, rows) : most)), dim3(block_of(TPR)), 0, s, x, M,
-                         (int)C, sx, w, wt, b, bt, eps, y, sy, mean, rstd, m0);
+    if constexpr (TPR <= 64) {
+      if (NV > 1 || M >= MANY_ROWS) {
+        const int64_t wgs = cdiv(M, 256 / TPR * (NV == 1 ? 2 : 1));
+        hipLaunchKernelGGL((layer_norm_many_kernel<DT, TPR, NV, FULL>), dim3((unsigned)(wgs < STAYING ? wgs : STAYING)), dim3(256), 0, s, x, M, (int)C, sx, w, wt, b, bt, eps,
+                           y, sy, mean, rstd);
+        return;
+      }
+    }
+    if constexpr (TPR > 64 || NV == 1) {
+      constexpr int64_t rows = block_of(TPR) / TPR, most = 1 << 21;  // (workgroups of a launch: 2^32 threads are its limit)
+      for (int64_t m0 = 0; m0 < M; m0 += most * rows)
+        hipLaunchKernelGGL((layer_norm_kernel<DT, TPR, NV, FULL>), dim3((unsigned)(cdiv(M - m0, rows) < most ? cdiv(M - m0, rows) : most)), dim3(block_of(TPR)), 0, s, x,
+                           M, (int)C, sx, w, wt, b, bt, eps, y, sy, mean, rstd, m0);
+    }
   }
 };
 
@@ -373,25 +528,26 @@ struct Backward {
   hipStream_t s;
   template <int DT, int TPR, int NV, int FULL>
   void run() const {
-    const int64_t wgs = cdiv(M, block_of(TPR) / TPR);
+    constexpr int BLOCK = backward_block(TPR), PARTS = backward_parts(TPR, NV);
+    const int64_t wgs = cdiv(M, BLOCK / TPR);
     const bool sums = dw || db;
-    const int n = (int)(sums ? (wgs < MAX_PARTS ? wgs : MAX_PARTS) : wgs < 2048 ? wgs : 2048);
+    const int n = (int)(sums ? (wgs < PARTS ? wgs : PARTS) : wgs < 2048 ? wgs : 2048);
     if (n && sums)
-      hipLaunchKernelGGL((layer_norm_backward_kernel<DT, TPR, NV, FULL, true>), dim3(n), dim3(block_of(TPR)), 0, s, dy, sdy, x, M, (int)C, sx, w, wt, mean, rstd, dx,
+      hipLaunchKernelGGL((layer_norm_backward_kernel<DT, TPR, NV, FULL, BLOCK, true>), dim3(n), dim3(BLOCK), 0, s, dy, sdy, x, M, (int)C, sx, w, wt, mean, rstd, dx,
                          sdx, parts);
     else if (n)
-      hipLaunchKernelGGL((layer_norm_backward_kernel<DT, TPR, NV, FULL, false>), dim3(n), dim3(block_of(TPR)), 0, s, dy, sdy, x, M, (int)C, sx, w, wt, mean, rstd, dx,
+      hipLaunchKernelGGL((layer_norm_backward_kernel<DT, TPR, NV, FULL, BLOCK, false>), dim3(n), dim3(BLOCK), 0, s, dy, sdy, x, M, (int)C, sx, w, wt, mean, rstd, dx,
                          sdx, nullptr);
     if (sums) join(n);
   }
   void join(int n) const {
-    hipLaunchKernelGGL(layer_norm_sums_kernel, dim3((unsigned)cdiv(C, 32), 2), dim3(256), 0, s, parts, n, (int)C, dw, wt, db, bt);
+    hipLaunchKernelGGL(layer_norm_sums_kernel, dim3((unsigned)cdiv(C, 16), 2), dim3(256), 0, s, parts, n, (int)C, dw, wt, db, bt);
   }
 };
 
-// Lanes a row and vectors a lane for rows of C columns: part of a wave up to 32 vectors, a wave up to 64 elements a lane, then a workgroup
-// of 256 up to 32 and one of 1024 up to 16 a lane.  False: longer ones.
-template <int DT, class Op>
+// Lanes a row, vectors a lane and how many of these are full for rows of C columns: part of a wave up to 32 vectors, a wave up to 32 elements a lane (forward 64),
+// two waves up to 32 (backward, whose sums take two registers an element), then a workgroup of 256 up to 32 and one of 1024 up to 16.  False: longer ones.
+template <int DT, bool BACKWARD, class Op>
 bool by_length(const Op& op, int64_t C) {
   constexpr int VE = RowType<DT>::VE;
   const int64_t vecs = cdiv(C, VE);
@@ -400,9 +556,19 @@ bool by_length(const Op& op, int64_t C) {
     op.template run<DT, tpr, nv, full>(); \
     return true;                           \
   }
-  TK_LN(8, 1, 0) TK_LN(16, 1, 0) TK_LN(32, 1, 0) TK_LN(64, 1, 0) TK_LN(64, 2, 1) TK_LN(64, 3, 2) TK_LN(64, 4, 3) TK_LN(64, 6, 4) TK_LN(64, 8, 6)
+  TK_LN(8, 1, 0) TK_LN(16, 1, 0) TK_LN(32, 1, 0) TK_LN(64, 1, 0) TK_LN(64, 2, 1) TK_LN(64, 3, 2) TK_LN(64, 4, 3)
+  if constexpr (BACKWARD && DT != TK_F32) {
+    TK_LN(128, 3, 2) TK_LN(128, 4, 3)
+  } else {
+    TK_LN(64, 6, 4) TK_LN(64, 8, 6)
+  }
+  if constexpr (BACKWARD && DT == TK_F32) {
+    TK_LN(128, 6, 4) TK_LN(128, 8, 6)
+  } else if constexpr (DT == TK_F32) {
+    TK_LN(64, 12, 8) TK_LN(64, 16, 12)
+  }
   if constexpr (DT == TK_F32) {
-    TK_LN(64, 12, 8) TK_LN(64, 16, 12) TK_LN(256, 8, 4) TK_LN(1024, 4, 2)
+    TK_LN(256, 8, 4) TK_LN(1024, 4, 2)
   } else {
     TK_LN(256, 4, 2) TK_LN(1024, 2, 1)
   }
@@ -412,13 +578,23 @@ bool by_length(const Op& op, int64_t C) {
 
 template <int DT>
 void forward(const Forward& f) {
-  if (!by_length<DT>(f, f.C))
+  const int64_t vecs = cdiv(f.C, RowType<DT>::VE);
+  if (f.M < MANY_ROWS && vecs > 64 && vecs <= 1024) {  // few rows: a workgroup a row
+    if (vecs <= 256)
+      f.run<DT, 256, 1, 0>();
+    else if (vecs <= 512)
+      f.run<DT, 256, 2, 1>();
+    else
+      f.run<DT, 256, 4, 2>();
+    return;
+  }
+  if (!by_length<DT, false>(f, f.C))
     hipLaunchKernelGGL(layer_norm_long_kernel<DT>, dim3(rows_grid(f.M)), dim3(256), 0, f.s, f.x, f.M, f.C, f.sx, f.w, f.wt, f.b, f.bt, f.eps, f.y, f.sy, f.mean, f.rstd);
 }
 
 template <int DT>
 void backward(const Backward& b) {
-  if (by_length<DT>(b, b.C)) return;
+  if (by_length<DT, true>(b, b.C)) return;
   if (b.dx && b.M)
     hipLaunchKernelGGL(layer_norm_dx_long_kernel<DT>, dim3(rows_grid(b.M)), dim3(256), 0, b.s, b.dy, b.sdy, b.x, b.M, b.C, b.sx, b.w, b.wt, b.mean, b.rstd, b.dx, b.sdx);
   if (!b.dw && !b.db) return;
@@ -449,7 +625,8 @@ extern "C" int32_t tk_layer_norm(const void* x, int32_t dtype, int64_t n_rows, i
 }
 
 extern "C" int64_t tk_layer_norm_backward_workspace_bytes(int64_t n_rows, int64_t n_cols) {
-  return n_rows > 0 && n_cols > 0 ? 2 * (n_rows < MAX_PARTS ? n_rows : MAX_PARTS) * n_cols * 4 : 0;
+  const int64_t parts = n_cols <= 512 ? 768 : 512;  // (a bound for each type)
+  return n_rows > 0 && n_cols > 0 ? 2 * (n_rows < parts ? n_rows : parts) * n_cols * 4 : 0;
 }
 
 extern "C" int32_t tk_layer_norm_backward(const void* dy, int64_t stride_dym, const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols,

@@ -69,6 +69,21 @@ struct RowType {
     return v;
   }
   static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int i, int end, uint32_t fill) { return load_vec_in(p, i, i, end, fill); }
+  // A row's last vectors without a branch, for rows of at least VE elements: load_last() takes the sixteen bytes that end with the row where those from i on pass its end,
+  // and last() moves them to their places, with zeros behind.  The move may wait until the vector is used.
+  static __device__ __forceinline__ row_u32x4 load_last(const void* p, int i, int end) { return load_vec(p, i < end - VE ? i : end - VE); }
+  static __device__ __forceinline__ row_u32x4 last(row_u32x4 v, int i, int end) {
+    const int n = left(i, end), drop = n >= VE ? 0 : n <= 0 ? 128 : (VE - n) * (8 * BYTES);
+    uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+    const bool half = drop >= 64;
+    const int s = drop & 63;
+    lo = half ? hi : lo;
+    hi = half ? 0 : hi;
+    const uint64_t carry = s ? hi << (64 - s) : 0;
+    lo = drop >= 128 ? 0 : lo >> s | carry;
+    hi = hi >> s;
+    return row_u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
   static __device__ __forceinline__ float element(row_u32x4 v, int e) {
     if constexpr (DT == TK_F32) return bits_f32(v[e]);
     if constexpr (DT == TK_BF16) return bits_f32(e & 1 ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
