@@ -64,7 +64,8 @@ def test_weight_and_bias_of_other_types_or_alone(dtype):
     _check(x, None, b.to(BF16), dy)
 
 
-@pytest.mark.parametrize("M,C", [(4099, 256), (4099, 40), (1031, 2880), (6000, 1023)])
+@pytest.mark.parametrize("M,C", [(4099, 256), (4099, 40), (1031, 2880), (6000, 1023), (2050, 7), (3001, 3), (2048, 512), (2047, 513), (2500, 1537), (2100, 2050), (2049, 4096),
+                                 (2200, 4100), (9001, 130), (2051, 8)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_many_rows(M, C, dtype):
     _check(*_make(M, C, dtype, F32))
@@ -146,6 +147,14 @@ def test_autograd_gives_the_same_and_only_what_is_asked(native, monkeypatch):
                 assert torch.equal(t.grad, want[i]), (mask, i)
             else:
                 assert t.grad is None
+    for weight, bias in ((None, None), (w, None), (None, b)):  # parameters that there are not
+        leaves = [t if t is None else t.clone().requires_grad_() for t in (x, weight, bias)]
+        y = layer_norm(*leaves)
+        y.backward(dy)
+        f = layer_norm_forward(x, weight, bias)
+        assert torch.equal(y, f[0])
+        for t, g in zip(leaves, layer_norm_backward(dy, x, f[1], f[2], weight, bias)):
+            assert t is None and g is None or torch.equal(t.grad, g)
     leaf = x.clone().requires_grad_()
     g, = torch.autograd.grad(layer_norm(leaf, w, b).sum(), leaf)
     assert torch.equal(g, layer_norm_backward(torch.ones_like(x), x, mean, rstd, w, b)[0])

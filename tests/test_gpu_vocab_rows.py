@@ -361,6 +361,85 @@ def test_in_graphs_that_are_replayed_in_turn(T, V):
                 assert torch.equal(x, y)
 
 
+def test_training_steps_in_a_graph():
+    """Forward and backward passes through autograd, captured together and replayed with other inputs between eager steps."""
+    T, V, K = 60, 3001, 20
+    z, tokens, a, b = _logits(T, V, BF16)
+    q, at = _teacher(z, K)
+    leaf = z.clone().requires_grad_()
+
+    def step(leaf):
+        r = token_logprobs(leaf, tokens, 5)
+        g1, = torch.autograd.grad((r.logprobs, r.entropy), leaf, (a, b))
+        loss = distill_topk(leaf, q, at, temperature=2.0)
+        g2, = torch.autograd.grad(loss, leaf, a)
+        y = layer_norm(leaf)
+        g3, = torch.autograd.grad(y, leaf, g2)
+        return r.logprobs.detach(), r.entropy.detach(), r.top_indx, g1, loss.detach(), g2, y.detach(), g3
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(leaf)
+    for seed in (3, 4, 5):
+        new = _logits(T, V, BF16, seed=seed)[0]
+        with torch.no_grad():
+            leaf.copy_(new)
+        graph.replay()
+        want = step(new.clone().requires_grad_())
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
+
+
+def test_calls_from_several_threads():
+    import threading
+    sets, want, got = [], [], [None] * 4
+    for i in range(4):
+        z, tokens, a, b = _logits(30 + i, 4000 + 111 * i, F16, seed=i)
+        sets.append((z, tokens, *_teacher(z, 30), a, b))
+        want.append(_everything(*sets[i]))
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = _everything(*sets[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i, )) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        for x, y in zip(got[i], want[i]):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_many_short_rows(dtype):
+    """Rows that have a wave each: with few and many alternatives, ties, masks, rows that are no distribution, more teacher entries than a wave holds."""
+    for T, V in ((1000, 1), (1100, 37), (1003, 1000), (1500, 2047), (1024, 2049), (1000, 8192)):
+        z, tokens, a, b = _logits(T, V, dtype)
+        z[3] = -INF
+        z[4, V // 2] = float("nan")
+        z[5] = 2.0
+        z[6, : V // 2] = -INF
+        z[7] = torch.finfo(dtype).min
+        tokens[8] = -1
+        for k in {min(V, 1), min(V, 32), min(V, 33), min(V, 128)}:
+            _check_logprobs(z, tokens, k, 1.0, (a, b) if k == min(V, 32) else None)
+        _check_logprobs(z, tokens, 0, 0.5, (a, b))
+        for K in {min(V, 5), min(V, 256), min(V, 300)}:
+            _check_distill(z, *_teacher(z, K, dtype=F32), 1.0, a)
+
+
 def test_rows_beyond_32_bit_offsets():
     T, V = 40000, 60000  # 4.8 GB
     z = torch.zeros((T, V), dtype=BF16, device="cuda")

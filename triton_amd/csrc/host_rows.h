@@ -72,7 +72,8 @@ variable_list layer_norm_forward(const Tensor& x, const Tensor& w, const Tensor&
 }
 
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, int64_t stream) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps, int64_t stream) {
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
     variable_list out = layer_norm_forward(x, w, b, eps, reinterpret_cast<void*>(stream), true);
     ctx->save_for_backward({x, w, b, out[1]});
     return out[0];
@@ -118,7 +119,8 @@ PyObject* run_layer_norm(PyObject* const* v) {
   if (!stream) return none();
   const Tensor no, &wt = w ? *w : no, &bt = b ? *b : no;
   if (wants_grad(*x) || (w && wants_grad(*w)) || (b && wants_grad(*b)))
-    return THPVariable_Wrap(LayerNormNode::apply(*x, wt, bt, eps, reinterpret_cast<int64_t>(*stream)));
+    return THPVariable_Wrap(LayerNormNode::apply(*x, w ? std::optional<Tensor>(*w) : std::nullopt, b ? std::optional<Tensor>(*b) : std::nullopt, eps,
+                                                 reinterpret_cast<int64_t>(*stream)));
   return THPVariable_Wrap(layer_norm_forward(*x, wt, bt, eps, *stream, false)[0]);
 }
 
