@@ -25,19 +25,25 @@ struct Scales {
 };
 
 // ---- the pass over the logits -------------------------------------------------------------------------------
-// Softmax statistics of the logits seen so far, as one pass takes them: m the largest, s = sum 2^d and e = sum 2^d d with
-// d = (x - m) c2.  A larger m rescales both: with f = 2^((m - m') c2), s' = f s and e' = f (e + s (m - m') c2).
-// (x - m) is taken before the scaling: the product x c2 of a mask of the type's lowest value would overflow.  d is bounded by
-// D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero in 32 bits.
-constexpr float D_MIN = -300.f;
+// Softmax statistics of the logits seen so far, as one pass takes them: m the largest, k = m c2 rounded to a whole number, s = sum 2^d and
+// e = sum 2^d d with d = x c2 - k.  The product and the difference are one operation and one rounding, and a larger m rescales both sums by a power of two,
+// exactly: s' = 2^(k - k') s, e' = 2^(k - k') (e + s (k - k')).  (x - m) c2 in two operations, which needs no whole number, took 4 to 7 % longer with
+// alternatives, where the vector unit bounds the pass; x c2 - m c2 with m c2 rounded is off by 1e-6 between lanes whose m differ.)
+// d is bounded by D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero in 32 bits.  Logits so large that m c2 is not
+// a number of 32 bits are left to Workgroup::wide().
+constexpr float D_MIN = -300.f, K_MAX = 3.3e38f;
 struct Softmax {
-  float m, s, e;
-  __device__ __forceinline__ float reference() const { return m == NEG_INF ? 0.f : m; }
+  float m, k, s, e;
+  float offset;  // of a row's whole sums: k - m c2, what its logarithms are off by from those around m
+  static __device__ __forceinline__ float reference(float m, float c2) { return fminf(fmaxf(rintf(m * c2), -K_MAX), K_MAX); }
+  static __device__ __forceinline__ Softmax nothing() { return {NEG_INF, -K_MAX, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ void raise(float to, float c2) {
-    const float d = m == NEG_INF ? 0.f : (m - to) * c2, f = __builtin_amdgcn_exp2f(d);  // (nothing seen yet: both sums are zero)
+    const float old = k;
+    m = to;
+    k = reference(to, c2);
+    const float d = old - k, f = __builtin_amdgcn_exp2f(d);
     e = f * fmaf(s, fmaxf(d, D_MIN), e);
     s *= f;
-    m = to;
   }
 };
 
@@ -55,12 +61,14 @@ struct Key {
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int column) { return (uint64_t)key << 32 | (uint32_t)~column; }
 
 struct RowResult {
-  float m, log_s;
+  float m, log_s, entropy;  // log_s = ln sum exp((x - m) / t)
   bool bad, empty;
   __device__ __forceinline__ RowResult(const Softmax& r) : m(r.m) {
     bad = !(r.s >= 0.f) || r.m == __builtin_inff();
     empty = !bad && r.s == 0.f;
-    log_s = bad ? __builtin_nanf("") : logf(r.s);
+    const float l = logf(r.s);
+    log_s = bad ? __builtin_nanf("") : empty ? NEG_INF : fmaf(LN2, r.offset, l);
+    entropy = bad ? __builtin_nanf("") : empty ? 0.f : l - LN2 * (r.e / r.s);
   }
   __device__ __forceinline__ float logprob(float x, float inv_t) const { return bad ? __builtin_nanf("") : empty ? NEG_INF : (x - m) * inv_t - log_s; }
 };
@@ -112,7 +120,9 @@ struct Workgroup {
 
   // A row's statistics in every lane, from those of the lanes; `buf`: 3 * WAVES floats of LDS.
   static __device__ __forceinline__ Softmax block_softmax(Softmax r, float c2, float* buf) {
-    r.raise(block_max<THREADS>(r.m, buf), c2);
+    const float m = block_max<THREADS>(r.m, buf);
+    r.raise(m, c2);
+    r.offset = fmaf(-m, c2, r.k);
     r.s = wave_sum_f32(r.s);
     r.e = wave_sum_f32(r.e);
     if constexpr (WAVES == 1) return r;
@@ -131,6 +141,25 @@ struct Workgroup {
     return r;
   }
 
+  // The sums of a row whose largest logit is finite but whose sums above are zero or infinite: its products with c2 are beyond 32 bits (a row of nothing but the type's
+  // lowest value, say).  Differences from m first, element by element.
+  template <int DT>
+  static __device__ __forceinline__ Softmax wide(const void* row, int V, Softmax r, float c2, float* buf) {
+    if (!(r.m > NEG_INF && r.m < __builtin_inff() && (r.s == 0.f || r.s == __builtin_inff()))) return r;
+    float s = 0.f, e = 0.f;
+    for (int v = threadIdx.x; v < V; v += THREADS) {
+      const float d = (RowType<DT>::load(row, v) - r.m) * c2, p = __builtin_amdgcn_exp2f(d);
+      s += p;
+      e = fmaf(p, fmaxf(d, D_MIN), e);
+    }
+    __syncthreads();
+    r.s = block_sum<THREADS>(s, buf);
+    __syncthreads();
+    r.e = block_sum<THREADS>(e, buf);
+    r.offset = 0.f;
+    return r;
+  }
+
   // Places [c0, c1) of a row from `begin` on; `keys` takes the order numbers of the groups' largest logits (group = place / GROUP; c0 is a multiple of
   // GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
   template <int DT, bool ENTROPY, bool TOP, int U, bool ONCE>
@@ -138,7 +167,7 @@ struct Workgroup {
     typedef RowType<DT> R;
     constexpr int VE = R::VE, STEP = THREADS * VE * U;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 64 * VE;
-    Softmax r = {NEG_INF, 0.f, 0.f};
+    Softmax r = Softmax::nothing();
     const auto fetch = [&](row_u32x4 (&raw)[U], int base) {
       const int at = base + (int)threadIdx.x * VE;
       if (base >= begin && base + STEP <= c1) {
@@ -158,43 +187,52 @@ struct Workgroup {
       for (int u = 0; u < U; ++u) raw[u] = next[u];
       if (base + STEP < c1) fetch(next, base + STEP);
       __builtin_amdgcn_sched_barrier(0);  // (the requests first)
-      float mx[U], top = NEG_INF;
+      const auto sum = [&](auto last) {  // (a row's last step: the waves skip as a whole what lies behind it)
+        const auto there = [&](int u) { return !decltype(last)::value || base + u * THREADS * VE + wave < c1; };
+        float mx[U], top = NEG_INF;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        mx[u] = NEG_INF;
-        if (base + u * THREADS * VE + wave >= c1) continue;  // (of a row's last step only; the wave as a whole)
-        mx[u] = R::element(raw[u], 0);
+        for (int u = 0; u < U; ++u) {
+          mx[u] = NEG_INF;
+          if (!there(u)) continue;
+          mx[u] = R::element(raw[u], 0);
 #pragma unroll
-        for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
-        top = fmaxf(top, mx[u]);
-      }
-      if (top > r.m) r.raise(top, c2);
-      const float ref = r.reference();
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (base + u * THREADS * VE + wave >= c1) continue;
-        float s = 0.f, en = 0.f;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float d = (R::element(raw[u], e) - ref) * c2, p = __builtin_amdgcn_exp2f(d);
-          s += p;
-          if (ENTROPY) en = fmaf(p, fmaxf(d, D_MIN), en);
+          for (int e = 1; e < VE; ++e) mx[u] = fmaxf(mx[u], R::element(raw[u], e));
+          top = fmaxf(top, mx[u]);
         }
-        r.s += s;
-        r.e += en;
-        if (TOP) {
-          int x = __builtin_bit_cast(int, mx[u]);
-#define TK_STEP(ctrl) \
-    x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl, 0xF, 0xF, false))));
-          TK_STEP(TK_DPP_QUAD_XOR1)
-          TK_STEP(TK_DPP_QUAD_XOR2)
-          TK_STEP(TK_DPP_ROW_HALF_MIRROR)
-          if (VE == 4) TK_STEP(TK_DPP_ROW_MIRROR)
+        if (top > r.m) r.raise(top, c2);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (!there(u)) continue;
+          float s = 0.f, en = 0.f;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float d = fmaf(R::element(raw[u], e), c2, -r.k), p = __builtin_amdgcn_exp2f(d);
+            s += p;
+            if (ENTROPY) en = fmaf(p, fmaxf(d, D_MIN), en);
+          }
+          r.s += s;
+          r.e += en;
+          if (TOP) {
+            uint32_t x = Key<DT>::of(mx[u]);
+#define TK_STEP(ctrl)                                                                        \
+  {                                                                                          \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xF, 0xF, true);     \
+    x = o > x ? o : x;                                                                       \
+  }
+            TK_STEP(TK_DPP_QUAD_XOR1)
+            TK_STEP(TK_DPP_QUAD_XOR2)
+            TK_STEP(TK_DPP_ROW_HALF_MIRROR)
+            if (VE == 4) TK_STEP(TK_DPP_ROW_MIRROR)
 #undef TK_STEP
-          const int c = at + u * THREADS * VE;
-          if ((threadIdx.x & (GROUP / VE - 1)) == 0 && c < c1) keys[c / GROUP] = Key<DT>::of(__builtin_bit_cast(float, x));
+            const int c = at + u * THREADS * VE;
+            if ((threadIdx.x & (GROUP / VE - 1)) == 0 && c < c1) keys[c / GROUP] = x;
+          }
         }
-      }
+      };
+      if (base + STEP <= c1)
+        sum(std::false_type());
+      else
+        sum(std::true_type());
     }
     return r;
   }
@@ -358,7 +396,7 @@ struct Workgroup {
     const RowResult o(r);
     if (threadIdx.x == 0) {
       d.logprobs[t] = token.live ? o.logprob(token.x, sc.inv_t) : 0.f;
-      d.entropy[t] = o.bad ? __builtin_nanf("") : o.empty ? 0.f : o.log_s - LN2 * (r.e / r.s);
+      d.entropy[t] = o.entropy;
       if (d.stats) {
         d.stats[t] = o.m;
         d.stats[(int64_t)d.n_rows + t] = o.log_s;
@@ -475,7 +513,7 @@ __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Sc
   const int end = p.begin + d.vocab;
   const Softmax mine = THREADS == 64 || t >= keep_from ? W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U, false>(p.base, p.begin, 0, end, sc.c2, keys)
                                                        : W::template stream<DT, OP != DISTILL, OP == LOGPROBS_TOP, U, THREADS != 64>(p.base, p.begin, 0, end, sc.c2, keys);
-  const Softmax r = W::block_softmax(mine, sc.c2, lds.softmax);
+  const Softmax r = W::template wide<DT>(row, d.vocab, W::block_softmax(mine, sc.c2, lds.softmax), sc.c2, lds.softmax);
   W::template finish<DT, OP>(d, sc, t, p, single, r, keys, lds);
 }
 
@@ -498,12 +536,12 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(tk_vocab_desc d, Scales
   const int t = blockIdx.x;
   const void* row = logits_row<DT>(d, t);
   const Wide::Single<DT, OP> single(d, t, row);
-  Softmax r = {NEG_INF, 0.f, 0.f};
+  Softmax r = Softmax::nothing();
   if ((int)threadIdx.x < n_chunks) {
     const float* p = parts + ((int64_t)t * n_chunks + threadIdx.x) * 3;
-    r = {p[0], p[1], p[2]};
+    r = {p[0], Softmax::reference(p[0], sc.c2), p[1], p[2], 0.f};
   }
-  r = Wide::block_softmax(r, sc.c2, lds.softmax);
+  r = Wide::wide<DT>(row, d.vocab, Wide::block_softmax(r, sc.c2, lds.softmax), sc.c2, lds.softmax);
   Wide::finish<DT, OP>(d, sc, t, placed<DT>(row), single, r, keys + (int64_t)t * groups, lds);
 }
 
