@@ -136,6 +136,36 @@ def test_masked_logits(V, dtype):
         _check_distill(z, q, at, 1.0, a)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,V", [(6, 30000), (1001, 1500), (1001, 20003)])
+@pytest.mark.parametrize("low", [-5e4, -1e9, -1e10, -1e20, -1e30])
+def test_masked_with_large_numbers(T, V, dtype, low):
+    """Masks whose products with log2(e) are further from whole numbers than an exponent can hold: in front of the logits that count, behind
+    them, in every other place, everywhere."""
+    z, tokens, a, b = _logits(T, V, dtype)
+    z[0::6, :V - 40] = low
+    z[1::6, 40:] = low
+    z[2::6, ::2] = low
+    z[3::6] = low
+    z[4::6, :V // 2] = low
+    z[4::6, V // 2:] = 2 * low
+    tokens[0::6] = V - 1
+    q, at = _teacher(z, 9)
+    n, k = 12, 20  # (rows that are compared; the others are there for the kernels that many rows have)
+    for t in (1.0, 0.7):
+        lp, h, top_lp, top, stats = logprobs_forward(z, tokens, k, t, True)
+        loss, distill_stats = distill_forward(z, q, at, t, True)
+        want = orc.token_logprobs(z[:n], tokens[:n], k, t)
+        assert torch.equal(top[:n].cpu().long(), want["top_indx"][0])
+        for name, got in (("logprobs", lp), ("entropy", h), ("top_logprobs", top_lp)):
+            orc.check(got[:n], *want[name], name)
+        orc.check(loss[:n], *orc.distill_topk(z[:n], q[:n], at[:n], t), "loss")
+        g = token_logprobs_backward(z, tokens, h, stats, a, b, t)
+        orc.check(g[:n], *orc.token_logprobs_backward(z[:n], tokens[:n], a[:n], b[:n], t), "dlogits")
+        g = distill_topk_backward(z, q, at, distill_stats, a, t)
+        orc.check(g[:n], *orc.distill_topk_backward(z[:n], q[:n], at[:n], a[:n], t), "dlogits of the distillation")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("V", [5, 777, 9000])
 def test_rows_that_are_no_distribution(V, dtype):
@@ -395,6 +425,33 @@ def test_training_steps_in_a_graph():
         torch.cuda.synchronize()
         for x, y in zip(out, want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused(native, monkeypatch):
+    """The refusal comes from the forward pass; nothing of a backward pass is captured while the leaves' gradients belong to the default stream."""
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
+    z, tokens, a, _ = _logits(20, 500, BF16)
+    q, at = _teacher(z, 5)
+    x, w, b = (torch.randn(s, device="cuda") for s in ((20, 64), 64, 64))
+    leaf, w = z.clone().requires_grad_(), w.requires_grad_()
+    calls = (lambda: token_logprobs(leaf, tokens).logprobs, lambda: distill_topk(leaf, q, at), lambda: layer_norm(x, w, b))
+    for f, wrt in zip(calls, (leaf, leaf, w)):
+        living = f()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            doubled = a * 2
+            with pytest.raises(RuntimeError, match="same leaf"):
+                f()
+            with torch.no_grad():
+                out = f()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, living) and torch.equal(doubled, a * 2)
+        assert torch.autograd.grad(living.sum(), wrt)[0].isfinite().all()
+        del living
 
 
 def test_calls_from_several_threads():

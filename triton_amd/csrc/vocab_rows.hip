@@ -28,14 +28,19 @@ struct Scales {
 // Softmax statistics of the logits seen so far, as one pass takes them: m the largest, k = m c2 rounded to a whole number, s = sum 2^d and
 // e = sum 2^d d with d = x c2 - k.  The product and the difference are one operation and one rounding, and a larger m rescales both sums by a power of two,
 // exactly: s' = 2^(k - k') s, e' = 2^(k - k') (e + s (k - k')).  (x - m) c2 in two operations, which needs no whole number, took 4 to 7 % longer with
-// alternatives, where the vector unit bounds the pass; x c2 - m c2 with m c2 rounded is off by 1e-6 between lanes whose m differ.)
-// d is bounded by D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero in 32 bits.  Logits so large that m c2 is not
-// a number of 32 bits are left to Workgroup::wide().
-constexpr float D_MIN = -300.f, K_MAX = 3.3e38f;
+// alternatives, where the vector unit bounds the pass; x c2 - m c2 with m c2 rounded is off by 1e-6 between lanes whose m differ.
+// From |m c2| = 2^24 on, numbers of 32 bits are further apart than one, and m c2 - k may be anything up to that distance.  So k is taken from a little above: no d is
+// much above zero, and no sum overflows that a larger logit (behind logits masked with -1e10, say) brings back to nothing.  The sums of a row whose largest
+// logit is so large are left to Workgroup::wide().  d is bounded by D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero
+// in 32 bits.
+constexpr float D_MIN = -300.f, K_MAX = 3.3e38f, WIDE = 2.f;
 struct Softmax {
   float m, k, s, e;
   float offset;  // of a row's whole sums: k - m c2, what its logarithms are off by from those around m
-  static __device__ __forceinline__ float reference(float m, float c2) { return fminf(fmaxf(rintf(m * c2), -K_MAX), K_MAX); }
+  static __device__ __forceinline__ float reference(float m, float c2) {
+    const float x = m * c2;
+    return fminf(fmaxf(rintf(fmaf(fabsf(x), 0x1p-23f, x)), -K_MAX), K_MAX);
+  }
   static __device__ __forceinline__ Softmax nothing() { return {NEG_INF, -K_MAX, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ void raise(float to, float c2) {
     const float old = k;
@@ -141,11 +146,11 @@ struct Workgroup {
     return r;
   }
 
-  // The sums of a row whose largest logit is finite but whose sums above are zero or infinite: its products with c2 are beyond 32 bits (a row of nothing but the type's
-  // lowest value, say).  Differences from m first, element by element.
+  // The sums of a row whose largest logit is finite but lies WIDE or more from its whole number (nothing but masked logits, say): differences from m first, element by
+  // element.
   template <int DT>
   static __device__ __forceinline__ Softmax wide(const void* row, int V, Softmax r, float c2, float* buf) {
-    if (!(r.m > NEG_INF && r.m < __builtin_inff() && (r.s == 0.f || r.s == __builtin_inff()))) return r;
+    if (!(r.m > NEG_INF && r.m < __builtin_inff() && !(fabsf(r.offset) < WIDE))) return r;
     float s = 0.f, e = 0.f;
     for (int v = threadIdx.x; v < V; v += THREADS) {
       const float d = (RowType<DT>::load(row, v) - r.m) * c2, p = __builtin_amdgcn_exp2f(d);
