@@ -109,6 +109,16 @@ def test_constant_rows_large_means_and_eps():
     _check(*_make(12, 384, BF16, F32, shift=-30.0))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [2, 9, 100, 1000])
+def test_constant_rows_of_large_numbers(C, dtype):
+    """Where the reciprocal deviation times the mean is beyond 32 bits, but no element's distance from the mean is."""
+    x, w, b, dy = _make(11, C, dtype, dtype)
+    x[3] = 2.0**121 if C <= 100 else 2.0**117
+    x[10] = -x[3]
+    _check(x, w, b, dy, eps=1e-5 if C <= 100 else 1e-9)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_infinities_and_nan_stay_in_their_rows(dtype):
     x, w, b, dy = _make(9, 200, dtype, dtype)

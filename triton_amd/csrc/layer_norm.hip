@@ -56,6 +56,12 @@ __device__ __forceinline__ void once_more(row_u32x4 (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
+// s / C, rounded once: the mean of equal elements whose sum is exact is that element, and their distances from it are zero.
+__device__ __forceinline__ float mean_of(float s, float C, float inv_c) {
+  const float q = s * inv_c;
+  return fmaf(fmaf(-q, C, s), inv_c, q);
+}
+
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 // One row's mean and reciprocal deviation from its registers (TPR lanes a row, NV vectors of 16 bytes a lane, the first FULL of them within any
@@ -69,7 +75,7 @@ __device__ __forceinline__ void row_statistics(row_u32x4 (&raw)[NV], int lane, i
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < VE; ++e) s += R::element(raw[v], e);
-  const float mu = row_sum<TPR>(s, buf[0]) * inv_c;
+  const float mu = mean_of(row_sum<TPR>(s, buf[0]), (float)C, inv_c);
   once_more(raw);
   s = 0.f;
 #pragma unroll
@@ -285,10 +291,11 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_backward_kernel(const void* 
     float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      const int here = v < FULL ? VE : R::left((v * TPR + lane) * VE, C);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        // (behind the last column dy is zero, and h is finite where the row's is)
-        const float g0 = R::element(gv[v], e), h = (R::element(xv[v], e) - mu) * r, g = g0 * bits_f32(wl[v][e / 4][lane][e % 4]);
+        // (behind the last column there is no x: of large equal ones (0 - mean) rstd may be infinite where their own h is zero)
+        const float g0 = R::element(gv[v], e), h = v < FULL || e < here ? (R::element(xv[v], e) - mu) * r : 0.f, g = g0 * bits_f32(wl[v][e / 4][lane][e % 4]);
         sg += g;
         sgh = fmaf(g, h, sgh);
         if constexpr (SUMS) {
