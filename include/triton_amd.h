@@ -533,7 +533,7 @@ int32_t tk_quant_fp8_rows(const void* x, int32_t dtype, int64_t M, int64_t K, in
  * Layer norm of the rows of x [n_rows, n_cols] (unit stride along the columns, rows at any element stride and address):
  *   y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps),   var = mean((x - mean)^2)
  * x and y share `dtype` (fp32 / bf16 / fp16); weight and bias [n_cols] are optional (NULL) and have a type of their own;
- * mean and rstd [n_rows] fp32 are optional outputs, which the backward pass reads.  Statistics and arithmetic in fp32, one
+ * mean and rstd [n_rows] fp32 are optional outputs (both or neither), which the backward pass reads.  Statistics and arithmetic in fp32, one
  * rounding to `dtype`.  No counterpart in the reference's operator library.
  */
 int32_t tk_layer_norm(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols, int64_t stride_xm, const void* weight,
@@ -570,6 +570,7 @@ int32_t tk_layer_norm_backward(const void* dy, int64_t stride_dym, const void* x
  *   - a logit of -inf has probability zero.  A row of nothing else: logprobs -inf, entropy 0, loss +inf, gradient 0;
  *   - a row with a NaN or +inf: logprobs, entropy, top_logprobs, loss and gradient are NaN, top_indx is -1;
  *   - a token outside [0, vocab): logprobs 0, and no gradient through it;
+ *   - a teacher entry with a NaN or +inf: loss and gradient are NaN;
  *   - a teacher entry whose index is outside [0, vocab), or whose logit is -inf, carries no weight; a row without any other has loss 0
  *     and gradient 0.  An index that occurs twice counts twice.
  * A row whose given gradients are all zero has the gradient zero.

@@ -97,6 +97,11 @@ def test_operators_refuse_what_they_do_not_take():
                         ((torch.zeros((3, 200)), tokens, 129), NotImplementedError), ((torch.zeros((3, 524289)), tokens, 1), NotImplementedError)):
         with pytest.raises(error):
             token_logprobs(*args)
+    for many in (torch.zeros((1, 1)).expand(2**31, 1), torch.zeros((1, 1)).expand(1, 2**30 + 1), torch.zeros((1, 1)).expand(1, 2**32 + 5)):
+        with pytest.raises(NotImplementedError, match="at most"):
+            token_logprobs(many, torch.zeros(1, dtype=torch.int64).expand(many.shape[0]))
+        with pytest.raises(NotImplementedError, match="at most"):
+            distill_topk(many, many[:, :1], torch.zeros((1, 1), dtype=torch.int64).expand(many.shape[0], 1))
     q, at = torch.zeros((3, 4)), torch.zeros((3, 4), dtype=torch.int32)
     with pytest.raises(RuntimeError, match="HIP device"):
         distill_topk(z, q, at)

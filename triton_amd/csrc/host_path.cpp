@@ -962,6 +962,7 @@ PyMethodDef methods[] = {
     METHOD("layer_norm", run_layer_norm, 4),
     METHOD("token_logprobs", run_token_logprobs, 4),
     METHOD("distill_topk", run_distill_topk, 4),
+    METHOD("kept_by_default_stream", run_kept_by_default_stream, 1),
     METHOD("x_extent", rule_x_extent, 4),
     METHOD("dma_runs_16bit", rule_dma_16bit, 5),
     METHOD("dma_block_m", rule_dma, 4),

@@ -18,6 +18,16 @@ bool row_dtype(const Tensor& t) {
 }
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool on_device_of(const Tensor& t, const Tensor& x) { return t.is_cuda() && t.get_device() == x.get_device(); }
+// Whether t is a leaf whose gradient is accumulated on the default stream, for the sake of a graph of this process that still lives.  A backward pass that is
+// captured would make the default stream wait for the capture, which ends the process.
+bool kept_by_default_stream(const Tensor& t) {
+  if (!t.requires_grad() || t.grad_fn()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  const auto stream = node ? node->stream() : std::nullopt;
+  return stream && stream->id() == 0;
+}
+// (the callers leave such leaves to the Python path unless the call itself is on the default stream, which is never captured)
+bool may_be_kept(const Tensor& t, void* stream) { return stream && kept_by_default_stream(t); }
 float* floats(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int32_t code_of(const Tensor& t) { return t.defined() ? dtype_code(t.scalar_type()) : TK_F32; }
@@ -118,9 +128,11 @@ PyObject* run_layer_norm(PyObject* const* v) {
   auto stream = stream_of(*x);
   if (!stream) return none();
   const Tensor no, &wt = w ? *w : no, &bt = b ? *b : no;
-  if (wants_grad(*x) || (w && wants_grad(*w)) || (b && wants_grad(*b)))
+  if (wants_grad(*x) || (w && wants_grad(*w)) || (b && wants_grad(*b))) {
+    if (may_be_kept(*x, *stream) || (w && may_be_kept(*w, *stream)) || (b && may_be_kept(*b, *stream))) return none();
     return THPVariable_Wrap(LayerNormNode::apply(*x, w ? std::optional<Tensor>(*w) : std::nullopt, b ? std::optional<Tensor>(*b) : std::nullopt, eps,
                                                  reinterpret_cast<int64_t>(*stream)));
+  }
   return THPVariable_Wrap(layer_norm_forward(*x, wt, bt, eps, *stream, false)[0]);
 }
 
@@ -209,6 +221,7 @@ PyObject* run_token_logprobs(PyObject* const* v) {
   if (!stream) return none();
   variable_list o;
   if (wants_grad(*z)) {
+    if (may_be_kept(*z, *stream)) return none();
     o = LogprobsNode::apply(*z, *tokens, k, temperature, reinterpret_cast<int64_t>(*stream));
   } else {
     auto f = logprobs_forward(*z, *tokens, k, temperature, *stream, false);
@@ -283,8 +296,16 @@ PyObject* run_distill_topk(PyObject* const* v) {
   if (dispatcher_heard()) return none();
   auto stream = stream_of(*z);
   if (!stream) return none();
-  if (wants_grad(*z)) return THPVariable_Wrap(DistillNode::apply(*z, *q, *at, temperature, reinterpret_cast<int64_t>(*stream)));
+  if (wants_grad(*z)) {
+    if (may_be_kept(*z, *stream)) return none();
+    return THPVariable_Wrap(DistillNode::apply(*z, *q, *at, temperature, reinterpret_cast<int64_t>(*stream)));
+  }
   return THPVariable_Wrap(distill_forward(*z, *q, *at, temperature, *stream, false)[0]);
+}
+
+PyObject* run_kept_by_default_stream(PyObject* const* v) {
+  const Tensor* t = tensor_of(v[0]);
+  return PyBool_FromLong(t && kept_by_default_stream(*t));
 }
 
 }  // namespace

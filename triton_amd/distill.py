@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nt
-from ._autograd import once
+from ._autograd import check_capture, once
 from .logprobs import DTYPES, check_index, check_logits, logits_desc, row_gradient, workspace
 
 MAX_TEACHER = 1024
@@ -95,6 +95,7 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distill_topk has no gradient for the teacher: pass its logits detached")
     if logits.requires_grad and torch.is_grad_enabled():
+        check_capture(logits)
         return _DistillTopK.apply(logits, teacher_logits, teacher_indx, temperature)
     return _forward(logits, teacher_logits, teacher_indx, temperature, False)[0]
 

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _native as nt
-from ._autograd import once
+from ._autograd import check_capture, once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -114,6 +114,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if y is not None:
         return y
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        check_capture(x, weight, bias)
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, with_stats=False)[0]
 

@@ -13,9 +13,10 @@ from typing import Optional
 import torch
 
 from . import _native as nt
-from ._autograd import once
+from ._autograd import check_capture, once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+MAX_ROWS, MAX_COLUMNS = 2**31 - 1, 2**30
 MAX_TOP = 128
 MAX_TOP_COLUMNS = 524288
 
@@ -34,6 +35,8 @@ def check_logits(logits, temperature):
         raise ValueError(f"logits must be [rows, vocabulary] (got shape {tuple(logits.shape)})")
     if logits.dtype not in DTYPES:
         raise NotImplementedError(f"logits must be fp32, bf16 or fp16 (got {logits.dtype})")
+    if logits.shape[0] > MAX_ROWS or logits.shape[1] > MAX_COLUMNS:
+        raise NotImplementedError(f"logits have at most {MAX_ROWS} rows and {MAX_COLUMNS} columns (got shape {tuple(logits.shape)})")
     if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError(f"temperature must be positive and finite (got {temperature})")
     return logits if logits.stride(1) == 1 else logits.contiguous()
@@ -145,6 +148,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0, tempe
         return TokenLogprobs(*r)
     logits = check_logits(logits, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
+        check_capture(logits)
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, k, temperature))
     return TokenLogprobs(*_forward(logits, tokens, k, temperature, False)[:4])
 
