@@ -112,6 +112,24 @@ def test_operators_refuse_what_they_do_not_take():
             distill_topk(*args)
 
 
+def test_backward_passes_refuse_what_no_forward_pass_gave():
+    from triton_kernels.distill import distill_topk_backward
+    from triton_kernels.logprobs import token_logprobs_backward
+    z, tokens, h, stats, g = torch.zeros((3, 10)), torch.zeros(3, dtype=torch.int64), torch.zeros(3), torch.zeros((2, 3)), torch.ones(3)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        token_logprobs_backward(z, tokens, h, stats, g, None)
+    for args in ((z, tokens, h[:2], stats, g, g), (z, tokens, h.double(), stats, g, g), (z, tokens, h, stats[0], g, g), (z, tokens, h, torch.zeros((3, 2)).t(), g, g),
+                 (z, tokens, h, stats, g[:2], g), (z, tokens, h, stats, g, g[:, None]), (z, tokens[:2], h, stats, g, g)):
+        with pytest.raises(ValueError):
+            token_logprobs_backward(*args)
+    q, at, stats = torch.zeros((3, 4)), torch.zeros((3, 4), dtype=torch.int32), torch.zeros((4, 3))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        distill_topk_backward(z, q, at, stats, g)
+    for args in ((z, q, at, stats[:2], g), (z, q, at, stats.double(), g), (z, q, at, stats, g[:1]), (z, q, at, stats, g[None]), (z, q[:2], at[:2], stats, g)):
+        with pytest.raises(ValueError):
+            distill_topk_backward(*args)
+
+
 def test_c_entries_refuse_bad_calls_before_any_launch():
     lib, p = nt.lib(), 64  # (an address that no entry reads)
     ln = lambda x=p, dt=nt.TK_BF16, m=4, c=8, w=p, wt=nt.TK_F32, eps=1e-5, y=p: lib.tk_layer_norm(x, dt, m, c, c, w, wt, None, 0, eps, y, c, None, None, None)  # noqa: E731

@@ -10,7 +10,7 @@ import torch
 
 from . import _native as nt
 from ._autograd import check_capture, once
-from .logprobs import DTYPES, check_index, check_logits, logits_desc, row_gradient, workspace
+from .logprobs import DTYPES, check_index, check_logits, check_saved, logits_desc, row_gradient, workspace
 
 MAX_TEACHER = 1024
 
@@ -51,11 +51,13 @@ def _forward(logits, teacher_logits, teacher_indx, temperature, with_stats):
 def distill_topk_backward(logits, teacher_logits, teacher_indx, stats, d_loss, temperature: float = 1.0):
     """The gradient of `logits` for that of the losses (`[T]`) and the forward pass' statistics."""
     logits = check_logits(logits, temperature)
-    d, keep = _desc(logits, teacher_logits, teacher_indx, temperature)
     T = logits.shape[0]
+    check_saved(stats, (4, T), logits, "stats")
+    d_l, stride, keep_g = row_gradient(d_loss, logits, "d_loss")
+    d, keep = _desc(logits, teacher_logits, teacher_indx, temperature)
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     d.stats, d.teacher_stats = stats.data_ptr(), stats.data_ptr() + 8 * T
-    d.d_loss, d.d_loss_stride, keep_g = row_gradient(d_loss, T)
+    d.d_loss, d.d_loss_stride = d_l, stride
     d.d_logits, d.d_logits_stride_m = d_logits.data_ptr(), d_logits.stride(0)
     nt.submit(nt.lib().tk_distill_topk_backward, d, logits.device)
     del keep, keep_g

@@ -63,10 +63,18 @@ def workspace(logits, k):
     return torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
 
 
-def row_gradient(g, T):
+def check_saved(t, shape, logits, name):
+    if t.shape != shape or t.dtype != torch.float32 or t.device != logits.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be the contiguous fp32 {list(shape)} of the forward pass")
+
+
+def row_gradient(g, logits, name):
     """A gradient of a row's output: its pointer, element stride and the tensor to keep alive."""
     if g is None:
         return None, 0, None
+    T = logits.shape[0]
+    if g.shape != (T, ) or g.device != logits.device:
+        raise ValueError(f"{name} must be [{T}] on {logits.device} (got {tuple(g.shape)} on {g.device})")
     g = g if g.dtype == torch.float32 else g.float()
     return g.data_ptr(), g.stride(0) if T > 1 else 0, g
 
@@ -98,17 +106,21 @@ def token_logprobs_backward(logits, tokens, entropy, stats, d_logprobs, d_entrop
     """The gradient of `logits` for those of the log probabilities and entropies (`[T]`, either may be None)."""
     logits = check_logits(logits, temperature)
     check_index(tokens, logits.shape[:1], logits, "tokens")
-    nt.require_gpu(logits, "logits")
     T = logits.shape[0]
+    check_saved(entropy, (T, ), logits, "entropy")
+    check_saved(stats, (2, T), logits, "stats")
+    d_lp, lp_stride, keep_lp = row_gradient(d_logprobs, logits, "d_logprobs")
+    d_h, h_stride, keep_h = row_gradient(d_entropy, logits, "d_entropy")
+    nt.require_gpu(logits, "logits")
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     d = logits_desc(logits, temperature)
     d.tokens, d.tokens_i64 = tokens.data_ptr(), int(tokens.dtype == torch.int64)
     d.entropy, d.stats = entropy.data_ptr(), stats.data_ptr()
-    d.d_logprobs, d.d_logprobs_stride, keep_lp = row_gradient(d_logprobs, T)
-    d.d_entropy, d.d_entropy_stride, keep_h = row_gradient(d_entropy, T)
+    d.d_logprobs, d.d_logprobs_stride, d.d_entropy, d.d_entropy_stride = d_lp, lp_stride, d_h, h_stride
     d.d_logits, d.d_logits_stride_m = d_logits.data_ptr(), d_logits.stride(0)
     nt.submit(nt.lib().tk_token_logprobs_backward, d, logits.device)
+    del keep_lp, keep_h
     return d_logits
 
 
