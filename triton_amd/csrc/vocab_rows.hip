@@ -506,6 +506,8 @@ struct Workgroup {
 };
 
 // A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
+// Bound by the logits' one read, and with alternatives by the vector unit as well: 4096 x 131072 bf16 174 us (6.2 TB/s), with 64 alternatives 192 (5.6); 2048 x 32000 fp32
+// 47.7 (5.5).
 template <int DT, int OP, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0, int keep_from) {
   typedef Workgroup<THREADS> W;
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Sc
   W::template finish<DT, OP>(d, sc, t, p, single, r, keys, lds);
 }
 
-// Few rows: pieces of a row, whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
+// Few rows: pieces of a row (61 x 50001 fp16 with 8 alternatives 11.5 us, both launches: latencies one after the other, not bytes), whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
 typedef Workgroup<256> Wide;
 template <int DT, int OP>
 __global__ __launch_bounds__(256) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
@@ -620,7 +622,7 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
 }
 
 // ---- gradients ----------------------------------------------------------------------------------------------
-// A piece of a row a workgroup: one read and one write of the row's size.  With p = 2^d2, d2 = (x - m) c2 - log2 s:
+// A piece of a row a workgroup: one read and one write of the row's size, which bound it (forward and backward of 1000 x 50001 bf16 59 us, 5.1 TB/s).  With p = 2^d2, d2 = (x - m) c2 - log2 s:
 //   log probabilities   g = p (A + B d2) everywhere, A = -(d_lp + d_h H) / t, B = -d_h ln 2 / t, and d_lp / t more at the token
 //   distillation        g = p G, G = d_loss / t, and a_j G less at the teacher's entry j
 // The teacher's few columns are written once more at the end, by the piece that they lie in: looking each column up while the row streams by
