@@ -55,6 +55,11 @@ def test_sizes_and_types(M, C, dtype, weights):
     _check(*_make(M, C, dtype, weights))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_long_rows_than_partial_sums(dtype):
+    _check(*_make(301, 16389, dtype, F32))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_weight_and_bias_of_other_types_or_alone(dtype):
     x, w, b, dy = _make(37, 264, dtype, F32)

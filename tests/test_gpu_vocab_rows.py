@@ -195,6 +195,17 @@ def test_large_logits_of_either_sign():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,V", [(5, 20001), (1001, 700)])
+@pytest.mark.parametrize("temperature", [2.0**-100, 2.0**-20, 2.0**20, 2.0**100])
+def test_temperatures_far_from_one(T, V, dtype, temperature):
+    z, tokens, a, b = _logits(T, V, dtype)
+    z[2] = z[2].round()  # (several largest ones)
+    _check_logprobs(z, tokens, 7, temperature, (a, b))
+    q, at = _teacher(z, 9)
+    _check_distill(z, q, at, temperature, a)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_tokens_out_of_range_and_no_gradient(dtype):
     z, tokens, a, b = _logits(8, 3001, dtype)
     tokens[0], tokens[1], tokens[2], tokens[3] = -1, -100, 3001, 2**40

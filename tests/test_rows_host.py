@@ -143,6 +143,7 @@ def test_c_entries_refuse_bad_calls_before_any_launch():
     for bad in (dict(m=-1), dict(c=0), dict(mean=None), dict(ws=None)):
         assert bw(**bad) == nt.TK_ERR_INVALID, bad
     assert bw(dt=nt.TK_U8) == nt.TK_ERR_UNSUPPORTED and bw(wt=nt.TK_I32) == nt.TK_ERR_UNSUPPORTED
+    assert [lib.tk_layer_norm_backward_workspace_bytes(5000, C) // (8 * C) for C in (1, 512, 513, 16384, 16385)] == [768, 768, 512, 512, 128]
     assert lib.tk_layer_norm_backward_workspace_bytes(0, 8) >= 0 and lib.tk_layer_norm_backward_workspace_bytes(5, 0) == 0
 
     def desc(**more):

@@ -150,8 +150,8 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x
   }
 }
 
-// Many rows (16384 x 2880 bf16 41.9 us, 4.5 TB/s both ways, 135168 x 128 18.5 us, 3.7): workgroups of four waves that stay, the weights read once each, into registers (up to 16 elements a lane) or LDS; a group's next
-// rows are requested before the present ones are summed.  AT rows a group at a time, so that short rows keep as many bytes under way as long ones.
+// Many rows (16384 x 2880 bf16 41.9 us, 4.5 TB/s both ways, 135168 x 128 18.5 us, 3.7): workgroups of four waves that stay, the weights read once each, into
+// registers (up to 16 elements a lane) or LDS; a group's next rows are requested before the present ones are summed.  AT rows a group at a time, so that short rows keep as many bytes under way as long ones.
 template <int DT, int TPR, int NV, int FULL>
 __global__ __launch_bounds__(256) void layer_norm_many_kernel(const void* x, int64_t M, int C, int64_t sx, const void* w, int wt, const void* b, int bt,
                                                               float eps, void* y, int64_t sy, float* mean, float* rstd) {
@@ -478,6 +478,7 @@ __global__ __launch_bounds__(256) void layer_norm_parts_long_kernel(const void* 
 }
 
 constexpr int64_t MAX_COLS = 1 << 30;
+constexpr int64_t LONG_PARTS = 128;  // partial rows of rows beyond 16384 columns
 // Lanes a workgroup of the backward pass, and the most workgroups, each of which leaves a row of partial sums: eight waves a CU carry long rows, short ones want more
 // (us at 256, 512, 768, 1024 workgroups: 65000 x 500 bf16 86, 59, 49, 50; 135168 x 128 43, 32, 29, 30; 32768 x 1024 64, 48, 49, 50; rows shared by two waves,
 // workgroups of eight: 16384 x 4096 85, 94, 104, 113).
@@ -605,7 +606,7 @@ void backward(const Backward& b) {
   if (b.dx && b.M)
     hipLaunchKernelGGL(layer_norm_dx_long_kernel<DT>, dim3(rows_grid(b.M)), dim3(256), 0, b.s, b.dy, b.sdy, b.x, b.M, b.C, b.sx, b.w, b.wt, b.mean, b.rstd, b.dx, b.sdx);
   if (!b.dw && !b.db) return;
-  const int n = (int)(b.M < 128 ? b.M : 128);
+  const int n = (int)(b.M < LONG_PARTS ? b.M : LONG_PARTS);
   if (n)
     hipLaunchKernelGGL(layer_norm_parts_long_kernel<DT>, dim3((unsigned)cdiv(b.C, 256), n), dim3(256), 0, b.s, b.dy, b.sdy, b.x, b.M, b.C, b.sx, b.mean, b.rstd,
                        b.parts);
@@ -632,7 +633,7 @@ extern "C" int32_t tk_layer_norm(const void* x, int32_t dtype, int64_t n_rows, i
 }
 
 extern "C" int64_t tk_layer_norm_backward_workspace_bytes(int64_t n_rows, int64_t n_cols) {
-  const int64_t parts = n_cols <= 512 ? 768 : 512;  // (a bound for each type)
+  const int64_t parts = n_cols <= 512 ? 768 : n_cols <= 16384 ? 512 : LONG_PARTS;  // (a bound for each type)
   return n_rows > 0 && n_cols > 0 ? 2 * (n_rows < parts ? n_rows : parts) * n_cols * 4 : 0;
 }
 
