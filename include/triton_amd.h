@@ -533,8 +533,8 @@ int32_t tk_quant_fp8_rows(const void* x, int32_t dtype, int64_t M, int64_t K, in
  * Layer norm of the rows of x [n_rows, n_cols] (unit stride along the columns, rows at any element stride and address):
  *   y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(var + eps),   var = mean((x - mean)^2)
  * x and y share `dtype` (fp32 / bf16 / fp16); weight and bias [n_cols] are optional (NULL) and have a type of their own;
- * mean and rstd [n_rows] fp32 are optional outputs (both or neither), which the backward pass reads.  Statistics and arithmetic in fp32, one
- * rounding to `dtype`.  No counterpart in the reference's operator library.
+ * mean and rstd [n_rows] fp32 are optional outputs (both or neither), which the backward pass reads.  Statistics and arithmetic in fp32 (the
+ * mean good to its own rounding, whatever the deviation), one rounding to `dtype`.  No counterpart in the reference's operator library.
  */
 int32_t tk_layer_norm(const void* x, int32_t dtype, int64_t n_rows, int64_t n_cols, int64_t stride_xm, const void* weight,
                       int32_t weight_dtype, const void* bias, int32_t bias_dtype, float eps, void* y, int64_t stride_ym,

@@ -108,8 +108,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """`(x - mean) / sqrt(var + eps) * weight + bias` over the last dimension of `x [..., C]` (biased variance), in x's type.
 
     x, weight and bias are fp32, bf16 or fp16, each its own; weight and bias are `[C]` and optional.  Rows may have any stride.
-    Sums and squares are taken in fp32: a row whose squared distances from its mean add up to more than that holds (distances of about
-    1e18 on) has no deviation to speak of, and gives the bias.
+    Statistics are taken in fp32; the mean is good to its own rounding also where it is large against the deviation, and a row of equal
+    elements gives the bias.  So does a row whose squared distances from its mean add up to more than fp32 holds (distances of about 1e18 on),
+    which has no deviation to speak of.
     Differentiable once in all three."""
     host = nt.host()
     y = host.layer_norm(x, weight, bias, eps) if host is not None else None
