@@ -1,0 +1,45 @@
+"""The row operators where autograd does more than call their backward pass: on other streams than the default one, in captures."""
+import pytest
+import torch
+
+from triton_amd import _native as nt
+from triton_kernels.distill import distill_topk
+from triton_kernels.layer_norm import layer_norm
+from triton_kernels.logprobs import token_logprobs
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+T, V, K, C = 20, 501, 5, 72
+
+
+def _inputs(dtype=F32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn((T, V), generator=g) * 3).to(dtype).cuda()
+    tokens = torch.randint(V, (T, ), generator=g).cuda()
+    q, at = torch.randn((T, K), generator=g).cuda(), torch.randint(V, (T, K), generator=g).cuda()
+    x, w, b = (torch.randn(s, generator=g).cuda() for s in ((T, C), C, C))
+    return z, tokens, q, at, x.to(dtype), w, b
+
+
+def _calls(z, tokens, q, at, x, w, b):
+    """(operator of one tensor to differentiate, that tensor)"""
+    return ((lambda t: token_logprobs(t, tokens, 3).logprobs, z), (lambda t: token_logprobs(t, tokens, 3).entropy, z), (lambda t: distill_topk(t, q, at), z),
+            (lambda t: layer_norm(t, w, b), x), (lambda t: layer_norm(x, t, b), w), (lambda t: layer_norm(x, w, t), b))
+
+
+def test_native_nodes_on_a_side_stream():
+    """Also where the leaves belong to a graph of the default stream, and with the same results."""
+    for f, t in _calls(*_inputs()):
+        leaf = t.clone().requires_grad_()
+        living = f(leaf)
+        want, = torch.autograd.grad(living.square().sum(), leaf, retain_graph=True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y = f(leaf)
+            got, = torch.autograd.grad(y.square().sum(), leaf)
+        torch.cuda.synchronize()
+        assert type(y.grad_fn) is type(living.grad_fn)
+        assert torch.equal(y, living) and torch.equal(got, want)
+        del living

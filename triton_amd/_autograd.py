@@ -11,7 +11,7 @@ from . import _native as nt
 def check_capture(*leaves):
     """Refuses a captured call with leaves that an earlier graph on the default stream still uses: their gradients are accumulated on that
     stream, and the backward pass would make it wait for the capture, which ends the process."""
-    if any(t is not None and nt.rules().kept_by_default_stream(t) for t in leaves) and torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_current_stream_capturing() and any(t is not None and nt.rules().kept_by_default_stream(t) for t in leaves):
         raise RuntimeError("a result computed on the default stream from the same leaf tensors is still alive: delete it before the capture "
                            "(or compute it on another stream)")
 

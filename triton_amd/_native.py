@@ -191,7 +191,8 @@ def _load_host():
     with _lock:
         if _host is None:
             table = {name: _c.cast(getattr(handle, name), _ptr).value for name in _HOST_ENTRIES}
-            table.update(check=check, raw_stream=_raw_stream, current_device=_current_device, tile_counters=matmul._tile_counters,
+            table.update(check=check, raw_stream=_raw_stream, current_device=_current_device,
+                         capturing=torch.cuda.is_current_stream_capturing, tile_counters=matmul._tile_counters,
                          combine_counters=matmul._combine_counters, decode_workspace=moe_decode._workspace, tensor_type=Tensor,
                          mx_value=GFX950MXValueLayout, mx_scale=GFX950MXScaleLayout, fp8_value=GFX950FP8ValueLayout, fp4=FP4,
                          metadata_type=RaggedTensorMetadata, routing_type=legacy.RoutingData, gather_type=legacy.GatherIndx,

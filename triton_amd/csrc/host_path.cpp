@@ -56,7 +56,7 @@ struct Bound {
   decltype(&tk_distill_topk) distill_topk = nullptr;
   decltype(&tk_distill_topk_backward) distill_topk_backward = nullptr;
   decltype(&tk_last_error) last_error = nullptr;
-  PyObject *check, *raw_stream, *current_device;              // _native.check, torch's raw stream and device getters
+  PyObject *check, *raw_stream, *current_device, *capturing;  // _native.check, torch's raw stream, device and capture getters
   PyObject *tile_counters, *combine_counters, *decode_workspace;  // per device and stream
   PyObject *tensor_type, *mx_value, *mx_scale, *fp8_value, *fp4;  // Tensor, its layouts, the FP4 data type
   PyObject *metadata_type, *routing_type, *gather_type, *scatter_type;
@@ -940,7 +940,7 @@ PyObject* bind(PyObject*, PyObject* dict) {
 #define OBJECT(name)                            \
   if (!(B.name = get(#name))) return nullptr;   \
   Py_INCREF(B.name);
-  OBJECT(check) OBJECT(raw_stream) OBJECT(current_device) OBJECT(tile_counters) OBJECT(combine_counters) OBJECT(decode_workspace)
+  OBJECT(check) OBJECT(raw_stream) OBJECT(current_device) OBJECT(capturing) OBJECT(tile_counters) OBJECT(combine_counters) OBJECT(decode_workspace)
   OBJECT(tensor_type) OBJECT(mx_value) OBJECT(mx_scale) OBJECT(fp8_value) OBJECT(fp4) OBJECT(metadata_type) OBJECT(routing_type)
   OBJECT(gather_type) OBJECT(scatter_type) OBJECT(default_flex) OBJECT(no_activation) OBJECT(no_epilogue)
 #undef OBJECT
