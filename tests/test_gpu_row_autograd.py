@@ -43,3 +43,35 @@ def test_native_nodes_on_a_side_stream():
         assert type(y.grad_fn) is type(living.grad_fn)
         assert torch.equal(y, living) and torch.equal(got, want)
         del living
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_captures_of_what_was_made_of_a_living_graphs_leaves_are_refused(native, monkeypatch):
+    """Transposed leaves, views and casts of leaves, results of the default stream; without gradients they are captured, and leaves of no other graph are with
+    them.  The refusal comes from the forward pass: no backward pass is captured."""
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
+    for f, t in _calls(*_inputs()):
+        turned = t.t().contiguous().t() if t.ndim == 2 else torch.stack((t, t), 1)[:, 0]
+        fresh = t.clone().requires_grad_()
+        for leaf, made in ((turned.detach(), lambda s: s), (t.clone(), lambda s: s.view(s.shape)), (t.clone(), lambda s: s.to(BF16)), (t.clone(), lambda s: (s * 2).exp())):
+            leaf.requires_grad_()
+            living = f(made(leaf))
+            before = made(leaf)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                for s in (lambda: made(leaf), lambda: before):
+                    with pytest.raises(RuntimeError, match="same leaf"):
+                        f(s())
+                with torch.no_grad():
+                    out = f(made(leaf))
+                own = f(fresh)
+                g, = torch.autograd.grad(own.sum(), fresh)
+            own, want = own.detach(), f(t)
+            for _ in range(2):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, living) and torch.equal(own, want) and g.isfinite().all()
+            assert torch.autograd.grad(living.sum(), leaf)[0].isfinite().all()
+            del living, before

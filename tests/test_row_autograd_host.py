@@ -1,0 +1,38 @@
+"""Row operators and autograd without a GPU."""
+import types
+
+import pytest
+import torch
+
+from triton_amd import _native as nt
+from triton_kernels.distill import distill_topk
+from triton_kernels.layer_norm import layer_norm
+from triton_kernels.logprobs import token_logprobs
+
+T, V, K, C = 6, 40, 5, 24
+
+
+def _inputs():
+    z, tokens = torch.randn((T, V)), torch.randint(V, (T, ))
+    q, at = torch.randn((T, K)), torch.randint(V, (T, K))
+    return z, tokens, q, at, torch.randn((T, C)), torch.randn(C), torch.randn(C)
+
+
+def _calls():
+    z, tokens, q, at, x, w, b = _inputs()
+    return ((lambda t: token_logprobs(t, tokens, 3).logprobs, z), (lambda t: distill_topk(t, q, at), z), (lambda t: layer_norm(t, w, b), x),
+            (lambda t: layer_norm(x, t, b), w), (lambda t: layer_norm(x, w, t), b))
+
+
+def test_captures_are_checked_for_the_tensors_of_the_caller(monkeypatch):
+    """With the two questions of the check answered by stubs: "is the stream being captured" with yes, "is it kept by the default stream" for leaves.
+    Rows that are copied for their strides are asked for as they come."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(nt, "rules", lambda: types.SimpleNamespace(kept_by_default_stream=lambda t: t.requires_grad and t.grad_fn is None))
+    for f, t in _calls():
+        strided = t.t().contiguous().t() if t.ndim == 2 else torch.stack((t, t), 1)[:, 0]
+        for leaf in (t.clone(), strided.detach()):
+            with pytest.raises(RuntimeError, match="same leaf"):
+                f(leaf.requires_grad_())
+            with pytest.raises(RuntimeError, match="HIP device"), torch.no_grad():
+                f(leaf)

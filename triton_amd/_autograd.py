@@ -8,12 +8,13 @@ import torch
 from . import _native as nt
 
 
-def check_capture(*leaves):
-    """Refuses a captured call with leaves that an earlier graph on the default stream still uses: their gradients are accumulated on that
-    stream, and the backward pass would make it wait for the capture, which ends the process."""
-    if torch.cuda.is_current_stream_capturing() and any(t is not None and nt.rules().kept_by_default_stream(t) for t in leaves):
+def check_capture(*tensors):
+    """Refuses a captured call with leaves that an earlier graph on the default stream still uses, and with what was made of such leaves: their
+    gradients are accumulated on that stream, and the backward pass would make it wait for the capture, which ends the process.  Asked of the
+    caller's own tensors, since a copy of a leaf is no leaf."""
+    if torch.cuda.is_current_stream_capturing() and any(t is not None and nt.rules().kept_by_default_stream(t) for t in tensors):
         raise RuntimeError("a result computed on the default stream from the same leaf tensors is still alive: delete it before the capture "
-                           "(or compute it on another stream)")
+                           "(or compute it on another stream; without a backward pass, capture the call under torch.no_grad())")
 
 
 def once(backward):

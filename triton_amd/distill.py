@@ -93,13 +93,12 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     loss = host.distill_topk(logits, teacher_logits, teacher_indx, temperature) if host is not None else None
     if loss is not None:
         return loss
-    logits = check_logits(logits, temperature)
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distill_topk has no gradient for the teacher: pass its logits detached")
     if logits.requires_grad and torch.is_grad_enabled():
         check_capture(logits)
-        return _DistillTopK.apply(logits, teacher_logits, teacher_indx, temperature)
-    return _forward(logits, teacher_logits, teacher_indx, temperature, False)[0]
+        return _DistillTopK.apply(check_logits(logits, temperature), teacher_logits, teacher_indx, temperature)
+    return _forward(check_logits(logits, temperature), teacher_logits, teacher_indx, temperature, False)[0]
 
 
 from .torch_twins import distill_topk_torch  # noqa: E402,F401  (plain twin; never called by `distill_topk`)

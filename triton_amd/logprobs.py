@@ -158,11 +158,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0, tempe
     r = host.token_logprobs(logits, tokens, k, temperature) if host is not None else None
     if r is not None:
         return TokenLogprobs(*r)
-    logits = check_logits(logits, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         check_capture(logits)
+        logits = check_logits(logits, temperature)
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, k, temperature))
-    return TokenLogprobs(*_forward(logits, tokens, k, temperature, False)[:4])
+    return TokenLogprobs(*_forward(check_logits(logits, temperature), tokens, k, temperature, False)[:4])
 
 
 from .torch_twins import token_logprobs_torch  # noqa: E402,F401  (plain twin; never called by `token_logprobs`)
