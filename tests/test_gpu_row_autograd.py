@@ -1,4 +1,5 @@
-"""The row operators where autograd does more than call their backward pass: on other streams than the default one, in captures."""
+"""The row operators where autograd does more than call their backward pass: other streams than the default one, captures, hooks on saved tensors,
+recomputation."""
 import pytest
 import torch
 
@@ -75,3 +76,63 @@ def test_captures_of_what_was_made_of_a_living_graphs_leaves_are_refused(native,
                 assert torch.equal(out, living) and torch.equal(own, want) and g.isfinite().all()
             assert torch.autograd.grad(living.sum(), leaf)[0].isfinite().all()
             del living, before
+
+
+def _both(monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
+
+
+def _gradient(f, leaf):
+    y = f(leaf)
+    return y.detach(), torch.autograd.grad(y.square().sum(), leaf)[0]
+
+
+HOOKS = {"offloaded": (lambda t: t.cpu(), lambda t: t.cuda()),
+         "other strides": (lambda t: (t.ndim, t.t().contiguous() if t.ndim == 2 else torch.stack((t, t), -1)), lambda p: p[1].t() if p[0] == 2 else p[1][..., 0]),
+         "rows between others": (lambda t: torch.stack((t, t), 1), lambda t: t[:, 1])}
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("hook", list(HOOKS))
+def test_saved_tensors_that_come_back_otherwise(hook, native, monkeypatch):
+    _both(monkeypatch, native)
+    for dtype in (F32, BF16):
+        for f, t in _calls(*_inputs(dtype)):
+            leaf = t.clone().requires_grad_()
+            want = _gradient(f, leaf)
+            with torch.autograd.graph.saved_tensors_hooks(*HOOKS[hook]):
+                got = _gradient(f, leaf)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_saved_tensors_that_are_not_what_was_saved(native, monkeypatch):
+    """Refused by the backward pass on the host: another device, other sizes, a type that their place does not take."""
+    _both(monkeypatch, native)
+    wrong = {"left on the host": lambda t: t.cpu(), "fewer": lambda t: t[:-1], "in 64 bits": lambda t: t.double(), "flat": lambda t: t[None]}
+    for unpack in wrong.values():
+        for f, t in _calls(*_inputs()):
+            leaf = t.clone().requires_grad_()
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = f(leaf)
+            with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+                torch.autograd.grad(y.sum(), leaf)
+    x = torch.randn((6, 40), device="cuda", requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.to(BF16), lambda t: t.float()):  # (rows kept in fewer bits are those rows)
+        y = layer_norm(x)
+    g, = torch.autograd.grad(y.sum(), x)
+    assert g.dtype == F32 and g.isfinite().all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_in_the_backward_pass(reentrant, native, monkeypatch):
+    from torch.utils.checkpoint import checkpoint
+    _both(monkeypatch, native)
+    for f, t in _calls(*_inputs()):
+        leaf = t.clone().requires_grad_()
+        want = _gradient(f, leaf)
+        y = checkpoint(lambda u: f(u * 1), leaf, use_reentrant=reentrant)
+        y.square().sum().backward()
+        assert torch.equal(y, want[0]) and torch.equal(leaf.grad, want[1])

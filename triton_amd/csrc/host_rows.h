@@ -19,6 +19,7 @@ using torch::autograd::variable_list;
 bool row_dtype(const Tensor& t) {
   return t.scalar_type() == ScalarType::Float || t.scalar_type() == ScalarType::BFloat16 || t.scalar_type() == ScalarType::Half;
 }
+bool index_type(const Tensor& t) { return t.scalar_type() == ScalarType::Long || t.scalar_type() == ScalarType::Int; }
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool on_device_of(const Tensor& t, const Tensor& x) { return t.is_cuda() && t.get_device() == x.get_device(); }
 // Whether a backward pass from t runs a node on the default stream: the accumulation of a leaf's gradient, for the sake of a graph of this process that still
@@ -76,6 +77,15 @@ void backward_call(const Tensor& t, F&& f) {
   TORCH_CHECK(status == TK_OK, B.last_error());
 }
 
+// A saved tensor as the kernels take it.  Hooks on saved tensors (offloading, compression, recomputation) may give back another layout, which is copied; another shape
+// or device, or a type that its place does not take, is an error before anything reads it.
+enum class Kind { ROWS, INDEX, STATS };
+Tensor unpacked(const Tensor& t, at::IntArrayRef sizes, const Tensor& like, Kind kind) {
+  const bool type = t.defined() && (kind == Kind::ROWS ? row_dtype(t) : kind == Kind::INDEX ? index_type(t) : t.scalar_type() == ScalarType::Float);
+  TORCH_CHECK(type && t.sizes() == sizes && t.device() == like.device(), "a tensor saved by the forward pass came back with another shape, type or device");
+  return kind == Kind::STATS || t.dim() != 2 || t.stride(1) != 1 ? t.contiguous() : t;
+}
+
 // Gradients that are themselves to be differentiated (create_graph) raise an error when they are.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -114,11 +124,14 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
+    const Tensor x = unpacked(saved[0], grads[0].sizes(), grads[0], Kind::ROWS);
+    const int64_t cols = x.size(-1);
+    const Tensor w = saved[1].defined() ? unpacked(saved[1], {cols}, x, Kind::ROWS) : saved[1], b = saved[2].defined() ? unpacked(saved[2], {cols}, x, Kind::ROWS) : saved[2];
+    const Tensor stats = unpacked(saved[3], {2, x.numel() / cols}, x, Kind::STATS);
     // (the numbers of the inputs count the tensors that there are)
     const bool need_x = ctx->needs_input_grad(0), need_w = w.defined() && ctx->needs_input_grad(1),
                need_b = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
-    const Tensor dy = dense_rows(grads[0]) ? grads[0] : grads[0].contiguous();
+    const Tensor g0 = grads[0].to(x.scalar_type()), dy = dense_rows(g0) ? g0 : g0.contiguous();
     const LayerNormRows r(x), g(dy);
     Tensor dx, dw, db;
     backward_call(x, [&](void* stream) {
@@ -166,8 +179,6 @@ bool plain_logits(const Tensor* z, double temperature) {
   return z && z->is_cuda() && z->dim() == 2 && z->numel() != 0 && z->stride(1) == 1 && row_dtype(*z) && temperature >= 1.2e-38 && temperature <= 3e38
          && z->size(0) <= 0x7FFFFFFF && z->size(1) <= 1 << 30;
 }
-bool index_type(const Tensor& t) { return t.scalar_type() == ScalarType::Long || t.scalar_type() == ScalarType::Int; }
-
 tk_vocab_desc vocab_desc(const Tensor& z, double temperature) {
   tk_vocab_desc d = {};
   d.logits = z.data_ptr(), d.logits_dtype = dtype_code(z.scalar_type()), d.logits_stride_m = z.stride(0);
@@ -205,6 +216,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
     auto o = logprobs_forward(z, tokens, k, temperature, reinterpret_cast<void*>(stream), true);
     ctx->save_for_backward({z, tokens, o[1], o[2]});
     ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["vocab"] = z.size(1);
     ctx->set_materialize_grads(false);
     if (!k) return {o[0], o[1]};
     ctx->mark_non_differentiable({o[3], o[4]});
@@ -212,18 +224,22 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &z = saved[0], &tokens = saved[1];
     Tensor dz;
-    if (grads[0].defined() || grads[1].defined())
+    if (grads[0].defined() || grads[1].defined()) {
+      const Tensor& g = grads[0].defined() ? grads[0] : grads[1];
+      const int64_t T = g.size(0);
+      const Tensor z = unpacked(saved[0], {T, ctx->saved_data["vocab"].toInt()}, g, Kind::ROWS), tokens = unpacked(saved[1], {T}, g, Kind::INDEX);
+      const Tensor entropy = unpacked(saved[2], {T}, g, Kind::STATS), stats = unpacked(saved[3], {2, T}, g, Kind::STATS);
       backward_call(z, [&](void* stream) {
         dz = empty(z.sizes(), z.scalar_type(), z);
         tk_vocab_desc d = vocab_desc(z, ctx->saved_data["temperature"].toDouble());
         d.tokens = tokens.data_ptr(), d.tokens_i64 = tokens.scalar_type() == ScalarType::Long;
-        d.entropy = floats(saved[2]), d.stats = floats(saved[3]);
+        d.entropy = floats(entropy), d.stats = floats(stats);
         d.d_logprobs = row_gradient(grads[0], &d.d_logprobs_stride), d.d_entropy = row_gradient(grads[1], &d.d_entropy_stride);
         d.d_logits = dz.data_ptr(), d.d_logits_stride_m = dz.size(1);
         return B.token_logprobs_backward(&d, stream);
       });
+    }
     return once({dz, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
@@ -285,17 +301,21 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
     auto o = distill_forward(z, q, at, temperature, reinterpret_cast<void*>(stream), true);
     ctx->save_for_backward({z, q, at, o[1]});
     ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["vocab"] = z.size(1);
+    ctx->saved_data["entries"] = q.size(1);
     return o[0];
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor& z = saved[0];
+    const int64_t T = grads[0].size(0), K = ctx->saved_data["entries"].toInt();
+    const Tensor z = unpacked(saved[0], {T, ctx->saved_data["vocab"].toInt()}, grads[0], Kind::ROWS), q = unpacked(saved[1], {T, K}, z, Kind::ROWS);
+    const Tensor at = unpacked(saved[2], {T, K}, z, Kind::INDEX), stats = unpacked(saved[3], {4, T}, z, Kind::STATS);
     Tensor dz;
     backward_call(z, [&](void* stream) {
       dz = empty(z.sizes(), z.scalar_type(), z);
       tk_vocab_desc d = vocab_desc(z, ctx->saved_data["temperature"].toDouble());
-      set_teacher(d, saved[1], saved[2]);
-      d.stats = floats(saved[3]), d.teacher_stats = d.stats + 2 * z.size(0);
+      set_teacher(d, q, at);
+      d.stats = floats(stats), d.teacher_stats = d.stats + 2 * z.size(0);
       d.d_loss = row_gradient(grads[0], &d.d_loss_stride);
       d.d_logits = dz.data_ptr(), d.d_logits_stride_m = dz.size(1);
       return B.distill_topk_backward(&d, stream);

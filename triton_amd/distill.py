@@ -76,7 +76,8 @@ class _DistillTopK(torch.autograd.Function):
     @staticmethod
     @once
     def backward(ctx, d_loss):
-        return distill_topk_backward(*ctx.saved_tensors, d_loss, ctx.temperature), None, None, None
+        logits, teacher_logits, teacher_indx, stats = ctx.saved_tensors
+        return distill_topk_backward(logits, teacher_logits, teacher_indx, stats.contiguous(), d_loss, ctx.temperature), None, None, None
 
 
 def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indx: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:

@@ -100,7 +100,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dweight, dbias = layer_norm_backward(dy, x, mean, rstd, weight, bias, need_dx=need[0], need_dweight=need[1], need_dbias=need[2])
+        dx, dweight, dbias = layer_norm_backward(dy, x, mean.contiguous(), rstd.contiguous(), weight, bias, need_dx=need[0], need_dweight=need[1], need_dbias=need[2])
         return dx, dweight, dbias, None
 
 

@@ -143,7 +143,7 @@ class _TokenLogprobs(torch.autograd.Function):
         logits, tokens, entropy, stats = ctx.saved_tensors
         if d_logprobs is None and d_entropy is None:
             return None, None, None, None
-        return token_logprobs_backward(logits, tokens, entropy, stats, d_logprobs, d_entropy, ctx.temperature), None, None, None
+        return token_logprobs_backward(logits, tokens, entropy.contiguous(), stats.contiguous(), d_logprobs, d_entropy, ctx.temperature), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
