@@ -462,9 +462,9 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_backward_kernel(const void* 
 
 // The partial sums' sums: 16 columns a workgroup, four lanes a row of 64 bytes, 64 rows at a time and eight such requested together; then over the lanes and
 // waves that hold the same columns.
-__global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts, int n, int C, void* dw, int wt, void* db, int bt) {
+__global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts, int n, int C, void* dw, int wt, void* db, int bt, int c0) {
   __shared__ float acc[4][16];
-  const int c = (int)blockIdx.x * 16 + (int)(threadIdx.x & 3) * 4;
+  const int first = c0 + (int)blockIdx.x * 16, c = first + (int)(threadIdx.x & 3) * 4;
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -486,8 +486,8 @@ __global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[threadIdx.x >> 6][(threadIdx.x & 3) * 4 + e] = s[e];
   __syncthreads();
-  if (threadIdx.x < 16 && (int)blockIdx.x * 16 + (int)threadIdx.x < C)
-    store_any(out, blockIdx.y ? bt : wt, (int)blockIdx.x * 16 + threadIdx.x, (acc[0][threadIdx.x] + acc[1][threadIdx.x]) + (acc[2][threadIdx.x] + acc[3][threadIdx.x]));
+  if (threadIdx.x < 16 && first + (int)threadIdx.x < C)
+    store_any(out, blockIdx.y ? bt : wt, first + (int)threadIdx.x, (acc[0][threadIdx.x] + acc[1][threadIdx.x]) + (acc[2][threadIdx.x] + acc[3][threadIdx.x]));
 }
 
 // ---- rows of any length: read once for each step ----------------------------------------------------------------
@@ -645,7 +645,9 @@ struct Backward {
     if (sums) join(n);
   }
   void join(int n) const {
-    hipLaunchKernelGGL(layer_norm_sums_kernel, dim3((unsigned)cdiv(C, 16), 2), dim3(256), 0, s, parts, n, (int)C, dw, wt, db, bt);
+    constexpr int64_t most = 1 << 27;  // columns of a launch: sixteen threads each, of which 2^32 are its limit
+    for (int64_t c0 = 0; c0 < C; c0 += most)
+      hipLaunchKernelGGL(layer_norm_sums_kernel, dim3((unsigned)cdiv(C - c0 < most ? C - c0 : most, 16), 2), dim3(256), 0, s, parts, n, (int)C, dw, wt, db, bt, (int)c0);
   }
 };
 
