@@ -21,3 +21,19 @@ def test_parameters_of_many_columns(C):
     assert dx is None
     assert torch.equal(db, dy[0].float())
     assert torch.equal(dw, dy[0].float() * ((x[0].float() - 0.25) * 1.5))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1.1**0.5, 0.7])
+def test_sums_of_long_rows(dtype, size):
+    """Elements of one size, whose squares each round the same way when they are added to a large sum; gradients likewise."""
+    C = 2**24 + 300
+    sign = torch.ones(C)
+    sign[1::2] = -1
+    x = (sign * size).to(dtype).cuda()[None]
+    dy = (sign * 0.3 + 0.2).to(dtype).cuda()[None]
+    y, mean, rstd = layer_norm_forward(x)
+    orc.check(y, *orc.layer_norm(x), "y")
+    want = 1 / (x.double().square().mean().item() + 1e-5)**0.5
+    assert abs(rstd.item() - want) <= (orc.LN_DEPTH / 2 + 8) * orc.U * want
+    orc.check(layer_norm_backward(dy, x, mean, rstd)[0], *orc.layer_norm_backward(dy, x)["dx"], "dx")

@@ -492,41 +492,58 @@ __global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts
 
 // ---- rows of any length: read once for each step ----------------------------------------------------------------
 
+// A thread's sums of N numbers over the columns of a row that are its own: add(column, sums).  Sums of 64, of 64 such and of these, so that
+// rows of 2^24 columns add no more than 64 numbers one after the other, and rows of 2^30 1024 (one sum for all of them: 4 million).
+template <int N, class F>
+__device__ __forceinline__ void long_sums(int64_t C, float (&out)[N], F&& add) {
+  constexpr int64_t STEP = 256, FEW = STEP * 64, MANY = FEW * 64;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = 0.f;
+  for (int64_t c0 = threadIdx.x; c0 < C; c0 += MANY) {
+    float many[N] = {};
+    for (int64_t c1 = c0; c1 < C && c1 < c0 + MANY; c1 += FEW) {
+      float few[N] = {};
+      const int64_t end = C < c1 + FEW ? C : c1 + FEW;
+      for (int64_t c = c1; c < end; c += STEP) add(c, few);
+#pragma unroll
+      for (int i = 0; i < N; ++i) many[i] += few[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] += many[i];
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void layer_norm_long_kernel(const void* x, int64_t M, int64_t C, int64_t sx, const void* w, int wt, const void* b, int bt,
                                                               float eps, void* y, int64_t sy, float* mean, float* rstd) {
   __shared__ StatisticsLds<4> lds;
   for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-    const auto sum = [&](float scale) {
-      float s = 0.f;
-      for (int64_t c = threadIdx.x; c < C; c += 256) s += RowType<DT>::load(x, m * sx + c) * scale;
-      return s;
-    };
-    float mu = block_sum<256>(sum(1.f), lds.sum) / (float)C;
-    if (!(fabsf(mu) < __builtin_inff())) mu = block_sum<256>(sum(0x1p-32f), lds.scaled) / (float)C * 0x1p32f;
-    float s = 0.f;
-    for (int64_t c = threadIdx.x; c < C; c += 256) {
-      const float d = RowType<DT>::load(x, m * sx + c) - mu;
-      s = fmaf(d, d, s);
+    const auto element = [&](int64_t c) { return RowType<DT>::load(x, m * sx + c); };
+    float s[1], d[2];
+    long_sums(C, s, [&](int64_t c, float (&o)[1]) { o[0] += element(c); });
+    float mu = block_sum<256>(s[0], lds.sum) / (float)C;
+    if (!(fabsf(mu) < __builtin_inff())) {
+      long_sums(C, s, [&](int64_t c, float (&o)[1]) { o[0] += element(c) * 0x1p-32f; });
+      mu = block_sum<256>(s[0], lds.scaled) / (float)C * 0x1p32f;
     }
-    float var = block_sum<256>(s, lds.squares) / (float)C;
+    long_sums(C, s, [&](int64_t c, float (&o)[1]) { o[0] = fmaf(element(c) - mu, element(c) - mu, o[0]); });
+    float var = block_sum<256>(s[0], lds.squares) / (float)C;
     if (beside_large_mean(mu, var))
       for (int turn = 0; turn < 2; ++turn) {
-        float s1 = 0.f, s2 = 0.f;
-        for (int64_t c = threadIdx.x; c < C; c += 256) {
-          const float d = RowType<DT>::load(x, m * sx + c) - mu;
-          s1 += d;
-          s2 = fmaf(d, d, s2);
-        }
-        row_sums<256>(s1, s2, lds.spread[turn]);
-        const Spread spread(s1 / (float)C, s2 / (float)C);
+        long_sums(C, d, [&](int64_t c, float (&o)[2]) {
+          const float x = element(c) - mu;
+          o[0] += x;
+          o[1] = fmaf(x, x, o[1]);
+        });
+        row_sums<256>(d[0], d[1], lds.spread[turn]);
+        const Spread spread(d[0] / (float)C, d[1] / (float)C);
         mu += spread.rest;
         var = spread.var;
         if (!spread.again) break;
       }
     const float r = 1.0f / sqrtf(var + eps);
     for (int64_t c = threadIdx.x; c < C; c += 256) {
-      const float h = (RowType<DT>::load(x, m * sx + c) - mu) * r;
+      const float h = (element(c) - mu) * r;
       RowType<DT>::store(y, m * sy + c, fmaf(h, w ? load_any(w, wt, c) : 1.0f, b ? load_any(b, bt, c) : 0.0f));
     }
     if (threadIdx.x == 0 && mean) {
@@ -542,14 +559,13 @@ __global__ __launch_bounds__(256) void layer_norm_dx_long_kernel(const void* dy,
   __shared__ float buf[2][4];
   for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
     const float mu = mean[m], r = rstd[m];
-    float sg = 0.f, sgh = 0.f;
-    for (int64_t c = threadIdx.x; c < C; c += 256) {
+    float sums[2];
+    long_sums(C, sums, [&](int64_t c, float (&o)[2]) {
       const float g = RowType<DT>::load(dy, m * sdy + c) * (w ? load_any(w, wt, c) : 1.0f);
-      sg += g;
-      sgh = fmaf(g, (RowType<DT>::load(x, m * sx + c) - mu) * r, sgh);
-    }
-    sg = block_sum<256>(sg, buf[0]) / (float)C;
-    sgh = block_sum<256>(sgh, buf[1]) / (float)C;
+      o[0] += g;
+      o[1] = fmaf(g, (RowType<DT>::load(x, m * sx + c) - mu) * r, o[1]);
+    });
+    const float sg = block_sum<256>(sums[0], buf[0]) / (float)C, sgh = block_sum<256>(sums[1], buf[1]) / (float)C;
     for (int64_t c = threadIdx.x; c < C; c += 256) {
       const float g = RowType<DT>::load(dy, m * sdy + c) * (w ? load_any(w, wt, c) : 1.0f), h = (RowType<DT>::load(x, m * sx + c) - mu) * r;
       RowType<DT>::store(dx, m * sdx + c, (g - sg - h * sgh) * r);
