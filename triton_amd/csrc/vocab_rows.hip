@@ -335,6 +335,8 @@ struct Workgroup {
     typedef RowType<DT> R;
     constexpr int VE = R::VE, BITS = Key<DT>::BITS, OWN = 8;
     const int groups = (end + GROUP - 1) / GROUP;
+    // (four waves have passed a barrier since the pass wrote the groups' numbers; one has not, and its lanes read each other's)
+    if constexpr (WAVES == 1) __syncthreads();
     if (threadIdx.x == 0) lds.n_groups = lds.n_found = 0;
     uint32_t most = 0, own[OWN];  // (the first OWN of a thread's stay in registers)
 #pragma unroll
