@@ -136,3 +136,22 @@ def test_recomputed_in_the_backward_pass(reentrant, native, monkeypatch):
         y = checkpoint(lambda u: f(u * 1), leaf, use_reentrant=reentrant)
         y.square().sum().backward()
         assert torch.equal(y, want[0]) and torch.equal(leaf.grad, want[1])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_other_transforms_are_refused(native, monkeypatch):
+    """Forward mode, whose dual tensors ask for no gradient, with and without a leaf beside them; vmap and grad of torch.func."""
+    import torch.autograd.forward_ad as fwad
+    _both(monkeypatch, native)
+    z, tokens, q, at, x, w, b = _inputs()
+    for f, t in _calls(z, tokens, q, at, x, w, b) + ((lambda s: distill_topk(z, s, at), q), (lambda s: layer_norm(x.clone().requires_grad_(), s, b), w)):
+        want = f(t)
+        with fwad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f(fwad.make_dual(t, torch.ones_like(t)))
+            assert torch.equal(f(t), want)
+        for call in (lambda: torch.func.jvp(f, (t, ), (torch.ones_like(t), )), lambda: torch.func.vmap(f)(torch.stack((t, t))),
+                     lambda: torch.func.grad(lambda s: f(s).sum())(t)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        assert torch.equal(f(t), want)

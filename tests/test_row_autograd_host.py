@@ -36,3 +36,18 @@ def test_captures_are_checked_for_the_tensors_of_the_caller(monkeypatch):
                 f(leaf.requires_grad_())
             with pytest.raises(RuntimeError, match="HIP device"), torch.no_grad():
                 f(leaf)
+
+
+def test_forward_mode_is_refused():
+    """Dual tensors ask for no gradient; without a refusal the result would be that of the primal, with a derivative of zero."""
+    import torch.autograd.forward_ad as fwad
+    z, tokens, q, at, x, w, b = _inputs()
+    calls = _calls() + ((lambda t: distill_topk(z, t, at), q), )
+    for f, t in calls:
+        with pytest.raises(NotImplementedError, match="forward mode"), fwad.dual_level():
+            f(fwad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward mode|storage"):
+            torch.func.jvp(f, (t, ), (torch.ones_like(t), ))
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="HIP device"):  # (others are taken in such a level)
+            fwad.make_dual(t, torch.ones_like(t))
+            f(t)

@@ -5,6 +5,8 @@ import functools
 
 import torch
 
+from torch.autograd import forward_ad
+
 from . import _native as nt
 
 
@@ -15,6 +17,12 @@ def check_capture(*tensors):
     if torch.cuda.is_current_stream_capturing() and any(t is not None and nt.rules().kept_by_default_stream(t) for t in tensors):
         raise RuntimeError("a result computed on the default stream from the same leaf tensors is still alive: delete it before the capture "
                            "(or compute it on another stream; without a backward pass, capture the call under torch.no_grad())")
+
+
+def check_forward_mode(who, *tensors):
+    """Refuses dual tensors, which ask for no gradient: an operator that computes from their primals alone would drop their tangents."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no derivative in forward mode")
 
 
 def once(backward):

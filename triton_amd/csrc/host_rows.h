@@ -20,6 +20,8 @@ bool row_dtype(const Tensor& t) {
   return t.scalar_type() == ScalarType::Float || t.scalar_type() == ScalarType::BFloat16 || t.scalar_type() == ScalarType::Half;
 }
 bool index_type(const Tensor& t) { return t.scalar_type() == ScalarType::Long || t.scalar_type() == ScalarType::Int; }
+// A dual tensor's tangent is dropped by whoever reads its data: such calls are left to the Python path, which refuses them.
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool on_device_of(const Tensor& t, const Tensor& x) { return t.is_cuda() && t.get_device() == x.get_device(); }
 // Whether a backward pass from t runs a node on the default stream: the accumulation of a leaf's gradient, for the sake of a graph of this process that still
@@ -156,10 +158,10 @@ PyObject* run_layer_norm(PyObject* const* v) {
     PyErr_Clear();
     return none();
   }
-  if (!x || !x->is_cuda() || x->dim() < 1 || x->numel() == 0 || !row_dtype(*x) || !dense_rows(*x) || !(eps >= 0. && eps <= 3e38)) return none();
+  if (!x || !x->is_cuda() || x->dim() < 1 || x->numel() == 0 || !row_dtype(*x) || !dense_rows(*x) || dual(*x) || !(eps >= 0. && eps <= 3e38)) return none();
   for (auto [t, o] : {std::pair(w, v[1]), std::pair(b, v[2])}) {
     if (!t && !is_none(o)) return none();
-    if (t && (!on_device_of(*t, *x) || !row_dtype(*t) || t->dim() != 1 || t->size(0) != x->size(-1) || !t->is_contiguous())) return none();
+    if (t && (!on_device_of(*t, *x) || !row_dtype(*t) || t->dim() != 1 || t->size(0) != x->size(-1) || !t->is_contiguous() || dual(*t))) return none();
   }
   if (dispatcher_heard()) return none();
   auto stream = stream_of(*x);
@@ -177,7 +179,7 @@ PyObject* run_layer_norm(PyObject* const* v) {
 
 bool plain_logits(const Tensor* z, double temperature) {
   return z && z->is_cuda() && z->dim() == 2 && z->numel() != 0 && z->stride(1) == 1 && row_dtype(*z) && temperature >= 1.2e-38 && temperature <= 3e38
-         && z->size(0) <= 0x7FFFFFFF && z->size(1) <= 1 << 30;
+         && z->size(0) <= 0x7FFFFFFF && z->size(1) <= 1 << 30 && !dual(*z);
 }
 tk_vocab_desc vocab_desc(const Tensor& z, double temperature) {
   tk_vocab_desc d = {};
@@ -334,7 +336,7 @@ PyObject* run_distill_topk(PyObject* const* v) {
   }
   if (!plain_logits(z, temperature) || !q || !at) return none();
   if (!on_device_of(*q, *z) || !row_dtype(*q) || q->dim() != 2 || q->size(0) != z->size(0) || q->size(1) < 1 || q->size(1) > TK_VOCAB_MAX_TEACHER
-      || q->stride(1) != 1 || wants_grad(*q))
+      || q->stride(1) != 1 || wants_grad(*q) || dual(*q))
     return none();
   if (!on_device_of(*at, *z) || !index_type(*at) || at->sizes() != q->sizes() || at->stride(1) != 1) return none();
   if (dispatcher_heard()) return none();

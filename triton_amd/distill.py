@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nt
-from ._autograd import check_capture, once
+from ._autograd import check_capture, check_forward_mode, once
 from .logprobs import DTYPES, check_index, check_logits, check_saved, logits_desc, row_gradient, workspace
 
 MAX_TEACHER = 1024
@@ -94,6 +94,7 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     loss = host.distill_topk(logits, teacher_logits, teacher_indx, temperature) if host is not None else None
     if loss is not None:
         return loss
+    check_forward_mode("distill_topk", logits, teacher_logits)
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distill_topk has no gradient for the teacher: pass its logits detached")
     if logits.requires_grad and torch.is_grad_enabled():

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _native as nt
-from ._autograd import check_capture, once
+from ._autograd import check_capture, check_forward_mode, once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -116,6 +116,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     y = host.layer_norm(x, weight, bias, eps) if host is not None else None
     if y is not None:
         return y
+    check_forward_mode("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         check_capture(x, weight, bias)
         return _LayerNorm.apply(x, weight, bias, eps)

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _native as nt
-from ._autograd import check_capture, once
+from ._autograd import check_capture, check_forward_mode, once
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_ROWS, MAX_COLUMNS = 2**31 - 1, 2**30
@@ -158,6 +158,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0, tempe
     r = host.token_logprobs(logits, tokens, k, temperature) if host is not None else None
     if r is not None:
         return TokenLogprobs(*r)
+    check_forward_mode("token_logprobs", logits)
     if logits.requires_grad and torch.is_grad_enabled():
         check_capture(logits)
         logits = check_logits(logits, temperature)
