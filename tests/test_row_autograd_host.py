@@ -51,3 +51,15 @@ def test_forward_mode_is_refused():
         with fwad.dual_level(), pytest.raises(RuntimeError, match="HIP device"):  # (others are taken in such a level)
             fwad.make_dual(t, torch.ones_like(t))
             f(t)
+
+
+def test_forward_mode_is_refused_by_the_other_differentiable_operators():
+    import torch.autograd.forward_ad as fwad
+    from triton_kernels.reduce import reduce
+    from triton_kernels.topk import topk
+    x, y, scale = torch.randn((T, 8)), torch.randn((T, 2, 16)), torch.rand((T, 2, 1))
+    for f, t in ((lambda s: topk(s, 2), x), (lambda s: reduce(s, 1), y), (lambda s: reduce(y, 1, scale=s), scale)):
+        with pytest.raises(NotImplementedError, match="forward mode"), fwad.dual_level():
+            f(fwad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(RuntimeError, match="HIP device"):
+            f(t)

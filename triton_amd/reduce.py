@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from . import _native as nt
+from ._autograd import check_forward_mode
 from .numerics import InFlexData, OutFlexData
 from .specialize import FnSpecs
 
@@ -102,6 +103,7 @@ def reduce(x: torch.Tensor, dim: int, mask: Optional[torch.Tensor] = None, scale
         raise NotImplementedError("reduce supports dim == 1 (the k-way combine)")
     if y_dtype is not None and y_dtype != x.dtype:
         raise NotImplementedError("reduce keeps the input dtype")
+    check_forward_mode("reduce", x, scale)
     if x.requires_grad and torch.is_grad_enabled():
         return _ReduceAutograd.apply(x, mask, scale, y), None
     return _reduce_forward(x, mask, scale, y)

@@ -13,6 +13,7 @@ from typing import Optional, Union
 import torch
 
 from . import _native as nt
+from ._autograd import check_forward_mode
 from .tensor import SparseMatrix, Tensor, wrap_torch_tensor
 from .tensor_details.bitmatrix import BitmatrixMetadata, _route
 from .tensor_details.dtype import BIT
@@ -120,6 +121,7 @@ def topk(x: Union[Tensor, torch.Tensor], k: int, apply_softmax: bool = True, dim
     assert dim == 1
     if all_gather or symm_mem_pool is not None:
         raise NotImplementedError("all_gather / symmetric-memory outputs are multi-GPU features")
+    check_forward_mode("topk", x)
     if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
         y_vals, y_indx, bm_t, col_sum, col_sorted, row_sorted = TopK.apply(x, k, apply_softmax, y_indx, n_rows)
         T, E = x.shape
