@@ -155,3 +155,23 @@ def test_other_transforms_are_refused(native, monkeypatch):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 call()
         assert torch.equal(f(t), want)
+
+
+@pytest.mark.parametrize("turned", [True, False])
+@pytest.mark.parametrize("native", [True, False])
+def test_results_changed_in_place(native, turned, monkeypatch):
+    """A mask over the log probabilities before they are added up; the entropies are theirs alone."""
+    _both(monkeypatch, native)
+    z, tokens, *_ = _inputs()
+    leaf = (z.t().contiguous().t() if turned else z.clone()).requires_grad_()
+    mask = (torch.arange(T, device="cuda") % 3 != 0).float()
+    want = token_logprobs(leaf, tokens)
+    g, = torch.autograd.grad((want.logprobs * mask).sum() + want.entropy.sum(), leaf)
+    r = token_logprobs(leaf, tokens)
+    r.logprobs.mul_(mask)
+    assert torch.equal(r.entropy, want.entropy) and torch.equal(r.logprobs, want.logprobs * mask)
+    assert torch.equal(torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), leaf)[0], g)
+    y = layer_norm(z.clone().requires_grad_())
+    loss = distill_topk(leaf, *_inputs()[2:4])
+    for out in (y, loss):
+        out.mul_(2).sum().backward()

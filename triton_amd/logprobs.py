@@ -89,7 +89,7 @@ def _forward(logits, tokens, k, temperature, with_stats):
     dev = logits.device
     nt.require_gpu(logits, "logits")
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    logprobs, entropy = torch.empty((2, T), dtype=torch.float32, device=dev)
+    logprobs, entropy = (torch.empty((T, ), dtype=torch.float32, device=dev) for _ in range(2))  # (not of one buffer: a caller may change one of them in place)
     stats = torch.empty((2, T), dtype=torch.float32, device=dev) if with_stats else None
     top_logprobs = torch.empty((T, k), dtype=torch.float32, device=dev) if k else None
     top_indx = torch.empty((T, k), dtype=torch.int32, device=dev) if k else None
