@@ -348,8 +348,10 @@ def layer_norm_torch(x, weight=None, bias=None, eps: float = 1e-5):
 
 
 def _log_softmax_rows(logits, temperature):
-    """fp32 log probabilities; rows of -inf alone stay -inf."""
+    """fp32 log probabilities; rows of -inf alone stay -inf, and rows of nothing empty."""
     x = logits.to(torch.float32)
+    if x.shape[1] == 0:
+        return x
     m = x.amax(1, keepdim=True)
     z = (x - torch.where(m == float("-inf"), torch.zeros_like(m), m)) / temperature
     s = z.exp().sum(1, keepdim=True)
