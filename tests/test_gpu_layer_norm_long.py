@@ -1,4 +1,5 @@
-"""Layer norm of rows far longer than a model's: sums of tens of thousands of numbers a lane, and parameters of more columns than one launch has threads for."""
+"""Layer norm of long rows and of many: sums of tens of thousands of numbers a lane, parameters of more columns than one launch has threads for,
+workgroups that take several of the longest rows that fit one, fp16."""
 import pytest
 import torch
 
@@ -37,3 +38,33 @@ def test_sums_of_long_rows(dtype, size):
     want = 1 / (x.double().square().mean().item() + 1e-5)**0.5
     assert abs(rstd.item() - want) <= (orc.LN_DEPTH / 2 + 8) * orc.U * want
     orc.check(layer_norm_backward(dy, x, mean, rstd)[0], *orc.layer_norm_backward(dy, x)["dx"], "dx")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float16])
+@pytest.mark.parametrize("M,C", [(600, 8200), (1100, 16384), (1030, 12001)])
+def test_many_rows_of_a_workgroup_each(M, C, dtype):
+    """More rows of 8193 to 16384 columns than the backward pass has workgroups for: the two buffers of its barrier, the row requested ahead, the running sums."""
+    g = torch.Generator(device="cuda").manual_seed(M + C)
+    x = (torch.randn((M, C), generator=g, device="cuda") * 1.5 + 0.3).to(dtype)
+    dy = torch.randn((M, C), generator=g, device="cuda").to(dtype)
+    w, b = torch.randn(C, generator=g, device="cuda"), torch.randn(C, generator=g, device="cuda")
+    y, mean, rstd = layer_norm_forward(x, w, b)
+    orc.check(y, *orc.layer_norm(x, w, b), "y")
+    want = orc.layer_norm_backward(dy, x, w, 1e-5, b)
+    for name, got in zip(("dx", "dweight", "dbias"), layer_norm_backward(dy, x, mean, rstd, w, b)):
+        orc.check(got, *want[name], name)
+    for name, got in zip(("dx", "dweight", "dbias"), layer_norm_backward(dy, x, mean, rstd, w, b, need_dx=False)):
+        assert got is None if name == "dx" else orc.check(got, *want[name], name) is None
+
+
+@pytest.mark.parametrize("M,C", [(4099, 256), (4099, 40), (6000, 1023), (2050, 7), (2048, 512), (2047, 513), (2049, 4096), (2200, 4100), (9001, 130)])
+def test_many_rows_in_fp16(M, C):
+    g = torch.Generator(device="cuda").manual_seed(M + C)
+    x, dy = (torch.randn((M, C), generator=g, device="cuda") for _ in range(2))
+    x, dy = (x * 1.5 + 0.3).half(), dy.half()
+    w, b = torch.randn(C, generator=g, device="cuda"), torch.randn(C, generator=g, device="cuda")
+    y, mean, rstd = layer_norm_forward(x, w, b)
+    orc.check(y, *orc.layer_norm(x, w, b), "y")
+    want = orc.layer_norm_backward(dy, x, w, 1e-5, b)
+    for name, got in zip(("dx", "dweight", "dbias"), layer_norm_backward(dy, x, mean, rstd, w, b)):
+        orc.check(got, *want[name], name)

@@ -1,4 +1,4 @@
-"""The row operators' twins where there is little to compute: no teacher entries, no rows, no alternatives, one column."""
+"""The row operators' twins and workspaces where there is little to compute: no teacher entries, no rows, no alternatives, one column."""
 import pytest
 import torch
 
@@ -31,3 +31,14 @@ def test_other_twins(T, V):
         assert r.logprobs.shape == r.entropy.shape == (T, )
         assert (r.top_indx is None) == (k == 0) and (k == 0 or r.top_indx.shape == r.top_logprobs.shape == (T, k))
     assert layer_norm_torch(z).shape == (T, V)
+
+
+def test_no_rows_need_no_workspace():
+    from triton_amd import _native as nt
+    lib = nt.lib()
+    for M, C in ((0, 8), (0, 20000), (5, 0), (-1, 8)):
+        assert lib.tk_layer_norm_backward_workspace_bytes(M, C) == 0
+    assert lib.tk_layer_norm_backward_workspace_bytes(3, 100) == 2 * 3 * 100 * 4
+    for T, V, k in ((0, 50000, 20), (-1, 50000, 0), (4, 0, 0), (2000, 50000, 20)):
+        assert lib.tk_vocab_workspace_bytes(T, V, k) == 0
+    assert lib.tk_vocab_workspace_bytes(1, 50000, 20) > 0
