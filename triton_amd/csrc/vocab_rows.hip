@@ -9,7 +9,7 @@ namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
 
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = (float)(1.44269504088896340736 - (double)LOG2E), LN2 = 0.69314718055994530942f;
 constexpr int MAX_GRID = 1 << 23;  // workgroups of a launch (2^32 threads are its limit)
 constexpr int GROUP = 64;      // consecutive columns whose largest logit is kept while a row streams by
 constexpr int MAX_CHUNKS = 256;  // pieces that a row is split into where there are few rows
@@ -642,7 +642,9 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
   const int c0 = (int)(place % (unsigned)n_chunks) * chunk;
   const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
   void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * R::BYTES;
+  // ln s / ln 2 in two parts: rounded to one number it is off by 7e-7 near 17, and every p of the row with it.  The second part is a factor of the row's A and B.
   const float m = d.stats[t], log_s = d.stats[(int64_t)d.n_rows + t], log2_s = log_s * LOG2E;
+  const float rest = __builtin_amdgcn_exp2f(-fmaf(log_s, LOG2E_REST, fmaf(log_s, LOG2E, -log2_s)));
   float A, B = 0.f, more = 0.f, qm = 0.f, log_qs = 0.f;
   int token = -1;
   bool zero;
@@ -662,9 +664,10 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
     B = -g_h * LN2 * sc.inv_t;
     more = g_lp * sc.inv_t;
   }
+  const float Ap = A * rest, Bp = B * rest;
   const auto gradient = [&](float x) {
     const float d2 = fmaf(x - m, sc.c2, -log2_s), p = __builtin_amdgcn_exp2f(d2);
-    return OP == DISTILL ? p * A : p * fmaf(fmaxf(d2, D_MIN), B, A);
+    return OP == DISTILL ? p * Ap : p * fmaf(fmaxf(d2, D_MIN), Bp, Ap);
   };
   for (int base = c0; base < c1; base += STEP) {
     const int at = base + (int)threadIdx.x * VE;
