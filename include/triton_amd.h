@@ -526,7 +526,7 @@ int32_t tk_quant_fp8_rows(const void* x, int32_t dtype, int64_t M, int64_t K, in
                           int64_t stride_qm, float* scales, tk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
- * Row operators around the experts
+ * Row operators around the experts.  Outputs do not overlap inputs.
  * ---------------------------------------------------------------------------------------------- */
 
 /*

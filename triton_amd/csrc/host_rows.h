@@ -1,9 +1,9 @@
-// The row operators' half of the native host path (included by host_path.cpp): layer norm, token log probabilities and distillation from top
-// logits, with their autograd nodes.
+// The row operators' half of the native host path (included by host_path.cpp): layer norm, token log probabilities and distillation from
+// top logits, with their autograd nodes.
 //
-// What bounds it: a training step's call makes an autograd node, whose backward pass runs on a thread of its own.  With nodes written in Python that
-// thread and the caller's pass the interpreter's lock to and fro: some 100 us a call of forward and backward where the kernels take 10.
-// These nodes need the lock for the stream's address only.
+// What bounds it: a training step's call makes an autograd node, whose backward pass runs on a thread of its own.  With nodes written in
+// Python that thread and the caller's pass the interpreter's lock to and fro: some 100 us a call of forward and backward where the kernels
+// take 10.  These nodes need the lock for the stream's address only.
 #pragma once
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -24,8 +24,9 @@ bool index_type(const Tensor& t) { return t.scalar_type() == ScalarType::Long ||
 bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool on_device_of(const Tensor& t, const Tensor& x) { return t.is_cuda() && t.get_device() == x.get_device(); }
-// Whether a backward pass from t runs a node on the default stream: the accumulation of a leaf's gradient, for the sake of a graph of this process that still
-// lives, or an operation in front of t.  A backward pass that is captured would make the default stream wait for the capture, which ends the process.
+// Whether a backward pass from t runs a node on the default stream: the accumulation of a leaf's gradient, for the sake of a graph of this
+// process that still lives, or an operation in front of t.  A backward pass that is captured would make the default stream wait for the
+// capture, which ends the process.
 bool on_default_stream(torch::autograd::Node* node) {
   const auto stream = node->stream();
   return stream && stream->id() == 0;
@@ -47,8 +48,9 @@ bool kept_by_default_stream(const Tensor& t) {
   }
   return false;
 }
-// Whether the current stream, `stream`, is being captured (the default stream never is).  The callers leave captured calls with such leaves to the Python path, which
-// refuses them; outside a capture the default stream may well wait, and the nodes of this file are 50 to 70 us a call faster than Python's.
+// Whether the current stream, `stream`, is being captured (the default stream never is).  The callers leave captured calls with such leaves
+// to the Python path, which refuses them; outside a capture the default stream may well wait, and the nodes of this file are 50 to 70 us a
+// call faster than Python's.
 bool captured(void* stream) {
   if (!stream) return false;
   Ref r(PyObject_CallNoArgs(B.capturing));
@@ -79,8 +81,8 @@ void backward_call(const Tensor& t, F&& f) {
   TORCH_CHECK(status == TK_OK, B.last_error());
 }
 
-// A saved tensor as the kernels take it.  Hooks on saved tensors (offloading, compression, recomputation) may give back another layout, which is copied; another shape
-// or device, or a type that its place does not take, is an error before anything reads it.
+// A saved tensor as the kernels take it.  Hooks on saved tensors (offloading, compression, recomputation) may give back another layout,
+// which is copied; another shape or device, or a type that its place does not take, is an error before anything reads it.
 enum class Kind { ROWS, INDEX, STATS };
 Tensor unpacked(const Tensor& t, at::IntArrayRef sizes, const Tensor& like, Kind kind) {
   const bool type = t.defined() && (kind == Kind::ROWS ? row_dtype(t) : kind == Kind::INDEX ? index_type(t) : t.scalar_type() == ScalarType::Float);

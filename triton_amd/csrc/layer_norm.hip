@@ -1,6 +1,9 @@
-// Layer norm of rows, forward and backward.  Both move each element of the rows once a pass and are bound by that; what the kernels
-// below arrange is that a row stays in registers between its reductions and its results, and that the sums over rows stay
-// in registers over many rows.
+// Layer norm of rows, forward and backward.  Both move each element of the rows once a pass and are bound by that; what the kernels below
+// arrange is that a row stays in registers between its reductions and its results, and that the sums over rows stay in registers over many
+// rows.
+//
+// Times in the comments are medians over replays of a captured graph of a few calls on the same buffers, so that what fits the last-level
+// cache (256 MB) may come from it; where two ways stand side by side, both were timed on one card when the choice between them was made.
 #include "row_math.h"
 
 namespace tk {
@@ -48,8 +51,8 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
   return v;
 }
 
-// Between two passes over a row's registers: without it the compiler keeps the first pass' 32-bit elements (and what else of it the second one
-// could use) beside the packed ones, at up to four times the registers.
+// Between two passes over a row's registers: without it the compiler keeps the first pass' 32-bit elements (and what else of it the second
+// one could use) beside the packed ones, at up to four times the registers.
 template <int N>
 __device__ __forceinline__ void once_more(row_u32x4 (&v)[N]) {
 #pragma unroll
@@ -64,7 +67,8 @@ __device__ __forceinline__ float mean_of(float s, float C, float inv_c) {
 
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
-// The sums of two numbers over the TPR lanes that share a row, in each of them; from 256 lanes on through `buf` (a pair a wave) and one barrier.
+// The sums of two numbers over the TPR lanes that share a row, in each of them; from 256 lanes on through `buf` (a pair a wave) and one
+// barrier.
 template <int TPR>
 __device__ __forceinline__ void row_sums(float& a, float& b, float2* buf) {
   if constexpr (TPR < 256) {
@@ -110,8 +114,8 @@ struct StatisticsLds {
   float2 spread[2][WAVES];
 };
 
-// One row's mean and reciprocal deviation from its registers (TPR lanes a row, NV vectors of 16 bytes a lane, the first FULL of them within any
-// row that comes here): the mean first, then the distances from it.  `lds`: not used below 256 lanes a row.
+// One row's mean and reciprocal deviation from its registers (TPR lanes a row, NV vectors of 16 bytes a lane, the first FULL of them within
+// any row that comes here): the mean first, then the distances from it.  `lds`: not used below 256 lanes a row.
 template <int DT, int TPR, int NV, int FULL>
 __device__ __forceinline__ void row_statistics(row_u32x4 (&raw)[NV], int lane, int C, float inv_c, float eps, StatisticsLds<16>* lds,
                                                float* mean, float* rstd) {
@@ -167,7 +171,8 @@ __device__ __forceinline__ void row_statistics(row_u32x4 (&raw)[NV], int lane, i
   *rstd = 1.0f / sqrtf(var + eps);
 }
 
-// A row's vectors, and what is to be done with them before they are used: elements behind the row's end are zero then.  (Rows shorter than a vector come element by element.)
+// A row's vectors, and what is to be done with them before they are used: elements behind the row's end are zero then.  (Rows shorter than
+// a vector come element by element.)
 template <int DT, int TPR, int NV, int FULL>
 __device__ __forceinline__ void load_row(const void* x, int64_t at, int lane, int C, row_u32x4 (&raw)[NV]) {
   typedef RowType<DT> R;
@@ -227,8 +232,9 @@ __global__ __launch_bounds__(block_of(TPR)) void layer_norm_kernel(const void* x
   }
 }
 
-// Many rows (16384 x 2880 bf16 41.9 us, 4.5 TB/s both ways, 135168 x 128 18.5 us, 3.7): workgroups of four waves that stay, the weights read once each, into
-// registers (up to 16 elements a lane) or LDS; a group's next rows are requested before the present ones are summed.  AT rows a group at a time, so that short rows keep as many bytes under way as long ones.
+// Many rows (16384 x 2880 bf16 34.0 us, 5.5 TB/s both ways, 135168 x 128 16.4 us, 4.2): workgroups of four waves that stay, the weights
+// read once each, into registers (up to 16 elements a lane) or LDS; a group's next rows are requested before the present ones are summed.
+// AT rows a group at a time, so that short rows keep as many bytes under way as long ones.
 template <int DT, int TPR, int NV, int FULL>
 __global__ __launch_bounds__(256) void layer_norm_many_kernel(const void* x, int64_t M, int C, int64_t sx, const void* w, int wt, const void* b, int bt,
                                                               float eps, void* y, int64_t sy, float* mean, float* rstd) {
@@ -301,16 +307,17 @@ __global__ __launch_bounds__(256) void layer_norm_many_kernel(const void* x, int
   }
 }
 
-// The gradients (16384 x 2880 bf16 66 us, 4.3 TB/s, with the sums' launch).  Workgroups stay for many rows: a lane's columns are the same in each of them, so that their sums over rows stay in
-// registers (`SUMS`), are joined over the workgroup's rows in LDS, and leave as one row of partial sums a workgroup (parts [2][gridDim.x][C]),
-// which layer_norm_sums_kernel adds in their order.  The weight lies in LDS in 32 bits, in the order in which lanes take it.
+// The gradients (16384 x 2880 bf16 66 us, 4.3 TB/s, with the sums' launch).  Workgroups stay for many rows: a lane's columns are the same
+// in each of them, so that their sums over rows stay in registers (`SUMS`), are joined over the workgroup's rows in LDS, and leave as one
+// row of partial sums a workgroup (parts [2][gridDim.x][C]), which layer_norm_sums_kernel adds in their order.  The weight lies in LDS in
+// 32 bits, in the order in which lanes take it.
 template <int DT, int TPR, int NV, int FULL, int BLOCK, bool SUMS>
 __global__ __launch_bounds__(BLOCK) void layer_norm_backward_kernel(const void* dy, int64_t sdy, const void* x, int64_t M, int C, int64_t sx, const void* w,
                                                                     int wt, const float* mean, const float* rstd, void* dx, int64_t sdx, float* parts) {
   typedef RowType<DT> R;
   constexpr int VE = R::VE, ROWS = BLOCK / TPR, WIDTH = NV * TPR * VE, WPR = TPR / 64;
-  // The next row is requested before the present one is summed, where there are registers for both (us without and with: 16384 x 2880 bf16 76.8, 65.6,
-  // x 4096 98.7, 92.4, 135168 x 128 31.7, 29.8).
+  // The next row is requested before the present one is summed, where there are registers for both (us without and with: 16384 x 2880 bf16
+  // 76.8, 65.6, x 4096 98.7, 92.4, 135168 x 128 31.7, 29.8).
   constexpr bool AHEAD = NV * VE <= 32;
   __shared__ float buf[2][2][16];
   __shared__ row_u32x4 wl[NV][VE / 4][TPR];
@@ -460,8 +467,8 @@ __global__ __launch_bounds__(BLOCK) void layer_norm_backward_kernel(const void* 
   }
 }
 
-// The partial sums' sums: 16 columns a workgroup, four lanes a row of 64 bytes, 64 rows at a time and eight such requested together; then over the lanes and
-// waves that hold the same columns.
+// The partial sums' sums: 16 columns a workgroup, four lanes a row of 64 bytes, 64 rows at a time and eight such requested together; then
+// over the lanes and waves that hold the same columns.
 __global__ __launch_bounds__(256) void layer_norm_sums_kernel(const float* parts, int n, int C, void* dw, int wt, void* db, int bt, int c0) {
   __shared__ float acc[4][16];
   const int first = c0 + (int)blockIdx.x * 16, c = first + (int)(threadIdx.x & 3) * 4;
@@ -591,14 +598,16 @@ __global__ __launch_bounds__(256) void layer_norm_parts_long_kernel(const void* 
 
 constexpr int64_t MAX_COLS = 1 << 30;
 constexpr int64_t LONG_PARTS = 128;  // partial rows of rows beyond 16384 columns
-// Lanes a workgroup of the backward pass, and the most workgroups, each of which leaves a row of partial sums: eight waves a CU carry long rows, short ones want more
-// (us at 256, 512, 768, 1024 workgroups: 65000 x 500 bf16 86, 59, 49, 50; 135168 x 128 43, 32, 29, 30; 32768 x 1024 64, 48, 49, 50; rows shared by two waves,
-// workgroups of eight: 16384 x 4096 85, 94, 104, 113).
+// Lanes a workgroup of the backward pass, and the most workgroups, each of which leaves a row of partial sums: eight waves a CU carry long
+// rows, short ones want more (us at 256, 512, 768, 1024 workgroups: 65000 x 500 bf16 86, 59, 49, 50; 135168 x 128 43, 32, 29, 30; 32768 x
+// 1024 64, 48, 49, 50; rows shared by two waves, workgroups of eight: 16384 x 4096 85, 94, 104, 113).
 constexpr int backward_block(int tpr) { return tpr == 128 ? 512 : block_of(tpr); }
 constexpr int backward_parts(int tpr, int nv) { return nv == 1 ? 768 : tpr == 128 ? 256 : 512; }
-// Rows from this many on go through workgroups that stay; fewer have a workgroup each (16 x 2880 bf16 4.0 us, by waves 6.4; 1024 x 2880 6.7, 9.4; 4096 x 2880 14.4, by workgroups 17.9).
+// Rows from this many on go through workgroups that stay; fewer have a workgroup each (16 x 2880 bf16 4.0 us, by waves 6.4; 1024 x 2880
+// 6.7, 9.4; 4096 x 2880 14.4, by workgroups 17.9).
 constexpr int64_t MANY_ROWS = 2048;
-constexpr int64_t STAYING = 2048;  // such workgroups, at most (16384 x 4096 bf16 with 1024, 2048, 4096: 53.6, 54.5, 51.2 us; 65000 x 500 fp16 42.0, 35.5, 36.0)
+// such workgroups, at most (16384 x 4096 bf16 with 1024, 2048, 4096: 53.6, 54.5, 51.2 us; 65000 x 500 fp16 42.0, 35.5, 36.0)
+constexpr int64_t STAYING = 2048;
 unsigned rows_grid(int64_t rows) { return (unsigned)(rows < 1 << 20 ? rows : 1 << 20); }
 
 struct Forward {
@@ -667,8 +676,9 @@ struct Backward {
   }
 };
 
-// Lanes a row, vectors a lane and how many of these are full for rows of C columns: part of a wave up to 32 vectors, a wave up to 32 elements a lane (forward 64),
-// two waves up to 32 (backward, whose sums take two registers an element), then a workgroup of 256 up to 32 and one of 1024 up to 16.  False: longer ones.
+// Lanes a row, vectors a lane and how many of these are full for rows of C columns: part of a wave up to 32 vectors, a wave up to 32
+// elements a lane (forward 64), two waves up to 32 (backward, whose sums take two registers an element), then a workgroup of 256 up to 32
+// and one of 1024 up to 16.  False: longer ones.
 template <int DT, bool BACKWARD, class Op>
 bool by_length(const Op& op, int64_t C) {
   constexpr int VE = RowType<DT>::VE;

@@ -46,9 +46,10 @@ struct RowType {
     asm volatile("" : "+v"(n));
     return n;
   }
-  // The same where the elements in front of `begin` and from `end` on are not there: they read as `fill` (a dword of it), and nothing there is
-  // touched.  Pairs of 16-bit elements are requested together, from the nearest element that there is, and chosen afterwards: one by one under their
-  // conditions, each waits for the one that it shares a register with, up to seven memory latencies in a row at the end of each row.
+  // The same where the elements in front of `begin` and from `end` on are not there: they read as `fill` (a dword of it), and nothing there
+  // is touched.  Pairs of 16-bit elements are requested together, from the nearest element that there is, and chosen afterwards: one by one
+  // under their conditions, each waits for the one that it shares a register with, up to seven memory latencies in a row at the end of each
+  // row.
   static __device__ __forceinline__ row_u32x4 load_vec_in(const void* p, int i, int begin, int end, uint32_t fill) {
     const int n = left(i, end), skip = begin - i;
     if (skip <= 0 && n >= VE) return load_vec(p, i);
@@ -69,8 +70,9 @@ struct RowType {
     return v;
   }
   static __device__ __forceinline__ row_u32x4 load_vec_to(const void* p, int i, int end, uint32_t fill) { return load_vec_in(p, i, i, end, fill); }
-  // A row's last vectors without a branch, for rows of at least VE elements: load_last() takes the sixteen bytes that end with the row where those from i on pass its end,
-  // and last() moves them to their places, with zeros behind.  The move may wait until the vector is used.
+  // A row's last vectors without a branch, for rows of at least VE elements: load_last() takes the sixteen bytes that end with the row
+  // where those from i on pass its end, and last() moves them to their places, with zeros behind.  The move may wait until the vector is
+  // used.
   static __device__ __forceinline__ row_u32x4 load_last(const void* p, int i, int end) { return load_vec(p, i < end - VE ? i : end - VE); }
   static __device__ __forceinline__ row_u32x4 last(row_u32x4 v, int i, int end) {
     const int n = left(i, end), drop = n >= VE ? 0 : n <= 0 ? 128 : (VE - n) * (8 * BYTES);

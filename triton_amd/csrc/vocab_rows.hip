@@ -1,5 +1,8 @@
 // Operators over rows of logits of a whole vocabulary: log probabilities of given tokens with entropy and top alternatives, the
 // distillation loss against a teacher's top logits, and the gradients of both.
+//
+// Times in the comments are medians over replays of a captured graph of a few calls on the same buffers, so that what fits the last-level
+// cache (256 MB) may come from it; where two ways stand side by side, both were timed on one card when the choice between them was made.
 #include <type_traits>
 
 #include "row_math.h"
@@ -26,13 +29,13 @@ struct Scales {
 
 // ---- the pass over the logits -------------------------------------------------------------------------------
 // Softmax statistics of the logits seen so far, as one pass takes them: m the largest, k = m c2 rounded to a whole number, s = sum 2^d and
-// e = sum 2^d d with d = x c2 - k.  The product and the difference are one operation and one rounding, and a larger m rescales both sums by a power of two,
-// exactly: s' = 2^(k - k') s, e' = 2^(k - k') (e + s (k - k')).  (x - m) c2 in two operations, which needs no whole number, took 4 to 7 % longer with
-// alternatives, where the vector unit bounds the pass; x c2 - m c2 with m c2 rounded is off by 1e-6 between lanes whose m differ.
-// From |m c2| = 2^24 on, numbers of 32 bits are further apart than one, and m c2 - k may be anything up to that distance.  So k is taken from a little above: no d is
-// much above zero, and no sum overflows that a larger logit (behind logits masked with -1e10, say) brings back to nothing.  The sums of a row whose largest
-// logit is so large are left to Workgroup::wide().  d is bounded by D_MIN in products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero
-// in 32 bits.
+// e = sum 2^d d with d = x c2 - k.  The product and the difference are one operation and one rounding, and a larger m rescales both sums by
+// a power of two, exactly: s' = 2^(k - k') s, e' = 2^(k - k') (e + s (k - k')).  (x - m) c2 in two operations, which needs no whole number,
+// took 4 to 7 % longer with alternatives, where the vector unit bounds the pass; x c2 - m c2 with m c2 rounded is off by 1e-6 between lanes
+// whose m differ.  From |m c2| = 2^24 on, numbers of 32 bits are further apart than one, and m c2 - k may be anything up to that distance.
+// So k is taken from a little above: no d is much above zero, and no sum overflows that a larger logit (behind logits masked with -1e10,
+// say) brings back to nothing.  The sums of a row whose largest logit is so large are left to Workgroup::wide().  d is bounded by D_MIN in
+// products only, where -inf times a probability of zero stands for zero; 2^D_MIN is zero in 32 bits.
 constexpr float D_MIN = -300.f, K_MAX = 3.3e38f, WIDE = 2.f;
 struct Softmax {
   float m, k, s, e;
@@ -104,8 +107,8 @@ __device__ __forceinline__ const void* logits_row(const tk_vocab_desc& d, int t)
   return static_cast<const char*>(d.logits) + (int64_t)t * d.logits_stride_m * RowType<DT>::BYTES;
 }
 
-// A row from the sixteen-byte boundary at or in front of it: place `begin` is its column 0, what lies in front is not touched.  Loads that do not begin at such
-// boundaries take a quarter longer (4096 x 130001 bf16 222 us, x 130000 180).
+// A row from the sixteen-byte boundary at or in front of it: place `begin` is its column 0, what lies in front is not touched.  Loads that
+// do not begin at such boundaries take a quarter longer (4096 x 130001 bf16 222 us, x 130000 180).
 struct Placed {
   const void* base;
   int begin;
@@ -146,8 +149,8 @@ struct Workgroup {
     return r;
   }
 
-  // The sums of a row whose largest logit is finite but lies WIDE or more from its whole number (nothing but masked logits, say): differences from m first, element by
-  // element.
+  // The sums of a row whose largest logit is finite but lies WIDE or more from its whole number (nothing but masked logits, say):
+  // differences from m first, element by element.
   template <int DT>
   static __device__ __forceinline__ Softmax wide(const void* row, int V, Softmax r, float c2, float* buf) {
     if (!(r.m > NEG_INF && r.m < __builtin_inff() && !(fabsf(r.offset) < WIDE))) return r;
@@ -165,8 +168,8 @@ struct Workgroup {
     return r;
   }
 
-  // Places [c0, c1) of a row from `begin` on; `keys` takes the order numbers of the groups' largest logits (group = place / GROUP; c0 is a multiple of
-  // GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
+  // Places [c0, c1) of a row from `begin` on; `keys` takes the order numbers of the groups' largest logits (group = place / GROUP; c0 is a
+  // multiple of GROUP).  U vectors of 16 bytes a lane are under way while the U before them are summed.
   template <int DT, bool ENTROPY, bool TOP, int U, bool ONCE>
   static __device__ __forceinline__ Softmax stream(const void* row, int begin, int c0, int c1, float c2, uint32_t* keys) {
     typedef RowType<DT> R;
@@ -244,12 +247,12 @@ struct Workgroup {
 
   // ---- the k largest ------------------------------------------------------------------------------------------
   // A row's k largest logits lie in the k groups whose largest logits are the largest (equal ones: the lower groups): were one of them in
-  // another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per
-  // group, and then at the k groups' elements again: the rest of the row is read once, whatever stands in it.
-  // A bound from below narrows both: k threads' largest group numbers are at least the k-th largest of the threads' largest ones, so that
-  // only groups, and then only elements, from there on can be among the k; as a rule they are few more than k, which are ranked by
-  // counting.  Where they are many (equal logits, logits masked to one value, neighbours sorted together), each of the two selections finds the
-  // k-th largest number bit by bit with a count over the workgroup, and takes the equal ones by a prefix sum in the order of the columns.
+  // another group, each of these k groups would hold an element in front of it.  So the selection looks at a number per group, and then at
+  // the k groups' elements again: the rest of the row is read once, whatever stands in it.  A bound from below narrows both: k threads'
+  // largest group numbers are at least the k-th largest of the threads' largest ones, so that only groups, and then only elements, from
+  // there on can be among the k; as a rule they are few more than k, which are ranked by counting.  Where they are many (equal logits,
+  // logits masked to one value, neighbours sorted together), each of the two selections finds the k-th largest number bit by bit with a
+  // count over the workgroup, and takes the equal ones by a prefix sum in the order of the columns.
   struct SelectLds {
     int count[2][WAVES];
     int scan[WAVES];
@@ -258,8 +261,8 @@ struct Workgroup {
     int group[MANY];
     uint64_t found[MANY];  // key << 32 | ~column: a larger one comes first
   };
-  // Calls take(slot, i) for the k first of n items in the order (larger key, then lower i), slots by i; at least k keys are not 0.  A thread looks
-  // at consecutive items.  This is the way for the rows that the ranking does not serve: it reads the keys again for each bit.
+  // Calls take(slot, i) for the k first of n items in the order (larger key, then lower i), slots by i; at least k keys are not 0.  A
+  // thread looks at consecutive items.  This is the way for the rows that the ranking does not serve: it reads the keys again for each bit.
   template <int BITS, class KeyOf, class F>
   static __device__ __forceinline__ void select(int n, int k, SelectLds& lds, KeyOf&& key_of, F&& take) {
     const int per = (n + THREADS - 1) / THREADS, i0 = (int)threadIdx.x * per, i1 = i0 + per < n ? i0 + per : n;
@@ -329,7 +332,8 @@ struct Workgroup {
     return from ? from : 1u;
   }
 
-  // Leaves at least the k largest of places [begin, end) of a row in lds.found, in any order, and returns how many; from the groups' numbers.
+  // Leaves at least the k largest of places [begin, end) of a row in lds.found, in any order, and returns how many; from the groups'
+  // numbers.
   template <int DT>
   static __device__ __forceinline__ int top_of_row(const void* row, int begin, int end, int k, const uint32_t* group_keys, SelectLds& lds) {
     typedef RowType<DT> R;
@@ -507,9 +511,9 @@ struct Workgroup {
   }
 };
 
-// A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).
-// Bound by the logits' one read, and with alternatives by the vector unit as well: 4096 x 131072 bf16 174 us (6.2 TB/s), with 64 alternatives 192 (5.6); 2048 x 32000 fp32
-// 47.7 (5.5).
+// A row a workgroup, from the first logit to the results; the groups' numbers stay in LDS (dynamic, with OP == LOGPROBS_TOP).  Bound by the
+// logits' one read, and with alternatives by the vector unit as well: 4096 x 131072 bf16 174 us (6.2 TB/s), with 64 alternatives 195 (5.5);
+// 2048 x 32000 fp32 43.7 (6.0).
 template <int DT, int OP, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Scales sc, int t0, int keep_from) {
   typedef Workgroup<THREADS> W;
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(THREADS) void vocab_rows_kernel(tk_vocab_desc d, Sc
   W::template finish<DT, OP>(d, sc, t, p, single, r, keys, lds);
 }
 
-// Few rows: pieces of a row (61 x 50001 fp16 with 8 alternatives 11.5 us, both launches: latencies one after the other, not bytes), whose statistics and groups' numbers go through the workspace to vocab_join_kernel.
+// Few rows: pieces of a row (61 x 50001 fp16 with 8 alternatives 12.2 us, both launches: latencies one after the other, not bytes), whose
+// statistics and groups' numbers go through the workspace to vocab_join_kernel.
 typedef Workgroup<256> Wide;
 template <int DT, int OP>
 __global__ __launch_bounds__(256) void vocab_chunk_kernel(tk_vocab_desc d, Scales sc, int chunk, int n_chunks, float* parts, uint32_t* keys, int groups) {
@@ -554,18 +559,22 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(tk_vocab_desc d, Scales
   Wide::finish<DT, OP>(d, sc, t, placed<DT>(row), single, r, keys + (int64_t)t * groups, lds);
 }
 
-// Gradients from this size on are read and written with the read-once hint: they would only push the logits, which come from the last-level cache in part, out
-// of it (forward and backward, us without and with: 2048 x 32000 fp32, 262 MB, 159, 129; 4096 x 131072 bf16, 1074 MB, 604, 590; 1000 x 50001 fp16,
-// 100 MB, 79, 74.5; 200 x 32000 bf16, 13 MB, 18, 18, where whoever reads the gradient next may find it cached).
+// Gradients from this size on are read and written with the read-once hint: they would only push the logits, which come from the last-level
+// cache in part, out of it (forward and backward, us without and with: 2048 x 32000 fp32, 262 MB, 159, 129; 4096 x 131072 bf16, 1074 MB,
+// 604, 590; 1000 x 50001 fp16, 100 MB, 79, 74.5; 200 x 32000 bf16, 13 MB, 18, 18, where whoever reads the gradient next may find it
+// cached).
 constexpr int64_t ONCE_BYTES = 64 << 20;
-// The forward pass reads its logits with the hint, too (nothing follows it: 4096 x 131072 bf16 189, 165, 2048 x 32000 fp32 48.6, 42.6), but where a backward pass is to follow,
-// the last rows without: that many bytes are still cached when it begins with them (forward and backward, all rows hinted, none, the last 192 MB not:
-// 2048 x 32000 fp32 143, 129, 127; 2048 x 64000 281, 270, 263; 4096 x 96000 bf16 422, 416, 400; 4096 x 131072 542, 586, 548; 8192 x 100000 978, 924, 960).
+// The forward pass reads its logits with the hint, too (nothing follows it: 4096 x 131072 bf16 189, 165, 2048 x 32000 fp32 48.6, 42.6), but
+// where a backward pass is to follow, the last rows without: that many bytes are still cached when it begins with them (forward and
+// backward, all rows hinted, none, the last 192 MB not: 2048 x 32000 fp32 143, 129, 127; 2048 x 64000 281, 270, 263; 4096 x 96000 bf16 422,
+// 416, 400; 4096 x 131072 542, 586, 548; 8192 x 100000 978, 924, 960).
 constexpr int64_t KEPT_BYTES = 192 << 20;
 
-// Pieces that the rows of a call are split into: about four workgroups a CU; no more, since a second launch joins them (us, pieces for 500, 1000
-// and 2048 workgroups: 1000 x 131072 bf16 with 20 alternatives 61, 61, 76; 300 x 131072 22.9, 22.5, 23.4; 100 x 131072 13.4, 12.6, 11.8; 61 x 50001
-// fp16 with 8 13.1, 14.4, 16.3).
+// Pieces that the rows of a call are split into: about four workgroups a CU; no more, since a second launch joins them (us, pieces for 500,
+// 1000 and 2048 workgroups: 1000 x 131072 bf16 with 20 alternatives 61, 61, 76; 300 x 131072 22.9, 22.5, 23.4; 100 x 131072 13.4, 12.6,
+// 11.8; 61 x 50001 fp16 with 8 13.1, 14.4, 16.3).  From some 400 rows on whole rows are as fast or faster, which this rule does not know
+// (in pieces and whole: 400 x 50001 fp16 15.5, 13.8; 600 19.9, 17.4; 999 27.6, 22.1, with 20 alternatives 37.4, 28.5; 400 x 131072 bf16
+// 25.6, 27.8; 600 33.4, 33.7; 999 50.2, 46.3; 999 x 32000 fp32 28.3, 24.1).
 struct Split {
   int n, chunk, groups;
   int64_t parts_bytes, bytes;
@@ -588,10 +597,10 @@ Split split_of(int32_t n_rows, int64_t vocab, int32_t k, int shift) {
 
 Scales scales_of(const tk_vocab_desc* d) { return {(float)(1.0 / d->temperature), (float)(1.4426950408889634 / d->temperature)}; }
 
-// Rows of up to SHORT_ROW columns have a wave each, where there are enough of them (us, a workgroup and a wave: 16000 x 1000 bf16 22.9, 12.1, its gradient
-// 35, 19; x 4000 23.5, 28, its gradient 52, 56), longer ones with alternatives up to SHORT_TOP, whose ranking is the same work for four waves and one
-// (with 20: 16000 x 2000 71, 34; x 4000 74, 44; x 8000 84, 67; x 16000 121, 118).  No more of those than half a wave ranks, nor more teacher
-// entries than four a lane.
+// Rows of up to SHORT_ROW columns have a wave each, where there are enough of them (us, a workgroup and a wave: 16000 x 1000 bf16 22.9,
+// 12.1, its gradient 35, 19; x 4000 23.5, 28, its gradient 52, 56), longer ones with alternatives up to SHORT_TOP, whose ranking is the
+// same work for four waves and one (with 20: 16000 x 2000 71, 34; x 4000 74, 44; x 8000 84, 67; x 16000 121, 118).  No more of those than
+// half a wave ranks, nor more teacher entries than four a lane.
 constexpr int SHORT_ROW = 2048, SHORT_TOP = 8192;
 
 template <int DT, int OP>
@@ -600,9 +609,11 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
   const Split s = split_of(d->n_rows, d->vocab, OP == LOGPROBS_TOP ? d->k : 0, aligned ? 0 : RowType<DT>::VE - 1);
   const Scales sc = scales_of(d);
   if (s.n == 1) {
-    // Four vectors a lane under way, or two: two waste less of a row's last step and start sooner, four carry long rows when the chip is full of them.
-    // us with two, four (softmax statistics alone; * with 64 alternatives): 4096 x 131072 bf16 196, 188 (* 208, 204); 2048 x 32000 fp32 50.2, 47.6;
-    // 1000 x 50001 fp16 25.4, 27.5, fp32 38.4, 39.8; 16000 x 4000 bf16 with 20 alternatives 74, 90.
+    // Four vectors a lane under way, or two: two waste less of a row's last step and start sooner, four carry long rows when the chip is
+    // full of them; us with two, four (statistics alone; * with 64 alternatives): 1000 x 131072 bf16 49.3, 46.0 (* 60.6, 58.8), 1500 66.5,
+    // 67.4 (* 78.9, 79.9), 2048 91.3, 94.8 (* 103, 106), 3000 134, 131 (* 151, 147), 4096 174, 174 (* 196, 195); x 50001 fp16 1000 23.6,
+    // 22.7 (* 34.0, 34.5), 2048 40.0, 42.5 (* 53.5, 59.3), 4096 75.6, 73.3 (* 92.9, 94.7); x 32000 fp32 1000 23.7, 24.1 (* 31.9, 32.7),
+    // 2048 46.4, 43.7 (* 57.6, 57.6), 4096 83.5, 82.5 (* 104, 100); 16000 x 4000 bf16 with 20 alternatives 74, 90.
     constexpr int STEP = 4 * 256 * RowType<DT>::VE;
     const bool wave = d->n_rows >= 1000 && (OP == LOGPROBS_TOP ? d->k <= 32 && d->vocab <= SHORT_TOP : d->vocab <= SHORT_ROW)
                       && (OP != DISTILL || d->n_teacher <= 64 * Workgroup<64>::ENTRIES);
@@ -624,11 +635,12 @@ int32_t forward(const tk_vocab_desc* d, hipStream_t stream, const char* who) {
 }
 
 // ---- gradients ----------------------------------------------------------------------------------------------
-// A piece of a row a workgroup: one read and one write of the row's size, which bound it (forward and backward of 1000 x 50001 bf16 59 us, 5.1 TB/s).  With p = 2^d2, d2 = (x - m) c2 - log2 s:
+// A piece of a row a workgroup: one read and one write of the row's size, which bound it (forward and backward of 1000 x 50001 bf16 57.9
+// us, 5.2 TB/s).  With p = 2^d2, d2 = (x - m) c2 - log2 s:
 //   log probabilities   g = p (A + B d2) everywhere, A = -(d_lp + d_h H) / t, B = -d_h ln 2 / t, and d_lp / t more at the token
 //   distillation        g = p G, G = d_loss / t, and a_j G less at the teacher's entry j
-// The teacher's few columns are written once more at the end, by the piece that they lie in: looking each column up while the row streams by
-// cost as much as the row where a wave's columns hold some of them (2000 x 1500 fp16 with 50 entries 31 us).
+// The teacher's few columns are written once more at the end, by the piece that they lie in: looking each column up while the row streams
+// by cost as much as the row where a wave's columns hold some of them (2000 x 1500 fp16 with 50 entries 31 us).
 constexpr int GRAD_CHUNK = 16384;
 
 template <int DT, int OP, int THREADS, bool ONCE>
@@ -642,7 +654,8 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
   const int c0 = (int)(place % (unsigned)n_chunks) * chunk;
   const int c1 = d.vocab - c0 < chunk ? d.vocab : c0 + chunk;
   void* out = static_cast<char*>(d.d_logits) + (int64_t)t * d.d_logits_stride_m * R::BYTES;
-  // ln s / ln 2 in two parts: rounded to one number it is off by 7e-7 near 17, and every p of the row with it.  The second part is a factor of the row's A and B.
+  // ln s / ln 2 in two parts: rounded to one number it is off by 7e-7 near 17, and every p of the row with it.  The second part is a factor
+  // of the row's A and B.
   const float m = d.stats[t], log_s = d.stats[(int64_t)d.n_rows + t], log2_s = log_s * LOG2E;
   const float rest = __builtin_amdgcn_exp2f(-fmaf(log_s, LOG2E_REST, fmaf(log_s, LOG2E, -log2_s)));
   float A, B = 0.f, more = 0.f, qm = 0.f, log_qs = 0.f;
@@ -703,7 +716,8 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
   }
   if constexpr (OP == DISTILL) {
     if (zero) return;
-    extern __shared__ uint32_t lds[];  // [n_teacher] columns, [n_teacher] logits, [chunk / 32] a bit a column that an entry names, whether two name one
+    // [n_teacher] columns, [n_teacher] logits, [chunk / 32] a bit a column that an entry names, whether two name one
+    extern __shared__ uint32_t lds[];
     const int n = d.n_teacher;
     uint32_t *column = lds, *logit = lds + n, *named = lds + 2 * n, *twice = named + chunk / 32;
     for (int i = threadIdx.x; i <= chunk / 32; i += THREADS) named[i] = 0;
@@ -716,7 +730,8 @@ __global__ __launch_bounds__(THREADS) void vocab_backward_kernel(tk_vocab_desc d
       const uint32_t bit = 1u << ((v - c0) & 31);
       if (v >= c0 && v < c1 && (atomicOr(&named[(v - c0) >> 5], bit) & bit)) *twice = 1;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's part of the row has arrived where the second writing of a column finds it)
+    // (this wave's part of the row has arrived where the second writing of a column finds it)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const auto weight = [&](int j) { return expf((bits_f32(logit[j]) - qm) * sc.inv_t - log_qs); };
     for (int j = threadIdx.x; j < n; j += THREADS) {
