@@ -572,7 +572,8 @@ int32_t tk_layer_norm_backward(const void* dy, int64_t stride_dym, const void* x
  *   - a token outside [0, vocab): logprobs 0, and no gradient through it;
  *   - a teacher entry with a NaN or +inf: loss and gradient are NaN;
  *   - a teacher entry whose index is outside [0, vocab), or whose logit is -inf, carries no weight; a row without any other has loss 0
- *     and gradient 0.  An index that occurs twice counts twice.
+ *     and gradient 0.  An index that occurs twice counts twice.  A student that gives one of the others no probability, or one whose
+ *     logarithm is beyond fp32 (logits masked with fp32's lowest value at a temperature below one), has loss +inf;
  * A row whose given gradients are all zero has the gradient zero.
  * No counterpart in the reference's operator library; tk/topk.py:25-141 is the router's selection.
  */

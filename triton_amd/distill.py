@@ -89,7 +89,8 @@ def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     `logits [T, V]` are the student's (fp32, bf16 or fp16), `teacher_logits [T, K]` the teacher's at `teacher_indx [T, K]` (int32 or
     int64; K up to 1024).  An entry whose index lies outside `[0, V)` or whose logit is -inf carries no weight; a row without any
     other has the loss 0 and no gradient (padding, fewer alternatives than K).  A student that gives one of the others no
-    probability has the loss +inf; one with a NaN or +inf, or a teacher with one, NaN.  Differentiable once in `logits`."""
+    probability, or one whose logarithm is beyond fp32 (a mask of fp32's lowest value at a temperature below one), has the loss +inf; one with a
+    NaN or +inf, or a teacher with one, NaN.  Differentiable once in `logits`."""
     host = nt.host()
     loss = host.distill_topk(logits, teacher_logits, teacher_indx, temperature) if host is not None else None
     if loss is not None:
