@@ -626,6 +626,104 @@ int32_t tk_distill_topk(const tk_vocab_desc* desc, tk_stream_t stream);
 int32_t tk_distill_topk_backward(const tk_vocab_desc* desc, tk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * e4m3 values with one fp32 scale for each block of 128 (no counterpart in the reference's operator library)
+ *
+ * A matrix [rows, cols] is cut into blocks of block_rows x 128 elements (block_rows 1: activations, 128: weights; the last
+ * ones may be smaller) and stands for values[r, c] * scales[r / block_rows, c / 128].
+ *
+ * tk_fp8_block_downcast: a block's scale is the smallest power of two, 2^-126 or more, that leaves its largest finite magnitude at
+ * most 448; 1 for a block of zeros.  An element is rounded to the nearest e4m3, ties to even; infinities and NaN become NaN.  Powers
+ * of two lose nothing against amax / 448 but a part of the subnormal numbers' range, and leave every value a number of four
+ * significant bits, which 16 bits hold exactly.  `values_t`, block_rows 128 only, may receive the transposed values [cols, rows] too.
+ * tk_fp8_block_upcast: values * scale in fp32, rounded once to out_dtype; scales of any size.
+ * All matrices have unit stride along cols (values_t: along rows); strides are in elements.  `batch` matrices in one call.
+ */
+int32_t tk_fp8_block_downcast(const void* x, int32_t dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_stride_b, int64_t x_stride_r,
+                              int32_t block_rows, uint8_t* values, int64_t v_stride_b, int64_t v_stride_r, uint8_t* values_t,
+                              int64_t t_stride_b, int64_t t_stride_c, float* scales, int64_t s_stride_b, int64_t s_stride_r, int64_t s_stride_c,
+                              tk_stream_t stream);
+int32_t tk_fp8_block_upcast(const uint8_t* values, int64_t batch, int64_t rows, int64_t cols, int64_t v_stride_b, int64_t v_stride_r, int32_t block_rows,
+                            const float* scales, int64_t s_stride_b, int64_t s_stride_r, int64_t s_stride_c, void* out, int32_t out_dtype,
+                            int64_t o_stride_b, int64_t o_stride_r, tk_stream_t stream);
+
+/*
+ * The ragged product of such operands: for row r of slice e
+ *     acc = sum over blocks b of K of (sum over k in b of x[src(r), k] w[e, k, n]) x_scale[src(r), b] w_scale[e, b, n / 128]
+ *     y[dst(r), n] = act(acc + bias[e, n]) * gammas[r]
+ * with fp32 sums, rounded once.  src(r) = gather_indx[r] or r; dst(r) = scatter_indx[r] (negative: the row is dropped; rows r >= scatter_len
+ * are dropped) or r.  act: none, or swiglu over interleaved (gate, linear) columns as in tk_moe_gemm.
+ * Rows of x and columns of w are contiguous along K, of any alignment.  slice_sizes NULL = one slice of M rows.  block_schedule = the
+ * schedule of row blocks of 64 ((block << 16) | slice, negative = none), grid_m entries.
+ * zero_rest: rows behind the last slice (from slice_offs[n_slices] on, below M) are set to zero; otherwise they stay as they were.
+ */
+typedef struct tk_fp8_gemm_desc {
+  const uint8_t* x; /* e4m3 [x_rows, K] */
+  int64_t x_stride_m, x_rows;
+  const float* x_scale; /* [x_rows, ceil(K / 128)] */
+  int64_t xs_stride_m, xs_stride_k;
+  const uint8_t* w; /* e4m3 [n_slices, K, N] */
+  int64_t w_stride_e, w_stride_n;
+  const float* w_scale; /* [n_slices, ceil(K / 128), ceil(N / 128)] */
+  int64_t ws_stride_e, ws_stride_k, ws_stride_n;
+  const void* bias; /* [n_slices, N] or NULL */
+  int32_t bias_dtype; /* TK_F32, TK_BF16 */
+  int64_t bias_stride_e;
+  const int32_t* gather_indx;  /* [M] or NULL */
+  const int32_t* scatter_indx; /* [scatter_len] or NULL */
+  int32_t scatter_len;
+  const void* gammas; /* [M] or NULL */
+  int32_t gammas_dtype; /* TK_F32, TK_BF16 */
+  const int32_t* slice_sizes;    /* [n_slices] or NULL */
+  const int32_t* slice_offs;     /* [n_slices + 1] */
+  const int32_t* block_schedule; /* [grid_m] */
+  int32_t n_slices, grid_m;
+  int32_t M, N, K;
+  void* y; /* [.., N], [.., N / 2] with swiglu */
+  int32_t y_dtype; /* TK_F32, TK_BF16, TK_F16 */
+  int64_t y_stride_m;
+  int32_t activation; /* TK_ACT_* */
+  float act_alpha, act_limit;
+  int32_t act_has_limit, zero_rest;
+} tk_fp8_gemm_desc;
+int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* desc, tk_stream_t stream);
+
+/*
+ * Gradient of the weights from an 8-bit activation: y[e, k, n] = sum over the rows t of slice e of x[t, k] x_scale[t, k / 128] dy[t, n],
+ * fp32 sums.  x times its scale is rounded to dy's type first (exact where the scales are powers of two as tk_fp8_block_downcast makes them, and
+ * limited to 65504 in fp16).  A slice without rows has the gradient zero.
+ */
+typedef struct tk_fp8_wgrad_desc {
+  const uint8_t* x; /* e4m3 [T, K] */
+  int64_t x_stride_t;
+  const float* x_scale; /* [T, ceil(K / 128)] */
+  int64_t xs_stride_t, xs_stride_k;
+  const void* dy; /* [T, N] */
+  int32_t dy_dtype; /* TK_BF16, TK_F16 */
+  int64_t dy_stride_t;
+  const int32_t* slice_sizes; /* [n_slices] or NULL: one slice of T rows */
+  const int32_t* slice_offs;
+  int32_t n_slices;
+  int32_t T, K, N;
+  void* y; /* [n_slices, K, N] */
+  int32_t y_dtype; /* TK_F32, TK_BF16, TK_F16 */
+  int64_t y_stride_e, y_stride_k;
+} tk_fp8_wgrad_desc;
+int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* desc, tk_stream_t stream);
+
+/*
+ * swiglu that keeps its input in 8 bits for the backward pass.  a [M, 2 n_out], interleaved (gate, linear) columns; out [M, n_out] =
+ * s (linear + 1), s = gate / (1 + exp(-alpha gate)), gate at most limit and linear within [-limit, limit] if there is one; values / scales = a as
+ * tk_fp8_block_downcast has it (block_rows 1; both NULL: not kept).  The backward call gives the gradient of a for that of out, taken at values * scales; an element beyond
+ * the limit has none.  NaN stays NaN.
+ */
+int32_t tk_swiglu_fp8(const void* a, int32_t dtype, int64_t M, int64_t n_out, int64_t a_stride_m, void* out, int64_t out_stride_m, uint8_t* values,
+                      int64_t v_stride_m, float* scales, int64_t s_stride_m, int64_t s_stride_c, float alpha, float limit, int32_t has_limit,
+                      tk_stream_t stream);
+int32_t tk_swiglu_fp8_backward(const void* d_out, int32_t dtype, int64_t M, int64_t n_out, int64_t d_out_stride_m, const uint8_t* values, int64_t v_stride_m,
+                               const float* scales, int64_t s_stride_m, int64_t s_stride_c, void* d_a, int64_t d_a_stride_m, float alpha, float limit,
+                               int32_t has_limit, tk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Host check hooks (no device work, no GPU needed)
  * ---------------------------------------------------------------------------------------------- */
 

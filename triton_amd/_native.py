@@ -108,6 +108,27 @@ class VocabDesc(_c.Structure):
     ]
 
 
+class Fp8GemmDesc(_c.Structure):
+    """struct tk_fp8_gemm_desc (field order and types follow include/triton_amd.h)."""
+    _fields_ = [
+        ("x", _ptr), ("x_stride_m", _i64), ("x_rows", _i64), ("x_scale", _ptr), ("xs_stride_m", _i64), ("xs_stride_k", _i64),
+        ("w", _ptr), ("w_stride_e", _i64), ("w_stride_n", _i64), ("w_scale", _ptr), ("ws_stride_e", _i64), ("ws_stride_k", _i64), ("ws_stride_n", _i64),
+        ("bias", _ptr), ("bias_dtype", _i32), ("bias_stride_e", _i64), ("gather_indx", _ptr), ("scatter_indx", _ptr), ("scatter_len", _i32),
+        ("gammas", _ptr), ("gammas_dtype", _i32), ("slice_sizes", _ptr), ("slice_offs", _ptr), ("block_schedule", _ptr), ("n_slices", _i32),
+        ("grid_m", _i32), ("M", _i32), ("N", _i32), ("K", _i32), ("y", _ptr), ("y_dtype", _i32), ("y_stride_m", _i64), ("activation", _i32),
+        ("act_alpha", _f32), ("act_limit", _f32), ("act_has_limit", _i32), ("zero_rest", _i32),
+    ]
+
+
+class Fp8WgradDesc(_c.Structure):
+    """struct tk_fp8_wgrad_desc (field order and types follow include/triton_amd.h)."""
+    _fields_ = [
+        ("x", _ptr), ("x_stride_t", _i64), ("x_scale", _ptr), ("xs_stride_t", _i64), ("xs_stride_k", _i64), ("dy", _ptr), ("dy_dtype", _i32),
+        ("dy_stride_t", _i64), ("slice_sizes", _ptr), ("slice_offs", _ptr), ("n_slices", _i32), ("T", _i32), ("K", _i32), ("N", _i32),
+        ("y", _ptr), ("y_dtype", _i32), ("y_stride_e", _i64), ("y_stride_k", _i64),
+    ]
+
+
 # name -> (restype, argtypes); must list every symbol include/triton_amd.h declares.
 SIGNATURES = {
     "tk_version": (_i32, []),
@@ -139,6 +160,12 @@ SIGNATURES = {
     "tk_token_logprobs_backward": (_i32, [_c.POINTER(VocabDesc), _ptr]),
     "tk_distill_topk": (_i32, [_c.POINTER(VocabDesc), _ptr]),
     "tk_distill_topk_backward": (_i32, [_c.POINTER(VocabDesc), _ptr]),
+    "tk_fp8_block_downcast": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr]),
+    "tk_fp8_block_upcast": (_i32, [_ptr, _i64, _i64, _i64, _i64, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _ptr]),
+    "tk_fp8_block_gemm": (_i32, [_c.POINTER(Fp8GemmDesc), _ptr]),
+    "tk_fp8_block_wgrad": (_i32, [_c.POINTER(Fp8WgradDesc), _ptr]),
+    "tk_swiglu_fp8": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _f32, _f32, _i32, _ptr]),
+    "tk_swiglu_fp8_backward": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _f32, _f32, _i32, _ptr]),
     # host check hooks (no device work)
     "tk_host_mx_convert": (_i32, [_ptr, _i64, _i32, _ptr]),
     "tk_host_mx_scale": (_i32, [_ptr, _i64, _i32, _i32, _ptr]),

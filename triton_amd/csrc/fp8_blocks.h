@@ -1,0 +1,249 @@
+// Pieces shared by the kernels of e4m3 matrices with one fp32 scale for each block of 128 (fp8_quant.hip, fp8_gemm*.hip, fp8_wgrad.hip).
+#pragma once
+#include "gemm_common.h"
+
+namespace tk {
+
+struct Fp8GemmParams {
+  const uint8_t* x;
+  int64_t x_stride_m;
+  const float* xs;
+  int64_t xs_m, xs_k;
+  const uint8_t* w;
+  int64_t w_e, w_n;
+  const float* ws;
+  int64_t ws_e, ws_k, ws_n;
+  const void* bias;
+  int64_t bias_e;
+  int32_t bias_is_f32;
+  const int32_t* gather;
+  const int32_t* scatter;
+  int32_t scatter_len;
+  const void* gammas;
+  int32_t gammas_is_f32;
+  const int32_t* slice_sizes;
+  const int32_t* slice_offs;
+  const int32_t* block_sched;
+  int32_t n_slices, grid_m, grid_n;
+  int32_t M, N, K;
+  void* y;
+  int64_t y_stride_m;
+  int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
+  float alpha, limit;  // (limit: +inf without one)
+  int32_t zero_rest;
+};
+
+namespace {
+
+constexpr int kFp8Block = 128;
+
+// ---- scales and conversions ----------------------------------------------------------------------------------------------------------------
+// The smallest power of two s >= 2^-126 with amax <= 448 s, from amax's own bits (448 = 1.75 * 2^8): no logarithm and no division, so every
+// place that quantises a block has the same scale.  Zero: 1.
+__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
+  if (amax_bits == 0) return 1.0f;
+  const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return bits_f32((uint32_t)(e < 1 ? 1 : e) << 23);
+}
+// 1 / s for such a scale: a power of two between 2^-120 and 2^126
+__device__ __forceinline__ float fp8_inverse(float s) { return bits_f32(0x7F000000u - f32_bits(s)); }
+
+// the magnitude that counts for the scale: none for infinities and NaN
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t u = f32_bits(v) & 0x7FFFFFFFu;
+  return u < 0x7F800000u ? u : 0u;
+}
+// the largest of sixteen lanes' numbers, in each of them
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+#define TK_STEP(ctrl)                                                                             \
+  {                                                                                               \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, false);     \
+    v = o > v ? o : v;                                                                            \
+  }
+  TK_STEP(0xB1)   // quad_perm [1,0,3,2]
+  TK_STEP(0x4E)   // quad_perm [2,3,0,1]
+  TK_STEP(0x141)  // row_half_mirror
+  TK_STEP(0x140)  // row_mirror
+#undef TK_STEP
+  return v;
+}
+// four numbers of at most 448 (or NaN; an infinity becomes NaN, e4m3 has none) to e4m3, nearest, ties to even
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {
+  int o = 0;
+  o = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, o, false);
+  o = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, o, true);
+  return (uint32_t)o;
+}
+__device__ __forceinline__ float no_infinity(float v) { return (f32_bits(v) & 0x7FFFFFFFu) == 0x7F800000u ? bits_f32(0x7FC00000u) : v; }
+__device__ __forceinline__ void from_e4m3(uint32_t q, float* o) {
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+  o[0] = lo[0], o[1] = lo[1], o[2] = hi[0], o[3] = hi[1];
+}
+
+template <int DT>
+__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+  if constexpr (DT == TK_F32) return static_cast<const float*>(p)[i];
+  if constexpr (DT == TK_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+  return f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
+  if constexpr (DT == TK_F32)
+    static_cast<float*>(p)[i] = v;
+  else if constexpr (DT == TK_BF16)
+    static_cast<uint16_t*>(p)[i] = f32_to_bf16_bits(v);
+  else
+    static_cast<uint16_t*>(p)[i] = f32_to_f16_bits(v);
+}
+// N (4 or 8) consecutive elements, of an address that N elements' size divides up to 16 bytes
+template <int DT, int N>
+__device__ __forceinline__ void load_vec(const void* p, int64_t i, float* v) {
+  if constexpr (DT == TK_F32) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+      const f32x4_t t = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i + c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[c + k] = t[k];
+    }
+  } else {
+    uint32_t w[N / 2];
+    if constexpr (N == 8) {
+      const u32x4_t t = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = t[k];
+    } else {
+      const u32x2_t t = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + i);
+      w[0] = t[0], w[1] = t[1];
+    }
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      if constexpr (DT == TK_BF16) {
+        v[2 * k] = bits_f32(w[k] << 16), v[2 * k + 1] = bits_f32(w[k] & 0xFFFF0000u);
+      } else {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, w[k]);
+        v[2 * k] = (float)h[0], v[2 * k + 1] = (float)h[1];
+      }
+    }
+  }
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_vec(void* p, int64_t i, const float* v) {
+  if constexpr (DT == TK_F32) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) *reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + i + c) = f32x4_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) w[k] = pack_out2<DT == TK_F16>(v[2 * k], v[2 * k + 1]);
+    if constexpr (N == 8)
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + i) = u32x4_t{w[0], w[1], w[2], w[3]};
+    else
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p) + i) = u32x2_t{w[0], w[1]};
+  }
+}
+
+// ---- swiglu ----------------------------------------------------------------------------------------------------------------------------------
+// sigma(x) = 1 / (1 + exp(-x)) as the product u v, and 1 - sigma.  With t = exp(-|x| / 2) nothing overflows, sigma and 1 - sigma have no difference in them, and
+// (y u) v is good as long as y sigma is a normal number, where exp(-|x|) itself no longer is.  For results of 16 bits the hardware's exp2 and reciprocal (1 ulp
+// each) of a once rounded x log2(e): off by |x| 2^-24, next to 2^-9 of the result's rounding.  For fp32 results (EXACT) that product is kept in two parts and the
+// reciprocal is a division.
+struct Sigmoid {
+  float u, v, rest;
+};
+template <bool EXACT>
+__device__ __forceinline__ Sigmoid sigmoid_of(float x) {
+  const float ax = fabsf(x), hi = ax * -1.44269504088896340736f;
+  float t = __builtin_amdgcn_exp2f(hi * 0.5f);
+  if constexpr (EXACT) {
+    const float lo = fmaf(ax, -1.44269504088896340736f, -hi) - ax * 1.92596299112661746887e-8f;  // (log2(e) less its fp32)
+    if (hi > -512.0f) t = fmaf(t, lo * 0.346573590279972654709f, t);
+  }
+  const float e = t * t, d = 1.0f + e, r = EXACT ? 1.0f / d : __builtin_amdgcn_rcpf(d);
+  const bool neg = x < 0.f;
+  return Sigmoid{neg ? t : 1.0f, neg ? t * r : r, neg ? r : e * r};
+}
+// (comparisons that keep NaN, as torch's clamp does)
+__device__ __forceinline__ float at_most(float v, float m) { return v > m ? m : v; }
+__device__ __forceinline__ float at_least(float v, float m) { return v < m ? m : v; }
+
+template <bool EXACT>
+__device__ __forceinline__ float swiglu_of(float gate, float lin, float alpha, float limit) {
+  gate = at_most(gate, limit);
+  lin = at_least(at_most(lin, limit), -limit);
+  const Sigmoid q = sigmoid_of<EXACT>(alpha * gate);
+  const float s = gate * q.u * q.v;
+  return fmaf(s, lin, s);
+}
+
+// ---- the product's epilogue ------------------------------------------------------------------------------------------------------------------
+// rows behind the last slice
+template <int YT, bool SWIGLU>
+__device__ __forceinline__ void fp8_zero_rest(const Fp8GemmParams& p) {
+  if (!p.zero_rest || !p.slice_sizes) return;
+  const int cols = SWIGLU ? p.N / 2 : p.N;
+  for (int64_t r = (int64_t)p.slice_offs[p.n_slices] + blockIdx.x; r < p.M; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) store_elem<YT>(p.y, r * p.y_stride_m + c, 0.f);
+}
+
+// acc[f][j] = 32 x 32 fragment of output columns ncol0 + f * 32 .. and rows off_m + (j * WM + mw) * 32 .. of the slice, as the MFMA leaves it with the
+// weights as its first operand (register i of lane half h: column Frag<32>::n_of(i, h) of row lr).  n_end: the first column that the tile does not have.
+template <int YT, bool SWIGLU, int WM, int MFW, int NFW>
+__device__ __forceinline__ void fp8_epilogue(const Fp8GemmParams& p, f32x16_t (&acc)[NFW][MFW], int expert, int off_m, int start_m, int eM, int ncol0, int n_end,
+                                             int mw, int lr, int h) {
+  float gam[MFW];
+  int64_t dst[MFW];
+#pragma unroll
+  for (int j = 0; j < MFW; ++j) {
+    const int row = off_m + (j * WM + mw) * 32 + lr, r = start_m + (row < eM ? row : eM - 1);
+    dst[j] = r;
+    if (p.scatter) dst[j] = r < p.scatter_len ? p.scatter[r] : -1;
+    if (row >= eM) dst[j] = -1;
+    gam[j] = p.gammas ? load_scalar(p.gammas, r, p.gammas_is_f32) : 1.0f;
+  }
+#pragma unroll
+  for (int f = 0; f < NFW; ++f)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int n0 = ncol0 + f * 32 + 16 * u + 8 * h;  // the lane's eight columns, after the halves' exchange
+      float b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = p.bias && n0 + i < n_end ? load_scalar(p.bias, expert * p.bias_e + n0 + i, p.bias_is_f32) : 0.f;
+#pragma unroll
+      for (int j = 0; j < MFW; ++j) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const auto s = __builtin_amdgcn_permlane32_swap(f32_bits(acc[f][j][8 * u + i]), f32_bits(acc[f][j][8 * u + 4 + i]), false, false);
+          v[i] = bits_f32(s[0]) + b[i];
+          v[4 + i] = bits_f32(s[1]) + b[4 + i];
+        }
+        if (dst[j] < 0) continue;
+        const int64_t row = dst[j] * p.y_stride_m;
+        if constexpr (SWIGLU) {
+          float o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = swiglu_of<YT == TK_F32>(v[2 * i], v[2 * i + 1], p.alpha, p.limit) * gam[j];
+          if (p.y_vec && n0 + 8 <= n_end) {
+            store_vec<YT, 4>(p.y, row + n0 / 2, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n0 + 2 * i < n_end) store_elem<YT>(p.y, row + n0 / 2 + i, o[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= gam[j];
+          if (p.y_vec && n0 + 8 <= n_end) {
+            store_vec<YT, 8>(p.y, row + n0, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n0 + i < n_end) store_elem<YT>(p.y, row + n0 + i, v[i]);
+          }
+        }
+      }
+    }
+}
+
+}  // namespace
+}  // namespace tk

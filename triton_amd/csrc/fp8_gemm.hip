@@ -1,0 +1,167 @@
+// The ragged product of e4m3 operands with one scale for each block of 128: the entry point, and the kernel for operands of any alignment.
+//
+// A block's sum is one chain of two scaled MFMAs (32 x 32 x 64, scales of one) on a cleared accumulator; it is then added to the running sum times the row's and the
+// weights' scale of the block: one fused operation for each accumulator register and block of K.  With the weights as the first operand a lane's registers are
+// output columns of one row, so a lane needs one row scale a fragment, and 32 columns share the weights' scale.
+#include "fp8_blocks.h"
+
+namespace tk {
+namespace {
+
+constexpr int kAnyRows = 64, kAnyCols = 64;
+
+__device__ __forceinline__ f32x16_t mfma_e4m3(i32x8_t w, i32x8_t x, f32x16_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+}
+
+// sixteen bytes at `k` of a row of K, whatever its address; zeros past K and without a row
+__device__ __forceinline__ u32x4_t load_piece(const uint8_t* row, int k, int K) {
+  u32x4_t v = {0, 0, 0, 0};
+  if (!row || k >= K) return v;
+  if (k + 16 <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+    for (int i = 0; i < K - k; ++i) v[i >> 2] |= (uint32_t)row[k + i] << (i & 3) * 8;
+  }
+  return v;
+}
+
+// The same product from the values' exact 16-bit form, for fp32 results: the e4m3 instructions add eight products at a time and drop what of one lies below 2^-13
+// of the power of two in the largest of them, which the rounding of a 16-bit result hides and that of an fp32 one does not.
+__device__ __forceinline__ f32x16_t mfma_e4m3_exact(i32x8_t w, i32x8_t x, f32x16_t c) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    bf16x8_t a, b;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bf16x2_t a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * t + i], 1.0f, false), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * t + i], 1.0f, true);
+      const bf16x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * t + i], 1.0f, false), b1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * t + i], 1.0f, true);
+      a[4 * i] = a0[0], a[4 * i + 1] = a0[1], a[4 * i + 2] = a1[0], a[4 * i + 3] = a1[1];
+      b[4 * i] = b0[0], b[4 * i + 1] = b0[1], b[4 * i + 2] = b1[0], b[4 * i + 3] = b1[1];
+    }
+    c = Frag<32>::mma(a, b, c);
+  }
+  return c;
+}
+
+// 64 x 64 tiles, four waves of 32 x 32; the next block of K is loaded into registers while this one is multiplied from LDS.
+template <int YT, bool SWIGLU>
+__global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams p) {
+  constexpr int PITCH = kFp8Block + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t xs[kAnyRows * PITCH], ws[kAnyCols * PITCH];
+  fp8_zero_rest<YT, SWIGLU>(p);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lr = lane & 31, h = lane >> 5, mw = wave & 1, nw = wave >> 1;
+  const int tile_n = blockIdx.x % p.grid_n, tile_m = blockIdx.x / p.grid_n;
+  int expert = 0, off_m = tile_m * kAnyRows, start_m = 0, eM = p.M;
+  if (p.slice_sizes) {
+    const int32_t where = p.block_sched[tile_m];
+    if (where < 0) return;
+    expert = where & 0xFFFF, off_m = (where >> 16) * kAnyRows;
+    start_m = p.slice_offs[expert], eM = p.slice_sizes[expert];
+  }
+  if (off_m >= eM) return;
+  const int n0 = tile_n * kAnyCols;
+  const int piece = (tid & 7) * 16, line = tid >> 3;
+  const uint8_t *x_row[2], *w_row[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = off_m + line + i * 32, n = n0 + line + i * 32;
+    x_row[i] = w_row[i] = nullptr;
+    if (m < eM) x_row[i] = p.x + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.x_stride_m;
+    if (n < p.N) w_row[i] = p.w + expert * p.w_e + n * p.w_n;
+  }
+  const int m = off_m + mw * 32 + lr;
+  const float* row_scale = nullptr;
+  if (m < eM) row_scale = p.xs + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.xs_m;
+  const int n_wave = n0 + nw * 32;
+  const float* col_scale = p.ws + expert * p.ws_e + (int64_t)((n_wave < p.N ? n_wave : 0) / kFp8Block) * p.ws_n;
+
+  f32x16_t acc[1][1];
+  const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  acc[0][0] = zero;
+  u32x4_t xr[2], wr[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], piece, p.K), wr[i] = load_piece(w_row[i], piece, p.K);
+  for (int k0 = 0, b = 0; k0 < p.K; k0 += kFp8Block, ++b) {
+    const float s = row_scale ? row_scale[b * p.xs_k] * col_scale[b * p.ws_k] : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<u32x4_t*>(xs + (line + i * 32) * PITCH + piece) = xr[i];
+      *reinterpret_cast<u32x4_t*>(ws + (line + i * 32) * PITCH + piece) = wr[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], k0 + kFp8Block + piece, p.K), wr[i] = load_piece(w_row[i], k0 + kFp8Block + piece, p.K);
+    f32x16_t part = zero;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      i32x8_t a, c;
+      __builtin_memcpy(&a, ws + (nw * 32 + lr) * PITCH + u * 64 + h * 32, 32);
+      __builtin_memcpy(&c, xs + (mw * 32 + lr) * PITCH + u * 64 + h * 32, 32);
+      part = YT == TK_F32 ? mfma_e4m3_exact(a, c, part) : mfma_e4m3(a, c, part);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[0][0][i] = fmaf(part[i], s, acc[0][0][i]);
+  }
+  fp8_epilogue<YT, SWIGLU, 2, 1, 1>(p, acc, expert, off_m, start_m, eM, n_wave, p.N, mw, lr, h);
+}
+
+int32_t launch_any(Fp8GemmParams p, int yt, bool swiglu, hipStream_t st) {
+  p.grid_n = (int)cdiv(p.N, kAnyCols);
+  const int64_t grid = (int64_t)p.grid_m * p.grid_n;
+  if (grid > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: grid too large");
+  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), 0, st, p); };
+  switch (yt) {
+    case TK_F32:
+      swiglu ? launch(fp8_block_any_kernel<TK_F32, true>) : launch(fp8_block_any_kernel<TK_F32, false>);
+      break;
+    case TK_BF16:
+      swiglu ? launch(fp8_block_any_kernel<TK_BF16, true>) : launch(fp8_block_any_kernel<TK_BF16, false>);
+      break;
+    default:
+      swiglu ? launch(fp8_block_any_kernel<TK_F16, true>) : launch(fp8_block_any_kernel<TK_F16, false>);
+  }
+  return check_launch("fp8_block_any_kernel");
+}
+
+}  // namespace
+}  // namespace tk
+
+using namespace tk;
+
+extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stream) {
+  if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: null descriptor");
+  if (d->M < 0 || d->N < 0 || d->K < 0 || d->n_slices < 0 || d->grid_m < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: negative size");
+  if (d->y_dtype != TK_F32 && d->y_dtype != TK_BF16 && d->y_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: the output is fp32, bf16 or fp16 (dtype %d)", d->y_dtype);
+  if (d->activation != TK_ACT_NONE && d->activation != TK_ACT_SWIGLU) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: bad activation %d", d->activation);
+  const bool swiglu = d->activation == TK_ACT_SWIGLU;
+  if (swiglu && d->N % 2) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: swiglu needs an even number of columns (got %d)", d->N);
+  if (d->bias && d->bias_dtype != TK_F32 && d->bias_dtype != TK_BF16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: the bias is fp32 or bf16 (dtype %d)", d->bias_dtype);
+  if (d->gammas && d->gammas_dtype != TK_F32 && d->gammas_dtype != TK_BF16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: gammas are fp32 or bf16 (dtype %d)", d->gammas_dtype);
+  if (d->M == 0 || d->N == 0) return TK_OK;
+  if (!d->y || (d->K > 0 && (!d->x || !d->x_scale || (d->n_slices > 0 && (!d->w || !d->w_scale))))) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: null operand");
+  if (d->slice_sizes) {
+    if (!d->slice_offs || !d->block_schedule) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: slices need their offsets and block schedule");
+    if (d->n_slices > 0xFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: up to 65535 slices (got %d)", d->n_slices);
+  } else if (d->n_slices != 1) {
+    return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: %d slices without their sizes", d->n_slices);
+  }
+  Fp8GemmParams p = {};
+  p.x = d->x, p.x_stride_m = d->x_stride_m, p.xs = d->x_scale, p.xs_m = d->xs_stride_m, p.xs_k = d->xs_stride_k;
+  p.w = d->w, p.w_e = d->w_stride_e, p.w_n = d->w_stride_n;
+  p.ws = d->w_scale, p.ws_e = d->ws_stride_e, p.ws_k = d->ws_stride_k, p.ws_n = d->ws_stride_n;
+  p.bias = d->bias, p.bias_e = d->bias_stride_e, p.bias_is_f32 = d->bias_dtype == TK_F32;
+  p.gather = d->gather_indx, p.scatter = d->scatter_indx, p.scatter_len = d->scatter_len;
+  p.gammas = d->gammas, p.gammas_is_f32 = d->gammas_dtype == TK_F32;
+  p.slice_sizes = d->slice_sizes, p.slice_offs = d->slice_offs, p.block_sched = d->block_schedule;
+  p.n_slices = d->n_slices, p.grid_m = d->slice_sizes ? d->grid_m : (int)cdiv(d->M, kAnyRows);
+  p.M = d->M, p.N = d->N, p.K = d->K;
+  p.y = d->y, p.y_stride_m = d->y_stride_m;
+  p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && d->y_stride_m * (d->y_dtype == TK_F32 ? 4 : 2) % 16 == 0;
+  p.alpha = d->act_alpha, p.limit = d->act_has_limit ? d->act_limit : INFINITY;
+  p.zero_rest = d->zero_rest;
+  if (p.grid_m == 0) return TK_OK;
+  return launch_any(p, d->y_dtype, swiglu, static_cast<hipStream_t>(stream));
+}

@@ -32,7 +32,9 @@ struct TileList {
   static __device__ __forceinline__ int n_short(int rows) { return rows > n_full(rows) * BM ? 1 : 0; }
 
   // n_cols = tiles of a row block; returns this workgroup's first index (it has none if that is not below t_end; the following ones are t_step apart)
-  __device__ __forceinline__ int init(const GemmParams& p, int lane, int n_cols) {
+  // (P: a kernel's parameters, with the slices, M and N under GemmParams' names)
+  template <class P>
+  __device__ __forceinline__ int init(const P& p, int lane, int n_cols) {
     int full = 0, brief = 0;
 #pragma unroll
     for (int c = 0; c < kSliceRegs; ++c) {

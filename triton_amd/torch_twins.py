@@ -383,3 +383,91 @@ def distill_topk_torch(logits, teacher_logits, teacher_indx, temperature: float 
     a = torch.where(live, la.exp(), lp.new_zeros(()))
     at = torch.where(live, teacher_indx, torch.zeros_like(teacher_indx)).to(torch.int64)
     return torch.where(a != 0, a * (la - lp.gather(1, at)), a).sum(1)
+
+
+# ---- e4m3 with a scale for each block of 128 ---------------------------------------------------------------
+
+def _fp8_block_view(x, block_rows):
+    """[..., R, C] as [..., R / block_rows, block_rows, C / 128, 128], filled up with zeros."""
+    R, C = x.shape[-2:]
+    x = torch.nn.functional.pad(x, (0, -C % 128, 0, -R % block_rows))
+    return x.unflatten(-1, (-1, 128)).unflatten(-3, (-1, block_rows))
+
+
+def downcast_to_fp8_blocks_torch(x, block_rows: int = 1):
+    """`(values, scales)`: the smallest power of two (2^-126 at least) as a scale that leaves a block's largest finite magnitude at most 448, 1 for a block of zeros."""
+    x2 = x[None] if x.ndim == 1 else x
+    b = _fp8_block_view(x2.to(torch.float32), block_rows)
+    amax = torch.where(b.isfinite(), b.abs(), b.new_zeros(())).amax((-3, -1))
+    fraction, exponent = torch.frexp(amax)
+    exponent = torch.where(fraction <= 0.875, exponent - 9, exponent - 8).clamp_min(-126)  # 448 = 0.875 * 2^9
+    scales = torch.where(amax == 0, torch.ones_like(amax), torch.ldexp(torch.ones_like(amax), exponent))
+    q = torch.where(b.isinf(), b.new_full((), float("nan")), b) / scales[..., :, None, :, None]
+    q = q.flatten(-2).flatten(-3, -2)[..., :x2.shape[-2], :x2.shape[-1]].to(torch.float8_e4m3fn)
+    return (q[0], scales[0]) if x.ndim == 1 else (q, scales)
+
+
+def upcast_from_fp8_blocks_torch(values, scales, dtype=torch.bfloat16, block_rows: int = 1):
+    """`values * scales` in fp32, rounded to `dtype`."""
+    v2, s2 = (values[None], scales[None]) if values.ndim == 1 else (values, scales)
+    b = _fp8_block_view(v2.to(torch.float32), block_rows) * s2[..., :, None, :, None]
+    out = b.flatten(-2).flatten(-3, -2)[..., :v2.shape[-2], :v2.shape[-1]].to(dtype)
+    return out[0] if values.ndim == 1 else out
+
+
+def _fp8_slices(md, rows):
+    if md is None:
+        return [(0, rows)]
+    offs = md.slice_offs.tolist()
+    return [(offs[e], offs[e] + n) for e, n in enumerate(md.slice_sizes.tolist())]
+
+
+def matmul_fp8_blocks_torch(a, a_scale, w, w_scale, bias=None, a_ragged_metadata=None, gather_indx=None, scatter_indx=None, gammas=None, fused_activation=None,
+                            out_dtype=torch.bfloat16):
+    """The ragged product of 8-bit operands in fp32; rows that nothing is written to are zero."""
+    w, w_scale = (w[None], w_scale[None]) if w.ndim == 2 else (w, w_scale)
+    x = upcast_from_fp8_blocks_torch(a, a_scale, torch.float32)
+    x = x if gather_indx is None else x[gather_indx.long()]
+    wf = upcast_from_fp8_blocks_torch(w, w_scale, torch.float32, 128)
+    y = x.new_zeros((x.shape[0], wf.shape[2]))
+    for e, (lo, hi) in enumerate(_fp8_slices(a_ragged_metadata, x.shape[0])):
+        y[lo:hi] = x[lo:hi] @ wf[e] + (0 if bias is None else (bias if bias.ndim == 2 else bias[None])[e].to(torch.float32))
+    if fused_activation is not None and fused_activation.specs.name == "swiglu":
+        y = _swiglu_parts(y, *fused_activation.fn_args)[0]
+    y = y if gammas is None else y * gammas.to(torch.float32)[:, None]
+    if scatter_indx is None:
+        return y.to(out_dtype)
+    out = y.new_zeros((scatter_indx.shape[0], y.shape[1]))
+    n = min(y.shape[0], scatter_indx.shape[0])
+    live = scatter_indx[:n] >= 0
+    out[scatter_indx[:n][live].long()] = y[:n][live]
+    return out.to(out_dtype)
+
+
+def weight_gradient_fp8_blocks_torch(x, x_scale, dy, ragged_metadata=None, out_dtype=None):
+    """`(x * x_scale)^T dy` of each slice in fp32, the first factor rounded to dy's type."""
+    top = torch.finfo(dy.dtype).max
+    xf = upcast_from_fp8_blocks_torch(x, x_scale, torch.float32).clamp(-top, top).to(dy.dtype).to(torch.float32)
+    out = torch.stack([xf[lo:hi].T @ dy[lo:hi].to(torch.float32) for lo, hi in _fp8_slices(ragged_metadata, x.shape[0])]).to(out_dtype or dy.dtype)
+    return out[0] if ragged_metadata is None else out
+
+
+def _swiglu_parts(a, alpha, limit=None):
+    gate, linear = a[..., 0::2], a[..., 1::2]
+    if limit is not None:
+        gate, linear = gate.clamp(max=limit), linear.clamp(-limit, limit)
+    sigmoid = torch.sigmoid(alpha * gate)
+    return gate * sigmoid * (linear + 1), gate, linear, sigmoid
+
+
+def swiglu_fp8_backward_torch(dh, values, scales, alpha, limit=None):
+    """The gradient of swiglu's input at its 8-bit copy, in fp32."""
+    a = upcast_from_fp8_blocks_torch(values, scales, torch.float32)
+    _, gate, linear, sigmoid = _swiglu_parts(a, alpha, limit)
+    d = dh.reshape(a.shape[0], -1).to(torch.float32)
+    da = torch.stack((d * (linear + 1) * sigmoid * (1 + alpha * gate * (1 - sigmoid)), d * gate * sigmoid), -1).flatten(-2)
+    if limit is not None:
+        beyond = a.abs() > limit
+        beyond[:, 0::2] = a[:, 0::2] > limit
+        da = torch.where(beyond, da.new_zeros(()), da)
+    return da.to(dh.dtype).view(*dh.shape[:-1], a.shape[1])
