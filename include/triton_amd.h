@@ -684,6 +684,7 @@ typedef struct tk_fp8_gemm_desc {
   int32_t activation; /* TK_ACT_* */
   float act_alpha, act_limit;
   int32_t act_has_limit, zero_rest;
+  int32_t pow2_scales; /* the caller vouches that all scales are powers of two from 2^-126 on, as tk_fp8_block_downcast makes them: the kernels may multiply by exponents */
 } tk_fp8_gemm_desc;
 int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* desc, tk_stream_t stream);
 

@@ -116,7 +116,7 @@ class Fp8GemmDesc(_c.Structure):
         ("bias", _ptr), ("bias_dtype", _i32), ("bias_stride_e", _i64), ("gather_indx", _ptr), ("scatter_indx", _ptr), ("scatter_len", _i32),
         ("gammas", _ptr), ("gammas_dtype", _i32), ("slice_sizes", _ptr), ("slice_offs", _ptr), ("block_schedule", _ptr), ("n_slices", _i32),
         ("grid_m", _i32), ("M", _i32), ("N", _i32), ("K", _i32), ("y", _ptr), ("y_dtype", _i32), ("y_stride_m", _i64), ("activation", _i32),
-        ("act_alpha", _f32), ("act_limit", _f32), ("act_has_limit", _i32), ("zero_rest", _i32),
+        ("act_alpha", _f32), ("act_limit", _f32), ("act_has_limit", _i32), ("zero_rest", _i32), ("pow2_scales", _i32),
     ]
 
 

@@ -31,11 +31,22 @@ struct Fp8GemmParams {
   int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
   float alpha, limit;  // (limit: +inf without one)
   int32_t zero_rest;
+  int32_t pow2;      // all scales are powers of two (fp8_scale's)
+  uint32_t x_bytes;  // with gather: the extent of x for a buffer resource
 };
+
+// 16-bit results, up to kDmaSlices slices, operands as fp8_tiles_run (fp8_gemm.hip) wants them; tile = 256 or 128
+int32_t fp8_gemm_launch_tiles(const Fp8GemmParams& p, int tile, int yt, bool swiglu, hipStream_t st);
 
 namespace {
 
 constexpr int kFp8Block = 128;
+
+// c + the product of 16 columns of w and 16 rows of x over a block of 128: lane l holds 32 consecutive k, from (l >> 4) * 32 on, of column / row l & 15.  The
+// scales are e8m0 bytes, the exponents of powers of two as fp32 numbers have them.
+__device__ __forceinline__ f32x4_t mfma_block(i32x8_t w, i32x8_t x, f32x4_t c, uint32_t w_exp = 0x7F7F7F7Fu, uint32_t x_exp = 0x7F7F7F7Fu) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, (int)w_exp, 0, (int)x_exp);
+}
 
 // ---- scales and conversions ----------------------------------------------------------------------------------------------------------------
 // The smallest power of two s >= 2^-126 with amax <= 448 s, from amax's own bits (448 = 1.75 * 2^8): no logarithm and no division, so every
@@ -185,64 +196,65 @@ __device__ __forceinline__ void fp8_zero_rest(const Fp8GemmParams& p) {
     for (int c = threadIdx.x; c < cols; c += blockDim.x) store_elem<YT>(p.y, r * p.y_stride_m + c, 0.f);
 }
 
-// acc[f][j] = 32 x 32 fragment of output columns ncol0 + f * 32 .. and rows off_m + (j * WM + mw) * 32 .. of the slice, as the MFMA leaves it with the
-// weights as its first operand (register i of lane half h: column Frag<32>::n_of(i, h) of row lr).  n_end: the first column that the tile does not have.
+// acc[f][j] = 16 x 16 fragment of output columns ncol0 + f * 16 .. and rows off_m + (j * WM + mw) * 16 .. of the slice, as the MFMA leaves it with the
+// weights as its first operand: register i of lane l is column (l >> 4) * 4 + i of row l & 15.  n_end: the first column that the tile does not have.
 template <int YT, bool SWIGLU, int WM, int MFW, int NFW>
-__device__ __forceinline__ void fp8_epilogue(const Fp8GemmParams& p, f32x16_t (&acc)[NFW][MFW], int expert, int off_m, int start_m, int eM, int ncol0, int n_end,
-                                             int mw, int lr, int h) {
+__device__ __forceinline__ void fp8_epilogue(const Fp8GemmParams& p, f32x4_t (&acc)[NFW][MFW], int expert, int off_m, int start_m, int eM, int ncol0, int n_end,
+                                             int mw, int lane) {
+  static_assert(NFW % 2 == 0, "fragments go in pairs");
+  const int lr = lane & 15, g4 = lane >> 4;
   float gam[MFW];
-  int64_t dst[MFW];
+  int dst[MFW];
 #pragma unroll
   for (int j = 0; j < MFW; ++j) {
-    const int row = off_m + (j * WM + mw) * 32 + lr, r = start_m + (row < eM ? row : eM - 1);
+    const int row = off_m + (j * WM + mw) * 16 + lr, r = start_m + (row < eM ? row : eM - 1);
     dst[j] = r;
     if (p.scatter) dst[j] = r < p.scatter_len ? p.scatter[r] : -1;
     if (row >= eM) dst[j] = -1;
     gam[j] = p.gammas ? load_scalar(p.gammas, r, p.gammas_is_f32) : 1.0f;
   }
 #pragma unroll
-  for (int f = 0; f < NFW; ++f)
+  for (int f = 0; f < NFW; f += 2) {
+    // after the exchange of the odd groups of sixteen lanes of the first fragment with the even ones of the second a lane has eight consecutive columns
+    const int n0 = ncol0 + f * 16 + (g4 & 1) * 16 + (g4 >> 1) * 8;
+    float b[8];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int n0 = ncol0 + f * 32 + 16 * u + 8 * h;  // the lane's eight columns, after the halves' exchange
-      float b[8];
+    for (int i = 0; i < 8; ++i) b[i] = p.bias && n0 + i < n_end ? load_scalar(p.bias, expert * p.bias_e + n0 + i, p.bias_is_f32) : 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = p.bias && n0 + i < n_end ? load_scalar(p.bias, expert * p.bias_e + n0 + i, p.bias_is_f32) : 0.f;
+    for (int j = 0; j < MFW; ++j) {
+      float v[8];
 #pragma unroll
-      for (int j = 0; j < MFW; ++j) {
-        float v[8];
+      for (int i = 0; i < 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(f32_bits(acc[f][j][i]), f32_bits(acc[f + 1][j][i]), false, false);
+        v[i] = bits_f32(s[0]) + b[i];
+        v[4 + i] = bits_f32(s[1]) + b[4 + i];
+      }
+      if (dst[j] < 0) continue;
+      const int64_t row = (int64_t)dst[j] * p.y_stride_m;
+      if constexpr (SWIGLU) {
+        float o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const auto s = __builtin_amdgcn_permlane32_swap(f32_bits(acc[f][j][8 * u + i]), f32_bits(acc[f][j][8 * u + 4 + i]), false, false);
-          v[i] = bits_f32(s[0]) + b[i];
-          v[4 + i] = bits_f32(s[1]) + b[4 + i];
-        }
-        if (dst[j] < 0) continue;
-        const int64_t row = dst[j] * p.y_stride_m;
-        if constexpr (SWIGLU) {
-          float o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = swiglu_of<YT == TK_F32>(v[2 * i], v[2 * i + 1], p.alpha, p.limit) * gam[j];
-          if (p.y_vec && n0 + 8 <= n_end) {
-            store_vec<YT, 4>(p.y, row + n0 / 2, o);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n0 + 2 * i < n_end) store_elem<YT>(p.y, row + n0 / 2 + i, o[i]);
-          }
+        for (int i = 0; i < 4; ++i) o[i] = swiglu_of<YT == TK_F32>(v[2 * i], v[2 * i + 1], p.alpha, p.limit) * gam[j];
+        if (p.y_vec && n0 + 8 <= n_end) {
+          store_vec<YT, 4>(p.y, row + n0 / 2, o);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= gam[j];
-          if (p.y_vec && n0 + 8 <= n_end) {
-            store_vec<YT, 8>(p.y, row + n0, v);
-          } else {
+          for (int i = 0; i < 4; ++i)
+            if (n0 + 2 * i < n_end) store_elem<YT>(p.y, row + n0 / 2 + i, o[i]);
+        }
+      } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (n0 + i < n_end) store_elem<YT>(p.y, row + n0 + i, v[i]);
-          }
+        for (int i = 0; i < 8; ++i) v[i] *= gam[j];
+        if (p.y_vec && n0 + 8 <= n_end) {
+          store_vec<YT, 8>(p.y, row + n0, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n0 + i < n_end) store_elem<YT>(p.y, row + n0 + i, v[i]);
         }
       }
     }
+  }
 }
 
 }  // namespace

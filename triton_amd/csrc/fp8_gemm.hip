@@ -1,18 +1,14 @@
 // The ragged product of e4m3 operands with one scale for each block of 128: the entry point, and the kernel for operands of any alignment.
 //
-// A block's sum is one chain of two scaled MFMAs (32 x 32 x 64, scales of one) on a cleared accumulator; it is then added to the running sum times the row's and the
-// weights' scale of the block: one fused operation for each accumulator register and block of K.  With the weights as the first operand a lane's registers are
-// output columns of one row, so a lane needs one row scale a fragment, and 32 columns share the weights' scale.
+// A block's sum is one MFMA (16 x 16 x 128) on a cleared accumulator; it is then added to the running sum times the row's and the weights' scale of the block: one fused
+// operation for each accumulator register and block of K.  With the weights as the first operand a lane's registers are output columns of one row, so a lane needs
+// one row scale a fragment, and the columns of a fragment share the weights' scale.
 #include "fp8_blocks.h"
 
 namespace tk {
 namespace {
 
 constexpr int kAnyRows = 64, kAnyCols = 64;
-
-__device__ __forceinline__ f32x16_t mfma_e4m3(i32x8_t w, i32x8_t x, f32x16_t c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
-}
 
 // sixteen bytes at `k` of a row of K, whatever its address; zeros past K and without a row
 __device__ __forceinline__ u32x4_t load_piece(const uint8_t* row, int k, int K) {
@@ -28,9 +24,9 @@ __device__ __forceinline__ u32x4_t load_piece(const uint8_t* row, int k, int K) 
 
 // The same product from the values' exact 16-bit form, for fp32 results: the e4m3 instructions add eight products at a time and drop what of one lies below 2^-13
 // of the power of two in the largest of them, which the rounding of a 16-bit result hides and that of an fp32 one does not.
-__device__ __forceinline__ f32x16_t mfma_e4m3_exact(i32x8_t w, i32x8_t x, f32x16_t c) {
+__device__ __forceinline__ f32x4_t mfma_block_exact(i32x8_t w, i32x8_t x, f32x4_t c) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < 4; ++t) {  // (eight of the lane's k each: any order does that is the same for both)
     bf16x8_t a, b;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -39,19 +35,19 @@ __device__ __forceinline__ f32x16_t mfma_e4m3_exact(i32x8_t w, i32x8_t x, f32x16
       a[4 * i] = a0[0], a[4 * i + 1] = a0[1], a[4 * i + 2] = a1[0], a[4 * i + 3] = a1[1];
       b[4 * i] = b0[0], b[4 * i + 1] = b0[1], b[4 * i + 2] = b1[0], b[4 * i + 3] = b1[1];
     }
-    c = Frag<32>::mma(a, b, c);
+    c = Frag<16>::mma(a, b, c);
   }
   return c;
 }
 
-// 64 x 64 tiles, four waves of 32 x 32; the next block of K is loaded into registers while this one is multiplied from LDS.
+// 64 x 64 tiles, four waves of 32 x 32 (two fragments by two); the next block of K is loaded into registers while this one is multiplied from LDS.
 template <int YT, bool SWIGLU>
 __global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams p) {
   constexpr int PITCH = kFp8Block + 16;
   __shared__ __attribute__((aligned(16))) uint8_t xs[kAnyRows * PITCH], ws[kAnyCols * PITCH];
   fp8_zero_rest<YT, SWIGLU>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int lr = lane & 31, h = lane >> 5, mw = wave & 1, nw = wave >> 1;
+  const int lr = lane & 15, g = lane >> 4, mw = wave & 1, nw = wave >> 1;
   const int tile_n = blockIdx.x % p.grid_n, tile_m = blockIdx.x / p.grid_n;
   int expert = 0, off_m = tile_m * kAnyRows, start_m = 0, eM = p.M;
   if (p.slice_sizes) {
@@ -71,20 +67,24 @@ __global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams 
     if (m < eM) x_row[i] = p.x + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.x_stride_m;
     if (n < p.N) w_row[i] = p.w + expert * p.w_e + n * p.w_n;
   }
-  const int m = off_m + mw * 32 + lr;
-  const float* row_scale = nullptr;
-  if (m < eM) row_scale = p.xs + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.xs_m;
+  const float* row_scale[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int m = off_m + (j * 2 + mw) * 16 + lr;
+    row_scale[j] = m < eM ? p.xs + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.xs_m : nullptr;
+  }
   const int n_wave = n0 + nw * 32;
   const float* col_scale = p.ws + expert * p.ws_e + (int64_t)((n_wave < p.N ? n_wave : 0) / kFp8Block) * p.ws_n;
 
-  f32x16_t acc[1][1];
-  const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  acc[0][0] = zero;
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t acc[2][2] = {{zero, zero}, {zero, zero}};
   u32x4_t xr[2], wr[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], piece, p.K), wr[i] = load_piece(w_row[i], piece, p.K);
   for (int k0 = 0, b = 0; k0 < p.K; k0 += kFp8Block, ++b) {
-    const float s = row_scale ? row_scale[b * p.xs_k] * col_scale[b * p.ws_k] : 0.f;
+    float s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = row_scale[j] ? row_scale[j][b * p.xs_k] * col_scale[b * p.ws_k] : 0.f;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -94,18 +94,22 @@ __global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams 
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], k0 + kFp8Block + piece, p.K), wr[i] = load_piece(w_row[i], k0 + kFp8Block + piece, p.K);
-    f32x16_t part = zero;
+    i32x8_t a[2], c[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      i32x8_t a, c;
-      __builtin_memcpy(&a, ws + (nw * 32 + lr) * PITCH + u * 64 + h * 32, 32);
-      __builtin_memcpy(&c, xs + (mw * 32 + lr) * PITCH + u * 64 + h * 32, 32);
-      part = YT == TK_F32 ? mfma_e4m3_exact(a, c, part) : mfma_e4m3(a, c, part);
+    for (int i = 0; i < 2; ++i) {
+      __builtin_memcpy(&a[i], ws + (nw * 32 + i * 16 + lr) * PITCH + g * 32, 32);
+      __builtin_memcpy(&c[i], xs + ((i * 2 + mw) * 16 + lr) * PITCH + g * 32, 32);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[0][0][i] = fmaf(part[i], s, acc[0][0][i]);
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f32x4_t part = YT == TK_F32 ? mfma_block_exact(a[f], c[j], zero) : mfma_block(a[f], c[j], zero);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][j][i] = fmaf(part[i], s[j], acc[f][j][i]);
+      }
   }
-  fp8_epilogue<YT, SWIGLU, 2, 1, 1>(p, acc, expert, off_m, start_m, eM, n_wave, p.N, mw, lr, h);
+  fp8_epilogue<YT, SWIGLU, 2, 2, 2>(p, acc, expert, off_m, start_m, eM, n_wave, p.N, mw, lane);
 }
 
 int32_t launch_any(Fp8GemmParams p, int yt, bool swiglu, hipStream_t st) {
@@ -124,6 +128,20 @@ int32_t launch_any(Fp8GemmParams p, int yt, bool swiglu, hipStream_t st) {
       swiglu ? launch(fp8_block_any_kernel<TK_F16, true>) : launch(fp8_block_any_kernel<TK_F16, false>);
   }
   return check_launch("fp8_block_any_kernel");
+}
+
+// What the kernels with memory-to-LDS transfers need: lines that begin at sixteen-byte boundaries, and offsets within a buffer resource (2 GiB) from the start of a
+// tile, or of x and its scales where rows are gathered.
+bool fp8_tiles_run(Fp8GemmParams& p, int64_t x_rows, int yt) {
+  const int64_t limit = (int64_t)1 << 31, K16 = (p.K + 15) & ~15, blocks = cdiv(p.K, kFp8Block), rows = p.gather ? x_rows : 256;
+  if (yt == TK_F32 || p.K == 0 || (p.slice_sizes && p.n_slices > kDmaSlices)) return false;
+  if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) return false;
+  if (p.x_stride_m < 0 || p.w_n < 0 || p.xs_m < 0 || p.xs_k < 0 || p.ws_k < 0 || p.ws_n < 0) return false;
+  const int64_t x_bytes = (rows - 1) * p.x_stride_m + K16;
+  if (x_bytes >= limit || 255 * p.w_n + K16 >= limit) return false;
+  if (((rows - 1) * p.xs_m + blocks * p.xs_k) * 4 >= limit || (p.ws_n + blocks * p.ws_k) * 4 >= limit) return false;
+  p.x_bytes = (uint32_t)x_bytes;
+  return true;
 }
 
 }  // namespace
@@ -161,7 +179,11 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   p.y = d->y, p.y_stride_m = d->y_stride_m;
   p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && d->y_stride_m * (d->y_dtype == TK_F32 ? 4 : 2) % 16 == 0;
   p.alpha = d->act_alpha, p.limit = d->act_has_limit ? d->act_limit : INFINITY;
-  p.zero_rest = d->zero_rest;
+  p.zero_rest = d->zero_rest, p.pow2 = d->pow2_scales;
   if (p.grid_m == 0) return TK_OK;
+  if (fp8_tiles_run(p, d->x_rows, d->y_dtype)) {
+    const int64_t slices = d->slice_sizes ? d->n_slices : 1;
+    return fp8_gemm_launch_tiles(p, d->M >= slices * 192 ? 256 : 128, d->y_dtype, swiglu, static_cast<hipStream_t>(stream));
+  }
   return launch_any(p, d->y_dtype, swiglu, static_cast<hipStream_t>(stream));
 }

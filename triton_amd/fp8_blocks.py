@@ -147,8 +147,9 @@ def _check_metadata(md, n_slices, device):
         raise ValueError(f"a_ragged_metadata must live on {device} (got {md.slice_sizes.device})")
 
 
-def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dtype, zero_rest):
-    """One launch; operands as checked by the callers, `w [E, K, N]` with K contiguous."""
+def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dtype, training):
+    """One launch; operands as checked by the callers, `w [E, K, N]` with K contiguous.  `training`: rows behind the slices become zero, and all scales are the
+    quantiser's."""
     M = a.shape[0] if gather is None else gather.shape[0]
     K, N = w.shape[1], w.shape[2]
     swiglu = act is not None
@@ -178,7 +179,7 @@ def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dt
     if swiglu:
         d.activation, d.act_alpha = nt.TK_ACT_SWIGLU, act[0]
         d.act_limit, d.act_has_limit = (act[1], 1) if act[1] is not None else (0.0, 0)
-    d.zero_rest = int(zero_rest)
+    d.zero_rest = d.pow2_scales = int(training)
     nt.submit(nt.lib().tk_fp8_block_gemm, d, a.device)
     return y
 
