@@ -8,6 +8,8 @@
 //   * Scales that are powers of two (a caller that had both operands quantised here says so) go into the matrix instruction as exponents, and it adds
 //     to the running sum itself.
 //   * The scales of a stage (one a row, one or two for the columns) come by transfers of four bytes a lane beside the operands.
+//   * A stage's columns are in registers from the end of the one before, so a second barrier in its middle frees their buffer and the transfers of the stage after
+//     next begin there; those of the rows follow behind the stage's last reads.
 //   * Transfers, the order of 16-byte pieces in LDS, the list of tiles and the run across tiles are those of moe_gemm_dma_kernel.h.
 //   * K that is no multiple of 16: the last piece of a row holds bytes of whatever follows; they are cleared in LDS before the last stage is read.
 #include "fp8_blocks.h"
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
 
   // A stage; its columns and its first row fragment are in registers.
   auto stage = [&](bool next_has_tail) __attribute__((always_inline)) {
-    constexpr int ALL = MFW * NFW, SKEW = 3;  // (up to NFW - 1: a result's registers are taken again NFW products later)
+    constexpr int MID = MFW / 2 - 1, ALL = MFW * NFW, SKEW = 3;  // (up to NFW - 1: a result's registers are taken again NFW products later)
     float s[2];
     auto add = [&](auto t_c) __attribute__((always_inline)) {  // product T's sums, times the scales
       constexpr int T = decltype(t_c)::value, J = T / NFW, F = T % NFW;
@@ -188,8 +190,8 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
       constexpr int T = decltype(t_c)::value, J = T / NFW, F = T % NFW;
       constexpr bool END = J == MFW - 1;
       if constexpr (END && F == 0) {
-        // every wave has read this stage, and the next one has landed
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // every wave has read this stage, and the next one has landed (in flight behind it: the columns that MID asked for)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::TR) : "memory");
         barrier();
         if (next_has_tail) clear_tail(b ^ 1);
       }
@@ -208,11 +210,16 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
       } else {
         if constexpr (F == 0) read_x(b ^ 1, 0);
         read_w(b ^ 1, F);
-        if constexpr (C::TR == NFW) {
-          fetch_w(F);
-          fetch_x(F);
-        }
+        fetch_x(F);
         if constexpr (F == NFW - 1) fetch_s();
+      }
+      if constexpr (J == MID) {
+        if constexpr (F == 0) {
+          // every wave has this stage's columns in registers
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        fetch_w(F);
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (T >= SKEW) add(template_int<T - SKEW>{});
