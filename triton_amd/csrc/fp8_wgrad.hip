@@ -18,6 +18,7 @@ struct WgradParams {
   uint8_t* y;
   int64_t y_e, y_k;
   int32_t tiles_k, tiles_n;
+  int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
 };
 
 // an e4m3 times its scale in dy's type (in fp16 at most its largest number)
@@ -82,6 +83,236 @@ __global__ __launch_bounds__(256) void fp8_wgrad_any_kernel(const WgradParams p)
   }
 }
 
+// ---- lines that begin at sixteen-byte boundaries -------------------------------------------------------------------------------------------------------
+//
+//   * A workgroup multiplies a T x T tile of a slice: 256 with eight waves of 128 x 64 (one per CU), or 128 with four waves of 64 x 64 (two per CU).  A stage is
+//     32 rows; two are in LDS, in the operands' own order, and are turned by the reads (read_frag_tr).
+//   * Both operands come through registers, asked for two stages ahead: that is where x is scaled and becomes dy's type, sixteen elements a thread and stage,
+//     once for all waves.  (A transfer straight into LDS would have x converted on its way out of it, by each of the waves that share it, row scales and all.)
+//   * One barrier a stage, between its two steps of sixteen rows: in front of it the next stage is written into the buffer that the last one has been read from.
+//   * Workgroups are persistent and the stream of stages runs on across tiles.  Every XCD takes an eighth of each slice's tiles, from the longest slice to the
+//     shortest (up to 64 of them), and its workgroups walk their list forth and back.
+
+constexpr int kStage = 32;
+template <int T>
+struct WgradCfg {
+  static constexpr int WM = 2, WN = T / 64, NW = WM * WN;
+  static constexpr int MF = T / WM / 32, NF = 2;  // fragments of a wave
+  static constexpr int PITCH = T * 2, OPERAND = kStage * PITCH, STAGE = 2 * OPERAND, LDS = 2 * STAGE;
+  static constexpr int THREADS = NW * 64;
+  static constexpr int PER_CU = T == 256 ? 1 : 2;
+  static constexpr int XP = kStage * T / 16 / THREADS, DP = kStage * T / 8 / THREADS;  // pieces of sixteen bytes a thread: x, dy
+};
+
+template <int DT, int YT, int T>
+__global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(const WgradParams p) {
+  typedef WgradCfg<T> C;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 31, h = lane >> 5;
+  const int mw = wave & 1, nw = wave >> 1;
+  const uint32_t lds0 = lds_addr(lds);
+
+  // ---- the slices, longest first (lane l: that of rank l), and this workgroup's tiles ----------------------------------------------------------------
+  const bool sorted = p.slice_sizes && p.n_slices <= 64;
+  int sz = 0, so = 0, id = lane;
+  if (sorted) {
+    const int mine = lane < p.n_slices ? p.slice_sizes[lane] : -1, first = lane < p.n_slices ? p.slice_offs[lane] : 0;
+    int rank = 0;
+    for (int o = 0; o < p.n_slices; ++o) {
+      const int other = __builtin_amdgcn_readlane(mine, o);
+      rank += other > mine || (other == mine && o < lane) ? 1 : 0;
+    }
+    // (a lane's rank is a place of its own; lanes without a slice keep theirs)
+    rank = lane < p.n_slices ? rank : lane;
+    sz = __builtin_amdgcn_ds_permute(rank * 4, mine);
+    so = __builtin_amdgcn_ds_permute(rank * 4, first);
+    id = __builtin_amdgcn_ds_permute(rank * 4, lane);
+  }
+  const uint32_t per_e = (uint32_t)(p.tiles_k * p.tiles_n), q = (per_e + 7) / 8, total = q * (uint32_t)p.n_slices;
+  const uint32_t xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3, wgs = gridDim.x >> 3, rounds = (total + wgs - 1) / wgs;
+  struct Where {
+    int id, rows, first, k0, n0;
+  };
+  auto next = [&](uint32_t& r, Where& w) __attribute__((always_inline)) -> bool {
+    for (; r < rounds; ++r) {
+      const uint32_t l = r * wgs + (r & 1 ? wgs - 1 - i8 : i8), rank = l / q, in = xcd * q + (l - rank * q);
+      if (l >= total || in >= per_e) continue;
+      // (bands of eight tiles down, in a band column by column, so that those in hand on an XCD share few operand columns)
+      const uint32_t band = in / (8u * (uint32_t)p.tiles_n), left = (uint32_t)p.tiles_k - band * 8u, bh = left < 8u ? left : 8u;
+      const uint32_t in_b = in - band * 8u * (uint32_t)p.tiles_n, tn = in_b / bh, tk = band * 8u + in_b - tn * bh;
+      if (sorted) {
+        w.id = __builtin_amdgcn_readlane(id, (int)rank), w.rows = __builtin_amdgcn_readlane(sz, (int)rank), w.first = __builtin_amdgcn_readlane(so, (int)rank);
+      } else {
+        w.id = (int)rank, w.rows = p.slice_sizes ? p.slice_sizes[rank] : p.T, w.first = p.slice_sizes ? p.slice_offs[rank] : 0;
+      }
+      w.k0 = (int)tk * T, w.n0 = (int)tn * T;
+      return true;
+    }
+    return false;
+  };
+  uint32_t cur_r = 0;
+  Where cur;
+  if (!next(cur_r, cur)) return;
+
+  // ---- loads: the next stage to ask for ------------------------------------------------------------------------------------------------------------------
+  uint32_t f_r = cur_r;
+  Where aim = cur;
+  int f_t = 0;       // its first row within the slice
+  bool more = true;
+  constexpr int XL = T / 16, DL = T / 8;  // threads of a row
+  struct Loads {
+    u32x4_t x[C::XP], d[C::DP];
+    float s[C::XP];
+  };
+  auto load = [&](Loads& l) __attribute__((always_inline)) {
+    const u32x4_t none = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < C::XP; ++i) {
+      const int row = tid / XL + i * (C::THREADS / XL), k = aim.k0 + tid % XL * 16;
+      const bool in = more && f_t + row < aim.rows && k < p.K;
+      const int64_t t = in ? (int64_t)aim.first + f_t + row : 0;
+      l.x[i] = in ? *reinterpret_cast<const u32x4_t*>(p.x + t * p.x_t + k) : none;
+      l.s[i] = in ? p.xs[t * p.xs_t + (int64_t)(k / kFp8Block) * p.xs_k] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < C::DP; ++i) {
+      const int row = tid / DL + i * (C::THREADS / DL), n = aim.n0 + tid % DL * 8;
+      const bool in = more && f_t + row < aim.rows && n < p.N;
+      const int64_t t = in ? (int64_t)aim.first + f_t + row : 0;
+      l.d[i] = in ? *reinterpret_cast<const u32x4_t*>(p.dy + t * p.dy_t + n) : none;
+    }
+    f_t += kStage;
+    if (f_t >= aim.rows && more) {
+      f_t = 0, ++f_r;
+      more = next(f_r, aim);
+    }
+  };
+  auto store = [&](const Loads& l, uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < C::XP; ++i) {
+      const int row = tid / XL + i * (C::THREADS / XL), piece = (tid % XL * 2) ^ ((row & 3) * 4);
+      u32x4_t o[2];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[4];
+        from_e4m3(l.x[i][c], v);
+        o[c >> 1][(c & 1) * 2] = scaled_pair<DT>(v[0], v[1], l.s[i]);
+        o[c >> 1][(c & 1) * 2 + 1] = scaled_pair<DT>(v[2], v[3], l.s[i]);
+      }
+      u32x4_t* to = reinterpret_cast<u32x4_t*>(lds + buf + row * C::PITCH + piece * 16);
+      to[0] = o[0], to[1] = o[1];
+    }
+#pragma unroll
+    for (int i = 0; i < C::DP; ++i) {
+      const int row = tid / DL + i * (C::THREADS / DL), piece = (tid % DL) ^ ((row & 3) * 4);
+      *reinterpret_cast<u32x4_t*>(lds + buf + C::OPERAND + row * C::PITCH + piece * 16) = l.d[i];
+    }
+  };
+
+  // ---- fragment reads: a lane's row of four, four columns; columns 32 j on are pieces 4 j on ----------------------------------------------------------------
+  const int l16 = lane & 15, pp = ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1);
+  const uint32_t rd0 = lds0 + (uint32_t)((h * 8 + (l16 >> 2)) * C::PITCH + (l16 & 1) * 8);
+  uint32_t at_a[C::MF], at_b[C::NF];
+#pragma unroll
+  for (int j = 0; j < C::MF; ++j) at_a[j] = rd0 + (uint32_t)(((mw * C::MF * 4 + j * 4 + pp) ^ ((l16 >> 2) * 4)) * 16);
+#pragma unroll
+  for (int f = 0; f < C::NF; ++f) at_b[f] = rd0 + C::OPERAND + (uint32_t)(((nw * C::NF * 4 + f * 4 + pp) ^ ((l16 >> 2) * 4)) * 16);
+  u32x4_t af[2][C::MF], bf[2][C::NF];
+  f32x16_t acc[C::NF][C::MF];
+  // step P of a stage: its products, while the operands of the next step (step 1 of the same stage, step 0 of the next) are read from `buf`
+  auto step = [&](auto p_c, uint32_t buf) __attribute__((always_inline)) {
+    constexpr int P = decltype(p_c)::value;
+#pragma unroll
+    for (int f = 0; f < C::NF; ++f) bf[1 - P][f] = read_frag_tr(at_b[f] + (uint32_t)((1 - P) * 16 * C::PITCH) + buf, C::PITCH);
+#pragma unroll
+    for (int j = 0; j < C::MF; ++j) {
+      af[1 - P][j] = read_frag_tr(at_a[j] + (uint32_t)((1 - P) * 16 * C::PITCH) + buf, C::PITCH);
+#pragma unroll
+      for (int f = 0; f < C::NF; ++f) {
+        acc[f][j] = mfma_k16<DT>(bf[P][f], af[P][j], acc[f][j]);
+        asm volatile("" : "+v"(acc[f][j]));  // (an empty use: the products stay where they are written)
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < C::NF; ++f)
+#pragma unroll
+      for (int j = 0; j < C::MF; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[f][j][i] = 0.f;
+  };
+  auto write = [&](const Where& w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < C::MF; ++j) {
+      const int k = w.k0 + (mw * C::MF + j) * 32 + lr;
+#pragma unroll
+      for (int f = 0; f < C::NF; ++f)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const auto s = __builtin_amdgcn_permlane32_swap(f32_bits(acc[f][j][8 * u + i]), f32_bits(acc[f][j][8 * u + 4 + i]), false, false);
+            v[i] = bits_f32(s[0]), v[4 + i] = bits_f32(s[1]);
+          }
+          const int n = w.n0 + (nw * C::NF + f) * 32 + 16 * u + 8 * h;
+          if (k >= p.K || n >= p.N) continue;
+          const int64_t to = w.id * p.y_e + k * p.y_k + n;
+          if (p.y_vec && n + 8 <= p.N) {
+            store_vec<YT, 8>(p.y, to, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i < p.N) store_elem<YT>(p.y, to + i, v[i]);
+          }
+        }
+    }
+  };
+
+  Loads l0, l1;
+  load(l0);
+  store(l0, 0);
+  load(l0);
+  load(l1);
+  barrier();
+#pragma unroll
+  for (int f = 0; f < C::NF; ++f) bf[0][f] = read_frag_tr(at_b[f], C::PITCH);
+#pragma unroll
+  for (int j = 0; j < C::MF; ++j) af[0][j] = read_frag_tr(at_a[j], C::PITCH);
+  clear();
+  int t = 0;
+  // a stage in buffer `buf`; `l` holds the next one, and then the one two further on
+  auto stage = [&](Loads& l, uint32_t buf) __attribute__((always_inline)) -> bool {
+    step(template_int<0>{}, buf);
+    store(l, buf ^ C::STAGE);
+    load(l);
+    barrier();
+    step(template_int<1>{}, buf ^ C::STAGE);
+    t += kStage;
+    if (t >= cur.rows) {
+      write(cur);
+      clear();
+      t = 0, ++cur_r;
+      return next(cur_r, cur);
+    }
+    return true;
+  };
+#pragma unroll 1
+  for (;;) {
+    if (!stage(l0, 0)) break;
+    if (!stage(l1, C::STAGE)) break;
+  }
+}
+
 int32_t launch_any(WgradParams p, int dt, int yt, hipStream_t st) {
   p.tiles_k = (int)cdiv(p.K, 64), p.tiles_n = (int)cdiv(p.N, 64);
   const int64_t grid = (int64_t)p.tiles_k * p.tiles_n * p.n_slices;
@@ -92,6 +323,24 @@ int32_t launch_any(WgradParams p, int dt, int yt, hipStream_t st) {
   else
     yt == TK_F32 ? launch(fp8_wgrad_any_kernel<TK_F16, TK_F32>) : yt == TK_BF16 ? launch(fp8_wgrad_any_kernel<TK_F16, TK_BF16>) : launch(fp8_wgrad_any_kernel<TK_F16, TK_F16>);
   return check_launch("fp8_wgrad_any_kernel");
+}
+
+template <int T>
+int32_t launch_tiles(WgradParams p, int dt, int yt, hipStream_t st) {
+  typedef WgradCfg<T> C;
+  p.tiles_k = (int)cdiv(p.K, T), p.tiles_n = (int)cdiv(p.N, T);
+  const int64_t lists = cdiv((int64_t)p.tiles_k * p.tiles_n, 8) * p.n_slices;  // tiles of an XCD
+  if (lists * 8 > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: grid too large");
+  const int64_t most = (int64_t)device_cu_count() * C::PER_CU / 8;
+  const unsigned grid = (unsigned)((lists < most ? lists : most) * 8);
+  auto launch = [&](auto kern) -> int32_t {
+    if (const int32_t rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), C::LDS)) return rc;
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(C::THREADS), C::LDS, st, p);
+    return check_launch("fp8_wgrad_kernel");
+  };
+  if (dt == TK_BF16)
+    return yt == TK_F32 ? launch(fp8_wgrad_kernel<TK_BF16, TK_F32, T>) : yt == TK_BF16 ? launch(fp8_wgrad_kernel<TK_BF16, TK_BF16, T>) : launch(fp8_wgrad_kernel<TK_BF16, TK_F16, T>);
+  return yt == TK_F32 ? launch(fp8_wgrad_kernel<TK_F16, TK_F32, T>) : yt == TK_BF16 ? launch(fp8_wgrad_kernel<TK_F16, TK_BF16, T>) : launch(fp8_wgrad_kernel<TK_F16, TK_F16, T>);
 }
 
 }  // namespace
@@ -113,5 +362,13 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
   p.slice_sizes = d->slice_sizes, p.slice_offs = d->slice_offs, p.n_slices = d->n_slices;
   p.T = d->T, p.K = d->K, p.N = d->N;
   p.y = static_cast<uint8_t*>(d->y), p.y_e = d->y_stride_e, p.y_k = d->y_stride_k;
-  return launch_any(p, d->dy_dtype, d->y_dtype, static_cast<hipStream_t>(stream));
+  const int ys = d->y_dtype == TK_F32 ? 4 : 2;
+  p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && p.y_e * ys % 16 == 0 && p.y_k * ys % 16 == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's)
+  if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0) {
+    const int64_t tiles = cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices;
+    return tiles >= 2 * device_cu_count() ? launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st) : launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
+  }
+  return launch_any(p, d->dy_dtype, d->y_dtype, st);
 }
