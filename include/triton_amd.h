@@ -708,6 +708,7 @@ typedef struct tk_fp8_wgrad_desc {
   void* y; /* [n_slices, K, N] */
   int32_t y_dtype; /* TK_F32, TK_BF16, TK_F16 */
   int64_t y_stride_e, y_stride_k;
+  int32_t pow2_scales; /* as in tk_fp8_gemm_desc */
 } tk_fp8_wgrad_desc;
 int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* desc, tk_stream_t stream);
 

@@ -125,7 +125,7 @@ class Fp8WgradDesc(_c.Structure):
     _fields_ = [
         ("x", _ptr), ("x_stride_t", _i64), ("x_scale", _ptr), ("xs_stride_t", _i64), ("xs_stride_k", _i64), ("dy", _ptr), ("dy_dtype", _i32),
         ("dy_stride_t", _i64), ("slice_sizes", _ptr), ("slice_offs", _ptr), ("n_slices", _i32), ("T", _i32), ("K", _i32), ("N", _i32),
-        ("y", _ptr), ("y_dtype", _i32), ("y_stride_e", _i64), ("y_stride_k", _i64),
+        ("y", _ptr), ("y_dtype", _i32), ("y_stride_e", _i64), ("y_stride_k", _i64), ("pow2_scales", _i32),
     ]
 
 

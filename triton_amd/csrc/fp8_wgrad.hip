@@ -18,6 +18,7 @@ struct WgradParams {
   uint8_t* y;
   int64_t y_e, y_k;
   int32_t tiles_k, tiles_n;
+  int32_t pow2;
   int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
 };
 
@@ -104,21 +105,22 @@ struct WgradCfg {
   static constexpr int XP = kStage * T / 16 / THREADS, DP = kStage * T / 8 / THREADS;  // pieces of sixteen bytes a thread: x, dy
 };
 
-template <int DT, int YT, int T>
+// POW2: bf16, and all scales powers of two: the conversion multiplies by the exponent.
+template <int DT, int YT, int T, bool POW2>
 __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(const WgradParams p) {
   typedef WgradCfg<T> C;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 31, h = lane >> 5;
-  const int mw = wave & 1, nw = wave >> 1;
+  const int h = lane >> 5, mw = wave & 1, nw = wave >> 1;
   const uint32_t lds0 = lds_addr(lds);
 
   // ---- the slices, longest first (lane l: that of rank l), and this workgroup's tiles ----------------------------------------------------------------
-  const bool sorted = p.slice_sizes && p.n_slices <= 64;
+  const bool sorted = p.n_slices <= 64;
   int sz = 0, so = 0, id = lane;
   if (sorted) {
-    const int mine = lane < p.n_slices ? p.slice_sizes[lane] : -1, first = lane < p.n_slices ? p.slice_offs[lane] : 0;
+    int mine = lane < p.n_slices ? p.T : -1, first = 0;  // (no slices: one of T rows)
+    if (p.slice_sizes && lane < p.n_slices) mine = p.slice_sizes[lane], first = p.slice_offs[lane];
     int rank = 0;
     for (int o = 0; o < p.n_slices; ++o) {
       const int other = __builtin_amdgcn_readlane(mine, o);
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
   };
   auto next = [&](uint32_t& r, Where& w) __attribute__((always_inline)) -> bool {
     for (; r < rounds; ++r) {
-      const uint32_t l = r * wgs + (r & 1 ? wgs - 1 - i8 : i8), rank = l / q, in = xcd * q + (l - rank * q);
+      const uint32_t l = r * wgs + (r & 1 ? wgs - 1 - i8 : i8), rank = (uint32_t)__builtin_amdgcn_readfirstlane((int)(l / q)), in = xcd * q + (l - rank * q);
       if (l >= total || in >= per_e) continue;
       // (bands of eight tiles down, in a band column by column, so that those in hand on an XCD share few operand columns)
       const uint32_t band = in / (8u * (uint32_t)p.tiles_n), left = (uint32_t)p.tiles_k - band * 8u, bh = left < 8u ? left : 8u;
@@ -145,9 +147,15 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
       if (sorted) {
         w.id = __builtin_amdgcn_readlane(id, (int)rank), w.rows = __builtin_amdgcn_readlane(sz, (int)rank), w.first = __builtin_amdgcn_readlane(so, (int)rank);
       } else {
-        w.id = (int)rank, w.rows = p.slice_sizes ? p.slice_sizes[rank] : p.T, w.first = p.slice_sizes ? p.slice_offs[rank] : 0;
+        // (scalar loads: the wait for a vector one would be a wait for the stages in flight)
+        typedef const __attribute__((address_space(4))) int32_t* scalar_t;
+        w.id = (int)rank, w.rows = reinterpret_cast<scalar_t>(reinterpret_cast<uintptr_t>(p.slice_sizes))[rank];
+        w.first = reinterpret_cast<scalar_t>(reinterpret_cast<uintptr_t>(p.slice_offs))[rank];
       }
-      w.k0 = (int)tk * T, w.n0 = (int)tn * T;
+      // (all of it is the same in every lane, which the compiler loses sight of)
+      w.id = __builtin_amdgcn_readfirstlane(w.id), w.rows = __builtin_amdgcn_readfirstlane(w.rows), w.first = __builtin_amdgcn_readfirstlane(w.first);
+      w.k0 = __builtin_amdgcn_readfirstlane((int)tk * T), w.n0 = __builtin_amdgcn_readfirstlane((int)tn * T);
+      r = (uint32_t)__builtin_amdgcn_readfirstlane((int)r);
       return true;
     }
     return false;
@@ -159,54 +167,78 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
   // ---- loads: the next stage to ask for ------------------------------------------------------------------------------------------------------------------
   uint32_t f_r = cur_r;
   Where aim = cur;
-  int f_t = 0;       // its first row within the slice
-  bool more = true;
   constexpr int XL = T / 16, DL = T / 8;  // threads of a row
+  constexpr int XR = C::THREADS / XL, DR = C::THREADS / DL;  // rows of a piece of all threads
   struct Loads {
     u32x4_t x[C::XP], d[C::DP];
     float s[C::XP];
   };
+  // A stage's resources begin at its first row, and end with the slice's last one: rows behind it read zeros, and no scale.  Columns behind K or N read what follows,
+  // or zeros, and end in rows and columns that are not there.
+  const uint32_t x_at = (uint32_t)(tid / XL) * (uint32_t)p.x_t + tid % XL * 16u, d_at = ((uint32_t)(tid / DL) * (uint32_t)p.dy_t + tid % DL * 8u) * 2u;
+  const uint32_t s_at = ((uint32_t)(tid / XL) * (uint32_t)p.xs_t + (uint32_t)(tid % XL * 16 / kFp8Block) * (uint32_t)p.xs_k) * 4u;
+  const bool s_in = tid % XL * 16 / kFp8Block == 0;  // (of a tile that ends within its first block of K the second has no scales)
+  const uint8_t* xb;
+  const uint16_t* db;
+  const float* sb;
+  int left;  // rows of the slice from the next stage on
+  int x_end, d_end;
+  bool second;
+  auto start = [&]() __attribute__((always_inline)) {
+    const int64_t t = aim.first;
+    xb = p.x + t * p.x_t + aim.k0, db = p.dy + t * p.dy_t + aim.n0, sb = p.xs + t * p.xs_t + (int64_t)(aim.k0 / kFp8Block) * p.xs_k;
+    left = aim.rows;
+    x_end = ((p.K + 15) & ~15) - aim.k0, d_end = (((p.N + 7) & ~7) - aim.n0) * 2;
+    second = aim.k0 + kFp8Block < p.K;
+  };
+  start();
   auto load = [&](Loads& l) __attribute__((always_inline)) {
-    const u32x4_t none = {0, 0, 0, 0};
+    const int rows = left < kStage ? left : kStage;
+    const int x_bytes = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)p.x_t + x_end : 0);
+    const int d_bytes = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)p.dy_t * 2 + d_end : 0);
+    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(xb), 0, x_bytes, 0x00020000);
+    const auto dr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(db), 0, d_bytes, 0x00020000);
+    const auto sr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(sb), 0, 0x7FFFFFFF, 0x00020000);
 #pragma unroll
     for (int i = 0; i < C::XP; ++i) {
-      const int row = tid / XL + i * (C::THREADS / XL), k = aim.k0 + tid % XL * 16;
-      const bool in = more && f_t + row < aim.rows && k < p.K;
-      const int64_t t = in ? (int64_t)aim.first + f_t + row : 0;
-      l.x[i] = in ? *reinterpret_cast<const u32x4_t*>(p.x + t * p.x_t + k) : none;
-      l.s[i] = in ? p.xs[t * p.xs_t + (int64_t)(k / kFp8Block) * p.xs_k] : 0.f;
+      l.x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_at + (uint32_t)(i * XR) * (uint32_t)p.x_t, 0, 0);
+      const bool in = tid / XL + i * XR < rows && (second || s_in);
+      l.s[i] = bits_f32(__builtin_amdgcn_raw_buffer_load_b32(sr, in ? s_at + (uint32_t)(i * XR) * (uint32_t)p.xs_t * 4u : 0x80000000u, 0, 0));
     }
 #pragma unroll
-    for (int i = 0; i < C::DP; ++i) {
-      const int row = tid / DL + i * (C::THREADS / DL), n = aim.n0 + tid % DL * 8;
-      const bool in = more && f_t + row < aim.rows && n < p.N;
-      const int64_t t = in ? (int64_t)aim.first + f_t + row : 0;
-      l.d[i] = in ? *reinterpret_cast<const u32x4_t*>(p.dy + t * p.dy_t + n) : none;
-    }
-    f_t += kStage;
-    if (f_t >= aim.rows && more) {
-      f_t = 0, ++f_r;
-      more = next(f_r, aim);
+    for (int i = 0; i < C::DP; ++i) l.d[i] = __builtin_amdgcn_raw_buffer_load_b128(dr, d_at + (uint32_t)(i * DR) * (uint32_t)p.dy_t * 2u, 0, 0);
+    left -= kStage;
+    if (left > 0) {
+      xb += kStage * p.x_t, db += kStage * p.dy_t, sb += kStage * p.xs_t;
+    } else if (f_r < rounds) {
+      ++f_r;
+      if (next(f_r, aim)) start();
     }
   };
   auto store = [&](const Loads& l, uint32_t buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < C::XP; ++i) {
-      const int row = tid / XL + i * (C::THREADS / XL), piece = (tid % XL * 2) ^ ((row & 3) * 4);
+      const int row = tid / XL + i * XR, piece = (tid % XL * 2) ^ ((row & 3) * 4);
+      const float s = l.s[i];
       u32x4_t o[2];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float v[4];
-        from_e4m3(l.x[i][c], v);
-        o[c >> 1][(c & 1) * 2] = scaled_pair<DT>(v[0], v[1], l.s[i]);
-        o[c >> 1][(c & 1) * 2 + 1] = scaled_pair<DT>(v[2], v[3], l.s[i]);
+        if constexpr (POW2) {
+          o[c >> 1][(c & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l.x[i][c], s, false));
+          o[c >> 1][(c & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l.x[i][c], s, true));
+        } else {
+          float v[4];
+          from_e4m3(l.x[i][c], v);
+          o[c >> 1][(c & 1) * 2] = scaled_pair<DT>(v[0], v[1], s);
+          o[c >> 1][(c & 1) * 2 + 1] = scaled_pair<DT>(v[2], v[3], s);
+        }
       }
       u32x4_t* to = reinterpret_cast<u32x4_t*>(lds + buf + row * C::PITCH + piece * 16);
       to[0] = o[0], to[1] = o[1];
     }
 #pragma unroll
     for (int i = 0; i < C::DP; ++i) {
-      const int row = tid / DL + i * (C::THREADS / DL), piece = (tid % DL) ^ ((row & 3) * 4);
+      const int row = tid / DL + i * DR, piece = (tid % DL) ^ ((row & 3) * 4);
       *reinterpret_cast<u32x4_t*>(lds + buf + C::OPERAND + row * C::PITCH + piece * 16) = l.d[i];
     }
   };
@@ -251,6 +283,9 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
         for (int i = 0; i < 16; ++i) acc[f][j][i] = 0.f;
   };
   auto write = [&](const Where& w) __attribute__((always_inline)) {
+    int l = tid & 63;
+    asm volatile("" : "+v"(l));  // (so that nothing of what follows is worked out before the loop and kept in registers)
+    const int lr = l & 31, h = l >> 5;
 #pragma unroll
     for (int j = 0; j < C::MF; ++j) {
       const int k = w.k0 + (mw * C::MF + j) * 32 + lr;
@@ -338,9 +373,13 @@ int32_t launch_tiles(WgradParams p, int dt, int yt, hipStream_t st) {
     hipLaunchKernelGGL(kern, dim3(grid), dim3(C::THREADS), C::LDS, st, p);
     return check_launch("fp8_wgrad_kernel");
   };
-  if (dt == TK_BF16)
-    return yt == TK_F32 ? launch(fp8_wgrad_kernel<TK_BF16, TK_F32, T>) : yt == TK_BF16 ? launch(fp8_wgrad_kernel<TK_BF16, TK_BF16, T>) : launch(fp8_wgrad_kernel<TK_BF16, TK_F16, T>);
-  return yt == TK_F32 ? launch(fp8_wgrad_kernel<TK_F16, TK_F32, T>) : yt == TK_BF16 ? launch(fp8_wgrad_kernel<TK_F16, TK_BF16, T>) : launch(fp8_wgrad_kernel<TK_F16, TK_F16, T>);
+  auto by_out = [&](auto dt_c, auto pow2_c) -> int32_t {
+    constexpr int DT = decltype(dt_c)::value;
+    constexpr bool POW2 = decltype(pow2_c)::value;
+    return yt == TK_F32 ? launch(fp8_wgrad_kernel<DT, TK_F32, T, POW2>) : yt == TK_BF16 ? launch(fp8_wgrad_kernel<DT, TK_BF16, T, POW2>) : launch(fp8_wgrad_kernel<DT, TK_F16, T, POW2>);
+  };
+  if (dt == TK_F16) return by_out(template_int<TK_F16>{}, std::false_type{});
+  return p.pow2 ? by_out(template_int<TK_BF16>{}, std::true_type{}) : by_out(template_int<TK_BF16>{}, std::false_type{});
 }
 
 }  // namespace
@@ -365,8 +404,12 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
   const int ys = d->y_dtype == TK_F32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && p.y_e * ys % 16 == 0 && p.y_k * ys % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's)
-  if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0) {
+  p.pow2 = d->pow2_scales;
+  // Lines that begin at sixteen-byte boundaries and do not overlap (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's), and offsets
+  // within a stage of 32 rows that fit a buffer resource.
+  const int64_t limit = (int64_t)1 << 31;
+  if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0 && p.x_t >= p.K && p.dy_t >= p.N &&
+      p.xs_t >= 0 && p.xs_k >= 0 && 32 * p.x_t < limit && 64 * p.dy_t < limit && (32 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
     const int64_t tiles = cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices;
     return tiles >= 2 * device_cu_count() ? launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st) : launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
   }

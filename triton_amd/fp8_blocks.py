@@ -311,6 +311,11 @@ def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch
         if getattr(md, "remapped_from", None) is not None:
             raise NotImplementedError("weight gradients need the metadata of all slices")
         _check_metadata(md, md.n_slices, x.device)
+    return _weight_gradient(x, x_scale, dy, md, out_dtype, False)
+
+
+def _weight_gradient(x, x_scale, dy, md, out_dtype, pow2):
+    """One launch; operands as checked by the callers.  `pow2`: the scales are the quantiser's."""
     dy = dy if dy.stride(1) == 1 or dy.shape[1] <= 1 else dy.contiguous()
     (T, K), N, E = x.shape, dy.shape[1], 1 if md is None else md.n_slices
     y = torch.empty((E, K, N), dtype=out_dtype, device=x.device)
@@ -321,6 +326,7 @@ def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch
         d.slice_sizes, d.slice_offs = md.slice_sizes.data_ptr(), md.slice_offs.data_ptr()
     d.n_slices, d.T, d.K, d.N = E, T, K, N
     d.y, d.y_dtype, d.y_stride_e, d.y_stride_k = y.data_ptr(), nt.TORCH_TO_TK[out_dtype], y.stride(0), y.stride(1)
+    d.pow2_scales = int(pow2)
     nt.submit(nt.lib().tk_fp8_block_wgrad, d, x.device)
     return y if md is not None else y[0]
 
@@ -360,13 +366,14 @@ class _LinearFp8(torch.autograd.Function):
     def backward(ctx, dy):
         names = ("x8", "x_scale", "w8", "w_scale")
         x8, xs, values_n, scales = (_check_saved(*v) for v in zip(ctx.saved_tensors, ctx.like, names))
+        x8 = x8 if x8.stride(1) == 1 or x8.shape[1] <= 1 else x8.contiguous()
         values_n = values_n if values_n.stride(2) == 1 or values_n.shape[2] <= 1 else values_n.contiguous()
         dx = dw = None
         if ctx.needs_input_grad[0]:
             d8, ds = _quantize_rows(dy)
             dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True)
         if ctx.needs_input_grad[1]:
-            dw = weight_gradient_fp8_blocks(x8, xs, dy.detach(), ctx.md, ctx.w_dtype).view(ctx.w_shape)
+            dw = _weight_gradient(x8, xs, dy, ctx.md, ctx.w_dtype, True).view(ctx.w_shape)
         return dx, dw, None, None, None, None
 
 
