@@ -87,14 +87,15 @@ __global__ __launch_bounds__(256) void fp8_wgrad_any_kernel(const WgradParams p)
 // ---- lines that begin at sixteen-byte boundaries -------------------------------------------------------------------------------------------------------
 //
 //   * A workgroup multiplies a T x T tile of a slice: 256 with eight waves of 128 x 64 (one per CU), or 128 with four waves of 64 x 64 (two per CU).  A stage is
-//     32 rows; two are in LDS, in the operands' own order, and are turned by the reads (read_frag_tr).
-//   * Both operands come through registers, asked for two stages ahead: that is where x is scaled and becomes dy's type, sixteen elements a thread and stage,
-//     once for all waves.  (A transfer straight into LDS would have x converted on its way out of it, by each of the waves that share it, row scales and all.)
-//   * One barrier a stage, between its two steps of sixteen rows: in front of it the next stage is written into the buffer that the last one has been read from.
+//     64 rows; two are in LDS, in the operands' own order, and are turned by the reads (read_frag_tr).
+//   * Both operands come through registers, asked for a stage and more ahead: that is where x is scaled and becomes dy's type, once for all waves.  (A transfer straight
+//     into LDS would have x converted on its way out of it, by each of the waves that share it, row scales and all.)
+//   * One barrier a stage, in front of the last of its four steps of sixteen rows: until there the next stage is written into the buffer that the last one has
+//     been read from, piece by piece beside the products of the other three steps, and the one behind it asked for.
 //   * Workgroups are persistent and the stream of stages runs on across tiles.  Every XCD takes an eighth of each slice's tiles, from the longest slice to the
 //     shortest (up to 64 of them), and its workgroups walk their list forth and back.
 
-constexpr int kStage = 32;
+constexpr int kStage = 64;
 template <int T>
 struct WgradCfg {
   static constexpr int WM = 2, WN = T / 64, NW = WM * WN;
@@ -169,10 +170,9 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
   Where aim = cur;
   constexpr int XL = T / 16, DL = T / 8;  // threads of a row
   constexpr int XR = C::THREADS / XL, DR = C::THREADS / DL;  // rows of a piece of all threads
-  struct Loads {
-    u32x4_t x[C::XP], d[C::DP];
-    float s[C::XP];
-  };
+  // what a thread holds of the stage to be written next: the pieces of x with their scales, and those of dy
+  u32x4_t lx[C::XP], ld[C::DP];
+  float ls[C::XP];
   // A stage's resources begin at its first row, and end with the slice's last one: rows behind it read zeros, and no scale.  Columns behind K or N read what follows,
   // or zeros, and end in rows and columns that are not there.
   const uint32_t x_at = (uint32_t)(tid / XL) * (uint32_t)p.x_t + tid % XL * 16u, d_at = ((uint32_t)(tid / DL) * (uint32_t)p.dy_t + tid % DL * 8u) * 2u;
@@ -192,21 +192,24 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
     second = aim.k0 + kFp8Block < p.K;
   };
   start();
-  auto load = [&](Loads& l) __attribute__((always_inline)) {
-    const int rows = left < kStage ? left : kStage;
+  typedef decltype(__builtin_amdgcn_make_buffer_rsrc((void*)nullptr, 0, 0, 0)) resource_t;
+  resource_t xr, dr, sr;
+  int rows;
+  auto resources = [&]() __attribute__((always_inline)) {  // of the stage to ask for
+    rows = left < kStage ? left : kStage;
     const int x_bytes = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)p.x_t + x_end : 0);
     const int d_bytes = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)p.dy_t * 2 + d_end : 0);
-    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(xb), 0, x_bytes, 0x00020000);
-    const auto dr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(db), 0, d_bytes, 0x00020000);
-    const auto sr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(sb), 0, 0x7FFFFFFF, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < C::XP; ++i) {
-      l.x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_at + (uint32_t)(i * XR) * (uint32_t)p.x_t, 0, 0);
-      const bool in = tid / XL + i * XR < rows && (second || s_in);
-      l.s[i] = bits_f32(__builtin_amdgcn_raw_buffer_load_b32(sr, in ? s_at + (uint32_t)(i * XR) * (uint32_t)p.xs_t * 4u : 0x80000000u, 0, 0));
-    }
-#pragma unroll
-    for (int i = 0; i < C::DP; ++i) l.d[i] = __builtin_amdgcn_raw_buffer_load_b128(dr, d_at + (uint32_t)(i * DR) * (uint32_t)p.dy_t * 2u, 0, 0);
+    xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(xb), 0, x_bytes, 0x00020000);
+    dr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(db), 0, d_bytes, 0x00020000);
+    sr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(sb), 0, 0x7FFFFFFF, 0x00020000);
+  };
+  auto load_x = [&](int i) __attribute__((always_inline)) {
+    lx[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_at + (uint32_t)(i * XR) * (uint32_t)p.x_t, 0, 0);
+    const bool in = tid / XL + i * XR < rows && (second || s_in);
+    ls[i] = bits_f32(__builtin_amdgcn_raw_buffer_load_b32(sr, in ? s_at + (uint32_t)(i * XR) * (uint32_t)p.xs_t * 4u : 0x80000000u, 0, 0));
+  };
+  auto load_d = [&](int i) __attribute__((always_inline)) { ld[i] = __builtin_amdgcn_raw_buffer_load_b128(dr, d_at + (uint32_t)(i * DR) * (uint32_t)p.dy_t * 2u, 0, 0); };
+  auto advance = [&]() __attribute__((always_inline)) {
     left -= kStage;
     if (left > 0) {
       xb += kStage * p.x_t, db += kStage * p.dy_t, sb += kStage * p.xs_t;
@@ -215,32 +218,35 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
       if (next(f_r, aim)) start();
     }
   };
-  auto store = [&](const Loads& l, uint32_t buf) __attribute__((always_inline)) {
+  auto store_x = [&](int i, uint32_t buf) __attribute__((always_inline)) {
+    const int row = tid / XL + i * XR, piece = (tid % XL * 2) ^ ((row & 3) * 4);
+    const float s = ls[i];
+    u32x4_t o[2];
 #pragma unroll
-    for (int i = 0; i < C::XP; ++i) {
-      const int row = tid / XL + i * XR, piece = (tid % XL * 2) ^ ((row & 3) * 4);
-      const float s = l.s[i];
-      u32x4_t o[2];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (POW2) {
-          o[c >> 1][(c & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l.x[i][c], s, false));
-          o[c >> 1][(c & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l.x[i][c], s, true));
-        } else {
-          float v[4];
-          from_e4m3(l.x[i][c], v);
-          o[c >> 1][(c & 1) * 2] = scaled_pair<DT>(v[0], v[1], s);
-          o[c >> 1][(c & 1) * 2 + 1] = scaled_pair<DT>(v[2], v[3], s);
-        }
+    for (int c = 0; c < 4; ++c) {
+      if constexpr (POW2) {
+        o[c >> 1][(c & 1) * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lx[i][c], s, false));
+        o[c >> 1][(c & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lx[i][c], s, true));
+      } else {
+        float v[4];
+        from_e4m3(lx[i][c], v);
+        o[c >> 1][(c & 1) * 2] = scaled_pair<DT>(v[0], v[1], s);
+        o[c >> 1][(c & 1) * 2 + 1] = scaled_pair<DT>(v[2], v[3], s);
       }
-      u32x4_t* to = reinterpret_cast<u32x4_t*>(lds + buf + row * C::PITCH + piece * 16);
-      to[0] = o[0], to[1] = o[1];
     }
-#pragma unroll
-    for (int i = 0; i < C::DP; ++i) {
-      const int row = tid / DL + i * DR, piece = (tid % DL) ^ ((row & 3) * 4);
-      *reinterpret_cast<u32x4_t*>(lds + buf + C::OPERAND + row * C::PITCH + piece * 16) = l.d[i];
-    }
+    u32x4_t* to = reinterpret_cast<u32x4_t*>(lds + buf + row * C::PITCH + piece * 16);
+    to[0] = o[0], to[1] = o[1];
+  };
+  auto store_d = [&](int i, uint32_t buf) __attribute__((always_inline)) {
+    const int row = tid / DL + i * DR, piece = (tid % DL) ^ ((row & 3) * 4);
+    *reinterpret_cast<u32x4_t*>(lds + buf + C::OPERAND + row * C::PITCH + piece * 16) = ld[i];
+  };
+  // part i of four of the stage held: written, and the same part of the one behind it asked for
+  static_assert(C::DP == 4 && C::XP == 2, "parts");
+  auto part = [&](auto i_c, uint32_t buf) __attribute__((always_inline)) {
+    constexpr int I = decltype(i_c)::value;
+    if constexpr (I < 2) store_x(I, buf), load_x(I);
+    store_d(I, buf), load_d(I);
   };
 
   // ---- fragment reads: a lane's row of four, four columns; columns 32 j on are pieces 4 j on ----------------------------------------------------------------
@@ -253,19 +259,21 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
   for (int f = 0; f < C::NF; ++f) at_b[f] = rd0 + C::OPERAND + (uint32_t)(((nw * C::NF * 4 + f * 4 + pp) ^ ((l16 >> 2) * 4)) * 16);
   u32x4_t af[2][C::MF], bf[2][C::NF];
   f32x16_t acc[C::NF][C::MF];
-  // step P of a stage: its products, while the operands of the next step (step 1 of the same stage, step 0 of the next) are read from `buf`
-  auto step = [&](auto p_c, uint32_t buf) __attribute__((always_inline)) {
-    constexpr int P = decltype(p_c)::value;
+  // step S of a stage: its products, while the operands of the next step (of the same stage, or the next one's first) are read from `from`; behind the first ones
+  // what `between` does
+  auto step = [&](auto s_c, uint32_t from, auto&& between) __attribute__((always_inline)) {
+    constexpr int S = decltype(s_c)::value, P = S & 1, NEXT = (S + 1) & 3;
 #pragma unroll
-    for (int f = 0; f < C::NF; ++f) bf[1 - P][f] = read_frag_tr(at_b[f] + (uint32_t)((1 - P) * 16 * C::PITCH) + buf, C::PITCH);
+    for (int f = 0; f < C::NF; ++f) bf[1 - P][f] = read_frag_tr(at_b[f] + (uint32_t)(NEXT * 16 * C::PITCH) + from, C::PITCH);
 #pragma unroll
     for (int j = 0; j < C::MF; ++j) {
-      af[1 - P][j] = read_frag_tr(at_a[j] + (uint32_t)((1 - P) * 16 * C::PITCH) + buf, C::PITCH);
+      af[1 - P][j] = read_frag_tr(at_a[j] + (uint32_t)(NEXT * 16 * C::PITCH) + from, C::PITCH);
 #pragma unroll
       for (int f = 0; f < C::NF; ++f) {
         acc[f][j] = mfma_k16<DT>(bf[P][f], af[P][j], acc[f][j]);
         asm volatile("" : "+v"(acc[f][j]));  // (an empty use: the products stay where they are written)
       }
+      if (j == 0) between();
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -313,11 +321,17 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
     }
   };
 
-  Loads l0, l1;
-  load(l0);
-  store(l0, 0);
-  load(l0);
-  load(l1);
+  // the first stage into LDS, the second into registers
+  resources();
+  static_for<0, 4>([&](auto i_c) __attribute__((always_inline)) {
+    constexpr int I = decltype(i_c)::value;
+    if constexpr (I < 2) load_x(I);
+    load_d(I);
+  });
+  advance();
+  resources();
+  static_for<0, 4>([&](auto i_c) __attribute__((always_inline)) { part(i_c, 0); });
+  advance();
   barrier();
 #pragma unroll
   for (int f = 0; f < C::NF; ++f) bf[0][f] = read_frag_tr(at_b[f], C::PITCH);
@@ -325,26 +339,25 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
   for (int j = 0; j < C::MF; ++j) af[0][j] = read_frag_tr(at_a[j], C::PITCH);
   clear();
   int t = 0;
-  // a stage in buffer `buf`; `l` holds the next one, and then the one two further on
-  auto stage = [&](Loads& l, uint32_t buf) __attribute__((always_inline)) -> bool {
-    step(template_int<0>{}, buf);
-    store(l, buf ^ C::STAGE);
-    load(l);
+  uint32_t buf = 0;
+#pragma unroll 1
+  for (;;) {
+    const uint32_t other = buf ^ C::STAGE;
+    resources();
+    step(template_int<0>{}, buf, [&]() __attribute__((always_inline)) { part(template_int<0>{}, other); });
+    step(template_int<1>{}, buf, [&]() __attribute__((always_inline)) { part(template_int<1>{}, other); });
+    step(template_int<2>{}, buf, [&]() __attribute__((always_inline)) { part(template_int<2>{}, other), part(template_int<3>{}, other); });
     barrier();
-    step(template_int<1>{}, buf ^ C::STAGE);
+    step(template_int<3>{}, other, []() {});
+    advance();
+    buf = other;
     t += kStage;
     if (t >= cur.rows) {
       write(cur);
       clear();
       t = 0, ++cur_r;
-      return next(cur_r, cur);
+      if (!next(cur_r, cur)) break;
     }
-    return true;
-  };
-#pragma unroll 1
-  for (;;) {
-    if (!stage(l0, 0)) break;
-    if (!stage(l1, C::STAGE)) break;
   }
 }
 
@@ -406,10 +419,10 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
   hipStream_t st = static_cast<hipStream_t>(stream);
   p.pow2 = d->pow2_scales;
   // Lines that begin at sixteen-byte boundaries and do not overlap (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's), and offsets
-  // within a stage of 32 rows that fit a buffer resource.
+  // within a stage of 64 rows that fit a buffer resource.
   const int64_t limit = (int64_t)1 << 31;
   if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0 && p.x_t >= p.K && p.dy_t >= p.N &&
-      p.xs_t >= 0 && p.xs_k >= 0 && 32 * p.x_t < limit && 64 * p.dy_t < limit && (32 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
+      p.xs_t >= 0 && p.xs_k >= 0 && 64 * p.x_t < limit && 128 * p.dy_t < limit && (64 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
     const int64_t tiles = cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices;
     return tiles >= 2 * device_cu_count() ? launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st) : launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
   }
