@@ -709,7 +709,10 @@ typedef struct tk_fp8_wgrad_desc {
   int32_t y_dtype; /* TK_F32, TK_BF16, TK_F16 */
   int64_t y_stride_e, y_stride_k;
   int32_t pow2_scales; /* as in tk_fp8_gemm_desc */
+  /* tk_fp8_block_wgrad_workspace_bytes bytes, 16-byte aligned, not cleared, or NULL: long slices are then not cut into parts that are summed side by side */
+  void* workspace;
 } tk_fp8_wgrad_desc;
+int64_t tk_fp8_block_wgrad_workspace_bytes(int32_t T, int32_t K, int32_t N, int32_t n_slices);
 int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* desc, tk_stream_t stream);
 
 /*

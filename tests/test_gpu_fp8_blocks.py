@@ -523,3 +523,16 @@ def test_hooks_on_saved_tensors():
     for out, d in ((y, dy), (h, dh)):
         with pytest.raises(ValueError, match="as the forward pass saved it"):
             torch.autograd.grad(out, x, d)
+
+
+@pytest.mark.parametrize("T,K,N,sizes", [(8192, 128, 72, None), (5000, 136, 520, [700, 0, 3300, 64, 900]), (4100, 256, 256, [4100, 0]), (1025, 16, 8, None), (20000, 64, 24, [1, 19999])])
+def test_weight_gradients_of_long_slices_in_parts(T, K, N, sizes):
+    g = _gen(T, K, N)
+    x, s = downcast_to_fp8_blocks(_rows(g, T, K))
+    dy = _rows(g, T, N, BF16, 0.02)
+    md = None if sizes is None else _metadata(sizes, T)
+    total = T if sizes is None else sum(sizes)
+    for out_dtype in (F32, BF16, F16):
+        dw = weight_gradient_fp8_blocks(x, s, dy, md, out_dtype)
+        check(dw.view(-1, K, N), *orc.weight_gradient(x[:total], s[:total], dy[:total], sizes, out_dtype), "dw")
+        assert torch.equal(weight_gradient_fp8_blocks(x, s, dy, md, out_dtype), dw)

@@ -125,7 +125,7 @@ class Fp8WgradDesc(_c.Structure):
     _fields_ = [
         ("x", _ptr), ("x_stride_t", _i64), ("x_scale", _ptr), ("xs_stride_t", _i64), ("xs_stride_k", _i64), ("dy", _ptr), ("dy_dtype", _i32),
         ("dy_stride_t", _i64), ("slice_sizes", _ptr), ("slice_offs", _ptr), ("n_slices", _i32), ("T", _i32), ("K", _i32), ("N", _i32),
-        ("y", _ptr), ("y_dtype", _i32), ("y_stride_e", _i64), ("y_stride_k", _i64), ("pow2_scales", _i32),
+        ("y", _ptr), ("y_dtype", _i32), ("y_stride_e", _i64), ("y_stride_k", _i64), ("pow2_scales", _i32), ("workspace", _ptr),
     ]
 
 
@@ -163,6 +163,7 @@ SIGNATURES = {
     "tk_fp8_block_downcast": (_i32, [_ptr, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr]),
     "tk_fp8_block_upcast": (_i32, [_ptr, _i64, _i64, _i64, _i64, _i64, _i32, _ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _ptr]),
     "tk_fp8_block_gemm": (_i32, [_c.POINTER(Fp8GemmDesc), _ptr]),
+    "tk_fp8_block_wgrad_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
     "tk_fp8_block_wgrad": (_i32, [_c.POINTER(Fp8WgradDesc), _ptr]),
     "tk_swiglu_fp8": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _f32, _f32, _i32, _ptr]),
     "tk_swiglu_fp8_backward": (_i32, [_ptr, _i32, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _f32, _f32, _i32, _ptr]),

@@ -18,6 +18,7 @@ struct WgradParams {
   uint8_t* y;
   int64_t y_e, y_k;
   int32_t tiles_k, tiles_n;
+  int32_t parts;  // parts of a slice's rows, each with sums of its own (y is the workspace then)
   int32_t pow2;
   int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
 };
@@ -133,15 +134,19 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
     so = __builtin_amdgcn_ds_permute(rank * 4, first);
     id = __builtin_amdgcn_ds_permute(rank * 4, lane);
   }
-  const uint32_t per_e = (uint32_t)(p.tiles_k * p.tiles_n), q = (per_e + 7) / 8, total = q * (uint32_t)p.n_slices;
+  // (of few tiles a slice, and of parts, an XCD takes every eighth)
+  const uint32_t per_e = (uint32_t)(p.tiles_k * p.tiles_n), parts = (uint32_t)p.parts, units = per_e * (uint32_t)p.n_slices * parts;
+  const bool flat = per_e < 64 || parts > 1;
+  const uint32_t q = (per_e + 7) / 8, total = flat ? (units + 7) / 8 : q * (uint32_t)p.n_slices;
   const uint32_t xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3, wgs = gridDim.x >> 3, rounds = (total + wgs - 1) / wgs;
   struct Where {
     int id, rows, first, k0, n0;
   };
   auto next = [&](uint32_t& r, Where& w) __attribute__((always_inline)) -> bool {
     for (; r < rounds; ++r) {
-      const uint32_t l = r * wgs + (r & 1 ? wgs - 1 - i8 : i8), rank = (uint32_t)__builtin_amdgcn_readfirstlane((int)(l / q)), in = xcd * q + (l - rank * q);
-      if (l >= total || in >= per_e) continue;
+      const uint32_t l = r * wgs + (r & 1 ? wgs - 1 - i8 : i8), v = flat ? (l * 8 + xcd) / per_e : l / q, in = flat ? l * 8 + xcd - v * per_e : xcd * q + (l - v * q);
+      if (l >= total || in >= per_e || v >= parts * (uint32_t)p.n_slices) continue;
+      const uint32_t rank = (uint32_t)__builtin_amdgcn_readfirstlane((int)(v / parts)), part = v - rank * parts;
       // (bands of eight tiles down, in a band column by column, so that those in hand on an XCD share few operand columns)
       const uint32_t band = in / (8u * (uint32_t)p.tiles_n), left = (uint32_t)p.tiles_k - band * 8u, bh = left < 8u ? left : 8u;
       const uint32_t in_b = in - band * 8u * (uint32_t)p.tiles_n, tn = in_b / bh, tk = band * 8u + in_b - tn * bh;
@@ -152,6 +157,11 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
         typedef const __attribute__((address_space(4))) int32_t* scalar_t;
         w.id = (int)rank, w.rows = reinterpret_cast<scalar_t>(reinterpret_cast<uintptr_t>(p.slice_sizes))[rank];
         w.first = reinterpret_cast<scalar_t>(reinterpret_cast<uintptr_t>(p.slice_offs))[rank];
+      }
+      if (parts > 1) {  // whole stages
+        const uint32_t stages = ((uint32_t)w.rows + kStage - 1) / kStage, from = (uint32_t)((uint64_t)stages * part / parts) * kStage;
+        const uint32_t to = (uint32_t)((uint64_t)stages * (part + 1) / parts) * kStage;
+        w.rows = (int)(to < (uint32_t)w.rows ? to : (uint32_t)w.rows) - (int)from, w.first += (int)from, w.id = w.id * (int)parts + (int)part;
       }
       // (all of it is the same in every lane, which the compiler loses sight of)
       w.id = __builtin_amdgcn_readfirstlane(w.id), w.rows = __builtin_amdgcn_readfirstlane(w.rows), w.first = __builtin_amdgcn_readfirstlane(w.first);
@@ -373,11 +383,35 @@ int32_t launch_any(WgradParams p, int dt, int yt, hipStream_t st) {
   return check_launch("fp8_wgrad_any_kernel");
 }
 
+// The parts' sums of one slice, added in their order.
+template <int YT>
+__global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float* ws, int parts, int64_t n_slices, int64_t K, int64_t N, int64_t pitch, void* y, int64_t y_e, int64_t y_k) {
+  const int64_t quads = pitch / 4, all = n_slices * K * quads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t line = i / quads, n = (i - line * quads) * 4, e = line / K, k = line - e * K;
+    const float* from = ws + (e * parts * K + k) * pitch + n;
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < parts; ++s) sum += *reinterpret_cast<const f32x4_t*>(from + s * K * pitch);
+    for (int c = 0; c < 4; ++c)
+      if (n + c < N) store_elem<YT>(y, e * y_e + k * y_k + n + c, sum[c]);
+  }
+}
+
+// Parts of a slice's rows: where tiles of 128 are fewer than half of the places for them and a slice has (expected) eight stages and more, so many that they fill those
+// places, of four stages at least.
+int wgrad_parts(int64_t T, int64_t K, int64_t N, int64_t n_slices) {
+  const int64_t tiles = cdiv(K, 128) * cdiv(N, 128) * n_slices, places = 512, stages = n_slices > 0 ? T / n_slices / kStage : 0;
+  if (tiles == 0 || tiles * 2 > places || stages < 8) return 1;
+  const int64_t by_places = places / tiles, by_stages = stages / 4;
+  return (int)(by_places < by_stages ? by_places : by_stages);
+}
+
 template <int T>
 int32_t launch_tiles(WgradParams p, int dt, int yt, hipStream_t st) {
   typedef WgradCfg<T> C;
   p.tiles_k = (int)cdiv(p.K, T), p.tiles_n = (int)cdiv(p.N, T);
-  const int64_t lists = cdiv((int64_t)p.tiles_k * p.tiles_n, 8) * p.n_slices;  // tiles of an XCD
+  const int64_t per_e = (int64_t)p.tiles_k * p.tiles_n;
+  const int64_t lists = per_e < 64 || p.parts > 1 ? cdiv(per_e * p.n_slices * p.parts, 8) : cdiv(per_e, 8) * p.n_slices;  // tiles of an XCD
   if (lists * 8 > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: grid too large");
   const int64_t most = (int64_t)device_cu_count() * C::PER_CU / 8;
   const unsigned grid = (unsigned)((lists < most ? lists : most) * 8);
@@ -399,6 +433,12 @@ int32_t launch_tiles(WgradParams p, int dt, int yt, hipStream_t st) {
 }  // namespace tk
 
 using namespace tk;
+
+extern "C" int64_t tk_fp8_block_wgrad_workspace_bytes(int32_t T, int32_t K, int32_t N, int32_t n_slices) {
+  if (T < 0 || K < 0 || N < 0 || n_slices < 0) return -1;
+  const int64_t parts = wgrad_parts(T, K, N, n_slices);
+  return parts > 1 ? parts * n_slices * K * (cdiv(N, 4) * 4) * 4 : 0;
+}
 
 extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t stream) {
   if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null descriptor");
@@ -423,6 +463,22 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
   const int64_t limit = (int64_t)1 << 31;
   if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0 && p.x_t >= p.K && p.dy_t >= p.N &&
       p.xs_t >= 0 && p.xs_k >= 0 && 64 * p.x_t < limit && 128 * p.dy_t < limit && (64 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
+    p.parts = d->workspace ? wgrad_parts(p.T, p.K, p.N, p.n_slices) : 1;
+    if (p.parts > 1) {
+      WgradParams q = p;
+      const int64_t pitch = cdiv(p.N, 4) * 4;
+      q.y = static_cast<uint8_t*>(d->workspace), q.y_e = p.K * pitch, q.y_k = pitch;
+      q.y_vec = reinterpret_cast<uintptr_t>(d->workspace) % 16 == 0;
+      if (!q.y_vec) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: the workspace is not 16-byte aligned");
+      if (const int32_t rc = launch_tiles<128>(q, d->dy_dtype, TK_F32, st)) return rc;
+      const int64_t blocks = cdiv(p.n_slices * p.K * (pitch / 4), 256);
+      auto join = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, static_cast<const float*>(d->workspace), p.parts, (int64_t)p.n_slices, (int64_t)p.K,
+                           (int64_t)p.N, pitch, static_cast<void*>(p.y), p.y_e, p.y_k);
+      };
+      d->y_dtype == TK_F32 ? join(fp8_wgrad_join_kernel<TK_F32>) : d->y_dtype == TK_BF16 ? join(fp8_wgrad_join_kernel<TK_BF16>) : join(fp8_wgrad_join_kernel<TK_F16>);
+      return check_launch("fp8_wgrad_join_kernel");
+    }
     const int64_t tiles = cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices;
     return tiles >= 2 * device_cu_count() ? launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st) : launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
   }

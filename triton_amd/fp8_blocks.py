@@ -327,6 +327,9 @@ def _weight_gradient(x, x_scale, dy, md, out_dtype, pow2):
     d.n_slices, d.T, d.K, d.N = E, T, K, N
     d.y, d.y_dtype, d.y_stride_e, d.y_stride_k = y.data_ptr(), nt.TORCH_TO_TK[out_dtype], y.stride(0), y.stride(1)
     d.pow2_scales = int(pow2)
+    n_ws = nt.lib().tk_fp8_block_wgrad_workspace_bytes(T, K, N, E)
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=x.device) if n_ws else None
+    d.workspace = nt.ptr(ws)
     nt.submit(nt.lib().tk_fp8_block_wgrad, d, x.device)
     return y if md is not None else y[0]
 
