@@ -202,16 +202,16 @@ def test_what_is_not_finite_stays_in_its_row_or_column(M):
 def test_rows_behind_the_slices_and_dropped_ones_stay():
     g, a, a_scale, w, w_scale = _operands(6, 90, 256, 64, 3)
     sizes = [20, 0, 31]
-    from triton_amd import fp8_blocks as mod
-    before, mod.torch.empty = torch.empty, lambda *s, **k: before(*s, **k).fill_(7) if k.get("dtype") == BF16 else before(*s, **k)
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)                               # (new memory holds NaN)
     try:
         y = matmul_fp8_blocks(a, a_scale, w, w_scale, None, _metadata(sizes, 90))
         at = torch.arange(90, dtype=torch.int32, device="cuda")
         at[::4] = -1
         z = matmul_fp8_blocks(a, a_scale, w, w_scale, None, _metadata(sizes, 90), scatter_indx=at)
     finally:
-        mod.torch.empty = before
-    assert (y[51:] == 7).all() and (z[51:] == 7).all() and (z[::4] == 7).all()
+        torch.use_deterministic_algorithms(before)
+    assert y[51:].isnan().all() and z[51:].isnan().all() and z[::4].isnan().all()
     want, bound, _ = orc.product(a[:51], a_scale[:51], w, w_scale, sizes)
     check(y[:51], want, bound, "y")
     assert torch.equal(z[1::4][:13], y[1::4][:13])
@@ -521,7 +521,7 @@ def test_hooks_on_saved_tensors():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:1]):
         y, h = linear_fp8_blocks(x, w), swiglu_fp8_checkpoint(x, 1.0)
     for out, d in ((y, dy), (h, dh)):
-        with pytest.raises(ValueError, match="as the forward pass saved it"):
+        with pytest.raises((ValueError, RuntimeError), match="as the forward pass saved it"):
             torch.autograd.grad(out, x, d)
 
 

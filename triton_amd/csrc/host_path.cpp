@@ -1,6 +1,6 @@
 // The host side of the common calls: a CPython extension module (`triton_amd._host`) that checks the operands, allocates the
 // results, fills the descriptor of the C ABI and launches, for the calls a layer is made of (routing, the expert GEMM, the top-k
-// combine, the quantisers, the ragged-K GEMM, the one-launch decode layer, and the row operators around them in host_rows.h).
+// combine, the quantisers, the ragged-K GEMM, the one-launch decode layer, the row operators around them in host_rows.h, and the experts in 8 bits in host_fp8.h).
 //
 // What bounds it: these calls come one after another from Python, and at small sizes the GPU waits for them.  The same steps
 // written in Python cost 15 us for a GEMM, 20 us for the router and 11 us for the combine, most of it attribute and tensor
@@ -55,6 +55,13 @@ struct Bound {
   decltype(&tk_token_logprobs_backward) token_logprobs_backward = nullptr;
   decltype(&tk_distill_topk) distill_topk = nullptr;
   decltype(&tk_distill_topk_backward) distill_topk_backward = nullptr;
+  decltype(&tk_fp8_block_downcast) fp8_downcast = nullptr;
+  decltype(&tk_fp8_block_upcast) fp8_upcast = nullptr;
+  decltype(&tk_fp8_block_gemm) fp8_gemm = nullptr;
+  decltype(&tk_fp8_block_wgrad) fp8_wgrad = nullptr;
+  decltype(&tk_fp8_block_wgrad_workspace_bytes) fp8_wgrad_workspace = nullptr;
+  decltype(&tk_swiglu_fp8) swiglu_fp8 = nullptr;
+  decltype(&tk_swiglu_fp8_backward) swiglu_fp8_backward = nullptr;
   decltype(&tk_last_error) last_error = nullptr;
   PyObject *check, *raw_stream, *current_device, *capturing;  // _native.check, torch's raw stream, device and capture getters
   PyObject *tile_counters, *combine_counters, *decode_workspace;  // per device and stream
@@ -811,6 +818,7 @@ PyObject* run_decode_layer(PyObject* const* v) {
 }  // namespace
 
 #include "host_rows.h"
+#include "host_fp8.h"
 
 namespace {
 
@@ -935,6 +943,13 @@ PyObject* bind(PyObject*, PyObject* dict) {
   ENTRY(token_logprobs_backward, tk_token_logprobs_backward)
   ENTRY(distill_topk, tk_distill_topk)
   ENTRY(distill_topk_backward, tk_distill_topk_backward)
+  ENTRY(fp8_downcast, tk_fp8_block_downcast)
+  ENTRY(fp8_upcast, tk_fp8_block_upcast)
+  ENTRY(fp8_gemm, tk_fp8_block_gemm)
+  ENTRY(fp8_wgrad, tk_fp8_block_wgrad)
+  ENTRY(fp8_wgrad_workspace, tk_fp8_block_wgrad_workspace_bytes)
+  ENTRY(swiglu_fp8, tk_swiglu_fp8)
+  ENTRY(swiglu_fp8_backward, tk_swiglu_fp8_backward)
   ENTRY(last_error, tk_last_error)
 #undef ENTRY
 #define OBJECT(name)                            \
@@ -962,6 +977,11 @@ PyMethodDef methods[] = {
     METHOD("layer_norm", run_layer_norm, 4),
     METHOD("token_logprobs", run_token_logprobs, 4),
     METHOD("distill_topk", run_distill_topk, 4),
+    METHOD("fp8_downcast", run_fp8_downcast, 2),
+    METHOD("fp8_upcast", run_fp8_upcast, 4),
+    METHOD("fp8_matmul", run_fp8_matmul, 11),
+    METHOD("fp8_linear", run_fp8_linear, 3),
+    METHOD("fp8_swiglu", run_fp8_swiglu, 3),
     METHOD("kept_by_default_stream", run_kept_by_default_stream, 1),
     METHOD("x_extent", rule_x_extent, 4),
     METHOD("dma_runs_16bit", rule_dma_16bit, 5),

@@ -82,6 +82,10 @@ def downcast_to_fp8_blocks(x: torch.Tensor, block_rows: int = 1):
 
     A block's scale is the smallest power of two that leaves its largest finite magnitude at most 448 (1 for a block of zeros, at least
     2^-126); elements are rounded to the nearest e4m3, ties to even.  Infinities and NaN become NaN and do not count for the scale."""
+    host = nt.host()
+    r = host.fp8_downcast(x, block_rows) if host is not None else None
+    if r is not None:
+        return r
     _check_block_rows(block_rows)
     _type(x, "x")
     _no_gradient("downcast_to_fp8_blocks", x=x)
@@ -99,6 +103,10 @@ def downcast_to_fp8_blocks(x: torch.Tensor, block_rows: int = 1):
 
 def upcast_from_fp8_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16, block_rows: int = 1) -> torch.Tensor:
     """`values * scales`, rounded once to `dtype` (fp32, bf16 or fp16); the arguments as `downcast_to_fp8_blocks` returns them, scales of any size."""
+    host = nt.host()
+    r = host.fp8_upcast(values, scales, dtype, block_rows) if host is not None else None
+    if r is not None:
+        return r
     _check_block_rows(block_rows)
     _type(values, "values", (_E4M3, ))
     if dtype not in DTYPES:
@@ -184,6 +192,14 @@ def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dt
     return y
 
 
+def _aligned(t, unit):
+    """`t [.., lines, length]` with lines at sixteen-byte boundaries (`unit` elements), copied if they are elsewhere."""
+    if t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1]):
+        return t
+    out = torch.empty((*t.shape[:-1], -(-t.shape[-1] // unit) * unit), dtype=t.dtype, device=t.device)[..., :t.shape[-1]]
+    return out.copy_(t)
+
+
 def _activation(fused_activation):
     """`(alpha, limit)` of a fused swiglu, None without one."""
     if fused_activation is None or (fused_activation.specs.fn is None and fused_activation.specs.name == "dflt"):
@@ -211,8 +227,11 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
     and keep of each what reaches 2^-13 of the largest one; for fp32 results they are taken from the exact 16-bit form of the values, at a fraction of the speed.
 
     Rows that no slice holds, and rows of the output that no index names, are not written.  No gradients: `linear_fp8_blocks` has them."""
-    check = dict(a_scale=a_scale, w_scale=w_scale, bias=bias, gammas=gammas)
-    _no_gradient("matmul_fp8_blocks", **check)
+    host = nt.host()
+    y = host.fp8_matmul(a, a_scale, w, w_scale, bias, a_ragged_metadata, gather_indx, scatter_indx, gammas, fused_activation, out_dtype) if host is not None else None
+    if y is not None:
+        return y
+    _no_gradient("matmul_fp8_blocks", a_scale=a_scale, w_scale=w_scale, bias=bias, gammas=gammas)
     _type(w, "w", (_E4M3, ))
     a = _operand_rows(a, a_scale)
     if w.ndim == 2:
@@ -257,6 +276,9 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
         raise NotImplementedError("batched weights need ragged metadata")
     if w.stride(1) != 1 and K > 1:
         w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    if M > 256 * E:
+        # (the fast kernels take lines at sixteen-byte boundaries; from about a hundred rows an expert a copy of all weights costs less than the kernel for any lines)
+        a, w = _aligned(a, 16), _aligned(w.transpose(1, 2), 16).transpose(1, 2)
     return _gemm(a, a_scale, w, w_scale, bias, md, gather_indx, scatter_indx, gammas, act, out_dtype, False)
 
 
@@ -317,6 +339,7 @@ def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch
 def _weight_gradient(x, x_scale, dy, md, out_dtype, pow2):
     """One launch; operands as checked by the callers.  `pow2`: the scales are the quantiser's."""
     dy = dy if dy.stride(1) == 1 or dy.shape[1] <= 1 else dy.contiguous()
+    x, dy = _aligned(x, 16), _aligned(dy, 8)  # (a copy costs less than the kernel for lines that begin anywhere)
     (T, K), N, E = x.shape, dy.shape[1], 1 if md is None else md.n_slices
     y = torch.empty((E, K, N), dtype=out_dtype, device=x.device)
     d = nt.Fp8WgradDesc()
@@ -390,6 +413,10 @@ def linear_fp8_blocks(x: torch.Tensor, w: torch.Tensor, a_ragged_metadata: Optio
     `x [rows, K]` is bf16 or fp16, the rows of the slices of `a_ragged_metadata` in order; `w [E, K, N]` (`[K, N]` without metadata) fp32, bf16 or fp16,
     contiguous along either of its last dimensions.  y and dx have x's type, dw has w's.  `quantized` = `quantize_fp8_weight(w)`, for steps that use the same weights several
     times; without it the call quantises w.  Rows behind the last slice give and receive zeros."""
+    host = nt.host() if quantized is None else None
+    y = host.fp8_linear(x, w, a_ragged_metadata) if host is not None else None
+    if y is not None:
+        return y
     _type(x, "x", (torch.bfloat16, torch.float16))
     _type(w, "w")
     if x.ndim != 2 or w.ndim not in (2, 3) or w.device != x.device or w.shape[-2] != x.shape[1]:
@@ -493,6 +520,10 @@ def swiglu_fp8_checkpoint(a: torch.Tensor, alpha: float, limit: Optional[float] 
     """swiglu of `a [..., 2n]` with interleaved (gate, linear) columns -> `[..., n]` in a's type (fp32, bf16 or fp16); for the backward pass a is kept in 8 bits
     (`downcast_to_fp8_blocks` of its rows), and the gradient is that at the kept values.  The same formula as `swiglu`, but NaN stays NaN also in front of a limit.  An element
     beyond the limit has the gradient zero.  Differentiable once; where no gradient is asked for nothing is kept."""
+    host = nt.host()
+    h = host.fp8_swiglu(a, alpha, limit) if host is not None else None
+    if h is not None:
+        return h
     check_forward_mode("swiglu_fp8_checkpoint", a)
     if torch.is_grad_enabled() and a.requires_grad:
         check_capture(a)
