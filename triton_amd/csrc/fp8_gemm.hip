@@ -114,8 +114,10 @@ bool fp8_tiles_run(Fp8GemmParams& p, int64_t x_rows, int yt) {
   return true;
 }
 
-// Tiles of a size that a call is expected to have: every slice's last row block is half full.
-int64_t expected_tiles(const Fp8GemmParams& p, int64_t slices, int64_t size) { return cdiv(2 * p.M + slices * size, 2 * size) * cdiv(p.N, size); }
+// Tiles of a size that a call is expected to have: every slice's last row block is half full (a single slice's is known).
+int64_t expected_tiles(const Fp8GemmParams& p, int64_t slices, int64_t size) {
+  return (p.slice_sizes ? cdiv(2 * p.M + slices * size, 2 * size) : cdiv(p.M, size)) * cdiv(p.N, size);
+}
 
 // Few rows a slice, and so few tiles of 128 that half of the CUs would have none.  us, few / tiles of 128 (K, N 4096 if not said): one slice, up to 32 rows 15 (the host's
 // time) / 32, 64 17 / 33, 128 32 / 34, 256 62 / 34; two, K 7168, N 2048, 32 rows each 22 / 52; eight of 8 rows, 256 tiles, 45 / 38; 32 of 4, K 2880, N 5760 155 / 115.
