@@ -28,7 +28,6 @@ struct Fp8GemmParams {
   int32_t M, N, K;
   void* y;
   int64_t y_stride_m;
-  int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
   float alpha, limit;  // (limit: +inf without one)
   int32_t zero_rest;
   int32_t pow2;      // all scales are powers of two (fp8_scale's)
@@ -137,32 +136,35 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
   else
     static_cast<uint16_t*>(p)[i] = f32_to_f16_bits(v);
 }
-// N (4 or 8) consecutive elements, of an address that N elements' size divides up to 16 bytes
+// N (4 or 8) consecutive elements at any element's address: wide loads and stores need no alignment here, but those that cross cache lines take two
+template <class V>
+__device__ __forceinline__ V load_wide(const void* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <class V>
+__device__ __forceinline__ void store_wide(void* p, V v) {
+  __builtin_memcpy(p, &v, sizeof(V));
+}
 template <int DT, int N>
 __device__ __forceinline__ void load_vec(const void* p, int64_t i, float* v) {
   if constexpr (DT == TK_F32) {
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
-      const f32x4_t t = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i + c);
+      const f32x4_t t = load_wide<f32x4_t>(static_cast<const float*>(p) + i + c);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[c + k] = t[k];
     }
   } else {
-    uint32_t w[N / 2];
-    if constexpr (N == 8) {
-      const u32x4_t t = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = t[k];
-    } else {
-      const u32x2_t t = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + i);
-      w[0] = t[0], w[1] = t[1];
-    }
+    typedef uint32_t words_t __attribute__((ext_vector_type(N / 2)));
+    const words_t w = load_wide<words_t>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
       if constexpr (DT == TK_BF16) {
         v[2 * k] = bits_f32(w[k] << 16), v[2 * k + 1] = bits_f32(w[k] & 0xFFFF0000u);
       } else {
-        const f16x2_t h = __builtin_bit_cast(f16x2_t, w[k]);
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, (uint32_t)w[k]);
         v[2 * k] = (float)h[0], v[2 * k + 1] = (float)h[1];
       }
     }
@@ -172,15 +174,13 @@ template <int DT, int N>
 __device__ __forceinline__ void store_vec(void* p, int64_t i, const float* v) {
   if constexpr (DT == TK_F32) {
 #pragma unroll
-    for (int c = 0; c < N; c += 4) *reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + i + c) = f32x4_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
+    for (int c = 0; c < N; c += 4) store_wide(static_cast<float*>(p) + i + c, f32x4_t{v[c], v[c + 1], v[c + 2], v[c + 3]});
   } else {
-    uint32_t w[N / 2];
+    typedef uint32_t words_t __attribute__((ext_vector_type(N / 2)));
+    words_t w;
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) w[k] = pack_out2<DT == TK_F16>(v[2 * k], v[2 * k + 1]);
-    if constexpr (N == 8)
-      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + i) = u32x4_t{w[0], w[1], w[2], w[3]};
-    else
-      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p) + i) = u32x2_t{w[0], w[1]};
+    store_wide(static_cast<uint16_t*>(p) + i, w);
   }
 }
 
@@ -266,7 +266,7 @@ __device__ __forceinline__ void fp8_epilogue(const Fp8GemmParams& p, f32x4_t (&a
         float o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = swiglu_of<YT == TK_F32>(v[2 * i], v[2 * i + 1], p.alpha, p.limit) * gam[j];
-        if (p.y_vec && n0 + 8 <= n_end) {
+        if (n0 + 8 <= n_end) {
           store_vec<YT, 4>(p.y, row + n0 / 2, o);
         } else {
 #pragma unroll
@@ -276,7 +276,7 @@ __device__ __forceinline__ void fp8_epilogue(const Fp8GemmParams& p, f32x4_t (&a
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= gam[j];
-        if (p.y_vec && n0 + 8 <= n_end) {
+        if (n0 + 8 <= n_end) {
           store_vec<YT, 8>(p.y, row + n0, v);
         } else {
 #pragma unroll

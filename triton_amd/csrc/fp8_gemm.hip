@@ -165,7 +165,6 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   p.n_slices = d->n_slices, p.grid_m = d->slice_sizes ? d->grid_m : (int)cdiv(d->M, kAnyRows);
   p.M = d->M, p.N = d->N, p.K = d->K;
   p.y = d->y, p.y_stride_m = d->y_stride_m;
-  p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && d->y_stride_m * (d->y_dtype == TK_F32 ? 4 : 2) % 16 == 0;
   p.alpha = d->act_alpha, p.limit = d->act_has_limit ? d->act_limit : INFINITY;
   p.zero_rest = d->zero_rest, p.pow2 = d->pow2_scales;
   if (p.grid_m == 0) return TK_OK;

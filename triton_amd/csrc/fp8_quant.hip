@@ -17,7 +17,7 @@ struct RowsParams {
   const void* d;  // swiglu's backward pass: the gradient of its output
   int64_t d_r;
   int64_t rows, cols, groups;  // groups = batch * rows * blocks of a row
-  uint32_t blocks, vec;
+  uint32_t blocks;
   int32_t block_rows;
   float alpha, limit;
 };
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const RowsParams p) {
     const int64_t at = w.b * p.x_b + w.r * p.x_r + w.col;
     const bool whole = w.col + 8 <= p.cols;
     float v[8];
-    if (p.vec && whole) {
+    if (whole) {
       load_vec<DT, 8>(p.x, at, v);
     } else {
 #pragma unroll
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const RowsParams p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = swiglu_of<DT == TK_F32>(v[2 * i], v[2 * i + 1], p.alpha, p.limit);
       const int64_t to = w.r * p.y_r + w.col / 2;
-      if (p.vec && whole) {
+      if (whole) {
         store_vec<DT, 4>(p.y, to, o);
       } else {
 #pragma unroll
@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const RowsParams p) {
     for (int i = 0; i < 8; ++i) v[i] = no_infinity(v[i]) * inv;
     const u32x2_t q = {to_e4m3(v[0], v[1], v[2], v[3]), to_e4m3(v[4], v[5], v[6], v[7])};
     uint8_t* out = p.v + w.b * p.v_b + w.r * p.v_r + w.col;
-    if (p.vec && whole) {
-      *reinterpret_cast<u32x2_t*>(out) = q;
+    if (whole) {
+      store_wide(out, q);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256) void fp8_upcast_kernel(const RowsParams p) {
     const float s = p.s[w.b * p.s_b + (p.block_rows == 1 ? w.r : w.r / p.block_rows) * p.s_r + (int64_t)w.c * p.s_c];
     const uint8_t* from = p.v + w.b * p.v_b + w.r * p.v_r + w.col;
     u32x2_t q = {0, 0};
-    if (p.vec && whole) {
-      q = *reinterpret_cast<const u32x2_t*>(from);
+    if (whole) {
+      q = load_wide<u32x2_t>(from);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void fp8_upcast_kernel(const RowsParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= s;
     const int64_t to = w.b * p.y_b + w.r * p.y_r + w.col;
-    if (p.vec && whole) {
+    if (whole) {
       store_vec<DT, 8>(p.y, to, v);
     } else {
 #pragma unroll
@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256) void swiglu_fp8_backward_kernel(const RowsPara
     const int64_t d_at = w.r * p.d_r + w.col / 2;
     u32x2_t q = {0, 0};
     float d[4];
-    if (p.vec && whole) {
-      q = *reinterpret_cast<const u32x2_t*>(from);
+    if (whole) {
+      q = load_wide<u32x2_t>(from);
       load_vec<DT, 4>(p.d, d_at, d);
     } else {
 #pragma unroll
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void swiglu_fp8_backward_kernel(const RowsPara
       v[2 * i + 1] = fabsf(lin0) > p.limit ? 0.f : d[i] * gate * t.u * t.v;
     }
     const int64_t to = w.r * p.y_r + w.col;
-    if (p.vec && whole) {
+    if (whole) {
       store_vec<DT, 8>(p.y, to, v);
     } else {
 #pragma unroll
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const RowsParams p, uint8
   for (int t = 0; t < 8; ++t) {
     const int64_t r = row0 + t * 16 + line;
     const int64_t at = b * p.x_b + r * p.x_r + col;
-    if (r < p.rows && whole && p.vec) {
+    if (r < p.rows && whole) {
       load_vec<DT, 8>(p.x, at, v[t]);
     } else {
 #pragma unroll
@@ -223,8 +223,8 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const RowsParams p, uint8
     const u32x2_t q = {to_e4m3(v[t][0], v[t][1], v[t][2], v[t][3]), to_e4m3(v[t][4], v[t][5], v[t][6], v[t][7])};
     if (r < p.rows) {
       uint8_t* out = p.v + b * p.v_b + r * p.v_r + col;
-      if (p.vec && whole) {
-        *reinterpret_cast<u32x2_t*>(out) = q;
+      if (whole) {
+        store_wide(out, q);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -244,8 +244,8 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const RowsParams p, uint8
     const uint32_t* from = reinterpret_cast<const uint32_t*>(turned + c * 132 + lane * 8);
     const u32x2_t q = {from[0], from[1]};
     uint8_t* out = vt + b * t_b + (col0 + c) * t_c + row0 + lane * 8;
-    if (((uint64_t)out & 7) == 0 && row0 + lane * 8 + 8 <= p.rows) {
-      *reinterpret_cast<u32x2_t*>(out) = q;
+    if (row0 + lane * 8 + 8 <= p.rows) {
+      store_wide(out, q);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -254,10 +254,6 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const RowsParams p, uint8
   }
 }
 
-bool aligned(const void* p, int64_t stride_b, int64_t stride_r, int size, int to) {
-  return reinterpret_cast<uintptr_t>(p) % to == 0 && stride_b * size % to == 0 && stride_r * size % to == 0;
-}
-int size_of(int dtype) { return dtype == TK_F32 ? 4 : 2; }
 bool is_float(int dtype) { return dtype == TK_F32 || dtype == TK_BF16 || dtype == TK_F16; }
 unsigned groups_grid(int64_t groups) {
   const int64_t n = cdiv(groups, 16), most = (int64_t)device_cu_count() * 8;
@@ -302,7 +298,6 @@ extern "C" int32_t tk_fp8_block_downcast(const void* x, int32_t dtype, int64_t b
   if (cdiv(cols, kFp8Block) > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_downcast: too many columns");
   p.blocks = (uint32_t)cdiv(cols, kFp8Block);
   p.groups = batch * rows * p.blocks;
-  p.vec = aligned(x, x_stride_b, x_stride_r, size_of(dtype), 16) && aligned(values, v_stride_b, v_stride_r, 1, 8);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (block_rows == 1) {
     by_type(dtype, [&](auto dt) { hipLaunchKernelGGL((fp8_rows_kernel<decltype(dt)::value, false, true>), dim3(groups_grid(p.groups)), dim3(256), 0, st, p); });
@@ -330,7 +325,6 @@ extern "C" int32_t tk_fp8_block_upcast(const uint8_t* values, int64_t batch, int
   if (cdiv(cols, kFp8Block) > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_upcast: too many columns");
   p.blocks = (uint32_t)cdiv(cols, kFp8Block);
   p.groups = batch * rows * p.blocks;
-  p.vec = aligned(out, o_stride_b, o_stride_r, size_of(out_dtype), 16) && aligned(values, v_stride_b, v_stride_r, 1, 8);
   by_type(out_dtype, [&](auto dt) { hipLaunchKernelGGL(fp8_upcast_kernel<decltype(dt)::value>, dim3(groups_grid(p.groups)), dim3(256), 0, static_cast<hipStream_t>(stream), p); });
   return check_launch("fp8_upcast_kernel");
 }
@@ -352,7 +346,6 @@ extern "C" int32_t tk_swiglu_fp8(const void* a, int32_t dtype, int64_t M, int64_
   p.blocks = (uint32_t)cdiv(p.cols, kFp8Block);
   p.groups = M * p.blocks;
   p.alpha = alpha, p.limit = has_limit ? limit : INFINITY;
-  p.vec = aligned(a, 0, a_stride_m, size_of(dtype), 16) && aligned(values, 0, v_stride_m, 1, 8) && aligned(out, 0, out_stride_m, size_of(dtype), 4 * size_of(dtype));
   by_type(dtype, [&](auto dt) {
     auto kern = values ? fp8_rows_kernel<decltype(dt)::value, true, true> : fp8_rows_kernel<decltype(dt)::value, true, false>;
     hipLaunchKernelGGL(kern, dim3(groups_grid(p.groups)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
@@ -377,7 +370,6 @@ extern "C" int32_t tk_swiglu_fp8_backward(const void* d_out, int32_t dtype, int6
   p.blocks = (uint32_t)cdiv(p.cols, kFp8Block);
   p.groups = M * p.blocks;
   p.alpha = alpha, p.limit = has_limit ? limit : INFINITY;
-  p.vec = aligned(d_a, 0, d_a_stride_m, size_of(dtype), 16) && aligned(values, 0, v_stride_m, 1, 8) && aligned(d_out, 0, d_out_stride_m, size_of(dtype), 4 * size_of(dtype));
   by_type(dtype, [&](auto dt) { hipLaunchKernelGGL(swiglu_fp8_backward_kernel<decltype(dt)::value>, dim3(groups_grid(p.groups)), dim3(256), 0, static_cast<hipStream_t>(stream), p); });
   return check_launch("swiglu_fp8_backward_kernel");
 }

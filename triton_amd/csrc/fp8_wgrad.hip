@@ -20,7 +20,6 @@ struct WgradParams {
   int32_t tiles_k, tiles_n;
   int32_t parts;  // parts of a slice's rows, each with sums of its own (y is the workspace then)
   int32_t pow2;
-  int32_t y_vec;  // rows of y allow 16-byte stores at every eighth column
 };
 
 // an e4m3 times its scale in dy's type (in fp16 at most its largest number)
@@ -320,7 +319,7 @@ __global__ __launch_bounds__(WgradCfg<T>::THREADS, 2) void fp8_wgrad_kernel(cons
           const int n = w.n0 + (nw * C::NF + f) * 32 + 16 * u + 8 * h;
           if (k >= p.K || n >= p.N) continue;
           const int64_t to = w.id * p.y_e + k * p.y_k + n;
-          if (p.y_vec && n + 8 <= p.N) {
+          if (n + 8 <= p.N) {
             store_vec<YT, 8>(p.y, to, v);
           } else {
 #pragma unroll
@@ -454,8 +453,6 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
   p.slice_sizes = d->slice_sizes, p.slice_offs = d->slice_offs, p.n_slices = d->n_slices;
   p.T = d->T, p.K = d->K, p.N = d->N;
   p.y = static_cast<uint8_t*>(d->y), p.y_e = d->y_stride_e, p.y_k = d->y_stride_k;
-  const int ys = d->y_dtype == TK_F32 ? 4 : 2;
-  p.y_vec = reinterpret_cast<uintptr_t>(d->y) % 16 == 0 && p.y_e * ys % 16 == 0 && p.y_k * ys % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   p.pow2 = d->pow2_scales;
   // Lines that begin at sixteen-byte boundaries and do not overlap (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's), and offsets
@@ -468,8 +465,7 @@ extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t st
       WgradParams q = p;
       const int64_t pitch = cdiv(p.N, 4) * 4;
       q.y = static_cast<uint8_t*>(d->workspace), q.y_e = p.K * pitch, q.y_k = pitch;
-      q.y_vec = reinterpret_cast<uintptr_t>(d->workspace) % 16 == 0;
-      if (!q.y_vec) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: the workspace is not 16-byte aligned");
+      if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: the workspace is not 16-byte aligned");
       if (const int32_t rc = launch_tiles<128>(q, d->dy_dtype, TK_F32, st)) return rc;
       const int64_t blocks = cdiv(p.n_slices * p.K * (pitch / 4), 256);
       auto join = [&](auto kern) {
