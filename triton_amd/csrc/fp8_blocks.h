@@ -36,6 +36,7 @@ struct Fp8GemmParams {
 
 // 16-bit results, up to kDmaSlices slices, operands as fp8_tiles_run (fp8_gemm.hip) wants them; tile = 256 or 128
 int32_t fp8_gemm_launch_tiles(const Fp8GemmParams& p, int tile, int yt, bool swiglu, hipStream_t st);
+int32_t fp8_gemm_launch_ring(const Fp8GemmParams& p, int yt, bool swiglu, hipStream_t st);  // operands as for the tiles, any number of slices
 int32_t fp8_gemm_launch_few(const Fp8GemmParams& p, bool aligned, int yt, bool swiglu, hipStream_t st);
 
 namespace {

@@ -104,7 +104,7 @@ int32_t launch_any(Fp8GemmParams p, int yt, bool swiglu, hipStream_t st) {
 // tile, or of x and its scales where rows are gathered.
 bool fp8_tiles_run(Fp8GemmParams& p, int64_t x_rows, int yt) {
   const int64_t limit = (int64_t)1 << 31, K16 = (p.K + 15) & ~15, blocks = cdiv(p.K, kFp8Block), rows = p.gather ? x_rows : 256;
-  if (yt == TK_F32 || p.K == 0 || (p.slice_sizes && p.n_slices > kDmaSlices)) return false;
+  if (yt == TK_F32 || p.K == 0) return false;
   if ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) return false;
   if (p.x_stride_m < 0 || p.w_n < 0 || p.xs_m < 0 || p.xs_k < 0 || p.ws_k < 0 || p.ws_n < 0) return false;
   const int64_t x_bytes = (rows - 1) * p.x_stride_m + K16;
@@ -119,17 +119,30 @@ int64_t expected_tiles(const Fp8GemmParams& p, int64_t slices, int64_t size) {
   return (p.slice_sizes ? cdiv(2 * p.M + slices * size, 2 * size) : cdiv(p.M, size)) * cdiv(p.N, size);
 }
 
-// Few rows a slice, and so few tiles of 128 that half of the CUs would have none.  us, few / tiles of 128 (K, N 4096 if not said): one slice, up to 32 rows 15 (the host's
-// time) / 32, 64 17 / 33, 128 32 / 34, 256 62 / 34; two, K 7168, N 2048, 32 rows each 22 / 52; eight of 8 rows, 256 tiles, 45 / 38; 32 of 4, K 2880, N 5760 155 / 115.
-bool few_rows_run(const Fp8GemmParams& p, int64_t slices) { return p.M <= slices * 96 && slices * cdiv(p.N, 128) <= 128; }
+// Whether the kernel for few rows runs: it reads each column's weights once for 64 rows and each row once for 16 columns, and a CU takes about as long for 32 rows as for two workgroups of 16,
+// so what decides is rows (16 for a slice that has fewer) times workgroups of columns.  us, it / the ring / `any` (rows, K, N of one slice; of four numbers: slices first), by that number: 1 4096
+// 4096 (4096) 6.8 / 14.4 / 26; 4 40 560 896 (3584) 4.3 / 5.6 / 7.1; 32 4096 4096 (8192) 11.3 / 14.5 / 30; 2 64 7168 2048 (8192) 21 / 22.6 / 62; 8 8 1024 1024 (8192) 4.7 / 7.1 / 8; 1 4096 14336
+// (14336) 18.7 / 15.1 / 33; 64 4096 4096 (16384) 17 / 14.7 / 35; 8 256 1024 1024 (16384) 10.9 / 6.9 / 11.4; 8 16 2048 2048 (16384) 8.8 / 10.1 / -; 96 4096 4096 (24576) 26 / 15 / 35; 8 16 1024 4096
+// (32768) 9.9 / 7.9 / 11.3; 8 512 1024 1024 (32768) 16 / 7.1 / 11.8; 256 4096 4096 (65536) 62 / 15.4 / 36; 32 128 2880 5760 (184320) 161 / 89 / 114.
+bool few_rows_run(const Fp8GemmParams& p, int64_t slices, bool dma) {
+  const int64_t in_use = slices < p.M ? slices : p.M, rows = p.M > 16 * in_use ? p.M : 16 * in_use;
+  return rows * cdiv(p.N, 16) <= (dma ? 8192 : 24576);
+}
 
-// 256 x 256 tiles (a round of 256 takes 2.5 us a block of K) or 128 x 128 (512: 1.55 us; 256 of them 1.3), whichever has the shorter rounds.  us, 128 / 256: one slice, K, N
-// 4096, 256 rows 34 / 63, 1024 42 / 73, 2048 50 / 76, 4096 91 / 80, 8192 173 / 146; 32 slices, 2880, 2048 rows 83 / 105, 4096 110 / 118, 8192 158 / 172; eight, 2048 rows 40 / 58, 4096
-// 70 / 62; eight of 1024, K 1024, N 2048 41 / 51.
+// Size of the tiles: 64 (the ring), 128 or 256, whichever is expected to take the least time.  A round of tiles (of 64 and 128 two a CU, of 256 one) takes the time of its blocks of K and
+// of a start and an end, in us (fitted to what is measured below).  With up to 16 rows a slice the weights' stream is all that counts, which the ring keeps up best.
+// us, 64 / 128 / 256 (a name of three numbers: rows, K and N of one slice; of four: slices first): 64 4096 4096 14.8 / 32.6 / 58.9; 256 4096 4096 15.8 / 33.6 / 61; 512 4096 4096 21.3 / 38 / 68; 1024 4096 4096 40.1 / 41.2 / 72;
+// 2048 4096 4096 86 / 50 / 76; 4096 4096 4096 - / 91 / 80; 1024 2048 2048 12.9 / 21 / 37; 2048 2048 2048 25.2 / 23.4 / 42; 4096 512 2048 21 / 16 / 20.6; 8 512 1024 1024 7.2 / 14.1 / 22.6; 8 1024 1024 1024 8.6 / 14.3 / 24.2; 8 2048
+// 1024 1024 14 / 14.7 / 24.5; 8 4096 1024 1024 22 / 18.3 / 25.4; 8 800 608 7296 26 / 23.1 / 23; 8 294 640 7312 17.5 / 14.5 / 19.4; 8 64 4096 4096 22.6 / 36.5 / 60; 32 128 2880 5760 90 / 113 / -; 32 512 2880 5760
+// 120 / 131 / 158; 32 1024 2880 5760 148 / 139 / 166; 32 2048 2880 2880 90 / 82 / 104; 32 4096 2880 2880 147 / 110 / 118; 8 4096 2880 2880 - / 70 / 62.
 int tile_size(const Fp8GemmParams& p, int64_t slices) {
-  const int64_t cus = device_cu_count(), small = expected_tiles(p, slices, 128), large = expected_tiles(p, slices, 256);
-  const int64_t by_small = small <= cus ? 130 : cdiv(small, 2 * cus) * 155, by_large = cdiv(large, cus) * 250;
-  return by_small <= by_large ? 128 : 256;
+  if (p.M <= slices * 16) return 64;
+  const int64_t cus = device_cu_count(), n64 = (int64_t)p.grid_m * cdiv(p.N, 64), n128 = expected_tiles(p, slices, 128), n256 = expected_tiles(p, slices, 256);
+  const double blocks = (double)cdiv(p.K, kFp8Block);
+  const double t64 = n64 <= cus ? 0.36 * blocks + 4.3 : (double)cdiv(n64, 2 * cus) * (0.56 * blocks + 3.4);
+  const double t128 = n128 <= cus / 2 ? 0.8 * blocks + 8 : (double)cdiv(n128, 2 * cus) * (1.3 * blocks + 6) + 6;
+  const double t256 = (double)cdiv(n256, cus) * (2.1 * blocks + 6) + 6;
+  return t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
 }
 
 }  // namespace
@@ -170,8 +183,10 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   if (p.grid_m == 0) return TK_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t slices = d->slice_sizes ? d->n_slices : 1;
-  if (few_rows_run(p, slices))
+  const bool dma = fp8_tiles_run(p, d->x_rows, d->y_dtype);
+  if (few_rows_run(p, slices, dma))
     return fp8_gemm_launch_few(p, ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) == 0, d->y_dtype, swiglu, st);
-  if (fp8_tiles_run(p, d->x_rows, d->y_dtype)) return fp8_gemm_launch_tiles(p, tile_size(p, slices), d->y_dtype, swiglu, st);
-  return launch_any(p, d->y_dtype, swiglu, st);
+  if (!dma) return launch_any(p, d->y_dtype, swiglu, st);
+  const int tile = tile_size(p, slices);
+  return tile == 64 || slices > kDmaSlices ? fp8_gemm_launch_ring(p, d->y_dtype, swiglu, st) : fp8_gemm_launch_tiles(p, tile, d->y_dtype, swiglu, st);
 }

@@ -109,9 +109,11 @@ __device__ __forceinline__ void few_rows(const Fp8GemmParams& p, float* sums, in
   }
 }
 
-template <int YT, bool SWIGLU, bool ALIGNED>
-__global__ __launch_bounds__(kFewWaves * 64) void fp8_block_few_kernel(const Fp8GemmParams p) {
-  __shared__ __attribute__((aligned(16))) float sums[kFewWaves * kFewRows * kFewCols];
+// ONE: no slice has more than 16 rows; two workgroups share a CU then (the compiler moves up to 19 of the registers to memory for it, before and after the loop), where
+// the registers for 64 rows allow one
+template <int YT, bool SWIGLU, bool ALIGNED, bool ONE>
+__global__ __launch_bounds__(kFewWaves * 64, ONE ? 4 : 2) void fp8_block_few_kernel(const Fp8GemmParams p) {
+  __shared__ __attribute__((aligned(16))) float sums[kFewWaves * (ONE ? 16 : kFewRows) * kFewCols];
   fp8_zero_rest<YT, SWIGLU>(p);
   const int tile_m = blockIdx.x / p.grid_n, n0 = (blockIdx.x - tile_m * p.grid_n) * kFewCols;
   int expert = 0, off_m = tile_m * kFewRows, start_m = 0, eM = p.M;
@@ -123,12 +125,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_block_few_kernel(const Fp8
   }
   if (off_m >= eM) return;
   const int rows = eM - off_m;
-  if (rows <= 16)
+  if (ONE || rows <= 16)
     few_rows<YT, SWIGLU, ALIGNED, 1>(p, sums, expert, off_m, start_m, eM, n0);
-  else if (rows <= 32)
-    few_rows<YT, SWIGLU, ALIGNED, 2>(p, sums, expert, off_m, start_m, eM, n0);
-  else
-    few_rows<YT, SWIGLU, ALIGNED, 4>(p, sums, expert, off_m, start_m, eM, n0);
+  else if constexpr (!ONE) {
+    if (rows <= 32)
+      few_rows<YT, SWIGLU, ALIGNED, 2>(p, sums, expert, off_m, start_m, eM, n0);
+    else
+      few_rows<YT, SWIGLU, ALIGNED, 4>(p, sums, expert, off_m, start_m, eM, n0);
+  }
 }
 
 }  // namespace
@@ -142,10 +146,14 @@ int32_t fp8_gemm_launch_few(const Fp8GemmParams& q, bool aligned, int yt, bool s
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kFewWaves * 64), 0, st, p);
     return check_launch("fp8_block_few_kernel");
   };
-  auto by_type = [&](auto yt_c) -> int32_t {
+  auto by_rows = [&](auto yt_c, auto swiglu_c, auto aligned_c) -> int32_t {
     constexpr int YT = decltype(yt_c)::value;
-    if (swiglu) return aligned ? go(fp8_block_few_kernel<YT, true, true>) : go(fp8_block_few_kernel<YT, true, false>);
-    return aligned ? go(fp8_block_few_kernel<YT, false, true>) : go(fp8_block_few_kernel<YT, false, false>);
+    constexpr bool SWIGLU = decltype(swiglu_c)::value, ALIGNED = decltype(aligned_c)::value;
+    return p.M <= 16 ? go(fp8_block_few_kernel<YT, SWIGLU, ALIGNED, true>) : go(fp8_block_few_kernel<YT, SWIGLU, ALIGNED, false>);
+  };
+  auto by_type = [&](auto yt_c) -> int32_t {
+    if (swiglu) return aligned ? by_rows(yt_c, std::true_type{}, std::true_type{}) : by_rows(yt_c, std::true_type{}, std::false_type{});
+    return aligned ? by_rows(yt_c, std::false_type{}, std::true_type{}) : by_rows(yt_c, std::false_type{}, std::false_type{});
   };
   return yt == TK_F32 ? by_type(template_int<TK_F32>{}) : yt == TK_BF16 ? by_type(template_int<TK_BF16>{}) : by_type(template_int<TK_F16>{});
 }
