@@ -192,3 +192,38 @@ def test_what_the_entries_refuse():
     assert act(m=0) == nt.TK_OK and act(v=None) == nt.TK_ERR_INVALID and act(o=None) == nt.TK_ERR_INVALID and act(dt=nt.TK_E4M3) == nt.TK_ERR_UNSUPPORTED
     back = lambda **k: lib.tk_swiglu_fp8_backward(*{**dict(d=p, dt=nt.TK_BF16, m=4, n=4, dm=4, v=p, vm=16, s=p, sm=1, sc=1, o=p, om=8, al=1.0, li=0.0, has=0, st=None), **k}.values())  # noqa: E731
     assert back(n=0) == nt.TK_OK and back(s=None) == nt.TK_ERR_INVALID and back(m=-1) == nt.TK_ERR_INVALID and back(dt=nt.TK_U8) == nt.TK_ERR_UNSUPPORTED
+
+
+def test_sizes_beyond_32_bits_and_long_slices_are_refused():
+    lib, p = nt.lib(), 4096
+
+    def gemm(**k):
+        d = nt.Fp8GemmDesc()
+        for name, v in {**dict(x=p, x_rows=4, x_stride_m=128, x_scale=p, w=p, w_stride_e=1024, w_stride_n=128, w_scale=p, n_slices=1, M=4, N=8, K=128, y=p, y_dtype=nt.TK_BF16), **k}.items():
+            setattr(d, name, v)
+        return lib.tk_fp8_block_gemm(d, None)
+
+    for bad in (dict(M=2**31 - 1), dict(N=2**31 - 256 + 1), dict(K=2**31 - 1)):
+        assert gemm(**bad) == nt.TK_ERR_UNSUPPORTED, bad
+    # a schedule counts up to 2^15 row blocks of 64 in a slice: beyond it only the kernels that need none
+    ragged = dict(slice_sizes=p, slice_offs=p, block_schedule=p, grid_m=2**15 + 1, n_slices=2, M=2**21 + 1)
+    for bad in (dict(y_dtype=nt.TK_F32), dict(x=p + 1), dict(w_stride_n=136), dict(K=0), dict(n_slices=300)):
+        assert gemm(**{**ragged, **bad}) == nt.TK_ERR_UNSUPPORTED, bad
+    d = nt.Fp8WgradDesc()
+    for name, v in dict(x=p, x_scale=p, dy=p, dy_dtype=nt.TK_BF16, n_slices=1, T=2**31 - 1, K=8, N=8, y=p, y_dtype=nt.TK_F32).items():
+        setattr(d, name, v)
+    assert lib.tk_fp8_block_wgrad(d, None) == nt.TK_ERR_UNSUPPORTED
+    for name in ("rows", "K", "N"):
+        _raises(NotImplementedError, f"got {name}=2147483648", ops._fit, **{name: 2**31})
+
+
+def test_operands_that_want_a_gradient_are_refused():
+    q, s = torch.ones((4, 256)).to(E4M3), torch.ones((4, 2))
+    w, ws = torch.ones((1, 64, 256)).to(E4M3).transpose(1, 2), torch.ones((1, 2, 1))
+    wants = lambda t: t.clone().requires_grad_()  # noqa: E731
+    _raises(NotImplementedError, "no gradient for a", ops.matmul_fp8_blocks, wants(q), s, w, ws)
+    _raises(NotImplementedError, "no gradient for w", ops.matmul_fp8_blocks, q, s, wants(w), ws)
+    _raises(NotImplementedError, "no gradient for values", ops.upcast_from_fp8_blocks, wants(q), s)
+    _raises(NotImplementedError, "no gradient for x", ops.weight_gradient_fp8_blocks, wants(q), s, torch.ones((4, 8), dtype=BF16))
+    _raises(NotImplementedError, "no gradient for a", ops.swiglu_fp8_forward, torch.ones((4, 8), requires_grad=True), 1.0)
+    _raises(NotImplementedError, "no gradient for dh", ops.swiglu_fp8_backward, torch.ones((4, 128), requires_grad=True), q, s, 1.0)

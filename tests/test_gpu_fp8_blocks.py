@@ -536,3 +536,94 @@ def test_weight_gradients_of_long_slices_in_parts(T, K, N, sizes):
         dw = weight_gradient_fp8_blocks(x, s, dy, md, out_dtype)
         check(dw.view(-1, K, N), *orc.weight_gradient(x[:total], s[:total], dy[:total], sizes, out_dtype), "dw")
         assert torch.equal(weight_gradient_fp8_blocks(x, s, dy, md, out_dtype), dw)
+
+
+@pytest.mark.parametrize("M,K,N,E", [(48, 264, 520, 1), (130, 1000, 1032, 4), (500, 384, 1024, 8), (400, 1048, 640, 280), (2500, 160, 264, 300), (20, 144, 4104, 12)])
+@pytest.mark.parametrize("out_dtype,swiglu", [(BF16, False), (F16, True)])
+def test_products_of_middle_sizes(M, K, N, E, out_dtype, swiglu):
+    g, a, a_scale, w, w_scale = _operands(12, M, K, N, E)
+    sizes = _deal(g, M, E)
+    _check_product(a, a_scale, w, w_scale, out_dtype, sizes, swiglu=swiglu, bias=torch.randn((E, N), generator=g).cuda())
+    at = torch.randint(M, (M, ), generator=g, dtype=torch.int32).cuda()
+    _check_product(a, a_scale, w, w_scale, out_dtype, sizes, swiglu=swiglu, gather=at)
+
+
+@pytest.mark.parametrize("M,E", [(900, 3), (257, 1)])
+def test_many_rows_of_lines_that_begin_anywhere(M, E):
+    K, N = 300, 136
+    g, a, a_scale, w, w_scale = _operands(13, M, K, N, E, 307)
+    odd = torch.full((E, N, K + 3), NAN, device="cuda").to(E4M3)
+    odd[:, :, 1:K + 1] = w.transpose(1, 2)
+    sizes = _deal(g, M, E)
+    y = _check_product(a, a_scale, odd[:, :, 1:K + 1].transpose(1, 2), w_scale, BF16, sizes)
+    assert torch.equal(matmul_fp8_blocks(a.contiguous(), a_scale, w, w_scale, None, _metadata(sizes)), y)
+
+
+def test_a_slice_of_more_rows_than_the_schedule_counts():
+    M, K, N = 2**21 + 300, 16, 16
+    g = _gen(14)
+    a = torch.randint(0, 120, (M, K), generator=g, dtype=torch.uint8).cuda().view(E4M3)
+    a_scale = (torch.rand((M, 1), generator=g) + 0.5).cuda()
+    _, _, _, w, w_scale = _operands(15, 4, K, N, 2)
+    sizes = [M - 100, 60]
+    md = _metadata(sizes, M)
+    y = matmul_fp8_blocks(a, a_scale, w, w_scale, None, md)
+    for lo, hi, e in ((0, 500, 0), (2**21 - 300, M - 100, 0), (M - 100, M - 40, 1)):
+        want, bound, _ = orc.product(a[lo:hi], a_scale[lo:hi], w[e:e + 1], w_scale[e:e + 1])
+        check(y[lo:hi], want, bound, "y")
+    with pytest.raises(NotImplementedError, match="more than 2097152 rows"):
+        matmul_fp8_blocks(a, a_scale, w, w_scale, None, md, out_dtype=F32)
+
+
+def test_linear_without_slices_or_row_blocks():
+    x = _rows(_gen(16), 30, 256)
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)                               # (new memory holds NaN)
+    try:
+        for E in (0, 2):
+            w = torch.ones((E, 256, 64), device="cuda", dtype=BF16)
+            for rows in (0, 30):                                           # (metadata of no rows have no row block)
+                xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+                y = linear_fp8_blocks(xg, wg, _metadata([0] * E, rows))
+                dx, dw = torch.autograd.grad(y, (xg, wg), torch.ones_like(y))
+                assert y.shape == (30, 64) and (y == 0).all() and (dx == 0).all() and (dw == 0).all() and dw.shape == w.shape
+    finally:
+        torch.use_deterministic_algorithms(before)
+
+
+@pytest.mark.parametrize("T,K,N", [(300, 264, 136), (2600, 512, 2056)])
+def test_linear_with_weights_of_other_scales(T, K, N):
+    from triton_kernels.fp8_blocks import Fp8Weight
+    g = _gen(T, K, N)
+    sizes = [T // 2, T - T // 2]
+    md = _metadata(sizes)
+    x, dy = _rows(g, T, K).requires_grad_(), _rows(g, T, N, BF16, 0.01)
+    w = (torch.randn((2, K, N), generator=g) * 0.05).cuda().requires_grad_()
+    q = quantize_fp8_weight(w)
+    q = Fp8Weight(q.values, q.values_n, q.scales * (torch.rand(q.scales.shape, generator=g).cuda() + 0.51))
+    y = linear_fp8_blocks(x, w, md, q)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x8, xs = downcast_to_fp8_blocks(x.detach())
+    d8, ds = downcast_to_fp8_blocks(dy)
+    check(y, *orc.product(x8, xs, q.values, q.scales, sizes)[:2], "y")
+    check(dx, *orc.product(d8, ds, q.values_n.transpose(1, 2), q.scales.transpose(1, 2), sizes)[:2], "dx")
+    check(dw, *orc.weight_gradient(x8, xs, dy, sizes, F32), "dw")
+
+
+@pytest.mark.parametrize("E,T,K,N", [(70, 900, 136, 200), (70, 45000, 16, 40), (129, 3000, 264, 520)])
+def test_weight_gradients_of_many_slices(E, T, K, N):
+    g = _gen(E, T, K, N)
+    sizes = _deal(g, T, E)
+    x, s = downcast_to_fp8_blocks(_rows(g, T, K))
+    dy = _rows(g, T, N, BF16, 0.02)
+    for out_dtype in (F32, BF16):
+        check(weight_gradient_fp8_blocks(x, s, dy, _metadata(sizes), out_dtype), *orc.weight_gradient(x, s, dy, sizes, out_dtype), "dw")
+
+
+def test_gradients_of_one_row_expanded():
+    x = _rows(_gen(17), 40, 256).requires_grad_()
+    w = (torch.randn((256, 64), generator=_gen(18)) * 0.1).cuda().requires_grad_()
+    row = _rows(_gen(19), 1, 64)
+    want = torch.autograd.grad(linear_fp8_blocks(x, w), (x, w), row.expand(40, 64).contiguous())
+    got = torch.autograd.grad(linear_fp8_blocks(x, w), (x, w), row.expand(40, 64))
+    assert all(torch.equal(p, q) for p, q in zip(want, got))

@@ -42,6 +42,7 @@ int32_t fp8_gemm_launch_few(const Fp8GemmParams& p, bool aligned, int yt, bool s
 namespace {
 
 constexpr int kFp8Block = 128;
+constexpr int kFp8Most = 0x7FFFFF00;  // of a size: with a tile more it is still a number of 32 bits
 
 // c + the product of 16 columns of w and 16 rows of x over a block of 128: lane l holds 32 consecutive k, from (l >> 4) * 32 on, of column / row l & 15.  The
 // scales are e8m0 bytes, the exponents of powers of two as fp32 numbers have them.

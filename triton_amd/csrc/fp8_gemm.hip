@@ -100,6 +100,20 @@ int32_t launch_any(Fp8GemmParams p, int yt, bool swiglu, hipStream_t st) {
   return check_launch("fp8_block_any_kernel");
 }
 
+// rows behind the slices alone: a call whose metadata have no row block
+template <int YT, bool SWIGLU>
+__global__ __launch_bounds__(256) void fp8_rest_kernel(const Fp8GemmParams p) {
+  fp8_zero_rest<YT, SWIGLU>(p);
+}
+int32_t launch_rest(const Fp8GemmParams& p, int yt, bool swiglu, hipStream_t st) {
+  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)(p.M < 1024 ? p.M : 1024)), dim3(256), 0, st, p); };
+  if (swiglu)
+    yt == TK_F32 ? launch(fp8_rest_kernel<TK_F32, true>) : yt == TK_BF16 ? launch(fp8_rest_kernel<TK_BF16, true>) : launch(fp8_rest_kernel<TK_F16, true>);
+  else
+    yt == TK_F32 ? launch(fp8_rest_kernel<TK_F32, false>) : yt == TK_BF16 ? launch(fp8_rest_kernel<TK_BF16, false>) : launch(fp8_rest_kernel<TK_F16, false>);
+  return check_launch("fp8_rest_kernel");
+}
+
 // What the kernels with memory-to-LDS transfers need: lines that begin at sixteen-byte boundaries, and offsets within a buffer resource (2 GiB) from the start of a
 // tile, or of x and its scales where rows are gathered.
 bool fp8_tiles_run(Fp8GemmParams& p, int64_t x_rows, int yt) {
@@ -153,6 +167,7 @@ using namespace tk;
 extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stream) {
   if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: null descriptor");
   if (d->M < 0 || d->N < 0 || d->K < 0 || d->n_slices < 0 || d->grid_m < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: negative size");
+  if (d->M > kFp8Most || d->N > kFp8Most || d->K > kFp8Most) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: sizes up to %d (got %d x %d x %d)", kFp8Most, d->M, d->K, d->N);
   if (d->y_dtype != TK_F32 && d->y_dtype != TK_BF16 && d->y_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: the output is fp32, bf16 or fp16 (dtype %d)", d->y_dtype);
   if (d->activation != TK_ACT_NONE && d->activation != TK_ACT_SWIGLU) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: bad activation %d", d->activation);
   const bool swiglu = d->activation == TK_ACT_SWIGLU;
@@ -180,13 +195,18 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   p.y = d->y, p.y_stride_m = d->y_stride_m;
   p.alpha = d->act_alpha, p.limit = d->act_has_limit ? d->act_limit : INFINITY;
   p.zero_rest = d->zero_rest, p.pow2 = d->pow2_scales;
-  if (p.grid_m == 0) return TK_OK;
+  if (p.grid_m == 0) return p.zero_rest ? launch_rest(p, d->y_dtype, swiglu, static_cast<hipStream_t>(stream)) : TK_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t slices = d->slice_sizes ? d->n_slices : 1;
   const bool dma = fp8_tiles_run(p, d->x_rows, d->y_dtype);
+  // A schedule has 15 bits for a row block of 64: a slice that may have more goes by tiles, which need none.
+  const bool long_slices = d->slice_sizes && d->M > (1 << 15) * kAnyRows;
+  if (long_slices && !(dma && slices <= kDmaSlices))
+    return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: more than %d rows in slices need 16-bit results, up to %d slices and operands whose lines begin at sixteen-byte boundaries (got %d rows)",
+                (1 << 15) * kAnyRows, kDmaSlices, d->M);
   if (few_rows_run(p, slices, dma))
     return fp8_gemm_launch_few(p, ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) == 0, d->y_dtype, swiglu, st);
   if (!dma) return launch_any(p, d->y_dtype, swiglu, st);
   const int tile = tile_size(p, slices);
-  return tile == 64 || slices > kDmaSlices ? fp8_gemm_launch_ring(p, d->y_dtype, swiglu, st) : fp8_gemm_launch_tiles(p, tile, d->y_dtype, swiglu, st);
+  return (tile == 64 && !long_slices) || slices > kDmaSlices ? fp8_gemm_launch_ring(p, d->y_dtype, swiglu, st) : fp8_gemm_launch_tiles(p, tile == 256 ? 256 : 128, d->y_dtype, swiglu, st);
 }

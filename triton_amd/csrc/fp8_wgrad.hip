@@ -442,6 +442,7 @@ extern "C" int64_t tk_fp8_block_wgrad_workspace_bytes(int32_t T, int32_t K, int3
 extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t stream) {
   if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null descriptor");
   if (d->T < 0 || d->K < 0 || d->N < 0 || d->n_slices < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: negative size");
+  if (d->T > kFp8Most || d->K > kFp8Most || d->N > kFp8Most) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: sizes up to %d (got %d x %d x %d)", kFp8Most, d->T, d->K, d->N);
   if (d->dy_dtype != TK_BF16 && d->dy_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: dy must be bf16 or fp16 (dtype %d)", d->dy_dtype);
   if (d->y_dtype != TK_F32 && d->y_dtype != TK_BF16 && d->y_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: the gradient is fp32, bf16 or fp16 (dtype %d)", d->y_dtype);
   if (d->slice_sizes ? !d->slice_offs : d->n_slices > 1) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: slices need their sizes and offsets");

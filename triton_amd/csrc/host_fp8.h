@@ -7,7 +7,7 @@
 
 namespace {
 
-constexpr int64_t kFp8 = 128, kFp8Rows = 64;  // a block; the row blocks of the schedule that the product's kernels go by
+constexpr int64_t kFp8 = 128, kFp8Rows = 64, kFp8Most = 0x7FFFFF00;  // a block; the row blocks of the schedule that the product's kernels go by; the most of a size
 int64_t fp8_blocks(int64_t n) { return (n + kFp8 - 1) / kFp8; }
 int64_t fp8_pitch(int64_t n) { return (n + 15) / 16 * 16; }
 bool is_e4m3(const Tensor& t) { return t.scalar_type() == ScalarType::Float8_e4m3fn; }
@@ -56,7 +56,7 @@ PyObject* run_fp8_downcast(PyObject* const* v) {
 PyObject* run_fp8_upcast(PyObject* const* v) {
   const Tensor *q = tensor_of(v[0]), *s = tensor_of(v[1]);
   const long block = PyLong_Check(v[3]) ? PyLong_AsLong(v[3]) : -1;
-  if (!q || !q->is_cuda() || q->dim() != 2 || q->numel() == 0 || q->stride(1) != 1 || !is_e4m3(*q) || !THPDtype_Check(v[2]) || (block != 1 && block != kFp8)) return none();
+  if (!q || !q->is_cuda() || q->dim() != 2 || q->numel() == 0 || q->stride(1) != 1 || !is_e4m3(*q) || wants_grad(*q) || !THPDtype_Check(v[2]) || (block != 1 && block != kFp8)) return none();
   const ScalarType out = reinterpret_cast<THPDtype*>(v[2])->scalar_type;
   const int64_t R = q->size(0), C = q->size(1);
   if ((out != ScalarType::Float && out != ScalarType::BFloat16 && out != ScalarType::Half) || !plain_scales(s, *q, {(R + block - 1) / block, fp8_blocks(C)})) return none();
@@ -108,8 +108,8 @@ bool lines_aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data
 // (a, a scale, w, w scale, bias, metadata, gather, scatter, gammas, activation, output type)
 PyObject* run_fp8_matmul(PyObject* const* v) {
   const Tensor *a = tensor_of(v[0]), *as = tensor_of(v[1]), *w = tensor_of(v[2]), *ws = tensor_of(v[3]), *gather, *scatter, *bias = nullptr, *gammas = nullptr;
-  if (!a || !a->is_cuda() || a->dim() != 2 || !is_e4m3(*a) || a->stride(1) != 1 || a->numel() == 0 || !plain_scales(as, *a, {a->size(0), fp8_blocks(a->size(1))})) return none();
-  if (!w || !on_device_of(*w, *a) || w->dim() != 3 || !is_e4m3(*w) || w->stride(1) != 1 || w->size(1) != a->size(1) || w->numel() == 0) return none();
+  if (!a || !a->is_cuda() || a->dim() != 2 || !is_e4m3(*a) || wants_grad(*a) || a->stride(1) != 1 || a->numel() == 0 || !plain_scales(as, *a, {a->size(0), fp8_blocks(a->size(1))})) return none();
+  if (!w || !on_device_of(*w, *a) || w->dim() != 3 || !is_e4m3(*w) || wants_grad(*w) || w->stride(1) != 1 || w->size(1) != a->size(1) || w->numel() == 0) return none();
   const int64_t E = w->size(0), K = w->size(1), N = w->size(2);
   if (!plain_scales(ws, *a, {E, fp8_blocks(K), fp8_blocks(N)})) return none();
   Activation act;
@@ -129,7 +129,7 @@ PyObject* run_fp8_matmul(PyObject* const* v) {
     gammas = tensor_of(v[8]);
     if (!gammas || !on_device_of(*gammas, *a) || gammas->dim() != 1 || gammas->size(0) != M || !gammas->is_contiguous() || !f32_or_bf16(*gammas) || wants_grad(*gammas) || dual(*gammas)) return none();
   }
-  if (M == 0 || M > 0x7FFFFFFF || (scatter && scatter->size(0) == 0)) return none();
+  if (M == 0 || M > kFp8Most || K > kFp8Most || N > kFp8Most || (scatter && (scatter->size(0) == 0 || scatter->size(0) > kFp8Most))) return none();
   // (many rows of lines that begin anywhere are copied first)
   if (M > E * 256 && ((uint64_t)w->stride(2) % 16 || !lines_aligned(*a))) return none();
   if (dispatcher_heard()) return none();
@@ -223,7 +223,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
       }
       if (ctx->needs_input_grad(1)) {
         Tensor g = dy;
-        if (reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 || g.stride(0) % 8) {  // (lines at sixteen-byte boundaries: a copy costs less than the kernel for any)
+        if (reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 || g.stride(0) % 8 || g.stride(0) < N) {  // (lines of their own at sixteen-byte boundaries: a copy costs less than the kernel for any)
           g = empty_strided({T, N}, {(N + 7) / 8 * 8, 1}, dy.scalar_type(), dy);
           g.copy_(dy);
         }
@@ -256,7 +256,7 @@ PyObject* run_fp8_linear(PyObject* const* v) {
   if (turned && w->stride(-2) != 1) return none();
   LinearFp8 f;
   f.E = w->dim() == 3 ? w->size(0) : 1, f.K = w->size(-2), f.N = w->size(-1);
-  if (!read_slices(v[2], *x, f.E, &f.md) || dispatcher_heard()) return none();
+  if (x->size(0) > kFp8Most || f.K > kFp8Most || f.N > kFp8Most || !read_slices(v[2], *x, f.E, &f.md) || dispatcher_heard()) return none();
   auto stream = stream_of(*x);
   if (!stream) return none();
   if (wants_grad(*x) || wants_grad(*w)) {

@@ -23,6 +23,7 @@ from .tensor_details.ragged_tensor import _BLOCK_SIZES
 FP8_BLOCK = 128
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _E4M3 = torch.float8_e4m3fn
+_MOST = 0x7FFFFF00  # of rows, K and N
 _SCHEDULE = 64  # row blocks of the kernel that goes by the schedule
 
 
@@ -39,7 +40,7 @@ def _no_gradient(who, **tensors):
     if torch.is_grad_enabled():
         for name, t in tensors.items():
             if t is not None and t.requires_grad:
-                raise NotImplementedError(f"{who} has no gradient for {name}: pass it detached, or call linear_fp8_blocks")
+                raise NotImplementedError(f"{who} has no gradient for {name}: pass it detached (linear_fp8_blocks and swiglu_fp8_checkpoint have gradients)")
     check_forward_mode(who, *tensors.values())
 
 
@@ -117,7 +118,7 @@ def upcast_from_fp8_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: to
     want = (*lead[:-1], -(-lead[-1] // block_rows), _blocks(values.shape[-1])) if lead else (_blocks(values.shape[-1]), )
     if tuple(scales.shape) != want or scales.dtype != torch.float32 or scales.device != values.device:
         raise ValueError(f"scales must be fp32 {want} on {values.device} (got {scales.dtype} {tuple(scales.shape)} on {scales.device})")
-    _no_gradient("upcast_from_fp8_blocks", scales=scales)
+    _no_gradient("upcast_from_fp8_blocks", values=values, scales=scales)
     nt.require_gpu(values, "values")
     v3 = _matrices(values, "values")
     s3 = scales.reshape(v3.shape[0], *((1, ) if not lead else ()), *scales.shape[-2:])
@@ -155,15 +156,22 @@ def _check_metadata(md, n_slices, device):
         raise ValueError(f"a_ragged_metadata must live on {device} (got {md.slice_sizes.device})")
 
 
-def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dtype, training):
-    """One launch; operands as checked by the callers, `w [E, K, N]` with K contiguous.  `training`: rows behind the slices become zero, and all scales are the
+def _fit(**sizes):
+    for name, n in sizes.items():
+        if n > _MOST:
+            raise NotImplementedError(f"sizes up to {_MOST} (got {name}={n})")
+
+
+def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dtype, zero_rest=False, pow2=False):
+    """One launch; operands as checked by the callers, `w [E, K, N]` with K contiguous.  `zero_rest`: rows behind the slices become zero; `pow2`: all scales are the
     quantiser's."""
     M = a.shape[0] if gather is None else gather.shape[0]
     K, N = w.shape[1], w.shape[2]
+    _fit(rows=M, K=K, N=N, scatter=0 if scatter is None else scatter.shape[0])
     swiglu = act is not None
     y = torch.empty((scatter.shape[0] if scatter is not None else M, N // 2 if swiglu else N), dtype=out_dtype, device=a.device)
-    if y.numel() == 0 or M == 0:
-        return y
+    if y.numel() == 0 or M == 0 or w.shape[0] == 0:
+        return y.zero_() if zero_rest else y
     d = nt.Fp8GemmDesc()
     d.x, d.x_stride_m, d.x_rows = a.data_ptr(), a.stride(0), a.shape[0]
     d.x_scale, d.xs_stride_m, d.xs_stride_k = a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1)
@@ -187,7 +195,7 @@ def _gemm(a, a_scale, w, w_scale, bias, md, gather, scatter, gammas, act, out_dt
     if swiglu:
         d.activation, d.act_alpha = nt.TK_ACT_SWIGLU, act[0]
         d.act_limit, d.act_has_limit = (act[1], 1) if act[1] is not None else (0.0, 0)
-    d.zero_rest = d.pow2_scales = int(training)
+    d.zero_rest, d.pow2_scales = int(zero_rest), int(pow2)
     nt.submit(nt.lib().tk_fp8_block_gemm, d, a.device)
     return y
 
@@ -231,7 +239,7 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
     y = host.fp8_matmul(a, a_scale, w, w_scale, bias, a_ragged_metadata, gather_indx, scatter_indx, gammas, fused_activation, out_dtype) if host is not None else None
     if y is not None:
         return y
-    _no_gradient("matmul_fp8_blocks", a_scale=a_scale, w_scale=w_scale, bias=bias, gammas=gammas)
+    _no_gradient("matmul_fp8_blocks", a=a, w=w, a_scale=a_scale, w_scale=w_scale, bias=bias, gammas=gammas)
     _type(w, "w", (_E4M3, ))
     a = _operand_rows(a, a_scale)
     if w.ndim == 2:
@@ -279,7 +287,7 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
     if M > 256 * E:
         # (the fast kernels take lines at sixteen-byte boundaries; from about a hundred rows an expert a copy of all weights costs less than the kernel for any lines)
         a, w = _aligned(a, 16), _aligned(w.transpose(1, 2), 16).transpose(1, 2)
-    return _gemm(a, a_scale, w, w_scale, bias, md, gather_indx, scatter_indx, gammas, act, out_dtype, False)
+    return _gemm(a, a_scale, w, w_scale, bias, md, gather_indx, scatter_indx, gammas, act, out_dtype)
 
 
 # ---- the linear layer for training -----------------------------------------------------------------------------------------
@@ -319,7 +327,7 @@ def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch
     """`dw[e] = (x * x_scale)^T dy` over the rows of slice e: `x [T, K]` e4m3 with `x_scale [T, ceil(K / 128)]` as `downcast_to_fp8_blocks` returns them, `dy [T, N]`
     bf16 or fp16; the result `[E, K, N]` (`[K, N]` without metadata) in `out_dtype` (dy's if not given).  fp32 sums; `x * x_scale` is rounded to dy's
     type first, which changes nothing where the scales are powers of two (in fp16: and the product within 65504, its largest number, which it is held to).  A slice without rows has the gradient zero."""
-    _no_gradient("weight_gradient_fp8_blocks", x_scale=x_scale, dy=dy)
+    _no_gradient("weight_gradient_fp8_blocks", x=x, x_scale=x_scale, dy=dy)
     _type(dy, "dy", (torch.bfloat16, torch.float16))
     out_dtype = out_dtype or dy.dtype
     if out_dtype not in DTYPES:
@@ -339,8 +347,10 @@ def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch
 def _weight_gradient(x, x_scale, dy, md, out_dtype, pow2):
     """One launch; operands as checked by the callers.  `pow2`: the scales are the quantiser's."""
     dy = dy if dy.stride(1) == 1 or dy.shape[1] <= 1 else dy.contiguous()
-    x, dy = _aligned(x, 16), _aligned(dy, 8)  # (a copy costs less than the kernel for lines that begin anywhere)
+    # (a copy costs less than the kernel for lines that begin anywhere, or overlap: a row expanded)
+    x, dy = (_aligned(t if t.stride(0) >= t.shape[1] else t.contiguous(), unit) for t, unit in ((x, 16), (dy, 8)))
     (T, K), N, E = x.shape, dy.shape[1], 1 if md is None else md.n_slices
+    _fit(rows=T, K=K, N=N)
     y = torch.empty((E, K, N), dtype=out_dtype, device=x.device)
     d = nt.Fp8WgradDesc()
     d.x, d.x_stride_t, d.x_scale, d.xs_stride_t, d.xs_stride_k = x.data_ptr(), x.stride(0), x_scale.data_ptr(), *x_scale.stride()
@@ -379,11 +389,11 @@ def _like(t):
 class _LinearFp8(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, x, w, values, values_n, scales, md):
+    def forward(ctx, x, w, values, values_n, scales, md, pow2):
         x8, xs = _quantize_rows(x)
-        y = _gemm(x8, xs, values, scales, None, md, None, None, None, None, x.dtype, True)
+        y = _gemm(x8, xs, values, scales, None, md, None, None, None, None, x.dtype, True, pow2)
         ctx.save_for_backward(x8, xs, values_n, scales)
-        ctx.md, ctx.w_shape, ctx.w_dtype = md, w.shape, w.dtype
+        ctx.md, ctx.pow2, ctx.w_shape, ctx.w_dtype = md, pow2, w.shape, w.dtype
         ctx.like = [_like(t) for t in (x8, xs, values_n, scales)]
         return y
 
@@ -397,10 +407,10 @@ class _LinearFp8(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             d8, ds = _quantize_rows(dy)
-            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True)
+            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True, ctx.pow2)
         if ctx.needs_input_grad[1]:
             dw = _weight_gradient(x8, xs, dy, ctx.md, ctx.w_dtype, True).view(ctx.w_shape)
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 def linear_fp8_blocks(x: torch.Tensor, w: torch.Tensor, a_ragged_metadata: Optional[RaggedTensorMetadata] = None, quantized: Optional[Fp8Weight] = None) -> torch.Tensor:
@@ -412,7 +422,7 @@ def linear_fp8_blocks(x: torch.Tensor, w: torch.Tensor, a_ragged_metadata: Optio
 
     `x [rows, K]` is bf16 or fp16, the rows of the slices of `a_ragged_metadata` in order; `w [E, K, N]` (`[K, N]` without metadata) fp32, bf16 or fp16,
     contiguous along either of its last dimensions.  y and dx have x's type, dw has w's.  `quantized` = `quantize_fp8_weight(w)`, for steps that use the same weights several
-    times; without it the call quantises w.  Rows behind the last slice give and receive zeros."""
+    times, or a `Fp8Weight` of other scales (a checkpoint's); without it the call quantises w.  Rows behind the last slice give and receive zeros."""
     host = nt.host() if quantized is None else None
     y = host.fp8_linear(x, w, a_ragged_metadata) if host is not None else None
     if y is not None:
@@ -438,13 +448,14 @@ def linear_fp8_blocks(x: torch.Tensor, w: torch.Tensor, a_ragged_metadata: Optio
                 raise ValueError(f"quantized.{name} must be {dtype} {shape} on {x.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
         if (quantized.values.stride(1) != 1 and K > 1) or (quantized.values_n.stride(2) != 1 and N > 1):
             raise ValueError("quantized must be as quantize_fp8_weight returns it (values contiguous along K, values_n along N)")
+    pow2 = quantized is None  # (nobody vouches for the scales of weights that are handed in)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         check_capture(x, w)
         q = quantize_fp8_weight(w) if quantized is None else quantized
-        return _LinearFp8.apply(x, w, *q, md)
+        return _LinearFp8.apply(x, w, *q, md, pow2)
     q = quantize_fp8_weight(w) if quantized is None else quantized
     x8, xs = _quantize_rows(x.detach())
-    return _gemm(x8, xs, q.values, q.scales, None, md, None, None, None, None, x.dtype, True)
+    return _gemm(x8, xs, q.values, q.scales, None, md, None, None, None, None, x.dtype, True, pow2)
 
 
 # ---- swiglu ----------------------------------------------------------------------------------------------------------------
@@ -466,6 +477,7 @@ def swiglu_fp8_forward(a: torch.Tensor, alpha: float, limit: Optional[float] = N
     """`(h, values, scales)`: swiglu of `a [..., 2n]`, and a's 8-bit copy as `downcast_to_fp8_blocks` makes it, from one pass over a (rows flattened; None unless
     `keep`)."""
     _type(a, "a")
+    _no_gradient("swiglu_fp8_forward", a=a)
     nt.require_gpu(a, "a")
     a2 = _swiglu_rows(a, "a")
     M, C = a2.shape
@@ -484,6 +496,7 @@ def swiglu_fp8_forward(a: torch.Tensor, alpha: float, limit: Optional[float] = N
 def swiglu_fp8_backward(dh: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, alpha: float, limit: Optional[float] = None) -> torch.Tensor:
     """The gradient of a for that of `swiglu_fp8_forward`'s output, at the 8-bit copy of a: `[..., 2n]` in dh's type."""
     _type(dh, "dh")
+    _no_gradient("swiglu_fp8_backward", dh=dh, values=values, scales=scales)
     values = _operand_rows(values, scales, "values")
     M, C = values.shape
     if dh.ndim < 1 or C % 2 or dh.shape[-1] * 2 != C or dh.numel() * 2 != M * C or dh.device != values.device:
