@@ -74,6 +74,12 @@ __device__ __forceinline__ u32x4_t load_piece(const uint8_t* row, int k, int K) 
   if (!row || k >= K) return v;
   if (k + 16 <= K) {
     __builtin_memcpy(&v, row + k, 16);
+  } else if (K >= 16) {  // the row's last sixteen bytes, moved down (byte by byte a row of 1000 took 3 us of its product's 9)
+    uint64_t q[2];
+    __builtin_memcpy(q, row + K - 16, 16);
+    const int drop = 8 * (k + 16 - K);  // 8 .. 120 bits
+    const uint64_t lo = drop < 64 ? q[0] >> drop | q[1] << (64 - drop) : q[1] >> (drop - 64), hi = drop < 64 ? q[1] >> drop : 0;
+    v = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
   } else {
     for (int i = 0; i < K - k; ++i) v[i >> 2] |= (uint32_t)row[k + i] << (i & 3) * 8;
   }

@@ -10,11 +10,14 @@ namespace {
 
 constexpr int kAnyRows = 64, kAnyCols = 64;
 
-// 64 x 64 tiles, four waves of 32 x 32 (two fragments by two); the next block of K is loaded into registers while this one is multiplied from LDS.
+// 64 x 64 tiles, four waves of 32 x 32 (two fragments by two).  A block of K and its scales are asked for into registers a block ahead, and go from there into one of two buffers in LDS; four
+// workgroups share a CU (the sixteen bit form of fp32 results leaves room for three).  us, this / three blocks ahead and two workgroups / one buffer and two barriers: three slices, 700 rows, K 1000, N
+// 1023 10.2 / 10.5 / 14.0; 128 rows, K 4100, N 4096 24 / 25 / 37; 16 slices, 1000 rows, K 1000, N 4099 35 / 41 / 42.
 template <int YT, bool SWIGLU>
-__global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams p) {
-  constexpr int PITCH = kFp8Block + 16;
-  __shared__ __attribute__((aligned(16))) uint8_t xs[kAnyRows * PITCH], ws[kAnyCols * PITCH];
+__global__ __launch_bounds__(256, YT == TK_F32 ? 3 : 4) void fp8_block_any_kernel(const Fp8GemmParams p) {
+  constexpr int PITCH = kFp8Block + 16, OPERAND = 64 * PITCH;
+  static_assert(kAnyRows == 64 && kAnyCols == 64, "lines of an operand");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2 * OPERAND];  // rows, columns
   fp8_zero_rest<YT, SWIGLU>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 15, g = lane >> 4, mw = wave & 1, nw = wave >> 1;
@@ -39,31 +42,41 @@ __global__ __launch_bounds__(256) void fp8_block_any_kernel(const Fp8GemmParams 
   }
   const float* row_scale[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int m = off_m + (j * 2 + mw) * 16 + lr;
-    row_scale[j] = m < eM ? p.xs + (int64_t)(p.gather ? p.gather[start_m + m] : start_m + m) * p.xs_m : nullptr;
+  for (int j = 0; j < 2; ++j) {  // (rows that are not there have the last one's)
+    const int m = off_m + (j * 2 + mw) * 16 + lr, r = start_m + (m < eM ? m : eM - 1);
+    row_scale[j] = p.xs + (int64_t)(p.gather ? p.gather[r] : r) * p.xs_m;
   }
   const int n_wave = n0 + nw * 32;
   const float* col_scale = p.ws + expert * p.ws_e + (int64_t)((n_wave < p.N ? n_wave : 0) / kFp8Block) * p.ws_n;
 
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
   f32x4_t acc[2][2] = {{zero, zero}, {zero, zero}};
+  const int nb = (p.K + kFp8Block - 1) / kFp8Block;
   u32x4_t xr[2], wr[2];
+  float sx[2], sc = 0.f, s[2];
+  auto load = [&](int b) __attribute__((always_inline)) {
+    if (b >= nb) return;
+    const int k = b * kFp8Block + piece;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], piece, p.K), wr[i] = load_piece(w_row[i], piece, p.K);
-  for (int k0 = 0, b = 0; k0 < p.K; k0 += kFp8Block, ++b) {
-    float s[2];
+    for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], k, p.K), wr[i] = load_piece(w_row[i], k, p.K);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s[j] = row_scale[j] ? row_scale[j][b * p.xs_k] * col_scale[b * p.ws_k] : 0.f;
-    __syncthreads();
+    for (int j = 0; j < 2; ++j) sx[j] = row_scale[j][b * p.xs_k];
+    sc = col_scale[b * p.ws_k];
+  };
+  load(0);
+  for (int b = 0; b < nb; ++b) {
+    uint8_t *xs = lds[b & 1], *ws = xs + OPERAND;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       *reinterpret_cast<u32x4_t*>(xs + (line + i * 32) * PITCH + piece) = xr[i];
       *reinterpret_cast<u32x4_t*>(ws + (line + i * 32) * PITCH + piece) = wr[i];
+      s[i] = sx[i] * sc;
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) xr[i] = load_piece(x_row[i], k0 + kFp8Block + piece, p.K), wr[i] = load_piece(w_row[i], k0 + kFp8Block + piece, p.K);
+    load(b + 1);
+    // (one barrier a block: the buffer that is written next is the one that was read before it.  No wait for what is on its way from memory.)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     i32x8_t a[2], c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -134,10 +147,11 @@ int64_t expected_tiles(const Fp8GemmParams& p, int64_t slices, int64_t size) {
 }
 
 // Whether the kernel for few rows runs: it reads each column's weights once for 64 rows and each row once for 16 columns, and a CU takes about as long for 32 rows as for two workgroups of 16,
-// so what decides is rows (16 for a slice that has fewer) times workgroups of columns.  us, it / the ring / `any` (rows, K, N of one slice; of four numbers: slices first), by that number: 1 4096
-// 4096 (4096) 6.8 / 14.4 / 26; 4 40 560 896 (3584) 4.3 / 5.6 / 7.1; 32 4096 4096 (8192) 11.3 / 14.5 / 30; 2 64 7168 2048 (8192) 21 / 22.6 / 62; 8 8 1024 1024 (8192) 4.7 / 7.1 / 8; 1 4096 14336
-// (14336) 18.7 / 15.1 / 33; 64 4096 4096 (16384) 17 / 14.7 / 35; 8 256 1024 1024 (16384) 10.9 / 6.9 / 11.4; 8 16 2048 2048 (16384) 8.8 / 10.1 / -; 96 4096 4096 (24576) 26 / 15 / 35; 8 16 1024 4096
-// (32768) 9.9 / 7.9 / 11.3; 8 512 1024 1024 (32768) 16 / 7.1 / 11.8; 256 4096 4096 (65536) 62 / 15.4 / 36; 32 128 2880 5760 (184320) 161 / 89 / 114.
+// so what decides is rows (16 for a slice that has fewer) times workgroups of columns (in brackets).  us (three numbers: rows, K, N of one slice; four: slices first),
+// it / the ring: 1 4096 4096 (4096) 6.8 / 14.4; 4 40 560 896 (3584) 4.3 / 5.6; 32 4096 4096 (8192) 11.3 / 14.5; 2 64 7168 2048 (8192) 21 / 22.6; 8 8 1024 1024 (8192) 4.7 / 7.1; 1 4096 14336 (14336)
+// 18.7 / 15.1; 64 4096 4096 (16384) 17 / 14.7; 8 256 1024 1024 (16384) 10.9 / 6.9; 8 16 2048 2048 (16384) 8.8 / 10.1; 8 16 1024 4096 (32768) 9.9 / 7.9; 256 4096 4096 (65536) 62 / 15.4;
+// it / `any`: 1 4100 4096 (4096) 8.1 / 23; 16 4100 16384 (16384) 22.5 / 24.8; 8 256 1000 1023 (16384) 9.8 / 10.1; 3 300 1000 1023 (19200) 9.8 / 10.2; 96 4100 4096 (24576) 23 / 25; 8 16 1000 4096 (32768)
+// 12.5 / 10.3; 128 4100 4096 (32768) 27.9 / 25.4; 3 700 1000 1023 (44800) 15.6 / 10.5.
 bool few_rows_run(const Fp8GemmParams& p, int64_t slices, bool dma) {
   const int64_t in_use = slices < p.M ? slices : p.M, rows = p.M > 16 * in_use ? p.M : 16 * in_use;
   return rows * cdiv(p.N, 16) <= (dma ? 8192 : 24576);
