@@ -8,8 +8,9 @@
 //   * Scales that are powers of two (a caller that had both operands quantised here says so) go into the matrix instruction as exponents, and it adds
 //     to the running sum itself.
 //   * The scales of a stage (one a row, one or two for the columns) come by transfers of four bytes a lane beside the operands.
-//   * A stage's columns are in registers from the end of the one before, so a second barrier in its middle frees their buffer and the transfers of the stage after
-//     next begin there; those of the rows follow behind the stage's last reads.
+//   * A stage's columns are in registers from the end of the one before, so a second barrier frees their buffer and the transfers of the stage after next begin there; those of the rows
+//     follow behind the stage's last reads.  The barrier stands in the stage's middle for tiles of 256, at its start for tiles of 128, whose stages are short beside a transfer's way (us, start /
+//     middle: 32 experts, 4096 rows, 2880 x 2880 108 / 113; 2048 rows 76 / 81; tiles of 256: one of 8192 rows, 8192 x 8192 608 / 575).
 //   * Transfers, the order of 16-byte pieces in LDS, the list of tiles and the run across tiles are those of moe_gemm_dma_kernel.h.
 //   * K that is no multiple of 16: the last piece of a row holds bytes of whatever follows; they are cleared in LDS before the last stage is read.
 #include "fp8_blocks.h"
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
 
   // A stage; its columns and its first row fragment are in registers.
   auto stage = [&](bool next_has_tail) __attribute__((always_inline)) {
-    constexpr int MID = MFW / 2 - 1, ALL = MFW * NFW, SKEW = 3;  // (up to NFW - 1: a result's registers are taken again NFW products later)
+    constexpr int MID = TILE == 128 ? 0 : MFW / 2 - 1, ALL = MFW * NFW, SKEW = 3;  // (up to NFW - 1: a result's registers are taken again NFW products later)
     float s[2];
     auto add = [&](auto t_c) __attribute__((always_inline)) {  // product T's sums, times the scales
       constexpr int T = decltype(t_c)::value, J = T / NFW, F = T % NFW;
@@ -195,6 +196,7 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
         barrier();
         if (next_has_tail) clear_tail(b ^ 1);
       }
+      if constexpr (T == 0 && MID == 0) barrier();  // every wave has this stage's columns in registers
       if constexpr (F == 0) s[J & 1] = sx[J & 1] * sc;
       if constexpr (POW2)
         acc[F][J] = mfma_block(w[F], x[J & 1], acc[F][J], f32_bits(sc) >> 23, f32_bits(sx[J & 1]) >> 23);
@@ -214,8 +216,8 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
         if constexpr (F == NFW - 1) fetch_s();
       }
       if constexpr (J == MID) {
-        if constexpr (F == 0) {
-          // every wave has this stage's columns in registers
+        if constexpr (F == 0 && MID > 0) {
+          // every wave has this stage's columns in registers (and multiplied by them)
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
