@@ -4,6 +4,7 @@
 //     sums are joined in LDS in the waves' order.  So a single row spreads 4096 columns over 256 workgroups, and a wave has all of its share of K = 4096 in flight at once.
 //   * Operands go from memory into registers as the matrix instruction wants them: a lane's 32 consecutive k of one column are a quarter of a cache line, and four
 //     lanes have the whole.
+//   * us: one row, 4096 x 4096 6.8 (2.5 TB/s of weights; an empty kernel takes 2), eight experts of a row, 1024 x 1024 4.7.
 #include "fp8_blocks.h"
 
 namespace tk {

@@ -6,6 +6,8 @@
 //     LDS behind the products of the one before.  One barrier a stage: behind it the next stage has landed and this one has been read, so its buffer is filled again.
 //   * Each wave makes the same number of transfers a stage (two of rows, two of columns, one of scales), so that one count of those in flight holds for all.
 //   * Row blocks of a slice that share columns run next to each other on one XCD.
+//   * us: one slice of 64 to 256 rows, 4096 x 4096 15 (weights at 1.1 TB/s: 64 workgroups' chain of 32 stages); 32 experts, 128 rows, K 2880, N 5760 with swiglu 89 (6 TB/s: HBM and the last-level
+//     cache); eight, 512 rows, 1024 x 1024 7.1.
 #include "fp8_blocks.h"
 #include "gemm_tiles.h"
 

