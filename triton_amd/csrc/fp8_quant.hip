@@ -1,8 +1,8 @@
 // e4m3 with one fp32 scale for each block of 128: writing it (rows, with swiglu in front where asked for, and 128 x 128 blocks), reading it back, and the
 // backward pass of swiglu from it.
 //
-// HBM bounds all of it: a pass over the data, eight consecutive elements a lane.  us: 16384 x 4096 bf16 written and read back 79 (5.1 TB/s, as a copy), eight matrices of 2880 x 5760 in both orders 111
-// (4.8), swiglu of 16384 x 11520 with its 8-bit copy 166 and its gradient 154 (4.7 together).
+// HBM bounds all of it: a pass over the data, eight consecutive elements a lane.  us: 16384 x 4096 bf16 written and read back 73 (5.5 TB/s; a copy of 1 GiB 5.0), eight matrices of 2880 x 5760 in both orders 111
+// (4.8), swiglu of 16384 x 11520 with its 8-bit copy and its gradient 291 (5.2).
 #include "fp8_blocks.h"
 
 namespace tk {
@@ -258,8 +258,10 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const RowsParams p, uint8
 }
 
 bool is_float(int dtype) { return dtype == TK_F32 || dtype == TK_BF16 || dtype == TK_F16; }
+// Workgroups, sixteen blocks a turn.  Eight times as many as a CU has room for: those that run have work side by side in memory, and few turns each.  us, 8 a CU / 16 / 64 / one turn each: 16384 x 11520
+// bf16 quantised 127 / 120 / 114 / 131, read back 110 / 109 / 101 / 108, swiglu's gradient 173 / 166 / 153 / 167; 16384 x 4096 fp32 read back 98 / 91 / 79 / 64.
 unsigned groups_grid(int64_t groups) {
-  const int64_t n = cdiv(groups, 16), most = (int64_t)device_cu_count() * 8;
+  const int64_t n = cdiv(groups, 16), most = (int64_t)device_cu_count() * 64;
   return (unsigned)(n < most ? n : most);
 }
 
