@@ -627,3 +627,27 @@ def test_gradients_of_one_row_expanded():
     want = torch.autograd.grad(linear_fp8_blocks(x, w), (x, w), row.expand(40, 64).contiguous())
     got = torch.autograd.grad(linear_fp8_blocks(x, w), (x, w), row.expand(40, 64))
     assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def test_offsets_past_32_bits():
+    R, K, N = 2**20 + 70_000, 4096, 64                                     # 4.6 GB in 8 bits
+    at = torch.tensor([0, 1, R // 2, 2**19 + 1, 2**20 + 3] + list(range(R - 60, R)), device="cuda")
+    a = torch.randint(0, 120, (R, K), dtype=torch.uint8, device="cuda").view(E4M3)
+    a_scale = torch.ldexp(torch.ones((), device="cuda"), torch.randint(-6, 6, (R, K // 128), device="cuda"))
+    _, _, _, w, w_scale = _operands(20, 4, K, N)
+    rows, scales = a.view(torch.uint8)[at].view(E4M3), a_scale[at]
+    for out_dtype in (BF16, F32):
+        want, bound, _ = orc.product(rows, scales, w, w_scale, out_dtype=out_dtype)
+        check(matmul_fp8_blocks(a, a_scale, w, w_scale, out_dtype=out_dtype)[at], want, bound, "y")
+        check(matmul_fp8_blocks(a, a_scale, w, w_scale, gather_indx=at.int(), out_dtype=out_dtype), want, bound, "gathered")
+    dy = torch.zeros((R, N), dtype=BF16, device="cuda")
+    dy[at] = _rows(_gen(21), len(at), N, BF16, 0.1)
+    check(weight_gradient_fp8_blocks(a, a_scale, dy, None, F32)[None], *orc.weight_gradient(rows, scales, dy[at]), "dw")
+    x = upcast_from_fp8_blocks(a, a_scale)
+    assert torch.equal(x[at].cpu(), orc.upcast(rows, scales).to(BF16))
+    v, s = downcast_to_fp8_blocks(x)
+    _same(v.view(torch.uint8)[at].view(E4M3), s[at], orc.downcast(x[at]))
+    h, v2, s2 = swiglu_fp8_forward(x, *ACT)
+    check(h[at], *orc.swiglu(x[at], *ACT), "h")
+    assert torch.equal(v2.view(torch.uint8), v.view(torch.uint8)) and torch.equal(s2, s)
+    check(swiglu_fp8_backward(h, v, s, *ACT)[at], *orc.swiglu_backward(h[at], v.view(torch.uint8)[at].view(E4M3), s[at], *ACT), "da")
