@@ -651,3 +651,17 @@ def test_offsets_past_32_bits():
     check(h[at], *orc.swiglu(x[at], *ACT), "h")
     assert torch.equal(v2.view(torch.uint8), v.view(torch.uint8)) and torch.equal(s2, s)
     check(swiglu_fp8_backward(h, v, s, *ACT)[at], *orc.swiglu_backward(h[at], v.view(torch.uint8)[at].view(E4M3), s[at], *ACT), "da")
+
+
+@pytest.mark.parametrize("M,K,N,E", [(70, 2057, 136, 1), (300, 2100, 520, 3), (40, 2176, 264, 1), (130, 4000, 1024, 2), (64, 2048, 16, 1), (97, 6150, 72, 2)])
+@pytest.mark.parametrize("out_dtype,swiglu", [(BF16, True), (F16, False)])
+def test_products_of_few_columns_and_long_rows(M, K, N, E, out_dtype, swiglu):
+    g, a, a_scale, w, w_scale = _operands(22, M, K, N, E)
+    wide = torch.full((E, N, -(-K // 16) * 16), NAN, device="cuda").to(E4M3)  # lines at sixteen-byte boundaries, NaN behind their ends
+    wide[:, :, :K] = w.transpose(1, 2)
+    a2 = torch.full((M, wide.shape[2]), NAN, device="cuda").to(E4M3)
+    a2[:, :K] = a
+    sizes = _deal(g, M, E)
+    y = _check_product(a2[:, :K], a_scale, wide[:, :, :K].transpose(1, 2), w_scale, out_dtype, sizes, swiglu=swiglu)
+    at = torch.arange(M, dtype=torch.int32, device="cuda")
+    assert torch.equal(_check_product(a2[:, :K], a_scale, wide[:, :, :K].transpose(1, 2), w_scale, out_dtype, sizes, swiglu=swiglu, gather=at), y)

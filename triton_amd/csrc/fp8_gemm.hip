@@ -148,18 +148,18 @@ int64_t expected_tiles(const Fp8GemmParams& p, int64_t slices, int64_t size) {
 
 // Whether the kernel for few rows runs: it reads each column's weights once for 64 rows and each row once for 16 columns, and a CU takes about as long for 32 rows as for two workgroups of 16,
 // so what decides is rows (16 for a slice that has fewer) times workgroups of columns (in brackets).  us (three numbers: rows, K, N of one slice; four: slices first),
-// it / the ring: 1 4096 4096 (4096) 6.8 / 14.4; 4 40 560 896 (3584) 4.3 / 5.6; 32 4096 4096 (8192) 11.3 / 14.5; 2 64 7168 2048 (8192) 21 / 22.6; 8 8 1024 1024 (8192) 4.7 / 7.1; 1 4096 14336 (14336)
-// 18.7 / 15.1; 64 4096 4096 (16384) 17 / 14.7; 8 256 1024 1024 (16384) 10.9 / 6.9; 8 16 2048 2048 (16384) 8.8 / 10.1; 8 16 1024 4096 (32768) 9.9 / 7.9; 256 4096 4096 (65536) 62 / 15.4;
+// it / the ring (which runs beyond 32 rows a slice in any case): 1 4096 4096 (4096) 6.8 / 12.5; 4 40 560 896 (3584) 4.3 / 5.6; 32 4096 4096 (8192) 11.3 / 12.8; 1 4096 8192 (8192) 10.9 / 12.7; 2 64 7168 2048 (8192) 20.8 / 19.1; 512 16384 256 (8192) 53 / 36; 8 8 1024 1024 (8192) 4.7 / 7.1; 1 4096 14336 (14336)
+// 18.7 / 13.8; 64 4096 4096 (16384) 17 / 12.9; 8 256 1024 1024 (16384) 10.9 / 6.9; 8 16 2048 2048 (16384) 8.8 / 9.0; 8 16 1024 4096 (32768) 9.9 / 7.9; 256 4096 4096 (65536) 62 / 14.3;
 // it / `any`: 1 4100 4096 (4096) 8.1 / 23; 16 4100 16384 (16384) 22.5 / 24.8; 8 256 1000 1023 (16384) 9.8 / 10.1; 3 300 1000 1023 (19200) 9.8 / 10.2; 96 4100 4096 (24576) 23 / 25; 8 16 1000 4096 (32768)
 // 12.5 / 10.3; 128 4100 4096 (32768) 27.9 / 25.4; 3 700 1000 1023 (44800) 15.6 / 10.5.
 bool few_rows_run(const Fp8GemmParams& p, int64_t slices, bool dma) {
   const int64_t in_use = slices < p.M ? slices : p.M, rows = p.M > 16 * in_use ? p.M : 16 * in_use;
-  return rows * cdiv(p.N, 16) <= (dma ? 8192 : 24576);
+  return dma ? p.M <= 32 * in_use && rows * cdiv(p.N, 16) <= 8192 : rows * cdiv(p.N, 16) <= 24576;
 }
 
 // Size of the tiles: 64 (the ring), 128 or 256, whichever is expected to take the least time.  A round of tiles (of 64 and 128 two a CU, of 256 one) takes the time of its blocks of K and
 // of a start and an end, in us (fitted to what is measured below).  With up to 16 rows a slice the weights' stream is all that counts, which the ring keeps up best.
-// us, 64 / 128 / 256 (a name of three numbers: rows, K and N of one slice; of four: slices first): 64 4096 4096 14.8 / 32.6 / 58.9; 256 4096 4096 15.8 / 33.6 / 61; 512 4096 4096 21.3 / 38 / 68; 1024 4096 4096 40.1 / 41.2 / 72;
+// us, 64 / 128 / 256 (a name of three numbers: rows, K and N of one slice; of four: slices first): 64 4096 4096 12.9 / 32.6 / 58.9; 256 4096 4096 14.3 / 33.6 / 61; 512 4096 4096 21.3 / 38 / 68; 1024 4096 4096 40.1 / 41.2 / 72;
 // 2048 4096 4096 86 / 50 / 76; 4096 4096 4096 - / 91 / 80; 1024 2048 2048 12.9 / 21 / 37; 2048 2048 2048 25.2 / 23.4 / 42; 4096 512 2048 21 / 16 / 20.6; 8 512 1024 1024 7.2 / 14.1 / 22.6; 8 1024 1024 1024 8.6 / 14.3 / 24.2; 8 2048
 // 1024 1024 14 / 14.7 / 24.5; 8 4096 1024 1024 22 / 18.3 / 25.4; 8 800 608 7296 26 / 23.1 / 23; 8 294 640 7312 17.5 / 14.5 / 19.4; 8 64 4096 4096 22.6 / 36.5 / 60; 32 128 2880 5760 90 / 113 / -; 32 512 2880 5760
 // 120 / 131 / 158; 32 1024 2880 5760 148 / 139 / 166; 32 2048 2880 2880 90 / 82 / 104; 32 4096 2880 2880 147 / 110 / 118; 8 4096 2880 2880 - / 70 / 62.

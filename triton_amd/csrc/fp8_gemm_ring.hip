@@ -4,9 +4,10 @@
 //     LDS, three on their way while the next one is read from it, and two workgroups share a CU.  (Eight stages and one workgroup: no change.)
 //   * Four waves of 32 x 32, four products of 16 x 16 each a stage, added to the running sums times the scales as in the kernel for large tiles.  A stage's operands are read from
 //     LDS behind the products of the one before.  One barrier a stage: behind it the next stage has landed and this one has been read, so its buffer is filled again.
+//   * Where there is a workgroup a CU at most and K is long, a workgroup has two such groups of four waves with a ring each, which take every other block of K.
 //   * Each wave makes the same number of transfers a stage (two of rows, two of columns, one of scales), so that one count of those in flight holds for all.
 //   * Row blocks of a slice that share columns run next to each other on one XCD.
-//   * us: one slice of 64 to 256 rows, 4096 x 4096 15 (weights at 1.1 TB/s: 64 workgroups' chain of 32 stages); 32 experts, 128 rows, K 2880, N 5760 with swiglu 89 (6 TB/s: HBM and the last-level
+//   * us: one slice of 64 to 256 rows, 4096 x 4096 13 to 14 (64 to 256 workgroups that each take in 50 GB/s, as a CU does however its stages are cut); 32 experts, 128 rows, K 2880, N 5760 with swiglu 89 (6 TB/s: HBM and the last-level
 //     cache); eight, 512 rows, 1024 x 1024 7.1.
 #include "fp8_blocks.h"
 #include "gemm_tiles.h"
@@ -18,8 +19,9 @@ constexpr int kRingTile = 64, kRingOperand = kRingTile * kFp8Block, kRingScales 
 constexpr int kRing = 4, kRingLds = kRing * kRingStage, kRingTransfers = 5;  // stages; transfers of a wave and stage
 static_assert(kRingLds <= 80 * 1024, "two workgroups of a CU");
 
-template <int YT, bool SWIGLU>
-__global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmParams p) {
+// KG groups of four waves: a stage is KG blocks of K, one for each group, and their sums are joined in the groups' order.
+template <int YT, bool SWIGLU, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void fp8_block_ring_kernel(const Fp8GemmParams p) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   fp8_zero_rest<YT, SWIGLU>(p);
   const int id = xcd_remap((int)blockIdx.x, (int)gridDim.x);
@@ -33,10 +35,10 @@ __global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmPar
   }
   if (off_m >= eM) return;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, g4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 8);
   const int mw = wave & 1, nw = wave >> 1;
-  const int nst = (p.K + kFp8Block - 1) / kFp8Block, tail = p.K & 15;
-  const uint32_t lds0 = lds_addr(lds);
+  const int nb = (p.K + kFp8Block - 1) / kFp8Block, nst = (nb + KG - 1) / KG, tail = p.K & 15;
+  const uint32_t mine = (uint32_t)group * kRingLds, lds0 = lds_addr(lds) + mine;
   const int rows = eM - off_m < kRingTile ? eM - off_m : kRingTile, cols = p.N - n0 < kRingTile ? p.N - n0 : kRingTile, first = start_m + off_m;
 
   // ---- transfers: eight lines each, as in the kernel for large tiles (lane -> line lane / 8, piece (lane % 8) ^ (line >> 1 & 7)) ------------------------------
@@ -65,14 +67,14 @@ __global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmPar
   }
   auto fetch = [&](int s) __attribute__((always_inline)) {
     const uint32_t at = lds0 + (uint32_t)(s % kRing) * kRingStage;
-    const int k = s * kFp8Block;
+    const int k = (s * KG + group) * kFp8Block;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool in = k + pc[i] * 16 < p.K;  // (none behind the last stage)
+      const bool in = k + pc[i] * 16 < p.K;  // (none behind the last block)
       lds_dma16(wdesc, at + kRingOperand + (wave * 2 + i) * 1024, in ? w_off[i] + (uint32_t)k : kOutOfRange);
       lds_dma16(xdesc, at + (wave * 2 + i) * 1024, in ? x_off[i] + (uint32_t)k : kOutOfRange);
     }
-    lds_dma4(sdesc, at + 2 * kRingOperand + (wave & 1) * 256, k < p.K ? s_off + (uint32_t)s * s_step : kOutOfRange);
+    lds_dma4(sdesc, at + 2 * kRingOperand + (wave & 1) * 256, k < p.K ? s_off + (uint32_t)(s * KG + group) * s_step : kOutOfRange);
   };
 
   // ---- LDS read side --------------------------------------------------------------------------------------------------------------------------------------
@@ -87,8 +89,9 @@ __global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmPar
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // clears what the last piece of each line of a stage holds past K
+  // clears what the last piece of each line of the last block holds past K
   auto clear_tail = [&](uint32_t at) __attribute__((always_inline)) {
+    at += (uint32_t)((nb - 1) % KG) * kRingLds;
     if (tid < 2 * kRingTile) {
       const int l = tid & 63, piece = ((p.K % kFp8Block) >> 4) ^ ((l >> 1) & 7);
       uint8_t* last = lds + at + (tid >> 6) * kRingOperand + l * 128 + piece * 16;
@@ -105,7 +108,7 @@ __global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmPar
   i32x8_t w[2], x[2];
   float sx[2], sc;
   auto read = [&](int s) __attribute__((always_inline)) {
-    const uint32_t at = (uint32_t)(s % kRing) * kRingStage;
+    const uint32_t at = mine + (uint32_t)(s % kRing) * kRingStage;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       w[i] = frag(at + kRingOperand + (uint32_t)((nw * 2 + i) * 2048));
@@ -148,6 +151,20 @@ __global__ __launch_bounds__(256, 2) void fp8_block_ring_kernel(const Fp8GemmPar
         for (int i = 0; i < 4; ++i) acc[f][j][i] = fmaf(part[f][j][i], scale[j], acc[f][j][i]);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last transfers write into this workgroup's LDS)
+  if constexpr (KG > 1) {
+    barrier();
+    f32x4_t* sums = reinterpret_cast<f32x4_t*>(lds) + (tid & 255);
+    if (group > 0) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f) sums[((group - 1) * 4 + f) * 256] = acc[f >> 1][f & 1];
+    }
+    barrier();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[f >> 1][f & 1] += sums[(g * 4 + f) * 256];
+  }
   fp8_epilogue<YT, SWIGLU, 2, 2, 2>(p, acc, expert, off_m, start_m, eM, n0 + nw * 32, p.N, mw, lane);
 }
 
@@ -158,13 +175,21 @@ int32_t fp8_gemm_launch_ring(const Fp8GemmParams& q, int yt, bool swiglu, hipStr
   p.grid_n = (int)cdiv(p.N, kRingTile);
   const int64_t grid = (int64_t)p.grid_m * p.grid_n;
   if (grid > 0x7FFFFFFF) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: grid too large");
-  auto go = [&](auto kern) -> int32_t {
-    if (const int32_t rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), kRingLds)) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), kRingLds, st, p);
+  // A workgroup a CU at most, and long chains of stages: two groups.  us, two / one: 64 rows, 4096 x 4096 12.9 / 14.8; 256 rows 14.3 / 15.7; 512 rows, 2048 x 2048 9.8 / 10.1; K 16384, N 256 36 / 46; but
+  // eight slices, 256 rows, 1024 x 1024 7.1 / 6.9; 2048 rows, 512 x 512 6.3 / 5.8.
+  const int groups = grid <= device_cu_count() && p.K >= 16 * kFp8Block ? 2 : 1;
+  auto go = [&](auto kern, int groups) -> int32_t {
+    if (const int32_t rc = allow_dynamic_lds(reinterpret_cast<const void*>(kern), groups * kRingLds)) return rc;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256 * groups), groups * kRingLds, st, p);
     return check_launch("fp8_block_ring_kernel");
   };
-  if (yt == TK_BF16) return swiglu ? go(fp8_block_ring_kernel<TK_BF16, true>) : go(fp8_block_ring_kernel<TK_BF16, false>);
-  return swiglu ? go(fp8_block_ring_kernel<TK_F16, true>) : go(fp8_block_ring_kernel<TK_F16, false>);
+  auto by_groups = [&](auto yt_c, auto swiglu_c) -> int32_t {
+    constexpr int YT = decltype(yt_c)::value;
+    constexpr bool SWIGLU = decltype(swiglu_c)::value;
+    return groups == 2 ? go(fp8_block_ring_kernel<YT, SWIGLU, 2>, 2) : go(fp8_block_ring_kernel<YT, SWIGLU, 1>, 1);
+  };
+  if (yt == TK_BF16) return swiglu ? by_groups(template_int<TK_BF16>{}, std::true_type{}) : by_groups(template_int<TK_BF16>{}, std::false_type{});
+  return swiglu ? by_groups(template_int<TK_F16>{}, std::true_type{}) : by_groups(template_int<TK_F16>{}, std::false_type{});
 }
 
 }  // namespace tk
