@@ -1,0 +1,58 @@
+"""Calls of the experts in 8 bits as programs make them: hooks that change what the backward pass was to read."""
+import pytest
+import torch
+
+from oracle import fp8_blocks as orc
+from oracle.rows import check
+from triton_amd import _native as nt
+from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks
+from triton_kernels.tensor import make_ragged_tensor_metadata
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def _both(monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(nt, "host", lambda: None)
+
+
+def _rows(g, R, C, dtype=BF16, scale=1.0):
+    return (torch.randn((R, C), generator=g) * (torch.rand((R, 1), generator=g) * 2 + 0.1) * scale).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N", [(40, 200, 72), (2300, 4104, 264)])       # (the second one's input gradient goes by tiles of 256)
+def test_scales_that_a_hook_gives_back_count_whole(T, K, N, dtype, native, monkeypatch):
+    _both(monkeypatch, native)
+    g = torch.Generator().manual_seed(T)
+    x = _rows(g, T, K, dtype).requires_grad_()
+    w = (torch.randn((1, K, N), generator=g) * 0.05).cuda().requires_grad_()
+    dy = _rows(g, T, N, dtype, 0.01)
+    md = make_ragged_tensor_metadata(torch.tensor([T], dtype=torch.int32, device="cuda"), T)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t * 1.25 if t.dtype == F32 else t):  # (the scales alone are fp32; three more bits)
+        y = linear_fp8_blocks(x, w, md)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x8, xs = downcast_to_fp8_blocks(x.detach())
+    w8, ws = downcast_to_fp8_blocks(w.detach(), 128)
+    d8, ds = downcast_to_fp8_blocks(dy)
+    some = torch.arange(0, T, max(1, T // 40), device="cuda")
+    check(dx[some], *orc.product(d8.view(torch.uint8)[some].view(E4M3), ds[some], w8.transpose(1, 2), ws.transpose(1, 2) * 1.25, out_dtype=dtype)[:2], "dx")
+    check(dw, *orc.weight_gradient(x8, xs * 1.25, dy), "dw")
+
+
+def test_scales_that_a_hook_of_one_node_gives_back_count_whole(monkeypatch):
+    """Hooks on the saved tensors of a node that Python has (weights that were handed in)."""
+    from triton_kernels.fp8_blocks import quantize_fp8_weight
+    g = torch.Generator().manual_seed(1)
+    x = _rows(g, 40, 200).requires_grad_()
+    w = (torch.randn((200, 72), generator=g) * 0.05).cuda().requires_grad_()
+    dy = _rows(g, 40, 72, BF16, 0.01)
+    y = linear_fp8_blocks(x, w, quantized=quantize_fp8_weight(w))
+    for saved in y.grad_fn._raw_saved_tensors:
+        saved.register_hooks(lambda t: t, lambda t: t * 1.25 if t.dtype == F32 else t)
+    dw, = torch.autograd.grad(y, w, dy)
+    x8, xs = downcast_to_fp8_blocks(x.detach())
+    check(dw[None], *orc.weight_gradient(x8, xs * 1.25, dy), "dw")

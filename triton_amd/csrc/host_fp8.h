@@ -4,6 +4,7 @@
 // What bounds it: in Python a product took 15 us, the quantiser with its inverse 30, a step of swiglu 113 and one of the linear layer 220, at sizes whose kernels take
 // 2 to 30.
 #pragma once
+#include <ATen/SavedTensorHooks.h>
 
 namespace {
 
@@ -190,7 +191,9 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
     if (sizes) f.md = {*sizes, *offs, *schedule};
     launch([&] { return f.forward(reinterpret_cast<void*>(stream)); });
     ctx->save_for_backward({f.x8.v, f.x8.s, f.n_first, f.scales, f.md.sizes, f.md.offs, f.md.schedule});
-    ctx->saved_data["dims"] = std::vector<int64_t>{f.E, f.K, f.N, w.dim(), (int64_t)w.scalar_type(), turned ? 1 : 0};
+    // (what hooks give back for the scales need not be the quantiser's: the backward pass takes those as any)
+    const bool hooked = !at::SavedTensorDefaultHooks::get_tls_state().stack.empty();
+    ctx->saved_data["dims"] = std::vector<int64_t>{f.E, f.K, f.N, w.dim(), (int64_t)w.scalar_type(), turned ? 1 : 0, hooked ? 0 : 1};
     return f.y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -198,6 +201,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
     const auto dims = ctx->saved_data["dims"].toIntVector();
     const int64_t E = dims[0], K = dims[1], N = dims[2], T = grads[0].size(0);
     const bool turned = dims[5] != 0;
+    const int32_t pow2 = (int32_t)dims[6];
     const Tensor dy = grads[0].stride(1) == 1 ? grads[0] : grads[0].contiguous();
     const Tensor x8 = fp8_saved(saved[0], {T, K}, ScalarType::Float8_e4m3fn, dy), xs = fp8_saved(saved[1], {T, fp8_blocks(K)}, ScalarType::Float, dy);
     const Tensor wn = fp8_saved(saved[2], {E, K, N}, ScalarType::Float8_e4m3fn, dy);
@@ -218,7 +222,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
         dx = empty({T, K}, dy.scalar_type(), dy);
         const int64_t r = ws.size(1), c = ws.size(2);
         tk_fp8_gemm_desc d = fp8_desc(d8.v, d8.s, {bytes(wn), wn.stride(0), wn.stride(1), floats(ws), r * c, turned ? c : 1, turned ? 1 : c}, E, T, K, md, dx);
-        d.zero_rest = d.pow2_scales = 1;
+        d.zero_rest = 1, d.pow2_scales = pow2;
         if (const int32_t rc = B.fp8_gemm(&d, stream)) return rc;
       }
       if (ctx->needs_input_grad(1)) {
@@ -235,7 +239,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
         if (md.sizes.defined()) d.slice_sizes = static_cast<int32_t*>(data(md.sizes)), d.slice_offs = static_cast<int32_t*>(data(md.offs));
         d.n_slices = (int32_t)E, d.T = (int32_t)T, d.K = (int32_t)K, d.N = (int32_t)N;
         d.y = dw.data_ptr(), d.y_dtype = dtype_code(wt), d.y_stride_e = K * N, d.y_stride_k = N;
-        d.pow2_scales = 1;
+        d.pow2_scales = pow2;
         const int64_t n = B.fp8_wgrad_workspace(d.T, d.K, d.N, d.n_slices);
         const Tensor ws2 = n > 0 ? empty({n}, ScalarType::Byte, dy) : Tensor();
         d.workspace = data(ws2);

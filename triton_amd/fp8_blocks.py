@@ -401,15 +401,16 @@ class _LinearFp8(torch.autograd.Function):
     @once
     def backward(ctx, dy):
         names = ("x8", "x_scale", "w8", "w_scale")
+        own = all(r.unpack_hook is None for r in ctx._raw_saved_tensors)  # (what a hook gives back for the scales need not be the quantiser's)
         x8, xs, values_n, scales = (_check_saved(*v) for v in zip(ctx.saved_tensors, ctx.like, names))
         x8 = x8 if x8.stride(1) == 1 or x8.shape[1] <= 1 else x8.contiguous()
         values_n = values_n if values_n.stride(2) == 1 or values_n.shape[2] <= 1 else values_n.contiguous()
         dx = dw = None
         if ctx.needs_input_grad[0]:
             d8, ds = _quantize_rows(dy)
-            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True, ctx.pow2)
+            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True, ctx.pow2 and own)
         if ctx.needs_input_grad[1]:
-            dw = _weight_gradient(x8, xs, dy, ctx.md, ctx.w_dtype, True).view(ctx.w_shape)
+            dw = _weight_gradient(x8, xs, dy, ctx.md, ctx.w_dtype, own).view(ctx.w_shape)
         return dx, dw, None, None, None, None, None
 
 
