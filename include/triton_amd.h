@@ -744,6 +744,12 @@ int32_t tk_swiglu_fp8_backward(const void* d_out, int32_t dtype, int64_t M, int6
 int32_t tk_host_mx_convert(const float* in, int64_t n, int32_t kind, uint8_t* out);
 int32_t tk_host_mx_scale(const float* absmax, int64_t n, int32_t kind, int32_t rounding, uint8_t* out);
 
+/*
+ * The kernel that tk_fp8_block_gemm takes for a call on a card with `cus` compute units: 0 none, 1 the one for lines that begin anywhere and fp32 results, 2 zeros behind the
+ * slices alone, 16 few rows, 64 the ring, 128 and 256 tiles of that size.  Checks the descriptor as the call does and follows none of its pointers.
+ */
+int32_t tk_host_fp8_block_gemm_kernel(const tk_fp8_gemm_desc* desc, int32_t cus, int32_t* kernel);
+
 #ifdef __cplusplus
 }
 #endif

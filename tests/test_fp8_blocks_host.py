@@ -227,3 +227,20 @@ def test_operands_that_want_a_gradient_are_refused():
     _raises(NotImplementedError, "no gradient for x", ops.weight_gradient_fp8_blocks, wants(q), s, torch.ones((4, 8), dtype=BF16))
     _raises(NotImplementedError, "no gradient for a", ops.swiglu_fp8_forward, torch.ones((4, 8), requires_grad=True), 1.0)
     _raises(NotImplementedError, "no gradient for dh", ops.swiglu_fp8_backward, torch.ones((4, 128), requires_grad=True), q, s, 1.0)
+
+
+@pytest.mark.parametrize("case,kernel", [
+    (dict(M=1, K=4096, N=4096), 16), (dict(M=1, K=4096, N=14336), 64), (dict(M=32, K=4096, N=4096), 16), (dict(M=64, K=4096, N=4096), 64), (dict(M=700, K=1000, N=1023, E=3), 64),
+    (dict(M=700, K=1000, N=1023, E=3, x=4097), 1), (dict(M=1, K=4096, N=4096, out_dtype=F32), 16), (dict(M=4096, K=4096, N=4096, out_dtype=F32), 1), (dict(M=128, K=2880, N=5760, E=32), 64),
+    (dict(M=4096, K=2880, N=2880, E=32), 128), (dict(M=2048, K=1024, N=2304), 128), (dict(M=16384, K=4096, N=14336, E=8, gather=True), 256), (dict(M=16384, K=2880, N=5760, E=8), 256),
+    (dict(M=16384, K=2880, N=5760, E=8, w_stride=2888), 1), (dict(M=4096, K=2880, N=2880, E=300), 64), (dict(M=2**21 + 64, K=16, N=16, E=2), 128), (dict(M=100, K=64, N=64, E=2, grid_m=0), 0),
+    (dict(M=100, K=64, N=64, E=2, grid_m=0, zero_rest=1), 2), (dict(M=0, K=64, N=64), 0)])
+def test_the_kernel_that_a_product_takes(case, kernel):
+    from fp8_cases import kernel_of, product_desc
+    assert kernel_of(product_desc(**case)) == kernel
+
+
+def test_the_kernel_of_a_refused_product():
+    from fp8_cases import kernel_of, product_desc
+    _raises(NotImplementedError, "sizes up to", kernel_of, product_desc(2**31 - 1, 16, 16))
+    _raises(ValueError, "bad argument", kernel_of, product_desc(1, 16, 16), 0)

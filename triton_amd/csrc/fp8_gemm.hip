@@ -163,9 +163,9 @@ bool few_rows_run(const Fp8GemmParams& p, int64_t slices, bool dma) {
 // 2048 4096 4096 86 / 50 / 76; 4096 4096 4096 - / 91 / 80; 1024 2048 2048 12.9 / 21 / 37; 2048 2048 2048 25.2 / 23.4 / 42; 4096 512 2048 21 / 16 / 20.6; 8 512 1024 1024 7.2 / 14.1 / 22.6; 8 1024 1024 1024 8.6 / 14.3 / 24.2; 8 2048
 // 1024 1024 14 / 14.7 / 24.5; 8 4096 1024 1024 22 / 18.3 / 25.4; 8 800 608 7296 26 / 23.1 / 23; 8 294 640 7312 17.5 / 14.5 / 19.4; 8 64 4096 4096 22.6 / 36.5 / 60; 32 128 2880 5760 90 / 113 / -; 32 512 2880 5760
 // 120 / 131 / 158; 32 1024 2880 5760 148 / 139 / 166; 32 2048 2880 2880 90 / 82 / 104; 32 4096 2880 2880 147 / 110 / 118; 8 4096 2880 2880 - / 70 / 62.
-int tile_size(const Fp8GemmParams& p, int64_t slices) {
+int tile_size(const Fp8GemmParams& p, int64_t slices, int64_t cus) {
   if (p.M <= slices * 16) return 64;
-  const int64_t cus = device_cu_count(), n64 = (int64_t)p.grid_m * cdiv(p.N, 64), n128 = expected_tiles(p, slices, 128), n256 = expected_tiles(p, slices, 256);
+  const int64_t n64 = (int64_t)p.grid_m * cdiv(p.N, 64), n128 = expected_tiles(p, slices, 128), n256 = expected_tiles(p, slices, 256);
   const double blocks = (double)cdiv(p.K, kFp8Block);
   const double t64 = n64 <= cus ? 0.36 * blocks + 4.3 : (double)cdiv(n64, 2 * cus) * (0.56 * blocks + 3.4);
   const double t128 = n128 <= cus / 2 ? 0.8 * blocks + 8 : (double)cdiv(n128, 2 * cus) * (1.3 * blocks + 6) + 6;
@@ -173,12 +173,12 @@ int tile_size(const Fp8GemmParams& p, int64_t slices) {
   return t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
 }
 
-}  // namespace
-}  // namespace tk
+// The kernels' numbers as the host check hook has them; tiles go by their size.
+enum { kNothing = 0, kAny = 1, kRest = 2, kFew = 16, kRing64 = 64 };
 
-using namespace tk;
-
-extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stream) {
+// Checks a call and chooses its kernel, on a card with `cus` compute units.
+int32_t plan(const tk_fp8_gemm_desc* d, int64_t cus, Fp8GemmParams& p, int32_t& kernel) {
+  kernel = kNothing;
   if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: null descriptor");
   if (d->M < 0 || d->N < 0 || d->K < 0 || d->n_slices < 0 || d->grid_m < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: negative size");
   if (d->M > kFp8Most || d->N > kFp8Most || d->K > kFp8Most) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: sizes up to %d (got %d x %d x %d)", kFp8Most, d->M, d->K, d->N);
@@ -196,7 +196,7 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   } else if (d->n_slices != 1) {
     return fail(TK_ERR_INVALID, "tk_fp8_block_gemm: %d slices without their sizes", d->n_slices);
   }
-  Fp8GemmParams p = {};
+  p = Fp8GemmParams{};
   p.x = d->x, p.x_stride_m = d->x_stride_m, p.xs = d->x_scale, p.xs_m = d->xs_stride_m, p.xs_k = d->xs_stride_k;
   p.w = d->w, p.w_e = d->w_stride_e, p.w_n = d->w_stride_n;
   p.ws = d->w_scale, p.ws_e = d->ws_stride_e, p.ws_k = d->ws_stride_k, p.ws_n = d->ws_stride_n;
@@ -209,8 +209,10 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   p.y = d->y, p.y_stride_m = d->y_stride_m;
   p.alpha = d->act_alpha, p.limit = d->act_has_limit ? d->act_limit : INFINITY;
   p.zero_rest = d->zero_rest, p.pow2 = d->pow2_scales;
-  if (p.grid_m == 0) return p.zero_rest ? launch_rest(p, d->y_dtype, swiglu, static_cast<hipStream_t>(stream)) : TK_OK;
-  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p.grid_m == 0) {
+    kernel = p.zero_rest ? kRest : kNothing;
+    return TK_OK;
+  }
   const int64_t slices = d->slice_sizes ? d->n_slices : 1;
   const bool dma = fp8_tiles_run(p, d->x_rows, d->y_dtype);
   // A schedule has 15 bits for a row block of 64: a slice that may have more goes by tiles, which need none.
@@ -218,9 +220,46 @@ extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stre
   if (long_slices && !(dma && slices <= kDmaSlices))
     return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: more than %d rows in slices need 16-bit results, up to %d slices and operands whose lines begin at sixteen-byte boundaries (got %d rows)",
                 (1 << 15) * kAnyRows, kDmaSlices, d->M);
-  if (few_rows_run(p, slices, dma))
-    return fp8_gemm_launch_few(p, ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) == 0, d->y_dtype, swiglu, st);
-  if (!dma) return launch_any(p, d->y_dtype, swiglu, st);
-  const int tile = tile_size(p, slices);
-  return (tile == 64 && !long_slices) || slices > kDmaSlices ? fp8_gemm_launch_ring(p, d->y_dtype, swiglu, st) : fp8_gemm_launch_tiles(p, tile == 256 ? 256 : 128, d->y_dtype, swiglu, st);
+  if (few_rows_run(p, slices, dma)) {
+    kernel = kFew;
+  } else if (!dma) {
+    kernel = kAny;
+  } else {
+    const int tile = tile_size(p, slices, cus);
+    kernel = (tile == 64 && !long_slices) || slices > kDmaSlices ? kRing64 : tile == 256 ? 256 : 128;
+  }
+  return TK_OK;
+}
+
+}  // namespace
+}  // namespace tk
+
+using namespace tk;
+
+extern "C" int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* d, tk_stream_t stream) {
+  Fp8GemmParams p;
+  int32_t kernel;
+  if (const int32_t rc = plan(d, device_cu_count(), p, kernel)) return rc;
+  const bool swiglu = kernel != kNothing && d->activation == TK_ACT_SWIGLU;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (kernel) {
+    case kNothing:
+      return TK_OK;
+    case kRest:
+      return launch_rest(p, d->y_dtype, swiglu, st);
+    case kAny:
+      return launch_any(p, d->y_dtype, swiglu, st);
+    case kFew:
+      return fp8_gemm_launch_few(p, ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w) | (uint64_t)p.x_stride_m | (uint64_t)p.w_e | (uint64_t)p.w_n) & 15) == 0, d->y_dtype, swiglu, st);
+    case kRing64:
+      return fp8_gemm_launch_ring(p, d->y_dtype, swiglu, st);
+    default:
+      return fp8_gemm_launch_tiles(p, kernel, d->y_dtype, swiglu, st);
+  }
+}
+
+extern "C" int32_t tk_host_fp8_block_gemm_kernel(const tk_fp8_gemm_desc* d, int32_t cus, int32_t* kernel) {
+  if (!kernel || cus <= 0) return fail(TK_ERR_INVALID, "tk_host_fp8_block_gemm_kernel: bad argument");
+  Fp8GemmParams p;
+  return plan(d, cus, p, *kernel);
 }
