@@ -749,6 +749,8 @@ int32_t tk_host_mx_scale(const float* absmax, int64_t n, int32_t kind, int32_t r
  * slices alone, 16 few rows, 64 the ring, 128 and 256 tiles of that size.  Checks the descriptor as the call does and follows none of its pointers.
  */
 int32_t tk_host_fp8_block_gemm_kernel(const tk_fp8_gemm_desc* desc, int32_t cus, int32_t* kernel);
+/* The same of tk_fp8_block_wgrad: tiles of 256 or 128, 64 the kernel for lines of any kind, 0 none; and the parts that a slice's rows are cut into. */
+int32_t tk_host_fp8_block_wgrad_kernel(const tk_fp8_wgrad_desc* desc, int32_t cus, int32_t* tile, int32_t* parts);
 
 #ifdef __cplusplus
 }

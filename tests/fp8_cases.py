@@ -30,3 +30,24 @@ def kernel_of(desc, cus=256):
     kernel = ctypes.c_int32(-1)
     nt.check(nt.lib().tk_host_fp8_block_gemm_kernel(desc, cus, kernel))
     return kernel.value
+
+
+def gradient_desc(T, K, N, E=1, *, workspace=True, dy_dtype=torch.bfloat16, **more):
+    """A descriptor of a weights' gradient from lines at sixteen-byte boundaries that nothing follows."""
+    d = nt.Fp8WgradDesc()
+    d.x, d.x_stride_t, d.x_scale, d.xs_stride_t, d.xs_stride_k = 4096, -(-K // 16) * 16, 4096, -(-K // 128), 1
+    d.dy, d.dy_dtype, d.dy_stride_t = 4096, nt.TORCH_TO_TK[dy_dtype], -(-N // 8) * 8
+    if E > 1:
+        d.slice_sizes, d.slice_offs = 4096, 4096
+    d.n_slices, d.T, d.K, d.N, d.y, d.y_dtype, d.y_stride_e, d.y_stride_k = E, T, K, N, 4096, nt.TK_F32, K * N, N
+    d.workspace = 4096 if workspace is True else workspace or None
+    for name, v in more.items():
+        setattr(d, name, v)
+    return d
+
+
+def gradient_kernel_of(desc, cus=256):
+    """`(tile, parts)`"""
+    tile, parts = ctypes.c_int32(-1), ctypes.c_int32(-1)
+    nt.check(nt.lib().tk_host_fp8_block_wgrad_kernel(desc, cus, tile, parts))
+    return tile.value, parts.value

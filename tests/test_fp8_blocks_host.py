@@ -244,3 +244,18 @@ def test_the_kernel_of_a_refused_product():
     from fp8_cases import kernel_of, product_desc
     _raises(NotImplementedError, "sizes up to", kernel_of, product_desc(2**31 - 1, 16, 16))
     _raises(ValueError, "bad argument", kernel_of, product_desc(1, 16, 16), 0)
+
+
+@pytest.mark.parametrize("case,kernel", [
+    (dict(T=16384, K=2880, N=5760, E=8), (256, 1)), (dict(T=333, K=520, N=776, E=5), (128, 1)), (dict(T=300, K=2300, N=2100, E=7), (256, 1)), (dict(T=400, K=1100, N=1100, E=3), (128, 1)),
+    (dict(T=8192, K=128, N=72), (128, 32)), (dict(T=8192, K=128, N=72, workspace=False), (128, 1)), (dict(T=8192, K=512, N=2048), (128, 8)), (dict(T=100, K=128, N=72, x=4097), (64, 1)),
+    (dict(T=100, K=128, N=72, dy_stride_t=76), (64, 1)), (dict(T=100, K=0, N=72), (0, 0)), (dict(T=0, K=128, N=72), (128, 1))])
+def test_the_kernel_that_a_gradient_takes(case, kernel):
+    from fp8_cases import gradient_desc, gradient_kernel_of
+    assert gradient_kernel_of(gradient_desc(**case)) == kernel
+
+
+def test_the_kernel_of_a_refused_gradient():
+    from fp8_cases import gradient_desc, gradient_kernel_of
+    _raises(ValueError, "not 16-byte aligned", gradient_kernel_of, gradient_desc(8192, 128, 72, workspace=4100))
+    _raises(ValueError, "bad argument", gradient_kernel_of, gradient_desc(1, 16, 16), 0)

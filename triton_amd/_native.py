@@ -171,6 +171,7 @@ SIGNATURES = {
     "tk_host_mx_convert": (_i32, [_ptr, _i64, _i32, _ptr]),
     "tk_host_mx_scale": (_i32, [_ptr, _i64, _i32, _i32, _ptr]),
     "tk_host_fp8_block_gemm_kernel": (_i32, [_c.POINTER(Fp8GemmDesc), _i32, _c.POINTER(_i32)]),
+    "tk_host_fp8_block_wgrad_kernel": (_i32, [_c.POINTER(Fp8WgradDesc), _i32, _c.POINTER(_i32), _c.POINTER(_i32)]),
 }
 
 _lib = None

@@ -430,6 +430,39 @@ int32_t launch_tiles(WgradParams p, int dt, int yt, hipStream_t st) {
   return p.pow2 ? by_out(template_int<TK_BF16>{}, std::true_type{}) : by_out(template_int<TK_BF16>{}, std::false_type{});
 }
 
+// Checks a call and chooses its kernel, on a card with `cus` compute units: tiles of 256 or 128 (with p.parts), 64 the one for any lines, 0 none.
+int32_t plan(const tk_fp8_wgrad_desc* d, int64_t cus, WgradParams& p, int32_t& tile) {
+  tile = 0;
+  if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null descriptor");
+  if (d->T < 0 || d->K < 0 || d->N < 0 || d->n_slices < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: negative size");
+  if (d->T > kFp8Most || d->K > kFp8Most || d->N > kFp8Most) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: sizes up to %d (got %d x %d x %d)", kFp8Most, d->T, d->K, d->N);
+  if (d->dy_dtype != TK_BF16 && d->dy_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: dy must be bf16 or fp16 (dtype %d)", d->dy_dtype);
+  if (d->y_dtype != TK_F32 && d->y_dtype != TK_BF16 && d->y_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: the gradient is fp32, bf16 or fp16 (dtype %d)", d->y_dtype);
+  if (d->slice_sizes ? !d->slice_offs : d->n_slices > 1) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: slices need their sizes and offsets");
+  if (d->n_slices == 0 || d->K == 0 || d->N == 0) return TK_OK;
+  if (!d->y || (d->T > 0 && (!d->x || !d->x_scale || !d->dy))) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null operand");
+  p = WgradParams{};
+  p.parts = 1;
+  p.x = d->x, p.x_t = d->x_stride_t, p.xs = d->x_scale, p.xs_t = d->xs_stride_t, p.xs_k = d->xs_stride_k;
+  p.dy = static_cast<const uint16_t*>(d->dy), p.dy_t = d->dy_stride_t;
+  p.slice_sizes = d->slice_sizes, p.slice_offs = d->slice_offs, p.n_slices = d->n_slices;
+  p.T = d->T, p.K = d->K, p.N = d->N;
+  p.y = static_cast<uint8_t*>(d->y), p.y_e = d->y_stride_e, p.y_k = d->y_stride_k;
+  p.pow2 = d->pow2_scales;
+  // Lines that begin at sixteen-byte boundaries and do not overlap (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's), and offsets
+  // within a stage of 64 rows that fit a buffer resource.
+  const int64_t limit = (int64_t)1 << 31;
+  if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0 && p.x_t >= p.K && p.dy_t >= p.N &&
+      p.xs_t >= 0 && p.xs_k >= 0 && 64 * p.x_t < limit && 128 * p.dy_t < limit && (64 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
+    if (d->workspace) p.parts = wgrad_parts(p.T, p.K, p.N, p.n_slices);
+    if (p.parts > 1 && reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: the workspace is not 16-byte aligned");
+    tile = p.parts == 1 && cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices >= 2 * cus ? 256 : 128;
+  } else {
+    tile = 64;
+  }
+  return TK_OK;
+}
+
 }  // namespace
 }  // namespace tk
 
@@ -442,44 +475,31 @@ extern "C" int64_t tk_fp8_block_wgrad_workspace_bytes(int32_t T, int32_t K, int3
 }
 
 extern "C" int32_t tk_fp8_block_wgrad(const tk_fp8_wgrad_desc* d, tk_stream_t stream) {
-  if (!d) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null descriptor");
-  if (d->T < 0 || d->K < 0 || d->N < 0 || d->n_slices < 0) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: negative size");
-  if (d->T > kFp8Most || d->K > kFp8Most || d->N > kFp8Most) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: sizes up to %d (got %d x %d x %d)", kFp8Most, d->T, d->K, d->N);
-  if (d->dy_dtype != TK_BF16 && d->dy_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: dy must be bf16 or fp16 (dtype %d)", d->dy_dtype);
-  if (d->y_dtype != TK_F32 && d->y_dtype != TK_BF16 && d->y_dtype != TK_F16) return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_wgrad: the gradient is fp32, bf16 or fp16 (dtype %d)", d->y_dtype);
-  if (d->slice_sizes ? !d->slice_offs : d->n_slices > 1) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: slices need their sizes and offsets");
-  if (d->n_slices == 0 || d->K == 0 || d->N == 0) return TK_OK;
-  if (!d->y || (d->T > 0 && (!d->x || !d->x_scale || !d->dy))) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: null operand");
-  WgradParams p = {};
-  p.x = d->x, p.x_t = d->x_stride_t, p.xs = d->x_scale, p.xs_t = d->xs_stride_t, p.xs_k = d->xs_stride_k;
-  p.dy = static_cast<const uint16_t*>(d->dy), p.dy_t = d->dy_stride_t;
-  p.slice_sizes = d->slice_sizes, p.slice_offs = d->slice_offs, p.n_slices = d->n_slices;
-  p.T = d->T, p.K = d->K, p.N = d->N;
-  p.y = static_cast<uint8_t*>(d->y), p.y_e = d->y_stride_e, p.y_k = d->y_stride_k;
+  WgradParams p;
+  int32_t tile;
+  if (const int32_t rc = plan(d, device_cu_count(), p, tile)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  p.pow2 = d->pow2_scales;
-  // Lines that begin at sixteen-byte boundaries and do not overlap (a line's last piece is read whole: its end lies in the sixteen bytes that hold the line's), and offsets
-  // within a stage of 64 rows that fit a buffer resource.
-  const int64_t limit = (int64_t)1 << 31;
-  if (((reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_t) & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.dy) | (uint64_t)(p.dy_t * 2)) & 15) == 0 && p.x_t >= p.K && p.dy_t >= p.N &&
-      p.xs_t >= 0 && p.xs_k >= 0 && 64 * p.x_t < limit && 128 * p.dy_t < limit && (64 * p.xs_t + 2 * p.xs_k) * 4 < limit) {
-    p.parts = d->workspace ? wgrad_parts(p.T, p.K, p.N, p.n_slices) : 1;
-    if (p.parts > 1) {
-      WgradParams q = p;
-      const int64_t pitch = cdiv(p.N, 4) * 4;
-      q.y = static_cast<uint8_t*>(d->workspace), q.y_e = p.K * pitch, q.y_k = pitch;
-      if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(TK_ERR_INVALID, "tk_fp8_block_wgrad: the workspace is not 16-byte aligned");
-      if (const int32_t rc = launch_tiles<128>(q, d->dy_dtype, TK_F32, st)) return rc;
-      const int64_t blocks = cdiv(p.n_slices * p.K * (pitch / 4), 256);
-      auto join = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, static_cast<const float*>(d->workspace), p.parts, (int64_t)p.n_slices, (int64_t)p.K,
-                           (int64_t)p.N, pitch, static_cast<void*>(p.y), p.y_e, p.y_k);
-      };
-      d->y_dtype == TK_F32 ? join(fp8_wgrad_join_kernel<TK_F32>) : d->y_dtype == TK_BF16 ? join(fp8_wgrad_join_kernel<TK_BF16>) : join(fp8_wgrad_join_kernel<TK_F16>);
-      return check_launch("fp8_wgrad_join_kernel");
-    }
-    const int64_t tiles = cdiv(p.K, 256) * cdiv(p.N, 256) * p.n_slices;
-    return tiles >= 2 * device_cu_count() ? launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st) : launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
-  }
-  return launch_any(p, d->dy_dtype, d->y_dtype, st);
+  if (tile == 0) return TK_OK;
+  if (tile == 64) return launch_any(p, d->dy_dtype, d->y_dtype, st);
+  if (tile == 256) return launch_tiles<256>(p, d->dy_dtype, d->y_dtype, st);
+  if (p.parts == 1) return launch_tiles<128>(p, d->dy_dtype, d->y_dtype, st);
+  WgradParams q = p;
+  const int64_t pitch = cdiv(p.N, 4) * 4;
+  q.y = static_cast<uint8_t*>(d->workspace), q.y_e = p.K * pitch, q.y_k = pitch;
+  if (const int32_t rc = launch_tiles<128>(q, d->dy_dtype, TK_F32, st)) return rc;
+  const int64_t blocks = cdiv(p.n_slices * p.K * (pitch / 4), 256);
+  auto join = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, static_cast<const float*>(d->workspace), p.parts, (int64_t)p.n_slices, (int64_t)p.K,
+                       (int64_t)p.N, pitch, static_cast<void*>(p.y), p.y_e, p.y_k);
+  };
+  d->y_dtype == TK_F32 ? join(fp8_wgrad_join_kernel<TK_F32>) : d->y_dtype == TK_BF16 ? join(fp8_wgrad_join_kernel<TK_BF16>) : join(fp8_wgrad_join_kernel<TK_F16>);
+  return check_launch("fp8_wgrad_join_kernel");
+}
+
+extern "C" int32_t tk_host_fp8_block_wgrad_kernel(const tk_fp8_wgrad_desc* d, int32_t cus, int32_t* tile, int32_t* parts) {
+  if (!tile || !parts || cus <= 0) return fail(TK_ERR_INVALID, "tk_host_fp8_block_wgrad_kernel: bad argument");
+  WgradParams p = {};
+  const int32_t rc = plan(d, cus, p, *tile);
+  *parts = *tile ? p.parts : 0;
+  return rc;
 }
