@@ -1,11 +1,12 @@
-"""Calls of the experts in 8 bits as programs make them: hooks that change what the backward pass was to read."""
+"""Calls of the experts in 8 bits as programs make them: hooks that change what the backward pass was to read, weights
+that begin at any address."""
 import pytest
 import torch
 
 from oracle import fp8_blocks as orc
 from oracle.rows import check
 from triton_amd import _native as nt
-from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks
+from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks, matmul_fp8_blocks
 from triton_kernels.tensor import make_ragged_tensor_metadata
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,24 @@ def test_scales_that_a_hook_of_one_node_gives_back_count_whole(monkeypatch):
     dw, = torch.autograd.grad(y, w, dy)
     x8, xs = downcast_to_fp8_blocks(x.detach())
     check(dw[None], *orc.weight_gradient(x8, xs * 1.25, dy), "dw")
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("shift,apart", [(1, 0), (0, 8), (8, 0)])
+@pytest.mark.parametrize("M", [900, 2**21 + 100])                          # (beyond 2^21 rows in slices only the kernels for lines at sixteen-byte boundaries run)
+def test_weights_of_even_lines_that_begin_anywhere(M, shift, apart, native, monkeypatch):
+    """Lines a multiple of sixteen bytes apart, matrices not: `shift` bytes behind a boundary, or `apart` bytes between them."""
+    _both(monkeypatch, native)
+    K, N, E = 32, 16, 2
+    g = torch.Generator().manual_seed(3)
+    a = torch.randint(0, 120, (M, K), generator=g, dtype=torch.uint8).cuda().view(E4M3)
+    a_scale = (torch.rand((M, 1), generator=g) + 0.5).cuda()
+    w = (torch.randn((E, N, K), generator=g) * 100).clamp(-448, 448).to(E4M3).cuda()
+    w_scale = (torch.rand((E, 1, 1), generator=g) + 0.5).cuda()
+    odd = torch.zeros(E * (N * K + apart) + 16, dtype=torch.uint8, device="cuda").as_strided((E, N, K), (N * K + apart, K, 1), shift)
+    odd.copy_(w.view(torch.uint8))
+    sizes = [M - 70, 60]
+    md = make_ragged_tensor_metadata(torch.tensor(sizes, dtype=torch.int32, device="cuda"), M)
+    y = matmul_fp8_blocks(a, a_scale, odd.view(E4M3).transpose(1, 2), w_scale, None, md)
+    for lo, hi, e in ((0, 300, 0), (M - 300, M - 70, 0), (M - 70, M - 10, 1)):
+        check(y[lo:hi], *orc.product(a[lo:hi], a_scale[lo:hi], w[e:e + 1].transpose(1, 2), w_scale[e:e + 1])[:2], "y")
