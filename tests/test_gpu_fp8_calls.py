@@ -78,3 +78,21 @@ def test_weights_of_even_lines_that_begin_anywhere(M, shift, apart, native, monk
     y = matmul_fp8_blocks(a, a_scale, odd.view(E4M3).transpose(1, 2), w_scale, None, md)
     for lo, hi, e in ((0, 300, 0), (M - 300, M - 70, 0), (M - 70, M - 10, 1)):
         check(y[lo:hi], *orc.product(a[lo:hi], a_scale[lo:hi], w[e:e + 1].transpose(1, 2), w_scale[e:e + 1])[:2], "y")
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_fp32_results_come_without_copies_of_the_operands(native, monkeypatch):
+    """Their kernel takes lines that begin anywhere."""
+    _both(monkeypatch, native)
+    M, K, N = 600, 1001, 264
+    g = torch.Generator().manual_seed(4)
+    a = torch.randint(0, 120, (M, K), generator=g, dtype=torch.uint8).cuda().view(E4M3)
+    w = torch.randint(0, 120, (1, N, K), generator=g, dtype=torch.uint8).cuda().view(E4M3).transpose(1, 2)
+    a_scale, w_scale = torch.ones((M, 8), device="cuda"), torch.ones((1, 8, 3), device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = matmul_fp8_blocks(a, a_scale, w, w_scale, out_dtype=F32)
+    assert torch.cuda.max_memory_allocated() - before < y.numel() * 4 + 4096
+    some = torch.arange(0, M, 37, device="cuda")
+    check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w, w_scale, out_dtype=F32)[:2], "y")

@@ -131,8 +131,8 @@ PyObject* run_fp8_matmul(PyObject* const* v) {
     if (!gammas || !on_device_of(*gammas, *a) || gammas->dim() != 1 || gammas->size(0) != M || !gammas->is_contiguous() || !f32_or_bf16(*gammas) || wants_grad(*gammas) || dual(*gammas)) return none();
   }
   if (M == 0 || M > kFp8Most || K > kFp8Most || N > kFp8Most || (scatter && (scatter->size(0) == 0 || scatter->size(0) > kFp8Most))) return none();
-  // (many rows of lines that begin anywhere are copied first)
-  if (M > E * 256 && ((reinterpret_cast<uintptr_t>(w->data_ptr()) | (uint64_t)w->stride(0) | (uint64_t)w->stride(2)) % 16 || !lines_aligned(*a))) return none();
+  // (many rows of lines that begin anywhere are copied first; the kernel for fp32 results takes any)
+  if (out != ScalarType::Float && M > E * 256 && ((reinterpret_cast<uintptr_t>(w->data_ptr()) | (uint64_t)w->stride(0) | (uint64_t)w->stride(2)) % 16 || !lines_aligned(*a))) return none();
   if (dispatcher_heard()) return none();
   auto stream = stream_of(*a);
   if (!stream) return none();

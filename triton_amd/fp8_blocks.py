@@ -284,8 +284,9 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
         raise NotImplementedError("batched weights need ragged metadata")
     if w.stride(1) != 1 and K > 1:
         w = w.transpose(1, 2).contiguous().transpose(1, 2)
-    if M > 256 * E:
-        # (the fast kernels take lines at sixteen-byte boundaries; from about a hundred rows an expert a copy of all weights costs less than the kernel for any lines)
+    if M > 256 * E and out_dtype != torch.float32:
+        # (the fast kernels take lines at sixteen-byte boundaries; beyond 256 rows an expert a copy of all weights costs less than the kernel for any lines.  fp32 results
+        # have no other kernel than that one: us, copied / not: 700 rows, 1000 x 1023 32 / 12; 2000, 2057 x 2048 57 / 44; eight experts, 16384, 2881 x 2880 600 / 566)
         a, w = _aligned(a, 16), _aligned(w.transpose(1, 2), 16).transpose(1, 2)
     return _gemm(a, a_scale, w, w_scale, bias, md, gather_indx, scatter_indx, gammas, act, out_dtype)
 
