@@ -655,8 +655,9 @@ int32_t tk_fp8_block_upcast(const uint8_t* values, int64_t batch, int64_t rows, 
  * Rows of x and columns of w are contiguous along K, of any alignment.  slice_sizes NULL = one slice of M rows.  block_schedule = the
  * schedule of row blocks of 64 ((block << 16) | slice, negative = none), grid_m entries.
  * zero_rest: rows behind the last slice (from slice_offs[n_slices] on, below M) are set to zero; otherwise they stay as they were.
- * M, N and K up to 2^31 - 256.  With slices and M > 2^21 (a schedule has 15 bits for a row block) only for 16-bit results, up to 256 slices, and operands whose lines
- * begin at sixteen-byte boundaries: TK_ERR_UNSUPPORTED otherwise.
+ * M, N and K up to 2^31 - 256.  With slices and M > 2^21 (a schedule has 15 bits for a row block) only for 16-bit results, up to 256 slices, operands whose lines
+ * begin at sixteen-byte boundaries and, with gather_indx, an x of less than 2 GiB: TK_ERR_UNSUPPORTED otherwise.  (Below that an x of 2 GiB and more that is gathered from
+ * is taken by the kernel for lines that begin anywhere: 1.5 to 2.5 times as long.)
  */
 typedef struct tk_fp8_gemm_desc {
   const uint8_t* x; /* e4m3 [x_rows, K] */

@@ -259,3 +259,14 @@ def test_the_kernel_of_a_refused_gradient():
     from fp8_cases import gradient_desc, gradient_kernel_of
     _raises(ValueError, "not 16-byte aligned", gradient_kernel_of, gradient_desc(8192, 128, 72, workspace=4100))
     _raises(ValueError, "bad argument", gradient_kernel_of, gradient_desc(1, 16, 16), 0)
+
+
+def test_gathered_rows_of_two_gibibytes():
+    """Beyond the reach of a buffer resource the kernel for any lines takes them, and where the schedule does not suffice the refusal says what for."""
+    from fp8_cases import kernel_of, product_desc
+    rows = 2**31 // 4096
+    for n, kernel in ((rows - 1, 256), (rows, 1)):
+        assert kernel_of(product_desc(16384, 4096, 14336, 8, gather=True, x_rows=n)) == kernel
+    assert kernel_of(product_desc(16384, 4096, 14336, 8, x_rows=rows)) == 256
+    assert kernel_of(product_desc(2**21 + 64, 4096, 256, 2, gather=True, x_rows=rows - 1)) in (128, 256)
+    _raises(NotImplementedError, "less than 2 GiB to gather from", kernel_of, product_desc(2**21 + 64, 4096, 256, 2, gather=True, x_rows=rows))

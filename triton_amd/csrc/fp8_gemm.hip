@@ -128,7 +128,7 @@ int32_t launch_rest(const Fp8GemmParams& p, int yt, bool swiglu, hipStream_t st)
 }
 
 // What the kernels with memory-to-LDS transfers need: lines that begin at sixteen-byte boundaries, and offsets within a buffer resource (2 GiB) from the start of a
-// tile, or of x and its scales where rows are gathered.
+// tile, or of x and its scales where rows are gathered (beyond it such a call takes the kernel for any lines).
 bool fp8_tiles_run(Fp8GemmParams& p, int64_t x_rows, int yt) {
   const int64_t limit = (int64_t)1 << 31, K16 = (p.K + 15) & ~15, blocks = cdiv(p.K, kFp8Block), rows = p.gather ? x_rows : 256;
   if (yt == TK_F32 || p.K == 0) return false;
@@ -218,7 +218,7 @@ int32_t plan(const tk_fp8_gemm_desc* d, int64_t cus, Fp8GemmParams& p, int32_t& 
   // A schedule has 15 bits for a row block of 64: a slice that may have more goes by tiles, which need none.
   const bool long_slices = d->slice_sizes && d->M > (1 << 15) * kAnyRows;
   if (long_slices && !(dma && slices <= kDmaSlices))
-    return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: more than %d rows in slices need 16-bit results, up to %d slices and operands whose lines begin at sixteen-byte boundaries (got %d rows)",
+    return fail(TK_ERR_UNSUPPORTED, "tk_fp8_block_gemm: more than %d rows in slices need 16-bit results, up to %d slices, operands whose lines begin at sixteen-byte boundaries and, where rows are gathered, less than 2 GiB to gather from (got %d rows)",
                 (1 << 15) * kAnyRows, kDmaSlices, d->M);
   if (few_rows_run(p, slices, dma)) {
     kernel = kFew;
