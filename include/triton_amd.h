@@ -635,7 +635,7 @@ int32_t tk_distill_topk_backward(const tk_vocab_desc* desc, tk_stream_t stream);
  * most 448; 1 for a block of zeros.  An element is rounded to the nearest e4m3, ties to even; infinities and NaN become NaN.  Powers
  * of two lose nothing against amax / 448 but a part of the subnormal numbers' range, and leave every value a number of four
  * significant bits, which 16 bits hold exactly.  `values_t`, block_rows 128 only, may receive the transposed values [cols, rows] too.
- * tk_fp8_block_upcast: values * scale in fp32, rounded once to out_dtype; scales of any size.
+ * tk_fp8_block_upcast: values * scale in fp32, rounded to out_dtype (two roundings where the scale is no power of two and out_dtype has 16 bits); scales of any size.
  * All matrices have unit stride along cols (values_t: along rows); strides are in elements.  `batch` matrices in one call.
  */
 int32_t tk_fp8_block_downcast(const void* x, int32_t dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_stride_b, int64_t x_stride_r,
@@ -693,8 +693,9 @@ int32_t tk_fp8_block_gemm(const tk_fp8_gemm_desc* desc, tk_stream_t stream);
 
 /*
  * Gradient of the weights from an 8-bit activation: y[e, k, n] = sum over the rows t of slice e of x[t, k] x_scale[t, k / 128] dy[t, n],
- * fp32 sums.  x times its scale is rounded to dy's type first (exact where the scales are powers of two as tk_fp8_block_downcast makes them, and
- * limited to 65504 in fp16).  A slice without rows has the gradient zero.
+ * fp32 sums.  x times its scale is rounded to dy's type first.  With scales that are powers of two as tk_fp8_block_downcast makes them that is exact in bf16 (from 2^-126
+ * on), and in fp16 where the product is a multiple of 2^-24, as all that was quantised from fp16 is: what was quantised from bf16 or fp32 loses what lies below, and
+ * numbers of less than 2^-25 altogether.  In fp16 it is held within 65504.  A slice without rows has the gradient zero.
  */
 typedef struct tk_fp8_wgrad_desc {
   const uint8_t* x; /* e4m3 [T, K] */

@@ -6,7 +6,7 @@ import torch
 from oracle import fp8_blocks as orc
 from oracle.rows import check
 from triton_amd import _native as nt
-from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks, matmul_fp8_blocks
+from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks, matmul_fp8_blocks, weight_gradient_fp8_blocks
 from triton_kernels.tensor import make_ragged_tensor_metadata
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +96,24 @@ def test_fp32_results_come_without_copies_of_the_operands(native, monkeypatch):
     assert torch.cuda.max_memory_allocated() - before < y.numel() * 4 + 4096
     some = torch.arange(0, M, 37, device="cuda")
     check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w, w_scale, out_dtype=F32)[:2], "y")
+
+
+@pytest.mark.parametrize("source", [BF16, F16, F32])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_what_the_weights_gradient_reads_in_16_bits(dtype, source):
+    """With the unit matrix behind it the gradient is x times its scale as it is multiplied: exact in fp16 where it is a multiple of 2^-24 within 65504, as all that was
+    quantised from fp16 is, the nearest such number otherwise; exact in bf16 from 2^-126 on."""
+    g = torch.Generator().manual_seed(6)
+    T, K = 64, 256
+    x = torch.randn((T, K), generator=g) * torch.ldexp(torch.ones(T, 1), torch.arange(T)[:, None] - 44)  # (up to 2^19 and more, beyond fp16, and far below 2^-24)
+    x = (x.clamp(-65504, 65504) if source == F16 else x).to(source).cuda()
+    x8, s = downcast_to_fp8_blocks(x)
+    dw = weight_gradient_fp8_blocks(x8, s, torch.eye(T, dtype=dtype, device="cuda"), None, F32).cpu().double().T
+    exact = orc.upcast(x8, s)
+    if dtype == BF16:
+        assert torch.equal(dw, exact)
+        return
+    held = exact.clamp(-65504, 65504)
+    whole = held * 2.0**24 == (held * 2.0**24).round()
+    assert torch.equal(dw[whole], held[whole]) and ((dw - held).abs() <= 2.0**-25).all()
+    assert whole.all() == (source == F16)

@@ -103,7 +103,8 @@ def downcast_to_fp8_blocks(x: torch.Tensor, block_rows: int = 1):
 
 
 def upcast_from_fp8_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16, block_rows: int = 1) -> torch.Tensor:
-    """`values * scales`, rounded once to `dtype` (fp32, bf16 or fp16); the arguments as `downcast_to_fp8_blocks` returns them, scales of any size."""
+    """`values * scales` in fp32, rounded to `dtype` (fp32, bf16 or fp16): two roundings where scales are no powers of two and `dtype` has 16 bits.  The arguments as
+    `downcast_to_fp8_blocks` returns them, scales of any size."""
     host = nt.host()
     r = host.fp8_upcast(values, scales, dtype, block_rows) if host is not None else None
     if r is not None:
@@ -326,8 +327,9 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
 def weight_gradient_fp8_blocks(x: torch.Tensor, x_scale: torch.Tensor, dy: torch.Tensor, ragged_metadata: Optional[RaggedTensorMetadata] = None,
                                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """`dw[e] = (x * x_scale)^T dy` over the rows of slice e: `x [T, K]` e4m3 with `x_scale [T, ceil(K / 128)]` as `downcast_to_fp8_blocks` returns them, `dy [T, N]`
-    bf16 or fp16; the result `[E, K, N]` (`[K, N]` without metadata) in `out_dtype` (dy's if not given).  fp32 sums; `x * x_scale` is rounded to dy's
-    type first, which changes nothing where the scales are powers of two (in fp16: and the product within 65504, its largest number, which it is held to).  A slice without rows has the gradient zero."""
+    bf16 or fp16; the result `[E, K, N]` (`[K, N]` without metadata) in `out_dtype` (dy's if not given).  fp32 sums; `x * x_scale` is rounded to dy's type first.  Where the
+    scales are powers of two that changes nothing in bf16, and in fp16 nothing of what was quantised from fp16 but numbers beyond 65504, which are held to it; of what was
+    quantised from bf16 or fp32 it loses in fp16 what lies below 2^-24: pass dy in bf16 there.  A slice without rows has the gradient zero."""
     _no_gradient("weight_gradient_fp8_blocks", x=x, x_scale=x_scale, dy=dy)
     _type(dy, "dy", (torch.bfloat16, torch.float16))
     out_dtype = out_dtype or dy.dtype
