@@ -650,7 +650,8 @@ int32_t tk_fp8_block_upcast(const uint8_t* values, int64_t batch, int64_t rows, 
  * The ragged product of such operands: for row r of slice e
  *     acc = sum over blocks b of K of (sum over k in b of x[src(r), k] w[e, k, n]) x_scale[src(r), b] w_scale[e, b, n / 128]
  *     y[dst(r), n] = act(acc + bias[e, n]) * gammas[r]
- * with fp32 sums, rounded once.  src(r) = gather_indx[r] or r; dst(r) = scatter_indx[r] (negative: the row is dropped; rows r >= scatter_len
+ * with fp32 sums, rounded once.  The two scales are multiplied first, in fp32: their product is to lie within its normal numbers (a smaller one loses bits, a larger
+ * one is infinite, also for blocks of zeros).  src(r) = gather_indx[r] or r; dst(r) = scatter_indx[r] (negative: the row is dropped; rows r >= scatter_len
  * are dropped) or r.  act: none, or swiglu over interleaved (gate, linear) columns as in tk_moe_gemm.
  * Rows of x and columns of w are contiguous along K, of any alignment.  slice_sizes NULL = one slice of M rows.  block_schedule = the
  * schedule of row blocks of 64 ((block << 16) | slice, negative = none), grid_m entries.

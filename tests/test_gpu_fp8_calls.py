@@ -117,3 +117,15 @@ def test_what_the_weights_gradient_reads_in_16_bits(dtype, source):
     whole = held * 2.0**24 == (held * 2.0**24).round()
     assert torch.equal(dw[whole], held[whole]) and ((dw - held).abs() <= 2.0**-25).all()
     assert whole.all() == (source == F16)
+
+
+@pytest.mark.parametrize("sa,sw", [(1.3 * 2.0**-63, 1.1 * 2.0**-62), (1.9 * 2.0**100, 1.1 * 2.0**-100), (1.7 * 2.0**60, 1.3 * 2.0**40), (1.1 * 2.0**-126, 1.9)])
+@pytest.mark.parametrize("M,K,N,out_dtype", [(3, 300, 64, BF16), (300, 304, 264, BF16), (300, 300, 264, F32), (6000, 272, 4201, BF16)])  # few rows, ring, any lines, tiles
+def test_scales_whose_product_is_a_normal_number(M, K, N, out_dtype, sa, sw):
+    g = torch.Generator().manual_seed(7)
+    a = torch.randint(0, 120, (M, -(-K // 16) * 16), generator=g, dtype=torch.uint8).cuda().view(E4M3)[:, :K]
+    w = (torch.randn((1, N, -(-K // 16) * 16), generator=g) * 100).clamp(-448, 448).cuda().to(E4M3)[:, :, :K].transpose(1, 2)
+    a_scale, w_scale = torch.full((M, -(-K // 128)), sa, device="cuda"), torch.full((1, -(-K // 128), -(-N // 128)), sw, device="cuda")
+    y = matmul_fp8_blocks(a, a_scale, w, w_scale, out_dtype=out_dtype)
+    some = torch.arange(0, M, max(1, M // 50), device="cuda")
+    check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w, w_scale, out_dtype=out_dtype)[:2], "y")

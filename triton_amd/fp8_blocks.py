@@ -229,7 +229,7 @@ def matmul_fp8_blocks(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w
         y[dst(r)] = act((a * a_scale)[src(r)] @ (w * w_scale)[e(r)] + bias[e(r)]) * gammas[r]
 
     `a [rows, K]` e4m3 with `a_scale [rows, ceil(K / 128)]`; `w [E, K, N]` (or `[K, N]`) e4m3 with `w_scale [E, ceil(K / 128), ceil(N / 128)]`, scales fp32
-    of any size and any strides.  Weights are contiguous along K, as a checkpoint's `[E, N, K]` transposed; others are copied for the call.  `a_ragged_metadata`, `gather_indx`,
+    of any size and any strides (the product of two of them is taken first, and is to be a normal number of fp32).  Weights are contiguous along K, as a checkpoint's `[E, N, K]` transposed; others are copied for the call.  `a_ragged_metadata`, `gather_indx`,
     `scatter_indx`, `gammas` and `fused_activation` (swiglu) as in `matmul`: the rows of the slices in order, src(r) = gather_indx[r], dst(r) =
     scatter_indx[r] (negative: dropped).  `bias [E, N]` and `gammas [rows]` are fp32 or bf16.  Blocks of 128 products are summed by themselves and added, times their scales,
     in fp32; the result is rounded once, to `out_dtype` (bf16, fp16 or fp32).  For results of 16 bits the products are those of the 8-bit matrix instructions, which add eight at a time
