@@ -1,12 +1,13 @@
 """Calls of the experts in 8 bits as programs make them: hooks that change what the backward pass was to read, weights
-that begin at any address."""
+that begin at any address, other transforms than a backward pass, several threads."""
 import pytest
 import torch
 
 from oracle import fp8_blocks as orc
 from oracle.rows import check
 from triton_amd import _native as nt
-from triton_kernels.fp8_blocks import downcast_to_fp8_blocks, linear_fp8_blocks, matmul_fp8_blocks, weight_gradient_fp8_blocks
+from triton_kernels.fp8_blocks import (downcast_to_fp8_blocks, linear_fp8_blocks, matmul_fp8_blocks, quantize_fp8_weight, swiglu_fp8_backward, swiglu_fp8_checkpoint,
+                                       swiglu_fp8_forward, upcast_from_fp8_blocks, weight_gradient_fp8_blocks)
 from triton_kernels.tensor import make_ragged_tensor_metadata
 
 pytestmark = pytest.mark.gpu
@@ -46,7 +47,6 @@ def test_scales_that_a_hook_gives_back_count_whole(T, K, N, dtype, native, monke
 
 def test_scales_that_a_hook_of_one_node_gives_back_count_whole(monkeypatch):
     """Hooks on the saved tensors of a node that Python has (weights that were handed in)."""
-    from triton_kernels.fp8_blocks import quantize_fp8_weight
     g = torch.Generator().manual_seed(1)
     x = _rows(g, 40, 200).requires_grad_()
     w = (torch.randn((200, 72), generator=g) * 0.05).cuda().requires_grad_()
@@ -129,3 +129,76 @@ def test_scales_whose_product_is_a_normal_number(M, K, N, out_dtype, sa, sw):
     y = matmul_fp8_blocks(a, a_scale, w, w_scale, out_dtype=out_dtype)
     some = torch.arange(0, M, max(1, M // 50), device="cuda")
     check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w, w_scale, out_dtype=out_dtype)[:2], "y")
+
+
+def _calls(g):
+    """(operator of one tensor, that tensor, whether it has a gradient)"""
+    x, w = _rows(g, 40, 256), (torch.randn((256, 64), generator=g) * 0.1).cuda()
+    x8, s = downcast_to_fp8_blocks(x)
+    q = quantize_fp8_weight(w)
+    h, v, t = swiglu_fp8_forward(x, 1.7, 2.0)
+    dy, bias, gammas = _rows(g, 40, 64), torch.randn((1, 64), generator=g).cuda(), torch.rand(40, generator=g).cuda()
+    return ((lambda p: downcast_to_fp8_blocks(p)[1], x, False), (lambda p: downcast_to_fp8_blocks(p, 128)[1], x, False), (lambda p: upcast_from_fp8_blocks(x8, p), s, False),
+            (lambda p: matmul_fp8_blocks(x8, p, q.values, q.scales), s, False), (lambda p: matmul_fp8_blocks(x8, s, q.values, p), q.scales, False),
+            (lambda p: matmul_fp8_blocks(x8, s, q.values, q.scales, p), bias, False), (lambda p: matmul_fp8_blocks(x8, s, q.values, q.scales, gammas=p), gammas, False),
+            (lambda p: weight_gradient_fp8_blocks(x8, s, p), dy, False), (lambda p: weight_gradient_fp8_blocks(x8, p, dy), s, False),
+            (lambda p: linear_fp8_blocks(p, w), x, True), (lambda p: linear_fp8_blocks(x, p), w, True), (lambda p: linear_fp8_blocks(p, w, quantized=q), x, True),
+            (lambda p: swiglu_fp8_forward(p, 1.7, 2.0)[0], x, False), (lambda p: swiglu_fp8_checkpoint(p, 1.7, 2.0), x, True), (lambda p: swiglu_fp8_backward(p, v, t, 1.7, 2.0), h, False))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_other_transforms_are_refused(native, monkeypatch):
+    """Forward mode, whose dual tensors ask for no gradient; vmap and grad of torch.func."""
+    import torch.autograd.forward_ad as fwad
+    _both(monkeypatch, native)
+    for f, t, differentiable in _calls(torch.Generator().manual_seed(8)):
+        want = f(t)
+        with fwad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f(fwad.make_dual(t, torch.ones_like(t)))
+            assert torch.equal(f(t), want)
+        for call in (lambda: torch.func.jvp(f, (t, ), (torch.ones_like(t), )), lambda: torch.func.vmap(f)(torch.stack((t, t))), lambda: torch.func.grad(lambda s: f(s).float().sum())(t)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        if not differentiable:
+            with pytest.raises(NotImplementedError, match="no gradient for"):
+                f(t.clone().requires_grad_())
+        assert torch.equal(f(t), want)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_threads_side_by_side(native, monkeypatch):
+    """Each on a stream of its own, forward and backward, many times over; a workspace of its own for each weights' gradient."""
+    import threading
+    _both(monkeypatch, native)
+    g = torch.Generator().manual_seed(9)
+    T, K, N = 2100, 144, 272                                               # (a gradient in parts)
+    sets = [(_rows(g, T, K), (torch.randn((K, N), generator=g) * 0.1).cuda(), _rows(g, T, N, BF16, 0.1), _rows(g, 60, 256)) for _ in range(4)]
+
+    def step(x, w, dy, a):
+        x, w, a = x.detach().requires_grad_(), w.detach().requires_grad_(), a.detach().requires_grad_()
+        y, h = linear_fp8_blocks(x, w), swiglu_fp8_checkpoint(a, 1.7, 2.0)
+        return (y, h) + torch.autograd.grad(y, (x, w), dy) + torch.autograd.grad(h, a, torch.ones_like(h))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = step(*sets[i])
+                    stream.synchronize()
+                    if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=run, args=(i, )) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
