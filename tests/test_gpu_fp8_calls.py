@@ -202,3 +202,12 @@ def test_threads_side_by_side(native, monkeypatch):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_dual_weights_are_not_quantised():
+    import torch.autograd.forward_ad as fwad
+    w = torch.ones((256, 64), device="cuda")
+    with fwad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            quantize_fp8_weight(fwad.make_dual(w, torch.ones_like(w)))
+    assert quantize_fp8_weight(w.requires_grad_()).scales.shape == (1, 2, 1)  # (a leaf's values: the linear layer has its gradient)

@@ -308,6 +308,7 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Weight:
     _type(w, "w")
     if w.ndim not in (2, 3):
         raise ValueError(f"w must be [E, K, N] (got {tuple(w.shape)})")
+    check_forward_mode("quantize_fp8_weight", w)
     nt.require_gpu(w, "w")
     w = w.detach()
     w3 = w[None] if w.ndim == 2 else w
