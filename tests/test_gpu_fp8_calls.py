@@ -1,5 +1,6 @@
 """Calls of the experts in 8 bits as programs make them: hooks that change what the backward pass was to read, weights
-that begin at any address, other transforms than a backward pass, several threads."""
+that begin at any address, other transforms than a backward pass, several threads, and a rank's own
+experts."""
 import pytest
 import torch
 
@@ -211,3 +212,33 @@ def test_dual_weights_are_not_quantised():
         with pytest.raises(NotImplementedError, match="forward mode"):
             quantize_fp8_weight(fwad.make_dual(w, torch.ones_like(w)))
     assert quantize_fp8_weight(w.requires_grad_()).scales.shape == (1, 2, 1)  # (a leaf's values: the linear layer has its gradient)
+
+
+@pytest.mark.parametrize("sizes,K,N,out_dtype", [([4, 1, 0, 13, 3, 5, 6, 1], 384, 96, BF16), ([40, 17, 0, 130, 33, 5, 64, 11], 400, 200, BF16), ([40, 17, 0, 130, 33, 5, 64, 11], 400, 200, F32),
+                                                 ([900, 300, 0, 2000, 77, 1100, 500, 1], 256, 4200, BF16)])  # few rows, ring, any lines, tiles
+def test_a_rank_multiplies_by_its_own_experts(sizes, K, N, out_dtype):
+    """Metadata of all slices restricted to a few: their rows are at their places, the other rows stay as they were."""
+    from triton_amd.tensor import remap_ragged_tensor_metadata
+    g = torch.Generator().manual_seed(10)
+    M, E, local = sum(sizes), len(sizes), [1, 3, 4, 6]
+    smap = torch.full((E, ), -1, dtype=torch.int32)
+    smap[local] = torch.arange(len(local), dtype=torch.int32)
+    a, a_scale = downcast_to_fp8_blocks(_rows(g, M, K))
+    w = (torch.randn((E, N, -(-K // 16) * 16), generator=g) * 100).clamp(-448, 448).cuda().to(E4M3)[:, :, :K].transpose(1, 2)
+    w_scale = (torch.rand((E, -(-K // 128), -(-N // 128)), generator=g) + 0.5).cuda()
+    md = remap_ragged_tensor_metadata(make_ragged_tensor_metadata(torch.tensor(sizes, dtype=torch.int32, device="cuda"), M), smap.cuda())
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)                               # (new memory holds NaN)
+    try:
+        mine = w.transpose(1, 2).view(torch.uint8)[local].view(E4M3).transpose(1, 2)
+        y = matmul_fp8_blocks(a, a_scale, mine, w_scale[local], None, md, out_dtype=out_dtype)
+    finally:
+        torch.use_deterministic_algorithms(before)
+    for e in range(E):
+        lo, hi = sum(sizes[:e]), sum(sizes[:e + 1])
+        if e not in local:
+            assert y[lo:hi].isnan().all()
+            continue
+        some = torch.arange(lo, hi, max(1, (hi - lo) // 40), device="cuda")
+        check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w[e:e + 1], w_scale[e:e + 1], out_dtype=out_dtype)[:2], "y")
+        assert y[lo:hi].isfinite().all()
