@@ -61,7 +61,7 @@ __global__ __launch_bounds__(TilesCfg<TILE>::NW * 64, 2) void fp8_block_tiles_ke
   uint32_t x_off[C::TR], w_off[C::TR], s_off;
   uint32_t s_step;  // bytes from a block's scale to the next one's, of what this wave fetches
   const uint32_t x_row = (uint32_t)p.x_stride_m, w_row = (uint32_t)p.w_n;
-  constexpr int SW = TILE / 64;  // waves 0 .. SW - 1 fetch the rows' scales, 64 each, wave SW - 1 + 1 (or the first again) the columns'
+  constexpr int SW = TILE / 64;  // waves 0 .. SW - 1 fetch the rows' scales, 64 each, wave SW the columns'
   // (what depends on the lane alone would be kept in registers over the whole loop, beside sums that need them: a lane number the compiler cannot follow is not)
   auto own_lane = [&]() __attribute__((always_inline)) -> int {
     int l = tid & 63;

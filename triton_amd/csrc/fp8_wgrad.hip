@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void fp8_wgrad_any_kernel(const WgradParams p)
 //     been read from, piece by piece beside the products of the other three steps, and the one behind it asked for.
 //   * Workgroups are persistent and the stream of stages runs on across tiles.  Every XCD takes an eighth of each slice's tiles, from the longest slice to the
 //     shortest (up to 64 of them), and its workgroups walk their list forth and back.
-//   * us: eight slices of 16384 rows in all, 2880 x 5760 600 to 640 (850 to 900 TFLOP/s), 4096 x 14336 1770 (1086; a library product of 8192 cubed in bf16 reaches 1200).  The matrix unit is busy
+//   * us: eight slices of 16384 rows in all, 2880 x 5760 545 to 640, by box (850 to 1000 TFLOP/s), 4096 x 14336 1770 (1086; a library product of 8192 cubed in bf16 reaches 1200).  The matrix unit is busy
 //     0.55 of the cycles at 1.98 GHz, LDS 0.42.  Four waves of 128 x 96 or 128 x 128, which read a third less from LDS, have one wave a SIMD and take 1.5 to 3 times as long.
 
 constexpr int kStage = 64;
@@ -399,7 +399,8 @@ __global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float* ws, in
 }
 
 // Parts of a slice's rows: where tiles of 128 are fewer than half of the places for them and a slice has (expected) eight stages and more, so many that they fill those
-// places, of four stages at least.
+// places, of four stages at least.  (Two places on each of 256 compute units, a constant: the workspace is asked for by sizes alone, before it is known on which device the call
+// will run, and both have to come to the same number.)
 int wgrad_parts(int64_t T, int64_t K, int64_t N, int64_t n_slices) {
   const int64_t tiles = cdiv(K, 128) * cdiv(N, 128) * n_slices, places = 512, stages = n_slices > 0 ? T / n_slices / kStage : 0;
   if (tiles == 0 || tiles * 2 > places || stages < 8) return 1;
