@@ -242,3 +242,54 @@ def test_a_rank_multiplies_by_its_own_experts(sizes, K, N, out_dtype):
         some = torch.arange(lo, hi, max(1, (hi - lo) // 40), device="cuda")
         check(y[some], *orc.product(a.view(torch.uint8)[some].view(E4M3), a_scale[some], w[e:e + 1], w_scale[e:e + 1], out_dtype=out_dtype)[:2], "y")
         assert y[lo:hi].isfinite().all()
+
+
+HOOKS = {"offloaded": (lambda t: t.cpu(), lambda t: t.cuda()),
+         "other strides": (lambda t: t.transpose(-1, -2).contiguous() if t.ndim > 1 else torch.stack((t, t), 1), lambda p: p.transpose(-1, -2) if p.dtype != torch.int32 or p.shape[1] != 2 else p[:, 0]),
+         "rows between others": (lambda t: torch.stack((t, t), t.ndim - 1), lambda p: p.select(p.ndim - 2, 1))}
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_saved_tensors_with_other_strides(dtype, native, hooks, monkeypatch):
+    _both(monkeypatch, native)
+    g = torch.Generator().manual_seed(11)
+    T, K, N, E = 90, 200, 72, 3
+    md = make_ragged_tensor_metadata(torch.tensor([30, 0, 50], dtype=torch.int32, device="cuda"), T)
+    x, a = _rows(g, T, K, dtype).requires_grad_(), _rows(g, 20, 300, dtype).requires_grad_()
+    w = (torch.randn((E, K, N), generator=g) * 0.05).cuda().requires_grad_()
+    k_first = w.detach().transpose(1, 2).contiguous().transpose(1, 2).requires_grad_()
+    dy, dh = _rows(g, T, N, dtype, 0.1), _rows(g, 20, 150, dtype)
+    step = lambda v: (linear_fp8_blocks(x, v, md), swiglu_fp8_checkpoint(a, 1.7, 2.0))  # noqa: E731
+    for v in (w, k_first):
+        y, h = step(v)
+        want = torch.autograd.grad(y, (x, v), dy) + torch.autograd.grad(h, a, dh)
+        with torch.autograd.graph.saved_tensors_hooks(*HOOKS[hooks]):
+            y, h = step(v)
+        got = torch.autograd.grad(y, (x, v), dy) + torch.autograd.grad(h, a, dh)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_layers(reentrant, native, monkeypatch):
+    from torch.utils.checkpoint import checkpoint
+    _both(monkeypatch, native)
+    g = torch.Generator().manual_seed(12)
+    T, d, f, E = 120, 136, 200, 2
+    md = make_ragged_tensor_metadata(torch.tensor([50, 70], dtype=torch.int32, device="cuda"), T)
+    x = _rows(g, T, d).requires_grad_()
+    w1, w2 = ((torch.randn(s, generator=g) * 0.05).cuda().requires_grad_() for s in ((E, d, 2 * f), (E, f, d)))
+    dy = _rows(g, T, d, BF16, 0.1)
+    block = lambda x, w1, w2: linear_fp8_blocks(swiglu_fp8_checkpoint(linear_fp8_blocks(x, w1, md), 1.7, 7.0), w2, md)  # noqa: E731
+
+    def gradients(y):
+        for t in (x, w1, w2):
+            t.grad = None
+        y.backward(dy)
+        return [t.grad for t in (x, w1, w2)]
+
+    y = block(x, w1, w2)
+    z = checkpoint(block, x, w1, w2, use_reentrant=reentrant)
+    assert torch.equal(y, z) and all(torch.equal(p, q) for p, q in zip(gradients(y), gradients(z)))
