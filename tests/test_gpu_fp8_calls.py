@@ -293,3 +293,18 @@ def test_recomputed_layers(reentrant, native, monkeypatch):
     y = block(x, w1, w2)
     z = checkpoint(block, x, w1, w2, use_reentrant=reentrant)
     assert torch.equal(y, z) and all(torch.equal(p, q) for p, q in zip(gradients(y), gradients(z)))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("changed", ["slice_sizes", "slice_offs", "block_schedule_data"])
+def test_metadata_changed_before_the_backward_pass(changed, native, monkeypatch):
+    """Slices written over for the next batch: the gradients of this one are gone, and the backward pass says so."""
+    _both(monkeypatch, native)
+    g = torch.Generator().manual_seed(13)
+    md = make_ragged_tensor_metadata(torch.tensor([30, 10, 50], dtype=torch.int32, device="cuda"), 90)
+    x = _rows(g, 90, 200).requires_grad_()
+    w = (torch.randn((3, 200, 72), generator=g) * 0.05).cuda().requires_grad_()
+    y = linear_fp8_blocks(x, w, md)
+    getattr(md, changed).add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

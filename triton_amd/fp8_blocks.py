@@ -397,25 +397,30 @@ class _LinearFp8(torch.autograd.Function):
     def forward(ctx, x, w, values, values_n, scales, md, pow2):
         x8, xs = _quantize_rows(x)
         y = _gemm(x8, xs, values, scales, None, md, None, None, None, None, x.dtype, True, pow2)
-        ctx.save_for_backward(x8, xs, values_n, scales)
+        slices = () if md is None else (md.slice_sizes, md.slice_offs, md.block_schedule_data)  # (saved, so that a change of them before the backward pass is an error)
+        ctx.save_for_backward(x8, xs, values_n, scales, *slices)
         ctx.md, ctx.pow2, ctx.w_shape, ctx.w_dtype = md, pow2, w.shape, w.dtype
-        ctx.like = [_like(t) for t in (x8, xs, values_n, scales)]
+        ctx.like = [_like(t) for t in (x8, xs, values_n, scales, *slices)]
         return y
 
     @staticmethod
     @once
     def backward(ctx, dy):
-        names = ("x8", "x_scale", "w8", "w_scale")
+        names = ("x8", "x_scale", "w8", "w_scale", "slice_sizes", "slice_offs", "block_schedule_data")
         own = all(r.unpack_hook is None for r in ctx._raw_saved_tensors)  # (what a hook gives back for the scales need not be the quantiser's)
-        x8, xs, values_n, scales = (_check_saved(*v) for v in zip(ctx.saved_tensors, ctx.like, names))
+        x8, xs, values_n, scales, *slices = (_check_saved(*v) for v in zip(ctx.saved_tensors, ctx.like, names))
+        md = None
+        if slices:
+            sizes, offs, schedule = (t.contiguous() for t in slices)
+            md = RaggedTensorMetadata(sizes, offs, ctx.md.block_offs_data, schedule)
         x8 = x8 if x8.stride(1) == 1 or x8.shape[1] <= 1 else x8.contiguous()
         values_n = values_n if values_n.stride(2) == 1 or values_n.shape[2] <= 1 else values_n.contiguous()
         dx = dw = None
         if ctx.needs_input_grad[0]:
             d8, ds = _quantize_rows(dy)
-            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, ctx.md, None, None, None, None, dy.dtype, True, ctx.pow2 and own)
+            dx = _gemm(d8, ds, values_n.transpose(1, 2), scales.transpose(1, 2), None, md, None, None, None, None, dy.dtype, True, ctx.pow2 and own)
         if ctx.needs_input_grad[1]:
-            dw = _weight_gradient(x8, xs, dy, ctx.md, ctx.w_dtype, own).view(ctx.w_shape)
+            dw = _weight_gradient(x8, xs, dy, md, ctx.w_dtype, own).view(ctx.w_shape)
         return dx, dw, None, None, None, None, None
 
 
